@@ -67,10 +67,12 @@ typedef struct CUstream_st *memt_stream_t;
  * NONE:        gate absent (log-decay 0 / factor 1)
  * PER_HEAD:    one value per (token, head): [L, H]          (BASELINE's g, beta)
  * PER_CHANNEL: one value per (token, head, channel): [L, H, D] (the reference's layout)
+ * CONSTANT:    one value per head for all tokens: [H]
  */
 #define MEMT_GATE_NONE 0
 #define MEMT_GATE_PER_HEAD 1
 #define MEMT_GATE_PER_CHANNEL 2
+#define MEMT_GATE_CONSTANT 3 /* one value per head, the same for every token: [H] (linear attention, steps) */
 
 /* Library version (major*10000 + minor*100 + patch).
  *   0.2.0  state pools by slot index (fields appended to the update, read and readout args)
@@ -368,15 +370,136 @@ typedef struct memt_latent_norm_args {
 
 int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream);
 
+/* ---- causal linear attention with a decay for each head ---------------------
+ *
+ * No counterpart in the reference: the recurrence of the update without its delta correction,
+ * with every token reading the state it has just written. Per sample, from initial_state, for
+ * each token t and value head h, with key head h / (num_heads / num_key_heads):
+ *     S_t = exp(g_t) S_{t-1} + k_t v_t^T,      out_t = cast(scale S_t^T q_t)
+ * final_state receives the last S (fp32). A sample without tokens keeps its initial state.
+ *
+ * dtype BF16: chunked on tensor cores. The fp32 state is kept exactly as the recurrence leaves it
+ *   up to fp32 rounding (k is split into three bf16 terms); the output is made from bf16 scores
+ *   and a bf16 copy of the state. dtype F32: exact fp32 token recurrence on CUDA cores.
+ * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] or
+ * decreasing ones are clamped. The tensors are read as token rows of *_stride elements (a
+ * multiple of 16 bytes), so split views of wider projections need no copy.
+ */
+typedef struct memt_linear_attention_args {
+  uint32_t struct_size;    /* sizeof(memt_linear_attention_args)                */
+  int32_t num_samples;     /* N >= 1                                            */
+  int32_t num_heads;       /* H value heads                                     */
+  int32_t num_key_heads;   /* Hk query and key heads, a divisor of H            */
+  int32_t head_dim;        /* D: 64, 128 or 256                                 */
+  int32_t dtype;           /* MEMT_BF16 or MEMT_F32: q, k, v and out            */
+  int64_t total_tokens;    /* rows L of q, k, v, out                            */
+  const int32_t *cu_seqlens; /* device [N+1]                                    */
+  const void *q;           int64_t q_stride;   /* [L,Hk,D]                      */
+  const void *k;           int64_t k_stride;   /* [L,Hk,D]                      */
+  const void *v;           int64_t v_stride;   /* [L,H,D]                       */
+  const float *g;          /* natural-log decay (<= 0): NONE, PER_HEAD [L,H], CONSTANT [H] */
+  int32_t g_layout;
+  float scale;
+  void *out;               int64_t out_stride; /* [L,H,D]                       */
+  const float *initial_state; /* [N,H,D,D] fp32, or NULL: zero states           */
+  float *final_state;         /* [N,H,D,D] fp32, may alias initial_state        */
+  /* Optional state pools, as in memt_gdn2_update_args. An input slot outside its pool starts
+   * from a zero state; an output slot outside its pool, or one that an earlier sample of the call
+   * writes, is not written. */
+  const int32_t *initial_slots;
+  int32_t num_initial_slots;
+  const int32_t *final_slots;
+  int32_t num_final_slots;
+} memt_linear_attention_args;
+
+/* Workspace bytes for these sizes (0 on invalid sizes). */
+size_t memt_linear_attention_workspace_size(int32_t num_samples, int64_t total_tokens, int32_t num_heads,
+                                            int32_t head_dim, int32_t dtype);
+
+/* workspace: device memory of at least the size above, 256-byte aligned. */
+int memt_linear_attention(const memt_linear_attention_args *args, void *workspace, size_t workspace_bytes,
+                          memt_stream_t stream);
+
+/* ---- one token of a recurrence, states in place --------------------------
+ *
+ * No counterpart in the reference (its executor commits through the chunked update): the
+ * single-token form of the two recurrences, one pass over the fp32 states. For sample n and
+ * value head h, key head h / (num_heads / num_key_heads):
+ *   RULE_LINEAR: S <- exp(g) S + k v^T,                        out = cast(scale S^T q)
+ *   RULE_GDN2:   k' = sqrt(beta) k,  S~ = diag(exp(g)) S,  d = write*v - S~^T (erase*k'),
+ *                S <- S~ + k' d^T,                             out = cast(scale S^T q)
+ * with read_incoming the output reads the state before the update, as a commit does. Arithmetic
+ * is fp32 whatever the dtype. beta and erase belong to key heads, g and write to value heads.
+ * A sample whose slot lies outside the pool, or whose slot an earlier sample of the call names,
+ * is skipped: neither its state nor its output row is written (pad a batch with slot -1). */
+#define MEMT_RULE_LINEAR 0
+#define MEMT_RULE_GDN2 1
+typedef struct memt_recurrent_step_args {
+  uint32_t struct_size;    /* sizeof(memt_recurrent_step_args)                  */
+  int32_t rule;            /* MEMT_RULE_LINEAR or MEMT_RULE_GDN2                */
+  int32_t num_samples;     /* N tokens, one per sample                          */
+  int32_t num_heads;       /* H value heads                                     */
+  int32_t num_key_heads;   /* Hk, a divisor of H                                */
+  int32_t head_dim;        /* 64, 128 or 256                                    */
+  int32_t dtype;           /* MEMT_BF16 or MEMT_F32: q, k, v, beta, erase, write, out */
+  int32_t read_incoming;   /* GDN2: read the state before the update            */
+  const void *q;           int64_t q_stride;   /* [N,Hk,D]                      */
+  const void *k;           int64_t k_stride;   /* [N,Hk,D]                      */
+  const void *v;           int64_t v_stride;   /* [N,H,D]                       */
+  const float *g;          /* NONE, PER_HEAD [N,H], CONSTANT [H]; GDN2 also PER_CHANNEL [N,H,D] */
+  int32_t g_layout;
+  int32_t beta_layout;     /* NONE, PER_HEAD [N,Hk], PER_CHANNEL [N,Hk,D]       */
+  const void *beta;
+  const void *erase;       /* NULL or [N,Hk,D]                                  */
+  const void *write;       /* NULL or [N,H,D]                                   */
+  float *states;           /* [N,H,D,D] fp32, or a pool [num_slots,H,D,D]       */
+  const int32_t *slots;    /* NULL or device [N]                                */
+  int32_t num_slots;
+  float scale;
+  void *out;               int64_t out_stride; /* [N,H,D]                       */
+} memt_recurrent_step_args;
+
+int memt_recurrent_step(const memt_recurrent_step_args *args, memt_stream_t stream);
+
+/* ---- rotary positions ------------------------------------------------------
+ *
+ * No counterpart in the reference's memory block. Pair i of the first rotary_dim elements of
+ * every head (elements i and i + rotary_dim/2, or 2i and 2i + 1 when interleaved) is turned by
+ * position * inv_freq[i] (by its negative when inverse) and multiplied by attention_scale; the
+ * elements behind rotary_dim are copied. Angles are formed in 64 bits, the rotation is fp32. The
+ * outputs may be the inputs (in place); otherwise they must not overlap them. */
+typedef struct memt_rotary_args {
+  uint32_t struct_size;    /* sizeof(memt_rotary_args)                          */
+  int32_t num_heads;       /* query heads                                       */
+  int32_t num_key_heads;   /* 0: no keys (k, k_out ignored)                     */
+  int32_t head_dim;
+  int32_t rotary_dim;      /* even, <= head_dim                                 */
+  int32_t dtype;           /* MEMT_BF16 or MEMT_F32                             */
+  int64_t total_tokens;
+  const void *q;           int64_t q_stride;   /* token rows of *_stride elements */
+  const void *k;           int64_t k_stride;
+  void *q_out;             int64_t q_out_stride;
+  void *k_out;             int64_t k_out_stride;
+  const void *positions;   /* int32 or int64 [total_tokens]                     */
+  int32_t positions_int64;
+  int32_t interleaved;
+  const double *inv_freq;  /* device fp64 [rotary_dim / 2], radians per position */
+  float attention_scale;
+  int32_t inverse;
+} memt_rotary_args;
+
+int memt_rotary(const memt_rotary_args *args, memt_stream_t stream);
+
 /* ---- kernel timing (benchmarks) ----------------------------------------
  *
  * No counterpart in the reference (its kernels are timed from Python). When enabled,
  * every kernel this library launches is bracketed by CUDA events on its own stream and
  * its device time is accumulated per kernel family; disabled (the default) it costs
  * nothing. Families: 0 plan, 1 intra (WY operands), 2 scan, 3 read (GEMV),
- * 4 read (tensor-core tiles), 5 fp32 recurrence, 6 prologue and latent norm.
+ * 4 read (tensor-core tiles), 5 fp32 recurrence, 6 prologue and latent norm, 7 linear attention,
+ * 8 single-token steps, 9 rotary.
  */
-#define MEMT_PROF_FAMILIES 7
+#define MEMT_PROF_FAMILIES 10
 int memt_profiler_enable(int on);
 int memt_profiler_reset(void);
 /* Synchronises the recorded events, then fills ms[i] (total device milliseconds) and

@@ -37,7 +37,10 @@ cudaError_t ensure_smem(Kernel kernel, size_t bytes) {
 
 // Optional per-launch CUDA-event timing (memt_profiler_*). Usage around a launch:
 //   ProfScope prof(kProfIntra, stream);  kernel<<<...>>>(...);
-enum ProfFamily { kProfPlan = 0, kProfIntra, kProfScan, kProfReadGemv, kProfReadTile, kProfRecurrent, kProfPrologue };
+enum ProfFamily {
+  kProfPlan = 0, kProfIntra, kProfScan, kProfReadGemv, kProfReadTile, kProfRecurrent, kProfPrologue,
+  kProfLinear, kProfStep, kProfRotary
+};
 void prof_begin(int family, cudaStream_t s, void** token);
 void prof_end(void* token, cudaStream_t s);
 struct ProfScope {
@@ -46,6 +49,14 @@ struct ProfScope {
   ProfScope(int family, cudaStream_t stream) : s(stream) { prof_begin(family, stream, &token); }
   ~ProfScope() { prof_end(token, s); }
 };
+
+// Multiprocessors of the current device.
+inline int device_sms(int* sms) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+  return cuda_status(e);
+}
 
 // CTAs of this kernel that fit on the device at once (SM count x occupancy), cached per
 // (kernel, device).

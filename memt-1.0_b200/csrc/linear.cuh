@@ -1,0 +1,120 @@
+// Causal linear attention with a decay for each head, packed samples: parameters of its kernels
+// and the token-by-token form.
+//
+//     S_t = e^{g_t} S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t
+//
+// The token-by-token kernel is the definition in fp32 on CUDA cores. It serves fp32 inputs (as
+// the fp32 mode of the update does) and is bound by the latency of the token chain.
+// One warp owns kCols value columns of one (sample, head): the state's D rows are spread over the
+// lanes (D / 32 rows each), so a token costs D / 32 * kCols * 2 multiply-adds a lane and one
+// butterfly sum over the lanes, without any barrier between warps. The next token's vectors are
+// fetched while this one is folded in.
+#pragma once
+
+#include "common.cuh"
+#include "step.cuh"
+
+namespace memt {
+
+struct LinearParams {
+  int32_t N, H, Hk;
+  int64_t L;
+  const int32_t* cu;
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t sq, sk, sv, so;  // elements per token row
+  const float* g;
+  int32_t g_layout;  // MEMT_GATE_NONE / PER_HEAD / CONSTANT
+  float scale;
+  void* out;
+  const float* h0;  // null: zero states
+  float* ht;
+  const int32_t* slots_in;
+  const int32_t* slots_out;
+  int32_t num_in, num_out;
+};
+
+// tokens [bos, eos) of sample n, clamped to the packed rows
+__device__ __forceinline__ void sample_range(const LinearParams& p, int n, int64_t& bos, int64_t& eos) {
+  bos = p.cu[n];
+  eos = p.cu[n + 1];
+  bos = bos < 0 ? 0 : (bos > p.L ? p.L : bos);
+  eos = eos < bos ? bos : (eos > p.L ? p.L : eos);
+}
+
+__device__ __forceinline__ float log_decay(const LinearParams& p, int64_t t, int h) {
+  return p.g_layout == 1 ? p.g[t * p.H + h] : (p.g_layout == 3 ? p.g[h] : 0.f);
+}
+
+// an earlier sample of this call writes the same slot
+__device__ __forceinline__ bool slot_taken(const int32_t* slots, int n, int64_t slot, int tid, int threads) {
+  bool taken = false;
+  if (slots != nullptr)
+    for (int i = tid; i < n; i += threads) taken |= slots[i] == static_cast<int32_t>(slot);
+  return taken;
+}
+
+struct LinearRecurrentCfg {
+  static constexpr int kCols = 4;   // value columns per warp
+  static constexpr int kWarps = 4;  // warps per CTA, consecutive column groups
+};
+
+template <int D, typename T>
+__global__ void __launch_bounds__(LinearRecurrentCfg::kWarps * 32) linear_recurrent_kernel(const LinearParams p) {
+  constexpr int C = LinearRecurrentCfg::kCols, W = LinearRecurrentCfg::kWarps, R = D / 32;
+  constexpr int kBlocks = D / (C * W);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int blk = blockIdx.x % kBlocks, nh = blockIdx.x / kBlocks;
+  const int h = nh % p.H, n = nh / p.H, hk = h / (p.H / p.Hk);
+  const int col = (blk * W + warp) * C, row = lane * R;
+  int64_t bos, eos;
+  sample_range(p, n, bos, eos);
+  const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
+  float S[R][C];
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < C; ++e)
+      S[i][e] = p.h0 != nullptr && in_slot >= 0 ? p.h0[((in_slot * p.H + h) * D + row + i) * D + col + e] : 0.f;
+  float q[R], k[R], v[C], g = 0.f;
+  auto fetch = [&](int64_t t) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      q[i] = load_f32<T>(p.q, t * p.sq + (int64_t)hk * D + row + i);
+      k[i] = load_f32<T>(p.k, t * p.sk + (int64_t)hk * D + row + i);
+    }
+#pragma unroll
+    for (int e = 0; e < C; ++e) v[e] = load_f32<T>(p.v, t * p.sv + (int64_t)h * D + col + e);
+    g = log_decay(p, t, h);
+  };
+  if (bos < eos) fetch(bos);
+  for (int64_t t = bos; t < eos; ++t) {
+    float o[C] = {0.f, 0.f, 0.f, 0.f};
+    const float a = expf(g);
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+      for (int e = 0; e < C; ++e) {
+        S[i][e] = fmaf(a, S[i][e], k[i] * v[e]);
+        o[e] = fmaf(S[i][e], q[i], o[e]);
+      }
+    if (t + 1 < eos) fetch(t + 1);
+#pragma unroll
+    for (int e = 0; e < C; ++e)
+#pragma unroll
+      for (int m = 16; m > 0; m >>= 1) o[e] += __shfl_xor_sync(0xffffffffu, o[e], m);
+    if (lane < C) {
+      const float x = lane == 0 ? o[0] : lane == 1 ? o[1] : lane == 2 ? o[2] : o[3];
+      store_f32(static_cast<T*>(p.out), t * p.so + (int64_t)h * D + col + lane, p.scale * x);
+    }
+  }
+  const bool taken = __any_sync(0xffffffffu, slot_taken(p.slots_out, n, out_slot, lane, 32));
+  if (out_slot < 0 || taken) return;
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < C; ++e) p.ht[((out_slot * p.H + h) * D + row + i) * D + col + e] = S[i][e];
+}
+
+}  // namespace memt

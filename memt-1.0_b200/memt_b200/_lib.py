@@ -25,6 +25,10 @@ MEMT_BF16 = 1
 GATE_NONE = 0
 GATE_PER_HEAD = 1
 GATE_PER_CHANNEL = 2
+GATE_CONSTANT = 3
+
+RULE_LINEAR = 0
+RULE_GDN2 = 1
 
 
 class _SizedArgs(ctypes.Structure):
@@ -92,6 +96,42 @@ class LatentNormArgs(_SizedArgs):
     ]
 
 
+class LinearAttentionArgs(_SizedArgs):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("num_samples", c_int32), ("num_heads", c_int32), ("num_key_heads", c_int32), ("head_dim", c_int32),
+        ("dtype", c_int32), ("total_tokens", c_int64), ("cu_seqlens", c_void_p),
+        ("q", c_void_p), ("q_stride", c_int64), ("k", c_void_p), ("k_stride", c_int64),
+        ("v", c_void_p), ("v_stride", c_int64), ("g", c_void_p), ("g_layout", c_int32), ("scale", c_float),
+        ("out", c_void_p), ("out_stride", c_int64), ("initial_state", c_void_p), ("final_state", c_void_p),
+        ("initial_slots", c_void_p), ("num_initial_slots", c_int32), ("final_slots", c_void_p),
+        ("num_final_slots", c_int32),
+    ]
+
+
+class RecurrentStepArgs(_SizedArgs):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("rule", c_int32), ("num_samples", c_int32), ("num_heads", c_int32), ("num_key_heads", c_int32),
+        ("head_dim", c_int32), ("dtype", c_int32), ("read_incoming", c_int32),
+        ("q", c_void_p), ("q_stride", c_int64), ("k", c_void_p), ("k_stride", c_int64),
+        ("v", c_void_p), ("v_stride", c_int64), ("g", c_void_p), ("g_layout", c_int32), ("beta_layout", c_int32),
+        ("beta", c_void_p), ("erase", c_void_p), ("write", c_void_p), ("states", c_void_p), ("slots", c_void_p),
+        ("num_slots", c_int32), ("scale", c_float), ("out", c_void_p), ("out_stride", c_int64),
+    ]
+
+
+class RotaryArgs(_SizedArgs):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("num_heads", c_int32), ("num_key_heads", c_int32), ("head_dim", c_int32), ("rotary_dim", c_int32),
+        ("dtype", c_int32), ("total_tokens", c_int64), ("q", c_void_p), ("q_stride", c_int64),
+        ("k", c_void_p), ("k_stride", c_int64), ("q_out", c_void_p), ("q_out_stride", c_int64),
+        ("k_out", c_void_p), ("k_out_stride", c_int64), ("positions", c_void_p), ("positions_int64", c_int32),
+        ("interleaved", c_int32), ("inv_freq", c_void_p), ("attention_scale", c_float), ("inverse", c_int32),
+    ]
+
+
 # name -> (restype, argtypes): every symbol include/memt_gdn2.h declares
 SIGNATURES = {
     "memt_version": (c_int, []),
@@ -109,12 +149,16 @@ SIGNATURES = {
     "memt_latent_rms_norm": (c_int, [POINTER(LatentNormArgs), c_void_p]),
     "memt_gdn2_update_noalloc": (c_int, [POINTER(UpdateArgs), c_void_p]),
     "memt_gdn2_noalloc_status": (c_int, [c_void_p, POINTER(c_int32)]),
+    "memt_linear_attention_workspace_size": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32]),
+    "memt_linear_attention": (c_int, [POINTER(LinearAttentionArgs), c_void_p, c_size_t, c_void_p]),
+    "memt_recurrent_step": (c_int, [POINTER(RecurrentStepArgs), c_void_p]),
+    "memt_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
     "memt_profiler_enable": (c_int, [c_int]),
     "memt_profiler_reset": (c_int, []),
     "memt_profiler_read": (c_int, [POINTER(ctypes.c_double), POINTER(c_int64), c_int]),
 }
 
-PROF_FAMILIES = ["plan", "intra", "scan", "read_gemv", "read_tile", "recurrent", "prologue"]
+PROF_FAMILIES = ["plan", "intra", "scan", "read_gemv", "read_tile", "recurrent", "prologue", "linear", "step", "rotary"]
 
 
 def profiler_enable(on: bool) -> None:

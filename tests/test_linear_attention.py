@@ -1,0 +1,600 @@
+"""Causal linear attention with a decay for each head and the single-token steps.
+
+CPU: refusals of the C entry points. GPU: every operator against the recurrence in 64 bits on the
+same (rounded) inputs.
+
+Tolerances are elementwise bounds. With u = 2^-24 (half an fp32 step) and A the same recurrence
+over absolute values (an upper bound of every partial sum):
+  * one recurrence step rounds the decay (expf: 2 steps), a product, a sum: <= 8 u of A a token;
+    a sum over D rows <= D u of A; hence (8 T + D + 8) u A for T tokens of the fp32 kernels;
+  * the chunked bf16 kernel keeps the state in fp32: weights exp(R) carry the rounding of the
+    exponent sum R (7 additions, |R| <= r: 7 r u) and of exp2 (4 u), the three-term split of k
+    leaves 2 u, 3 x 64 truncating additions of a chunk <= 2 u each, the carry 4 u a chunk:
+    (7 r + 6 + 384 + 4 chunks) u A;
+  * its output rounds scores, state copy and result to bf16 (half a step: 2^-8 each):
+    2^-8 (1 + 2^-7) (A_o + |o|) plus the fp32 share above.
+"""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import memt_b200 as M
+from memt_b200 import _lib
+
+gpu = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: U}
+
+
+# ---------------------------------------------------------------------------
+# refusals of the C entry points (nothing is launched)
+# ---------------------------------------------------------------------------
+
+def _linear_args(**over):
+    f = dict(num_samples=1, num_heads=4, num_key_heads=2, head_dim=64, dtype=_lib.MEMT_BF16, total_tokens=8,
+             cu_seqlens=16, q=16, q_stride=128, k=16, k_stride=128, v=16, v_stride=256, g=16,
+             g_layout=_lib.GATE_PER_HEAD, scale=1.0, out=16, out_stride=256, final_state=16)
+    f.update(over)
+    return _lib.LinearAttentionArgs(**f)
+
+
+BAD_LINEAR = [
+    (dict(struct_size=8), "INVALID_ARGUMENT"), (dict(num_samples=0), "INVALID_ARGUMENT"),
+    (dict(num_heads=3), "INVALID_ARGUMENT"), (dict(num_key_heads=0), "INVALID_ARGUMENT"),
+    (dict(total_tokens=-1), "INVALID_ARGUMENT"), (dict(total_tokens=2 ** 31), "INVALID_ARGUMENT"),
+    (dict(dtype=5), "INVALID_ARGUMENT"), (dict(head_dim=96), "UNSUPPORTED"), (dict(q=None), "INVALID_ARGUMENT"),
+    (dict(final_state=None), "INVALID_ARGUMENT"), (dict(g=None), "INVALID_ARGUMENT"),
+    (dict(g_layout=_lib.GATE_NONE), "INVALID_ARGUMENT"), (dict(g_layout=_lib.GATE_PER_CHANNEL), "INVALID_ARGUMENT"),
+    (dict(q_stride=120), "INVALID_ARGUMENT"), (dict(v_stride=128), "INVALID_ARGUMENT"),
+    (dict(out_stride=128), "INVALID_ARGUMENT"), (dict(k_stride=132), "MISALIGNED"), (dict(v=24), "MISALIGNED"),
+    (dict(initial_slots=16, num_initial_slots=1), "INVALID_ARGUMENT"),
+    (dict(final_slots=16, num_final_slots=0), "INVALID_ARGUMENT"),
+]
+
+
+@pytest.mark.parametrize("over,error", BAD_LINEAR)
+def test_linear_attention_refuses(over, error):
+    a = _linear_args(**over)
+    assert _lib.load().memt_linear_attention(ctypes.byref(a), 256, 1 << 40, None) == getattr(_lib, "MEMT_ERR_" + error)
+
+
+def test_linear_attention_refuses_workspace():
+    lib, a = _lib.load(), _linear_args()
+    assert lib.memt_linear_attention(None, 256, 1 << 40, None) == _lib.MEMT_ERR_INVALID_ARGUMENT
+    assert lib.memt_linear_attention(ctypes.byref(a), None, 1 << 40, None) == _lib.MEMT_ERR_WORKSPACE
+    assert lib.memt_linear_attention(ctypes.byref(a), 256, 0, None) == _lib.MEMT_ERR_WORKSPACE
+    assert lib.memt_linear_attention(ctypes.byref(a), 264, 1 << 40, None) == _lib.MEMT_ERR_WORKSPACE
+    f = lib.memt_linear_attention_workspace_size
+    assert f(1, 0, 1, 64, _lib.MEMT_BF16) >= 256 and f(1, 100, 1, 96, _lib.MEMT_BF16) == 0
+    assert f(0, 100, 1, 64, _lib.MEMT_BF16) == 0 and f(1, 100, 1, 64, 9) == 0
+
+
+def _step_args(**over):
+    f = dict(rule=_lib.RULE_GDN2, num_samples=0, num_heads=4, num_key_heads=2, head_dim=64, dtype=_lib.MEMT_BF16,
+             q=16, q_stride=128, k=16, k_stride=128, v=16, v_stride=256, g=16, g_layout=_lib.GATE_PER_HEAD,
+             states=16, scale=1.0, out=16, out_stride=256)
+    f.update(over)
+    return _lib.RecurrentStepArgs(**f)
+
+
+BAD_STEP = [
+    (dict(struct_size=8), "INVALID_ARGUMENT"), (dict(rule=2), "INVALID_ARGUMENT"),
+    (dict(num_samples=-1), "INVALID_ARGUMENT"), (dict(num_heads=5), "INVALID_ARGUMENT"),
+    (dict(dtype=2), "INVALID_ARGUMENT"), (dict(head_dim=32), "UNSUPPORTED"), (dict(states=None), "INVALID_ARGUMENT"),
+    (dict(states=20), "MISALIGNED"), (dict(g=None), "INVALID_ARGUMENT"), (dict(g_layout=4), "INVALID_ARGUMENT"),
+    (dict(beta=16), "INVALID_ARGUMENT"), (dict(beta_layout=1), "INVALID_ARGUMENT"),
+    (dict(q_stride=64), "INVALID_ARGUMENT"), (dict(out_stride=8), "INVALID_ARGUMENT"),
+    (dict(slots=16, num_slots=0), "INVALID_ARGUMENT"),
+    (dict(rule=_lib.RULE_LINEAR, write=16), "UNSUPPORTED"), (dict(rule=_lib.RULE_LINEAR, read_incoming=1), "UNSUPPORTED"),
+    (dict(rule=_lib.RULE_LINEAR, g_layout=_lib.GATE_PER_CHANNEL), "UNSUPPORTED"),
+]
+
+
+@pytest.mark.parametrize("over,error", BAD_STEP)
+def test_step_refuses(over, error):
+    a = _step_args(**over)
+    assert _lib.load().memt_recurrent_step(ctypes.byref(a), None) == getattr(_lib, "MEMT_ERR_" + error)
+
+
+def test_empty_step_launches_nothing():
+    assert _lib.load().memt_recurrent_step(ctypes.byref(_step_args()), None) == _lib.MEMT_OK
+    assert _lib.load().memt_recurrent_step(None, None) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+def test_operators_refuse_host_tensors():
+    x, s = torch.zeros(3, 2, 64), torch.zeros(3, 2, 64, 64)
+    with pytest.raises(ValueError):
+        M.linear_attention(x, x, x, None, s, torch.tensor([0, 1, 2, 3]))
+    with pytest.raises(ValueError):
+        M.linear_attention_step(x, x, x, None, s)
+    with pytest.raises(ValueError):
+        M.gdn2_step(x, x, x, None, s)
+
+
+# ---------------------------------------------------------------------------
+# the definition in 64 bits
+# ---------------------------------------------------------------------------
+
+def _recurrence(q, k, v, g, h0, cu, scale):
+    """fp64 (o, final) and the same recurrence over absolute values (A_o, A_final). CPU tensors."""
+    L, H, D = v.shape
+    rep = H // q.shape[1]
+    q, k, v = (x.double() for x in (q.repeat_interleave(rep, 1), k.repeat_interleave(rep, 1), v))
+    a = torch.ones(L, H, dtype=torch.float64) if g is None else torch.exp(g.double()).expand(L, H)
+    S, B = h0.double().clone(), h0.double().abs()
+    o, A = torch.zeros(L, H, D, dtype=torch.float64), torch.zeros(L, H, D, dtype=torch.float64)
+    for n in range(len(cu) - 1):
+        for t in range(int(cu[n]), int(cu[n + 1])):
+            S[n] = a[t][:, None, None] * S[n] + k[t][:, :, None] * v[t][:, None, :]
+            B[n] = a[t][:, None, None] * B[n] + (k[t][:, :, None] * v[t][:, None, :]).abs()
+            o[t] = scale * torch.einsum("hk,hkv->hv", q[t], S[n])
+            A[t] = abs(scale) * torch.einsum("hk,hkv->hv", q[t].abs(), B[n])
+    return o, S, A, B
+
+
+def _inputs(seed, lengths, Hk, H, D, dtype, decay, gscale=1.0):
+    gen = torch.Generator().manual_seed(seed)
+    L, N = sum(lengths), len(lengths)
+    unit = lambda x: x / (x.square().sum(-1, keepdim=True) + 1e-6).sqrt()  # noqa: E731
+    q = unit(torch.randn(L, Hk, D, generator=gen)).to(dtype)
+    k = unit(torch.randn(L, Hk, D, generator=gen)).to(dtype)
+    v = torch.randn(L, H, D, generator=gen).to(dtype)
+    g = {"none": None, "head": -torch.exp2(-8.0 * torch.arange(1, H + 1) / H),
+         "token": torch.nn.functional.logsigmoid(2 + 0.5 * torch.randn(L, H, generator=gen))}[decay]
+    g = None if g is None else g * gscale
+    h0 = 0.5 * torch.randn(N, H, D, D, generator=gen)
+    cu = torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32)
+    return q, k, v, g, h0, cu
+
+
+def _dev(*xs):
+    return tuple(None if x is None else x.cuda() for x in xs)
+
+
+def _check(got, ref, tol, what):
+    err = (got.double().cpu() - ref).abs()
+    bad = err > tol
+    assert not bool(bad.any()) and not bool(torch.isnan(err).any()), \
+        f"{what}: worst {float((err / (tol + 1e-300)).max()):.3g} of its bound"
+
+
+def _tolerances(ref, lengths, D, dtype, g, H):
+    o, S, A, B = ref
+    T = max(lengths)
+    if dtype == torch.float32:
+        return (8 * T + D + 8) * U * A + U * o.abs() + 1e-40, (8 * T + 8) * U * B + 1e-40
+    r = 0.0 if g is None else 64 * float(g.abs().max()) * 1.4427
+    share = (7 * r + 390 + 4 * (T / 64 + 1)) * U
+    return HALF[dtype] * (1 + 2.0 ** -7) * (A + o.abs()) + (share + D * U) * A + 1e-40, share * B + 1e-40
+
+
+def _run_and_check(lengths, Hk, H, D, dtype, decay, seed=0, gscale=1.0):
+    q, k, v, g, h0, cu = _inputs(seed, lengths, Hk, H, D, dtype, decay, gscale)
+    scale = D ** -0.5
+    ref = _recurrence(q, k, v, g, h0, cu, scale)
+    dq, dk, dv, dg, dh, dcu = _dev(q, k, v, g, h0, cu)
+    before = dh.clone()
+    o, final = M.linear_attention(dq, dk, dv, dg, dh, dcu)
+    torch.cuda.synchronize()
+    to, ts = _tolerances(ref, lengths, D, dtype, g, H)
+    _check(final, ref[1], ts, "state")
+    _check(o, ref[0], to, "output")
+    assert torch.equal(dh, before)
+    return o, final
+
+
+# ---------------------------------------------------------------------------
+# linear_attention
+# ---------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths", [[1], [63], [64], [65], [128, 1, 0, 200], [0, 3, 130]])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_attention_lengths(cuda, D, lengths, dtype):
+    _run_and_check(lengths, 2, 2, D, dtype, "token", seed=D + len(lengths))
+
+
+@gpu
+@pytest.mark.parametrize("decay", ["none", "head", "token"])
+@pytest.mark.parametrize("Hk,H", [(1, 3), (2, 4), (3, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_linear_attention_heads_and_decays(cuda, decay, Hk, H, dtype):
+    _run_and_check([150, 70], Hk, H, 64, dtype, decay, seed=H)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_linear_attention_many_chunks(cuda, D):
+    _run_and_check([1100], 1, 2, D, torch.bfloat16, "head", seed=3)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strong_decays_and_resets(cuda, dtype):
+    """Decays from none to a full reset (g = -inf forgets everything before the token)."""
+    lengths, H, D = [200, 90], 2, 64
+    q, k, v, g, h0, cu = _inputs(5, lengths, H, H, D, dtype, "token")
+    g[::7] = -40.0
+    g[::31] = 0.0
+    g[50] = -float("inf")
+    g[64] = -float("inf")
+    g[127:131] = -float("inf")
+    g[230] = -1e4
+    ref = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    dq, dk, dv, dg, dh, dcu = _dev(q, k, v, g, h0, cu)
+    o, final = M.linear_attention(dq, dk, dv, dg, dh, dcu)
+    torch.cuda.synchronize()
+    # exponents: sums between two tokens that still see each other stay below 60 in magnitude
+    # where the weight is above 2^-86; smaller weights are below every bound here
+    to, ts = _tolerances(ref, lengths, D, dtype, torch.tensor([1.0]), H)
+    _check(final, ref[1], ts + 1e-20, "state")
+    _check(o, ref[0], to + 1e-20, "output")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_masked_places_do_not_leak(cuda, dtype):
+    """NaN and infinities in rows behind a sample's end, in other samples and in other heads stay
+    there; rows of out that belong to no sample are left as they were."""
+    lengths, H, D = [70, 33, 65], 2, 64
+    q, k, v, g, h0, cu = _inputs(6, lengths, H, H, D, dtype, "token")
+    pad = 40
+    rows = sum(lengths)
+
+    def padded(x, value):
+        return torch.cat([x, torch.full((pad, *x.shape[1:]), value, dtype=x.dtype)])
+
+    q, k, v, g = padded(q, float("nan")), padded(k, float("inf")), padded(v, float("nan")), padded(g, float("nan"))
+    bad = slice(70, 103)  # the middle sample
+    k[bad, 0], v[bad, 0] = float("nan"), float("inf")
+    ref = _recurrence(q[:rows], k[:rows], v[:rows], g[:rows], h0, cu, D ** -0.5)
+    out = torch.full((rows + pad, H, D), 7.0, dtype=dtype, device="cuda")
+    dq, dk, dv, dg, dh, dcu = _dev(q, k, v, g, h0, cu)
+    o, final = M.linear_attention(dq, dk, dv, dg, dh, dcu, out=out)
+    torch.cuda.synchronize()
+    assert bool((o[rows:] == 7.0).all())
+    to, ts = _tolerances(ref, lengths, D, dtype, g[:rows], H)
+    clean = [r for r in range(rows) if not 70 <= r < 103]
+    _check(o[clean], ref[0][clean], to[clean], "output")
+    _check(o[bad, 1], ref[0][bad, 1], to[bad, 1], "other head")
+    for n in (0, 2):
+        _check(final[n], ref[1][n], ts[n], "state")
+    _check(final[1, 1], ref[1][1, 1], ts[1, 1], "other head's state")
+    assert bool(torch.isnan(final[1, 0]).all()) and bool(torch.isnan(o[bad, 0].float()).all())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_views_pools_and_in_place(cuda, dtype):
+    """Split views of one projection, an output inside a wider buffer, pools updated in place, an
+    input slot outside the pool (zeros), an output slot outside it and one named twice."""
+    lengths, Hk, H, D = [40, 77, 5, 64], 1, 2, 64
+    q, k, v, g, h0, cu = _inputs(8, lengths, Hk, H, D, dtype, "head")
+    L = sum(lengths)
+    wide = torch.zeros(L, (2 * Hk + H) * D + 64, dtype=dtype)
+    wide[:, :D], wide[:, D:2 * D], wide[:, 2 * D:4 * D] = q[:, 0], k[:, 0], v.reshape(L, H * D)
+    wide = wide.cuda()
+    q2, k2, v2 = wide[:, :D].view(L, 1, D), wide[:, D:2 * D].view(L, 1, D), wide[:, 2 * D:4 * D].view(L, H, D)
+    pool = torch.randn(7, H, D, D, generator=torch.Generator().manual_seed(1))
+    ins, outs = [3, 9, 0, 5], [3, 1, -1, 3]
+    start = torch.stack([pool[s] if 0 <= s < 7 else torch.zeros_like(pool[0]) for s in ins])
+    ref = _recurrence(q, k, v, g, start, cu, 0.3)
+    dpool, dg, dcu = _dev(pool, g, cu)
+    slots = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    buffer = torch.full((L, H * D + 128), -3.0, dtype=dtype, device="cuda")
+    o, final = M.linear_attention(q2, k2, v2, dg, dpool, dcu, scale=0.3, initial_slots=slots(ins),
+                                  final_state=dpool, final_slots=slots(outs),
+                                  out=buffer[:, 64:64 + H * D].view(L, H, D))
+    torch.cuda.synchronize()
+    assert final.data_ptr() == dpool.data_ptr() and o.data_ptr() == buffer[:, 64:].data_ptr()
+    assert bool((buffer[:, :64] == -3).all()) and bool((buffer[:, 64 + H * D:] == -3).all())
+    to, ts = _tolerances(ref, lengths, D, dtype, g, H)
+    _check(o, ref[0], to, "output")
+    _check(final[3], ref[1][0], ts[0], "slot 3 (first of two)")
+    _check(final[1], ref[1][1], ts[1], "slot 1")
+    for s in (0, 2, 4, 5, 6):
+        assert torch.equal(final[s].cpu(), pool[s])
+
+
+@gpu
+def test_no_initial_state_is_zeros_and_host_offsets(cuda):
+    q, k, v, g, h0, cu = _inputs(9, [50, 90], 2, 2, 64, torch.bfloat16, "token")
+    dq, dk, dv, dg, dh, dcu = _dev(q, k, v, g, torch.zeros_like(h0), cu)
+    a = M.linear_attention(dq, dk, dv, dg, dh, dcu)
+    b = M.linear_attention(dq[None], dk[None], dv[None], dg[None], None, cu.long())
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@gpu
+def test_samples_are_independent_of_the_pack(cuda):
+    """A sample's result does not depend on what it is packed with, bit for bit."""
+    lengths = [130, 64, 300]
+    q, k, v, g, h0, cu = _dev(*_inputs(10, lengths, 2, 2, 128, torch.bfloat16, "token"))
+    o, final = M.linear_attention(q, k, v, g, h0, cu)
+    at = 0
+    for n, T in enumerate(lengths):
+        s = slice(at, at + T)
+        o1, f1 = M.linear_attention(q[s], k[s], v[s], g[s], h0[n:n + 1], torch.tensor([0, T]))
+        assert torch.equal(o[s], o1) and torch.equal(final[n], f1[0])
+        at += T
+
+
+@gpu
+def test_bad_offsets_are_clamped(cuda):
+    """Device offsets outside the rows or decreasing never reach outside the tensors."""
+    q, k, v, g, h0, _ = _dev(*_inputs(11, [64, 64], 1, 1, 64, torch.bfloat16, "token"))
+    for bad in ([0, 200, 128], [-5, 64, 1 << 30], [100, 20, 128]):
+        o, final = M.linear_attention(q, k, v, g, h0, torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        assert bool(torch.isfinite(final).all())
+
+
+@gpu
+def test_linear_attention_refuses_arguments(cuda):
+    q, k, v, g, h0, cu = _dev(*_inputs(12, [20, 12], 2, 2, 64, torch.bfloat16, "token"))
+    f = M.linear_attention
+    slots = torch.zeros(2, dtype=torch.int32, device="cuda")
+    bad = [
+        lambda: f(q.half(), k.half(), v.half(), g, h0, cu), lambda: f(q.float(), k, v, g, h0, cu),
+        lambda: f(q[:, :, :32], k[:, :, :32], v[:, :, :32], g, h0, cu), lambda: f(q[:10], k, v, g, h0, cu),
+        lambda: f(q.repeat(1, 2, 1)[:, :3], k.repeat(1, 2, 1)[:, :3], v, g, h0, cu),
+        lambda: f(q, k, v, g.double(), h0, cu), lambda: f(q, k, v, g[:5], h0, cu),
+        lambda: f(q, k, v, g, h0[:1], cu), lambda: f(q, k, v, g, h0.half(), cu),
+        lambda: f(q, k, v, g, h0, cu[:1]), lambda: f(q, k, v, g, h0, cu.float()),
+        lambda: f(q, k, v, g, h0, torch.tensor([0, 40, 32])), lambda: f(q, k, v, g, h0, torch.tensor([0, 20, 33])),
+        lambda: f(q, k, v, g, None, cu, initial_slots=slots), lambda: f(q, k, v, g, h0, cu, final_slots=slots),
+        lambda: f(q, k, v, g, h0, cu, initial_slots=slots.long()), lambda: f(q, k, v, g, h0, cu, out=v),
+        lambda: f(q, k, v, g, h0, cu, out=torch.empty_like(v).float()),
+        lambda: f(q, k, v, g, h0, cu, final_state=torch.empty(2, 2, 64, 128, device="cuda")[..., :64]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was accepted")
+
+
+@gpu
+def test_graphs_streams_and_replays(cuda):
+    """Two captured graphs of one stream, replayed together on two streams, and an eager call give
+    the same results: no scratch is shared."""
+    cases = [_dev(*_inputs(20 + i, [700, 300], 2, 4, 128, torch.bfloat16, "token")) for i in range(2)]
+    eager = [M.linear_attention(*c) for c in cases]
+    stream = torch.cuda.Stream()
+    graphs, outs = [], []
+    for c in cases:
+        with torch.cuda.stream(stream):
+            M.linear_attention(*c)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(M.linear_attention(*c))
+        graphs.append(graph)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for s, graph in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+    torch.cuda.synchronize()
+    for (o, f), (eo, ef) in zip(outs, eager):
+        assert torch.equal(o, eo) and torch.equal(f, ef)
+    again = [M.linear_attention(*c) for c in cases]
+    for (o, f), (eo, ef) in zip(again, eager):
+        assert torch.equal(o, eo) and torch.equal(f, ef)
+
+
+# ---------------------------------------------------------------------------
+# single-token steps
+# ---------------------------------------------------------------------------
+
+def _step_inputs(seed, N, Hk, H, D, dtype):
+    gen = torch.Generator().manual_seed(seed)
+    unit = lambda x: x / (x.square().sum(-1, keepdim=True) + 1e-6).sqrt()  # noqa: E731
+    q, k = (unit(torch.randn(N, Hk, D, generator=gen)).to(dtype) for _ in range(2))
+    v = torch.randn(N, H, D, generator=gen).to(dtype)
+    sig = lambda *s: torch.sigmoid(torch.randn(*s, generator=gen)).to(dtype)  # noqa: E731
+    return gen, q, k, v, sig
+
+
+def _step_reference(q, k, v, g, S, beta=None, erase=None, write=None, delta=False, incoming=False, scale=1.0):
+    """fp64 (o, S_new, A_o, A_S)"""
+    rep = v.shape[1] // q.shape[1]
+    up = lambda x: x.double().repeat_interleave(rep, 1)  # noqa: E731
+    q, k, v, S = up(q), up(k), v.double(), S.double()
+    a = torch.ones((), dtype=torch.float64) if g is None else torch.exp(g.double())
+    if g is not None:
+        a = a[:, :, :, None] if a.dim() == 3 else (a[None, :] if a.dim() == 1 else a)[:, :, None, None]
+    new, mag = a * S, a * S.abs()
+    if delta:
+        if beta is not None:
+            b = beta.double().sqrt()
+            k = k * up(b if b.dim() == 3 else b[:, :, None])
+        kb = k if erase is None else k * up(erase)
+        v = v if write is None else v * write.double()
+        vm = v.abs() + torch.einsum("nhk,nhkv->nhv", kb.abs(), mag)
+        v = v - torch.einsum("nhk,nhkv->nhv", kb, new)
+    else:
+        vm = v.abs()
+    new = new + k[..., :, None] * v[..., None, :]
+    mag = mag + k.abs()[..., :, None] * vm[..., None, :]
+    src, smag = (S, S.abs()) if incoming else (new, mag)
+    return (scale * torch.einsum("nhk,nhkv->nhv", q, src), new,
+            scale * torch.einsum("nhk,nhkv->nhv", q.abs(), smag), mag)
+
+
+def _check_step(o, states, ref, D, dtype):
+    # the delta rule's extra sum over D rows enters the state too: (D + 16) u
+    _check(states, ref[1], (D + 16) * U * ref[3] + 1e-40, "state")
+    _check(o, ref[0], (2 * D + 24) * U * ref[2] + HALF[dtype] * ref[0].abs() * 1.01 + 1e-40, "output")
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("N,Hk,H", [(1, 1, 1), (3, 2, 4), (5, 3, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("decay", ["none", "head", "token"])
+def test_linear_attention_step(cuda, D, N, Hk, H, dtype, decay):
+    gen, q, k, v, _ = _step_inputs(D + N, N, Hk, H, D, dtype)
+    g = {"none": None, "head": -torch.rand(H, generator=gen), "token": -torch.rand(N, H, generator=gen)}[decay]
+    S = torch.randn(N, H, D, D, generator=gen)
+    ref = _step_reference(q, k, v, g, S, scale=D ** -0.5)
+    dq, dk, dv, dg, dS = _dev(q, k, v, g, S)
+    o = M.linear_attention_step(dq, dk, dv, dg, dS)
+    torch.cuda.synchronize()
+    _check_step(o, dS, ref, D, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gates", ["none", "head", "channel", "erase", "constant"])
+@pytest.mark.parametrize("incoming", [False, True])
+def test_gdn2_step(cuda, D, dtype, gates, incoming):
+    N, Hk, H = 4, 2, 4
+    gen, q, k, v, sig = _step_inputs(D, N, Hk, H, D, dtype)
+    g = {"none": None, "constant": -torch.rand(H, generator=gen)}.get(
+        gates, -torch.rand(*((N, H) if gates == "head" else (N, H, D)), generator=gen))
+    beta = {"head": sig(N, Hk), "channel": sig(N, Hk, D), "constant": sig(N, Hk)}.get(gates)
+    erase = sig(N, Hk, D) if gates == "erase" else None
+    write = sig(N, H, D) if gates in ("channel", "erase") else None
+    S = torch.randn(N, H, D, D, generator=gen)
+    ref = _step_reference(q, k, v, g, S, beta, erase, write, True, incoming, 0.25)
+    dq, dk, dv, dg, dS, db, de, dw = _dev(q, k, v, g, S, beta, erase, write)
+    o = M.gdn2_step(dq, dk, dv, dg, dS, beta=db, erase=de, write=dw, scale=0.25, read_incoming=incoming)
+    torch.cuda.synchronize()
+    _check_step(o, dS, ref, D, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("rule", ["linear", "gdn2"])
+def test_step_pools_views_and_skipped_rows(cuda, rule):
+    """Slots of a pool; a slot outside it and a slot named twice are skipped, with their rows of o;
+    q, k, v as split views, o inside a wider buffer."""
+    N, H, D = 6, 2, 128
+    gen, q, k, v, _ = _step_inputs(1, N, H, H, D, torch.bfloat16)
+    g = -torch.rand(N, H, generator=gen)
+    pool = torch.randn(9, H, D, D, generator=gen)
+    slots = [8, -1, 2, 9, 8, 0]
+    live = [0, 2, 5]
+    at = [slots[i] for i in live]
+    ref = _step_reference(q[live], k[live], v[live], g[live], pool[at], delta=rule == "gdn2", scale=0.5)
+    wide = torch.cat([q.reshape(N, -1), k.reshape(N, -1), v.reshape(N, -1)], 1).cuda()
+    qv, kv, vv = (wide[:, i * H * D:(i + 1) * H * D].view(N, H, D) for i in range(3))
+    dpool, dg = _dev(pool, g)
+    buffer = torch.full((N, H * D + 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    step = M.gdn2_step if rule == "gdn2" else M.linear_attention_step
+    o = step(qv, kv, vv, dg, dpool, scale=0.5, slots=torch.tensor(slots, dtype=torch.int32, device="cuda"),
+             out=buffer[:, 64:].view(N, H, D))
+    torch.cuda.synchronize()
+    _check_step(o[live], dpool[at], ref, D, torch.bfloat16)
+    assert bool((o[[1, 3, 4]] == 5.0).all()) and bool((buffer[:, :64] == 5.0).all())
+    for s in (1, 3, 4, 5, 6, 7):
+        assert torch.equal(dpool[s].cpu(), pool[s])
+
+
+@gpu
+def test_empty_batch_and_refused_steps(cuda):
+    _, q, k, v, sig = _step_inputs(2, 3, 2, 2, 64, torch.bfloat16)
+    dq, dk, dv = _dev(q, k, v)
+    S = torch.zeros(3, 2, 64, 64, device="cuda")
+    assert M.linear_attention_step(dq[:0], dk[:0], dv[:0], None, S[:0]).shape == (0, 2, 64)
+    g3 = torch.zeros(3, 2, 64, device="cuda")
+    b = sig(3, 2).cuda()
+    bad = [
+        lambda: M.linear_attention_step(dq, dk, dv, g3, S), lambda: M.linear_attention_step(dq, dk, dv, None, S[:2]),
+        lambda: M.linear_attention_step(dq, dk, dv, None, S.half()),
+        lambda: M.linear_attention_step(dq, dk, dv, None, S.transpose(0, 1)),
+        lambda: M.linear_attention_step(dq, dk, dv, None, S, slots=torch.zeros(3, device="cuda", dtype=torch.int64)),
+        lambda: M.linear_attention_step(dq, dk, dv, None, S, out=dv), lambda: M.gdn2_step(dq, dk, dv, None, S, beta=b.float()),
+        lambda: M.gdn2_step(dq, dk, dv, None, S, beta=b[:, :1]), lambda: M.gdn2_step(dq, dk, dv, None, S, erase=b),
+        lambda: M.gdn2_step(dq, dk, dv, None, S, write=dv.float()),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was accepted")
+
+
+@gpu
+def test_step_matches_the_update_it_stands_beside(cuda):
+    """gdn2_step in fp32 is gdn2_update's fp32 recurrence on one-token samples: fp32 rounding of
+    two orders of the same sums ((D + 16) u each)."""
+    N, H, D = 5, 3, 64
+    gen, q, k, v, sig = _step_inputs(4, N, H, H, D, torch.float32)
+    g, S = -torch.rand(N, H, generator=gen), torch.randn(N, H, D, D, generator=gen)
+    beta, write = sig(N, H), sig(N, H, D)
+    ref = _step_reference(q, k, v, g, S, beta, None, write, True)
+    dq, dk, dv, dg, dS, db, dw = _dev(q, k, v, g, S, beta, write)
+    final = M.gdn2_update(dk, dv, dg, dS, torch.arange(N + 1, dtype=torch.int32, device="cuda"), num_samples=N,
+                          total_tokens=N, beta=db, write=dw)
+    M.gdn2_step(dq, dk, dv, dg, dS, beta=db, write=dw)
+    torch.cuda.synchronize()
+    _check(final, dS.double().cpu(), 2 * (D + 16) * U * ref[3], "state")
+
+
+@gpu
+def test_step_in_a_graph_advances_the_states(cuda):
+    N, H, D = 3, 2, 128
+    gen, q, k, v, _ = _step_inputs(6, N, H, H, D, torch.bfloat16)
+    dq, dk, dv, dg, S = _dev(q, k, v, -torch.rand(N, H, generator=gen), torch.randn(N, H, D, D, generator=gen))
+    eager = S.clone()
+    for _ in range(4):
+        want = M.linear_attention_step(dq, dk, dv, dg, eager)
+    out = torch.empty_like(dv)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    keep = S.clone()
+    with torch.cuda.stream(stream):
+        M.linear_attention_step(dq, dk, dv, dg, S, out=out)
+    stream.synchronize()
+    S.copy_(keep)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        M.linear_attention_step(dq, dk, dv, dg, S, out=out)
+    for _ in range(4):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(S, eager) and torch.equal(out, want)
+
+
+# ---------------------------------------------------------------------------
+# a serving run: rotary, prompts, then decode steps
+# ---------------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_prompt_then_steps_equal_one_long_prompt(cuda, dtype):
+    """Rotated prompts through linear_attention into a pool, then six decode tokens through rotary
+    and linear_attention_step, against the 64-bit recurrence over the whole sequences."""
+    prompts, extra, Hk, H, D = [90, 17], 6, 2, 4, 64
+    full = [p + extra for p in prompts]
+    q, k, v, g, h0, cu = _inputs(30, full, Hk, H, D, dtype, "token")
+    inv, att = M.rotary_frequencies(32, scaling="yarn", factor=4.0, trained_tokens=64)
+    pos = torch.cat([torch.arange(n) for n in full]) + 1000
+    dq, dk, dv, dg, dpos = _dev(q, k, v, g, pos)
+    rq, rk = M.rotary(dq, dk, dpos, inv, attention_scale=att)
+    scale = D ** -0.5
+    ref = _recurrence(rq.cpu(), rk.cpu(), v, g, h0, cu, scale)
+    pool = torch.zeros(4, H, D, D, device="cuda")
+    slots = torch.tensor([2, 0], dtype=torch.int32, device="cuda")
+    pool[slots.long()] = h0.cuda()
+    start = [0, full[0]]
+    rows = torch.cat([torch.arange(s, s + p) for s, p in zip(start, prompts)]).cuda()
+    pq, pk = M.rotary(dq[rows], dk[rows], dpos[rows], inv, attention_scale=att)
+    cu_p = torch.tensor([0, prompts[0], sum(prompts)], dtype=torch.int32, device="cuda")
+    o, _ = M.linear_attention(pq, pk, dv[rows], dg[rows], pool, cu_p, initial_slots=slots, final_state=pool,
+                              final_slots=slots)
+    to, ts = _tolerances(ref, full, D, dtype, g, H)
+    got = torch.zeros(sum(full), H, D, device="cuda", dtype=dtype)
+    got[rows] = o
+    for i in range(extra):
+        at = torch.tensor([s + p + i for s, p in zip(start, prompts)], device="cuda")
+        sq, sk = M.rotary(dq[at], dk[at], dpos[at], inv, attention_scale=att)
+        got[at] = M.linear_attention_step(sq, sk, dv[at], dg[at], pool, slots=slots)
+    torch.cuda.synchronize()
+    _check(got, ref[0], to, "outputs")
+    _check(pool[[2, 0]], ref[1], ts + (8 * extra + 8) * U * ref[3], "states")
+    assert bool((pool[[1, 3]] == 0).all())
