@@ -420,6 +420,11 @@ size_t memt_linear_attention_workspace_size(int32_t num_samples, int64_t total_t
 int memt_linear_attention(const memt_linear_attention_args *args, void *workspace, size_t workspace_bytes,
                           memt_stream_t stream);
 
+/* Status of the bf16 calls on the current device since the last call, then cleared: bit 0 = a
+ * bounded wait inside the kernel ran out (results of that call are incomplete). Synchronises the
+ * stream; intended for tests and debugging. */
+int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
+
 /* ---- one token of a recurrence, states in place --------------------------
  *
  * No counterpart in the reference (its executor commits through the chunked update): the

@@ -1,6 +1,7 @@
 // memt_linear_attention: argument checks and launch of the causal linear attention.
 #include "launch.h"
 #include "linear.cuh"
+#include "linear_tc.cuh"
 
 namespace {
 
@@ -8,22 +9,47 @@ using namespace memt;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int D, typename T>
+template <int D>
 int launch_recurrent_form(const LinearParams& p, cudaStream_t s) {
   constexpr int kBlocks = D / (LinearRecurrentCfg::kCols * LinearRecurrentCfg::kWarps);
   const int64_t grid = int64_t(p.N) * p.H * kBlocks;
   if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   ProfScope prof(kProfLinear, s);
-  linear_recurrent_kernel<D, T><<<static_cast<unsigned>(grid), LinearRecurrentCfg::kWarps * 32, 0, s>>>(p);
+  linear_recurrent_kernel<D><<<static_cast<unsigned>(grid), LinearRecurrentCfg::kWarps * 32, 0, s>>>(p);
   return cuda_status(cudaGetLastError());
 }
 
-template <typename T>
 int launch_recurrent_form(int D, const LinearParams& p, cudaStream_t s) {
   switch (D) {
-    case 64: return launch_recurrent_form<64, T>(p, s);
-    case 128: return launch_recurrent_form<128, T>(p, s);
-    default: return launch_recurrent_form<256, T>(p, s);
+    case 64: return launch_recurrent_form<64>(p, s);
+    case 128: return launch_recurrent_form<128>(p, s);
+    default: return launch_recurrent_form<256>(p, s);
+  }
+}
+
+template <int D>
+int launch_chunked(const LinearParams& p, cudaStream_t s) {
+  using Cfg = LinearTcCfg<D>;
+  LinearTcParams P;
+  P.p = p;
+  const uint64_t rows = static_cast<uint64_t>(p.L);
+  cudaError_t e = make_tmap_bf16_2d(&P.q_map, p.q, uint64_t(p.Hk) * D, rows, uint64_t(p.sq) * 2, 64, kTile);
+  if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.k_map, p.k, uint64_t(p.Hk) * D, rows, uint64_t(p.sk) * 2, 64, kTile);
+  if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.v_map, p.v, uint64_t(p.H) * D, rows, uint64_t(p.sv) * 2, 64, kTile);
+  if (e == cudaSuccess) e = ensure_smem(linear_tc_kernel<D, true>, Cfg::kSmem);
+  if (e != cudaSuccess) return cuda_status(e);
+  const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;
+  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  ProfScope prof(kProfLinear, s);
+  linear_tc_kernel<D, true><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
+  return cuda_status(cudaGetLastError());
+}
+
+int launch_chunked(int D, const LinearParams& p, cudaStream_t s) {
+  switch (D) {
+    case 64: return launch_chunked<64>(p, s);
+    case 128: return launch_chunked<128>(p, s);
+    default: return launch_chunked<256>(p, s);
   }
 }
 
@@ -34,12 +60,13 @@ int check_linear(const memt_linear_attention_args* a) {
     return MEMT_ERR_INVALID_ARGUMENT;
   const int D = a->head_dim;
   if (D != 64 && D != 128 && D != 256) return MEMT_ERR_UNSUPPORTED;
-  if (a->cu_seqlens == nullptr || a->q == nullptr || a->k == nullptr || a->v == nullptr || a->out == nullptr ||
-      a->final_state == nullptr)
+  if (a->cu_seqlens == nullptr || a->final_state == nullptr) return MEMT_ERR_INVALID_ARGUMENT;
+  if (a->total_tokens > 0 && (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->out == nullptr))
     return MEMT_ERR_INVALID_ARGUMENT;
   if (a->g_layout != MEMT_GATE_NONE && a->g_layout != MEMT_GATE_PER_HEAD && a->g_layout != MEMT_GATE_CONSTANT)
     return MEMT_ERR_INVALID_ARGUMENT;
-  if ((a->g_layout == MEMT_GATE_NONE) != (a->g == nullptr)) return MEMT_ERR_INVALID_ARGUMENT;
+  if (a->g_layout == MEMT_GATE_NONE ? a->g != nullptr : a->g == nullptr && a->total_tokens > 0)
+    return MEMT_ERR_INVALID_ARGUMENT;
   const int64_t row = int64_t(a->num_heads) * D, krow = int64_t(a->num_key_heads) * D;
   if (a->q_stride < krow || a->k_stride < krow || a->v_stride < row || a->out_stride < row)
     return MEMT_ERR_INVALID_ARGUMENT;
@@ -96,8 +123,22 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   p.slots_out = a->final_slots;
   p.num_out = a->num_final_slots;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == MEMT_F32 ? launch_recurrent_form<float>(a->head_dim, p, s)
-                              : launch_recurrent_form<__nv_bfloat16>(a->head_dim, p, s);
+  // without tokens the states are only copied
+  if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_recurrent_form(a->head_dim, p, s);
+  return launch_chunked(a->head_dim, p, s);
+}
+
+int memt_linear_attention_status(memt_stream_t stream, int32_t* status_out) {
+  if (status_out == nullptr) return MEMT_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int zero = 0;
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_linear_status, sizeof(v), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_linear_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return cuda_status(e);
+  *status_out = v;
+  return MEMT_OK;
 }
 
 }  // extern "C"

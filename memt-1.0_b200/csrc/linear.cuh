@@ -60,7 +60,7 @@ struct LinearRecurrentCfg {
   static constexpr int kWarps = 4;  // warps per CTA, consecutive column groups
 };
 
-template <int D, typename T>
+template <int D>
 __global__ void __launch_bounds__(LinearRecurrentCfg::kWarps * 32) linear_recurrent_kernel(const LinearParams p) {
   constexpr int C = LinearRecurrentCfg::kCols, W = LinearRecurrentCfg::kWarps, R = D / 32;
   constexpr int kBlocks = D / (C * W);
@@ -81,11 +81,11 @@ __global__ void __launch_bounds__(LinearRecurrentCfg::kWarps * 32) linear_recurr
   auto fetch = [&](int64_t t) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      q[i] = load_f32<T>(p.q, t * p.sq + (int64_t)hk * D + row + i);
-      k[i] = load_f32<T>(p.k, t * p.sk + (int64_t)hk * D + row + i);
+      q[i] = load_f32<float>(p.q, t * p.sq + (int64_t)hk * D + row + i);
+      k[i] = load_f32<float>(p.k, t * p.sk + (int64_t)hk * D + row + i);
     }
 #pragma unroll
-    for (int e = 0; e < C; ++e) v[e] = load_f32<T>(p.v, t * p.sv + (int64_t)h * D + col + e);
+    for (int e = 0; e < C; ++e) v[e] = load_f32<float>(p.v, t * p.sv + (int64_t)h * D + col + e);
     g = log_decay(p, t, h);
   };
   if (bos < eos) fetch(bos);
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(LinearRecurrentCfg::kWarps * 32) linear_recurr
       for (int m = 16; m > 0; m >>= 1) o[e] += __shfl_xor_sync(0xffffffffu, o[e], m);
     if (lane < C) {
       const float x = lane == 0 ? o[0] : lane == 1 ? o[1] : lane == 2 ? o[2] : o[3];
-      store_f32(static_cast<T*>(p.out), t * p.so + (int64_t)h * D + col + lane, p.scale * x);
+      store_f32(static_cast<float*>(p.out), t * p.so + (int64_t)h * D + col + lane, p.scale * x);
     }
   }
   const bool taken = __any_sync(0xffffffffu, slot_taken(p.slots_out, n, out_slot, lane, 32));

@@ -151,6 +151,7 @@ SIGNATURES = {
     "memt_gdn2_noalloc_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "memt_linear_attention_workspace_size": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32]),
     "memt_linear_attention": (c_int, [POINTER(LinearAttentionArgs), c_void_p, c_size_t, c_void_p]),
+    "memt_linear_attention_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "memt_recurrent_step": (c_int, [POINTER(RecurrentStepArgs), c_void_p]),
     "memt_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
     "memt_profiler_enable": (c_int, [c_int]),
