@@ -36,6 +36,8 @@ int launch_chunked(const LinearParams& p, cudaStream_t s) {
   cudaError_t e = make_tmap_bf16_2d(&P.q_map, p.q, uint64_t(p.Hk) * D, rows, uint64_t(p.sq) * 2, 64, kTile);
   if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.k_map, p.k, uint64_t(p.Hk) * D, rows, uint64_t(p.sk) * 2, 64, kTile);
   if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.v_map, p.v, uint64_t(p.H) * D, rows, uint64_t(p.sv) * 2, 64, kTile);
+  if (e == cudaSuccess)
+    e = make_tmap_bf16_2d_sw64(&P.o_map, p.out, uint64_t(p.H) * D, rows, uint64_t(p.so) * 2, Cfg::kOutTokens);
   if (e == cudaSuccess) e = ensure_smem(linear_tc_kernel<D, true>, Cfg::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;

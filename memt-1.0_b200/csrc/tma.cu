@@ -20,20 +20,30 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-cudaError_t make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
-                              uint64_t row_stride, uint32_t box_inner, uint32_t box_rows) {
+static cudaError_t encode_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
+                                  uint64_t row_stride, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (fn == nullptr) return cudaErrorNotSupported;
-  if (reinterpret_cast<uintptr_t>(base) % 16 != 0 || row_stride % 16 != 0 || box_inner * 2 != 128)
-    return cudaErrorInvalidValue;
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0 || row_stride % 16 != 0) return cudaErrorInvalidValue;
   const cuuint64_t dims[2] = {inner, rows};
   const cuuint64_t strides[1] = {row_stride};
   const cuuint32_t box[2] = {box_inner, box_rows};
   const cuuint32_t estride[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box,
-                        estride, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        estride, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+cudaError_t make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
+                              uint64_t row_stride, uint32_t box_inner, uint32_t box_rows) {
+  if (box_inner * 2 != 128) return cudaErrorInvalidValue;
+  return encode_bf16_2d(map, base, inner, rows, row_stride, box_inner, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+cudaError_t make_tmap_bf16_2d_sw64(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
+                                   uint64_t row_stride, uint32_t box_rows) {
+  return encode_bf16_2d(map, base, inner, rows, row_stride, 32, box_rows, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 }  // namespace memt

@@ -15,6 +15,11 @@ namespace memt {
 cudaError_t make_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
                               uint64_t row_stride, uint32_t box_inner, uint32_t box_rows);
 
+// The same with boxes of 32 elements (64 bytes) x box_rows and the 64-byte swizzle: 16-byte chunk c of
+// row r lies at chunk c ^ ((r >> 1) & 3).
+cudaError_t make_tmap_bf16_2d_sw64(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows,
+                                   uint64_t row_stride, uint32_t box_rows);
+
 #ifdef __CUDACC__
 // Load the box at (x elements, y rows) into shared memory (1024-byte aligned for the
 // 128-byte swizzle); completion is signalled on the mbarrier as transaction bytes.
