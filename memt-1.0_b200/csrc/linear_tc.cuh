@@ -26,12 +26,14 @@
 // its row's 16-token block start, of whole blocks between, and to its column's block end; inside a
 // block of 16 it is one difference. So every factor is <= 1 for any decay, a reset (e^g = 0) included.
 //
-// Roles (20 warps): warp 0 issues MMAs, warp 1 loads tiles, warp 2 makes the decay tables; warps 4-7
-// split e^R V and make P from Sc; warps 8-11 make the outputs from X and Y; warps 12-19 hold the state,
-// half of the keys each warpgroup, fold U into it and write bf16(S). U of a chunk does not
-// depend on the state, so no MMA waits for another one's chunk: the groups work on neighbouring
-// chunks at the same time, and the only chain is fold, fold, ... in registers. A form in which 16 warps
-// did all of this in lockstep took 6200 cycles a chunk at D = 128, most of it the latency of its phases.
+// Roles (20 warps): warp 0 issues MMAs, warp 1 loads tiles, warps 2 and 3 make the decay tables of
+// alternate chunks; warps 4-11 split e^R V of a chunk and then make the outputs of the previous one,
+// half of the tokens each warpgroup; warps 12-19 hold the state, half of the keys each warpgroup: they
+// write bf16(S), make P from Sc (alternate column blocks) and fold U into S. U of a chunk does not depend on
+// the state, so no MMA waits for another one's chunk; the loop that closes is U -> e^R V of the next
+// chunk -> U. A form in which 16 warps did all of this in lockstep took 6200 cycles a chunk at D = 128, most of
+// it the latency of its phases; one with a role for each product was bound by instruction fetch
+// (every role's code runs once a chunk), hence few roles and rolled loops.
 // The last chunk of a sample is padded with whatever the TMA brings (the next sample's rows, or
 // zeros past the last row): those columns of P are masked by selection, those rows of K's and V's
 // tiles are set to zero (0 x NaN would not be), and those tokens' outputs are not stored.
@@ -86,8 +88,8 @@ struct LinearTcCfg {
   static constexpr uint32_t kOffK = kOffQ + kStages * kBytesQK;
   static constexpr uint32_t kOffV = kOffK + kStages * kBytesQK;
   static constexpr uint32_t kOffP = kOffV + kStages * kBytesV;
-  static constexpr uint32_t kOffOut = kOffP + kPanel;           // 4 KB per output warp
-  static constexpr uint32_t kOffTab = kOffOut + 4 * 4096;
+  static constexpr uint32_t kOffOut = kOffP + kPanel;           // 2 KB per output warp
+  static constexpr uint32_t kOffTab = kOffOut + 8 * 2048;
   static constexpr uint32_t kOffBar = kOffTab + kTables * sizeof(DecayTable);
   static constexpr size_t kSmem = kOffBar + 512 + 1024;
   // tensor memory columns: U^T of one unit, the three terms of (e^R V)^T, bf16(S)^T, X^T, Y^T, Sc
@@ -98,7 +100,7 @@ struct LinearTcCfg {
   // registers per thread after the split of the launch's 5 x 96 over the warpgroups
   static constexpr int kRegsControl = D == 256 ? 32 : 64, kRegsState = D == 256 ? 152 : 104,
                        kRegsWork = D == 256 ? 72 : 104;
-  static constexpr int kOutTokens = D >= 128 ? kTile : kTile / 2;  // tokens of an output warp
+  static constexpr int kOutTokens = D >= 128 ? kTile / 2 : kTile / 4;  // tokens of an output warp
   static constexpr int kCols = D == 256 ? 8 : 16;  // columns of U that a state thread holds at a time
   static_assert(kRegsControl + 2 * kRegsState + 2 * kRegsWork <= 5 * 96, "no more than the launch's registers");
   static_assert(kColSc + 64 <= 512 && kSmem <= 227 * 1024, "one CTA's resources");
@@ -161,10 +163,9 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
   if (tid == 0) {
     for (int i = 0; i < NBAR; ++i) {
       uint32_t count = 1;                                      // TMA, tcgen05.commit or one thread
-      if (i == VW || i == BP || i == OE) count = 4;
-      if (i >= TE && i < VW) count = OUT ? 16 : 12;     // every warp that reads the table
+      if (i == VW || i == BP || i == OE || i == SB) count = 8;
+      if (i >= TE && i < VW) count = 16;                // every warp that reads the table
       if (i >= UE && i < SC) count = NP == 1 ? 8 : 4;   // the state warps that read the unit
-      if (i == SB) count = 8;
       mbar_init(B(i), count);
     }
     mbar_fence_init();
@@ -322,22 +323,30 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
           mbar_wait_clock(B(VF + c % NS), (c / NS) & 1);
         }
       }
-    } else if (warp == 2) {
+    } else {
       // ---------------- decay tables: lane l has tokens 2 l and 2 l + 1, eight lanes a block of 16 ----------------
-      for (int c = 0; c < nchunks; ++c) {
-        const int64_t y = bos + (int64_t)c * kTile;
+      constexpr float kLog2e = 1.44269504f;
+      float next[2];
+      auto fetch = [&](int c) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int64_t t = bos + (int64_t)c * kTile + 2 * lane + e;
+          next[e] = t < eos ? log_decay(p, t, h) : 0.f;
+        }
+      };
+      fetch(warp - 2);
+      for (int c = warp - 2; c < nchunks; c += 2) {
         const int len = chunk_len(c);
-        constexpr float kLog2e = 1.44269504f;
         float g[2];
         double total = 0.0;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int t = 2 * lane + e;
-          const float x = t < len ? log_decay(p, y + t, h) : 0.f;
+          const float x = next[e];
           // below 2^-160 a decay is a reset in fp32 whatever it multiplies; NaN stays NaN
           g[e] = x * kLog2e < -160.f ? -160.f : x * kLog2e;
           total += x < -111.f ? -111.0 : static_cast<double>(x);
         }
+        if (c + 2 < nchunks) fetch(c + 2);
         float fwd = g[0] + g[1], bwd = fwd;
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) {
@@ -391,31 +400,30 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         arrive(TF + ts);
       }
     }
-  } else if (warp < 8) {
-    // ---------------- (e^R V)^T in three bf16 terms into tensor memory; P from the scores ----------------
+  } else if (warp < 12) {
+    // ---------------- (e^R V)^T in three bf16 terms into tensor memory; outputs from X and Y ----------------
     if constexpr (Cfg::kRegsWork > 96) regs_inc<Cfg::kRegsWork>(); else regs_dec<Cfg::kRegsWork>();
+    const int half = (warp - 4) >> 2;        // tokens 32 half ..
+    const int pair = 2 * (lane & 3);         // first column of a fragment
     // Values go through registers in the fragment layout: ldmatrix turns 8 x 8 pieces of V's tile, so that
     // a register holds two tokens of one value, and the fragment store puts them in that value's lane.
-    // Lane's row of the four pieces (two of tokens by two of values) that one ldmatrix turns:
-    const int lrow = 8 * (lane >> 4) + (lane & 7), lval = 8 * ((lane >> 3) & 1);
-    // ... and of the four pieces of P (two of rows by two of columns) that one stmatrix writes
-    const int prow = 16 * quad + 8 * ((lane >> 3) & 1) + (lane & 7), pcol = lane >> 4;
-    const int r0 = 16 * quad + (lane >> 2), pair = 2 * (lane & 3);  // first row and column of a fragment
-    for (int c = 0; c < nchunks; ++c) {
+    // This lane's row of the four pieces (two of tokens by two of values) of an ldmatrix or stmatrix:
+    const int prow = 8 * (lane >> 4) + (lane & 7), pval = (lane >> 3) & 1;
+    auto split_v = [&](int c) {
       const int s = c % NS, len = chunk_len(c);
-      unsigned char* v = sm + Cfg::kOffV + s * Cfg::kBytesV;
+      const uint32_t v = base + Cfg::kOffV + s * Cfg::kBytesV;
       wait(VF + s, c / NS);
       if (len < kTile) {  // rows of K and V behind the sample
         wait(KF + s, c / NS);
         const int pieces = (kTile - len) * 8;
-        for (int i = tid - 128; i < (D / 64 + 2) * pieces; i += 128) {
+        for (int i = tid - 128; i < (D / 64 + 2) * pieces; i += 256) {
           const int pan = i / pieces;
-          unsigned char* tile = pan < 2 ? v + pan * Cfg::kPanel
+          unsigned char* tile = pan < 2 ? sm + Cfg::kOffV + s * Cfg::kBytesV + pan * Cfg::kPanel
                                         : sm + Cfg::kOffK + s * Cfg::kBytesQK + (pan - 2) * Cfg::kPanel;
           *reinterpret_cast<uint4*>(tile + len * 128 + (i % pieces) * 16) = make_uint4(0, 0, 0, 0);
         }
         tc::fence_smem_async();
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the four warps read each other's zeros below
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight warps read each other's zeros
       }
       wait(TF + c % NT, c / NT);
       const DecayTable& t = tab[c % NT];
@@ -424,22 +432,21 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         __syncwarp();
         tc::fence_after();
       }
-      const uint32_t vbase = base + Cfg::kOffV + s * Cfg::kBytesV;
 #pragma unroll 1
-      for (int e = 0; e < 4; ++e) {  // 16 values by 32 tokens
-        const int val = (32 * quad + 16 * (e >> 1)) % Cfg::kVB + lval, tok = 32 * (e & 1);
+      for (int e = 0; e < 2; ++e) {  // 16 values by 32 tokens
+        const int val = (32 * quad + 16 * e) % Cfg::kVB + 8 * pval;
         uint32_t r[3][8];
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
           uint32_t x[4];
-          const int t = tok + 16 * q + lrow;
-          ldsm_x4_t(x, vbase + (val >> 6) * Cfg::kPanel + t * 128 + ((((val & 63) >> 3) ^ (t & 7)) << 4));
+          const int tok = 32 * half + 16 * q + prow;
+          ldsm_x4_t(x, v + (val >> 6) * Cfg::kPanel + tok * 128 + ((((val & 63) >> 3) ^ (tok & 7)) << 4));
 #pragma unroll
           for (int i = 0; i < 4; ++i) r[0][4 * q + i] = x[i];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float2 w = *reinterpret_cast<const float2*>(&t.w[tok + 8 * i + pair]);
+          const float2 w = *reinterpret_cast<const float2*>(&t.w[32 * half + 8 * i + pair]);
           const uint64_t ww = f32x2_pack(w.x, w.y);
 #pragma unroll
           for (int j = 2 * i; j < 2 * i + 2; ++j) {
@@ -453,19 +460,133 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         }
 #pragma unroll
         for (int term = 0; term < 3; ++term)
-          tc::st_frag16(tc::lane_addr(tW, 32 * quad + 16 * (e >> 1), 32 * term + tok / 2), r[term]);
+          tc::st_frag16(tc::lane_addr(tW, 32 * quad + 16 * e, 32 * term + 16 * half), r[term]);
       }
       tc::wait_st();
       tc::fence_before();
       arrive(VW);
+      if (!OUT && lane == 0) mbar_arrive(B(TE + c % NT));
+    };
+    // Outputs: fragments of 16 values by tokens, a register pair is two tokens of one value. stmatrix
+    // turns them into token rows of this warp's 32 values (64 bytes, the 64-byte swizzle), which leave
+    // as one TMA box; a chunk that ends inside leaves row by row instead.
+    constexpr int kTok = Cfg::kOutTokens, kGroups = kTok / 8;
+    const int t0 = 32 * half + (D >= 128 ? 0 : kTok * (quad >> 1));
+    const int col = h * D + vblk * Cfg::kVB + (D >= 128 ? 32 * quad : 32 * (quad & 1));
+    const uint32_t turn = base + Cfg::kOffOut + (warp - 4) * 2048;
+    auto write_out = [&](int c) {
+      const DecayTable& t = tab[c % NT];
+      const int len = chunk_len(c);
+      wait(XY, c);
+      if (lane == 0) bulk_wait_read();  // the previous box has left the rows
+      __syncwarp();
+      tc::fence_after();
+#pragma unroll 1
+      for (int e = 0; e < 2; ++e) {
+        uint32_t x[4 * kGroups], y[4 * kGroups];
+        tc::ld_frag2<kGroups>(tc::lane_addr(tX, 32 * quad + 16 * e, t0), tc::lane_addr(tY, 32 * quad + 16 * e, t0), x, y);
+        if (e == 1) {
+          tc::fence_before();
+          arrive(OE);
+        }
+#pragma unroll
+        for (int i = 0; i < kGroups; i += 2) {
+          uint32_t z[4];  // tokens 8 (i + j) + pair, + 1: of value lane / 4, of value lane / 4 + 8
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 f = *reinterpret_cast<const float2*>(&t.f[t0 + 8 * (i + j) + pair]);
+            const uint64_t ff = f32x2_pack(f.x, f.y);
+#pragma unroll
+            for (int v8 = 0; v8 < 2; ++v8) {
+              const int k = 4 * (i + j) + 2 * v8;
+              z[2 * j + v8] = f32x2_to_bf16x2(fma_f32x2(ff, (static_cast<uint64_t>(x[k + 1]) << 32) | x[k],
+                                                        (static_cast<uint64_t>(y[k + 1]) << 32) | y[k]));
+            }
+          }
+          const int tok = 8 * i + prow;
+          stsm_x4_t(turn + tok * 64 + (((2 * e + pval) ^ ((tok >> 1) & 3)) << 4), z[0], z[1], z[2], z[3]);
+        }
+      }
+      if (lane == 0) mbar_arrive(B(TE + c % NT));
+      const int64_t tok0 = bos + (int64_t)c * kTile + t0;
+      if (len == kTile) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&P.o_map, col, static_cast<int>(tok0), turn);
+          bulk_commit();
+        }
+      } else {
+        __syncwarp();
+        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + tok0 * p.so + col + 8 * (lane & 3);
+        for (int tok = lane >> 2; tok < kTok && t0 + tok < len; tok += 8) {
+          uint4 z;
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
+                       : "r"(turn + tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4)) : "memory");
+          *reinterpret_cast<uint4*>(o + tok * p.so) = z;
+        }
+        __syncwarp();
+      }
+    };
+    // With the scores on Y's columns the next ones wait for the outputs, which then come first.
+    for (int c = 0; c < nchunks; ++c) {
+      split_v(c);
       if constexpr (OUT) {
+        if (Cfg::kAlias) write_out(c);
+        else if (c > 0) write_out(c - 1);
+      }
+    }
+    if (OUT && !Cfg::kAlias && nchunks > 0) write_out(nchunks - 1);
+    if (lane == 0) bulk_wait_all();
+  } else {
+    // ---------------- the state: value row of this lane, keys KT half .. ----------------
+    regs_inc<Cfg::kRegsState>();
+    const int half = (warp - 12) >> 2;
+    const int vr = (32 * quad + lane) % Cfg::kVB;
+    const bool writes = D >= 128 || quad < 2;  // at D = 64 quadrants 2 and 3 repeat 0 and 1
+    const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
+    const int64_t col_off = (int64_t)(KT * half) * D + vblk * Cfg::kVB + vr;
+    // P's fragments: first row and column of this lane's, and its row of the four pieces (two of rows by
+    // two of columns) that one stmatrix writes
+    const int r0 = 16 * quad + (lane >> 2), pair = 2 * (lane & 3);
+    const int prow = 16 * quad + 8 * ((lane >> 3) & 1) + (lane & 7), pcol = lane >> 4;
+    uint64_t S[KT / 2];  // pairs of fp32: keys KT half + 2 i, + 2 i + 1 of value vr
+    if (p.h0 != nullptr && in_slot >= 0) {
+      const float* src = p.h0 + (in_slot * p.H + h) * D * D + col_off;
+#pragma unroll
+      for (int i = 0; i < KT; i += 2) S[i / 2] = f32x2_pack(src[i * D], src[(i + 1) * D]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) S[i] = 0;
+    }
+    for (int c = 0; c < nchunks; ++c) {
+      if constexpr (OUT) {  // bf16(S)^T before chunk c: keys 2 i, 2 i + 1 in column i
+        if (c > 0) wait(XD, c - 1);
+        __syncwarp();
+        tc::fence_after();
+#pragma unroll
+        for (int q = 0; q < KT / 16; ++q) {
+          uint32_t r[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) r[i] = f32x2_to_bf16x2(S[8 * q + i]);
+          tc::st8(tc::lane_addr(tSb, 32 * quad, (KT * half + 16 * q) / 2), r);
+        }
+        tc::wait_st();
+        tc::fence_before();
+        arrive(SB);
+      }
+      wait(TF + c % NT, c / NT);
+      const DecayTable& t = tab[c % NT];
+      if constexpr (OUT) {
+        const int len = chunk_len(c);
         const uint32_t row = base + Cfg::kOffP + prow * 128;
         wait(SC, c);
         __syncwarp();
         tc::fence_after();
         const float f0 = t.row[r0], f1 = t.row[r0 + 8];
 #pragma unroll 1
-        for (int J = 0; J <= quad; ++J) {  // 16 x 16 blocks up to the diagonal: decays, then bf16 into the operand
+        for (int J = half; J <= quad; J += 2) {  // 16 x 16 blocks up to the diagonal: decays, then bf16 into the operand
           uint32_t x[8], z[4];  // x: columns 8 e + pair, + 1 of row r0, then of row r0 + 8, e = 0, 1
           tc::ld_frag<2>(tc::lane_addr(tSc, 32 * quad, 16 * J), x);
           if (J < quad) {
@@ -504,121 +625,10 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         tc::fence_before();
         arrive(BP);
       }
-      if (lane == 0) mbar_arrive(B(TE + c % NT));
-    }
-  } else if (warp < 12) {
-    // ---------------- outputs from X and Y ----------------
-    if constexpr (Cfg::kRegsWork > 96) regs_inc<Cfg::kRegsWork>(); else regs_dec<Cfg::kRegsWork>();
-    if constexpr (OUT) {
-      // Fragments of 16 values by tokens: a register pair is two tokens of one value. stmatrix turns
-      // them into token rows of this warp's 32 values (64 bytes, the 64-byte swizzle), which leave as one
-      // TMA box; a chunk that ends inside leaves row by row instead.
-      constexpr int kTok = Cfg::kOutTokens, kSet = D == 256 ? 4 : kTok / 8;  // groups of 8 tokens held at a time
-      const int t0 = D >= 128 ? 0 : kTok * (quad >> 1);
-      const int col = h * D + vblk * Cfg::kVB + (D >= 128 ? 32 * quad : 32 * (quad & 1));
-      const int pair = 2 * (lane & 3);
-      const uint32_t turn = base + Cfg::kOffOut + quad * 4096;
-      const int srow = 8 * (lane >> 4) + (lane & 7), sval = (lane >> 3) & 1;  // this lane's row of the four pieces
-      for (int c = 0; c < nchunks; ++c) {
-        const DecayTable& t = tab[c % NT];
-        const int len = chunk_len(c);
-        wait(TF + c % NT, c / NT);
-        wait(XY, c);
-        if (lane == 0) bulk_wait_read();  // the previous box has left the rows
-        __syncwarp();
-        tc::fence_after();
-#pragma unroll 1
-        for (int hf = 0; hf < 2; ++hf) {
-#pragma unroll 1
-          for (int g = 0; g < kTok / 8; g += kSet) {
-            uint32_t x[4 * kSet], y[4 * kSet];
-            tc::ld_frag2<kSet>(tc::lane_addr(tX, 32 * quad + 16 * hf, t0 + 8 * g),
-                               tc::lane_addr(tY, 32 * quad + 16 * hf, t0 + 8 * g), x, y);
-            if (hf == 1 && g + kSet == kTok / 8) {
-              tc::fence_before();
-              arrive(OE);
-            }
-#pragma unroll
-            for (int i = 0; i < kSet; i += 2) {
-              uint32_t z[4];  // tokens 8 (g + i + e) + pair, + 1: of value lane / 4, of value lane / 4 + 8
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float2 f = *reinterpret_cast<const float2*>(&t.f[t0 + 8 * (g + i + e) + pair]);
-                const uint64_t ff = f32x2_pack(f.x, f.y);
-#pragma unroll
-                for (int v8 = 0; v8 < 2; ++v8) {
-                  const int k = 4 * (i + e) + 2 * v8;
-                  z[2 * e + v8] = f32x2_to_bf16x2(fma_f32x2(ff, (static_cast<uint64_t>(x[k + 1]) << 32) | x[k],
-                                                            (static_cast<uint64_t>(y[k + 1]) << 32) | y[k]));
-                }
-              }
-              const int tok = 8 * (g + i) + srow;
-              stsm_x4_t(turn + tok * 64 + (((2 * hf + sval) ^ ((tok >> 1) & 3)) << 4), z[0], z[1], z[2], z[3]);
-            }
-          }
-        }
-        if (lane == 0) mbar_arrive(B(TE + c % NT));
-        const int64_t tok0 = bos + (int64_t)c * kTile + t0;
-        if (len == kTile) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&P.o_map, col, static_cast<int>(tok0), turn);
-            bulk_commit();
-          }
-        } else {
-          __syncwarp();
-          __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + tok0 * p.so + col + 8 * (lane & 3);
-          for (int tok = lane >> 2; tok < kTok && t0 + tok < len; tok += 8) {
-            uint4 z;
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
-                         : "r"(turn + tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4)) : "memory");
-            *reinterpret_cast<uint4*>(o + tok * p.so) = z;
-          }
-          __syncwarp();
-        }
-      }
-      if (lane == 0) bulk_wait_all();
-    }
-  } else {
-    // ---------------- the state: value row of this lane, keys KT half .. ----------------
-    regs_inc<Cfg::kRegsState>();
-    const int half = (warp - 12) >> 2;
-    const int vr = (32 * quad + lane) % Cfg::kVB;
-    const bool writes = D >= 128 || quad < 2;  // at D = 64 quadrants 2 and 3 repeat 0 and 1
-    const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
-    const int64_t col_off = (int64_t)(KT * half) * D + vblk * Cfg::kVB + vr;
-    uint64_t S[KT / 2];  // pairs of fp32: keys KT half + 2 i, + 2 i + 1 of value vr
-    if (p.h0 != nullptr && in_slot >= 0) {
-      const float* src = p.h0 + (in_slot * p.H + h) * D * D + col_off;
-#pragma unroll
-      for (int i = 0; i < KT; i += 2) S[i / 2] = f32x2_pack(src[i * D], src[(i + 1) * D]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) S[i] = 0;
-    }
-    for (int c = 0; c < nchunks; ++c) {
-      if constexpr (OUT) {  // bf16(S)^T before chunk c: keys 2 i, 2 i + 1 in column i
-        if (c > 0) wait(XD, c - 1);
-        __syncwarp();
-        tc::fence_after();
-#pragma unroll
-        for (int q = 0; q < KT / 16; ++q) {
-          uint32_t r[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) r[i] = f32x2_to_bf16x2(S[8 * q + i]);
-          tc::st8(tc::lane_addr(tSb, 32 * quad, (KT * half + 16 * q) / 2), r);
-        }
-        tc::wait_st();
-        tc::fence_before();
-        arrive(SB);
-      }
       // S = a S + U; a unit is both halves' keys, or at D = 256 this half's
       const int u = NP == 2 ? half : 0;
       const uint32_t col = tU + (NP == 2 ? 0 : KT * half);
-      wait(TF + c % NT, c / NT);
-      const uint64_t ah = f32x2_splat(tab[c % NT].a_hi), al = f32x2_splat(tab[c % NT].a_lo);
+      const uint64_t ah = f32x2_splat(t.a_hi), al = f32x2_splat(t.a_lo);
       arrive(TE + c % NT);
       wait(BU + u, c);
       __syncwarp();
