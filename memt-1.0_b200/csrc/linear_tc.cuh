@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
   extern __shared__ __align__(1024) unsigned char smem_linear_tc[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_linear_tc) + 1023) &
                                                        ~static_cast<uintptr_t>(1023));
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, quad = warp & 3;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(~0u, tid >> 5, 0), quad = warp & 3;  // uniform: so are the roles' branches
   const int vblk = blockIdx.x % Cfg::kBlocks, nh = blockIdx.x / Cfg::kBlocks;
   const int h = nh % p.H, n = nh / p.H, hk = h / (p.H / p.Hk);
 
@@ -217,13 +218,13 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         wait(QF + s, c / NS);
         wait(KF + s, c / NS);
         if (go()) {
-          const uint32_t q = base + Cfg::kOffQ + s * Cfg::kBytesQK, k = base + Cfg::kOffK + s * Cfg::kBytesQK;
-          uint64_t dq = tc::desc_kmajor(q, 0), dk = tc::desc_kmajor(k, 0);
-#pragma unroll 1
-          for (int pan = 0; pan < D / 64; ++pan, dq += Cfg::kPanel >> 4, dk += Cfg::kPanel >> 4)
+        const uint64_t dq = tc::desc_kmajor(base + Cfg::kOffQ + s * Cfg::kBytesQK, 0);
+        const uint64_t dk = tc::desc_kmajor(base + Cfg::kOffK + s * Cfg::kBytesQK, 0);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) tc::mma_bf16(tSc, dq + 2 * ks, dk + 2 * ks, kIdSc, (pan | ks) > 0);
-          tc::commit(B(SC));
+        for (int i = 0; i < D / 16; ++i)
+          tc::mma_bf16(tSc, dq + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2,
+                            dk + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2, kIdSc, i > 0);
+        tc::commit(B(SC));
         }
         __syncwarp();
       };
@@ -236,17 +237,15 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         if (u > 0) wait(UE, c);
         else if (c > 0) wait(UE + NP - 1, c - 1);
         if (go()) {
-          const uint32_t k = base + Cfg::kOffK + s * Cfg::kBytesQK + u * (Cfg::kPanelKeys / 64) * Cfg::kPanel;
-          const uint64_t dk = tc::desc_mnmajor(k, Cfg::kPanel, 0);
-          // smallest term first, so that the accumulator's truncations are those of small sums
-#pragma unroll 1
-          for (int term = 2; term >= 0; --term)
+        const uint64_t dk = tc::desc_mnmajor(
+            base + Cfg::kOffK + s * Cfg::kBytesQK + u * (Cfg::kPanelKeys / 64) * Cfg::kPanel, Cfg::kPanel, 0);
+        // smallest term first, so that the accumulator's truncations are those of small sums
 #pragma unroll
-            for (int ks = 0; ks < kTile / 16; ++ks)
-              tc::mma_bf16_ts(tU, tW + 32 * term + 8 * ks, dk + 128 * ks, kIdU, term < 2 || ks > 0);
-          tc::commit(B(BU + u));
-          if (u == NP - 1) tc::commit(B(KE + s));
-          if (!OUT && u == NP - 1) tc::commit(B(VE + s));
+        for (int i = 0; i < 12; ++i)
+          tc::mma_bf16_ts(tU, tW + 8 * i, dk + 128 * (i & 3), kIdU, i > 0);
+        tc::commit(B(BU + u));
+        if (u == NP - 1) tc::commit(B(KE + s));
+        if (!OUT && u == NP - 1) tc::commit(B(VE + s));
         }
         __syncwarp();
       };
@@ -255,24 +254,22 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         wait(SB, c);
         if (!Cfg::kAlias && c > 0) wait(OE, c - 1);
         if (go()) {
-          const uint32_t q = base + Cfg::kOffQ + s * Cfg::kBytesQK;
-          uint64_t dq = tc::desc_kmajor(q, 0);
-#pragma unroll 1
-          for (int pan = 0; pan < D / 64; ++pan, dq += Cfg::kPanel >> 4)
+        const uint64_t dq = tc::desc_kmajor(base + Cfg::kOffQ + s * Cfg::kBytesQK, 0);
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) tc::mma_bf16_ts(tX, tSb + 32 * pan + 8 * ks, dq + 2 * ks, kIdX, (pan | ks) > 0);
-          tc::commit(B(XD));
-          tc::commit(B(QE + s));
+        for (int i = 0; i < D / 16; ++i)
+          tc::mma_bf16_ts(tX, tSb + 8 * i, dq + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2, kIdX, i > 0);
+        tc::commit(B(XD));
+        tc::commit(B(QE + s));
         }
         __syncwarp();
         wait(BP, c);
         if (go()) {
-          const uint64_t dv = tc::desc_mnmajor(base + Cfg::kOffV + s * Cfg::kBytesV, Cfg::kPanel, 0);
-          const uint64_t dp = tc::desc_kmajor(base + Cfg::kOffP, 0);
+        const uint64_t dv = tc::desc_mnmajor(base + Cfg::kOffV + s * Cfg::kBytesV, Cfg::kPanel, 0);
+        const uint64_t dp = tc::desc_kmajor(base + Cfg::kOffP, 0);
 #pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks) tc::mma_bf16(tY, dv + 128 * ks, dp + 2 * ks, kIdY, ks > 0);
-          tc::commit(B(XY));
-          tc::commit(B(VE + s));
+        for (int i = 0; i < kTile / 16; ++i) tc::mma_bf16(tY, dv + 128 * i, dp + 2 * i, kIdY, i > 0);
+        tc::commit(B(XY));
+        tc::commit(B(VE + s));
         }
         __syncwarp();
       };
@@ -460,7 +457,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         }
 #pragma unroll
         for (int term = 0; term < 3; ++term)
-          tc::st_frag16(tc::lane_addr(tW, 32 * quad + 16 * e, 32 * term + 16 * half), r[term]);
+          tc::st_frag16(tc::lane_addr(tW, 32 * quad + 16 * e, 32 * (2 - term) + 16 * half), r[term]);
       }
       tc::wait_st();
       tc::fence_before();
