@@ -27,8 +27,40 @@ int launch_recurrent_form(int D, const LinearParams& p, cudaStream_t s) {
   }
 }
 
+// Multiprocessors the split is planned for (the workspace size is known without a device).
+constexpr int kPlanSms = 148;
+
+// 64-token chunks per segment, or 0: one CTA per (sample, head, value block) walks a whole sample. Few of
+// them leave SMs idle for as long as a sample takes: 16 heads of one 65536-token sample 1.5 ms. Segments
+// fill the SMs once, at the price of a first pass that sums their states (k and v are read twice) and
+// a pass that joins them: 0.36 ms. A chunk takes about 1.7 us in one CTA, 1.1 us in the first pass, the
+// two further launches about 12 us, which decides whether the split pays.
+int plan_segment_chunks(int64_t N, int64_t L, int64_t H, int D) {
+  const int64_t ctas = N * H * (D == 256 ? 2 : 1);
+  const int64_t split = kPlanSms / ctas;
+  if (split < 2) return 0;
+  const int64_t chunks = (L + kTile - 1) / kTile / N;  // of a mean sample
+  if (chunks * (1.7 - 2.8 / split) < 12.0) return 0;
+  return static_cast<int>((chunks + split - 1) / split);
+}
+int64_t max_segments(int64_t N, int64_t L, int seg_chunks) { return L / (int64_t(seg_chunks) * kTile) + N; }
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
+
+template <int D, bool OUT>
+int launch_pass(const LinearTcParams& P, int64_t units, cudaStream_t s) {
+  using Cfg = LinearTcCfg<D>;
+  const cudaError_t e = ensure_smem(linear_tc_kernel<D, OUT>, Cfg::kSmem);
+  if (e != cudaSuccess) return cuda_status(e);
+  const int64_t grid = units * P.p.H * Cfg::kBlocks;
+  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  ProfScope prof(kProfLinear, s);
+  linear_tc_kernel<D, OUT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
+  return cuda_status(cudaGetLastError());
+}
+
 template <int D>
-int launch_chunked(const LinearParams& p, cudaStream_t s) {
+int launch_chunked(const LinearParams& p, void* workspace, cudaStream_t s) {
   using Cfg = LinearTcCfg<D>;
   LinearTcParams P;
   P.p = p;
@@ -38,20 +70,37 @@ int launch_chunked(const LinearParams& p, cudaStream_t s) {
   if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.v_map, p.v, uint64_t(p.H) * D, rows, uint64_t(p.sv) * 2, 64, kTile);
   if (e == cudaSuccess)
     e = make_tmap_bf16_2d_sw64(&P.o_map, p.out, uint64_t(p.H) * D, rows, uint64_t(p.so) * 2, Cfg::kOutTokens);
-  if (e == cudaSuccess) e = ensure_smem(linear_tc_kernel<D, true>, Cfg::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
-  const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;
-  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
-  ProfScope prof(kProfLinear, s);
-  linear_tc_kernel<D, true><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
-  return cuda_status(cudaGetLastError());
+  const int seg_chunks = plan_segment_chunks(p.N, p.L, p.H, D);
+  if (seg_chunks == 0) {
+    // more CTAs than SMs: the longest samples first, so that no SM ends with one (16 samples of 1 to 16384
+    // tokens, 16 heads, d = 128: 617 us in order of the samples, 498 us by length)
+    P.p.by_length = p.N > 1 && p.N <= 256 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms;
+    return launch_pass<D, true>(P, p.N, s);
+  }
+  const int64_t units = max_segments(p.N, p.L, seg_chunks);
+  P.p.seg_chunks = seg_chunks;
+  P.p.max_segments = static_cast<int32_t>(units);
+  P.p.seg_states = static_cast<float*>(workspace);
+  P.p.seg_decays = reinterpret_cast<float2*>(static_cast<unsigned char*>(workspace) +
+                                             align256(size_t(units) * p.H * D * D * sizeof(float)));
+  int st = launch_pass<D, false>(P, units, s);
+  if (st != MEMT_OK) return st;
+  {
+    ProfScope prof(kProfLinear, s);
+    const unsigned grid = static_cast<unsigned>(p.N * p.H * ((D * D / 4 + 255) / 256));  // fewer CTAs than SMs ran: small
+    linear_segments_kernel<<<grid, 256, 0, s>>>(P.p, D);
+    st = cuda_status(cudaGetLastError());
+    if (st != MEMT_OK) return st;
+  }
+  return launch_pass<D, true>(P, units, s);
 }
 
-int launch_chunked(int D, const LinearParams& p, cudaStream_t s) {
+int launch_chunked(int D, const LinearParams& p, void* workspace, cudaStream_t s) {
   switch (D) {
-    case 64: return launch_chunked<64>(p, s);
-    case 128: return launch_chunked<128>(p, s);
-    default: return launch_chunked<256>(p, s);
+    case 64: return launch_chunked<64>(p, workspace, s);
+    case 128: return launch_chunked<128>(p, workspace, s);
+    default: return launch_chunked<256>(p, workspace, s);
   }
 }
 
@@ -90,7 +139,10 @@ extern "C" {
 size_t memt_linear_attention_workspace_size(int32_t N, int64_t L, int32_t H, int32_t D, int32_t dtype) {
   if (N < 1 || L < 0 || H < 1 || (D != 64 && D != 128 && D != 256)) return 0;
   if (dtype != MEMT_F32 && dtype != MEMT_BF16) return 0;
-  return 256;
+  const int seg_chunks = dtype == MEMT_BF16 ? plan_segment_chunks(N, L, H, D) : 0;
+  if (seg_chunks == 0) return 256;
+  const size_t units = static_cast<size_t>(max_segments(N, L, seg_chunks));
+  return align256(units * H * D * D * sizeof(float)) + align256(units * H * sizeof(float2));
 }
 
 int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, size_t workspace_bytes,
@@ -127,7 +179,7 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // without tokens the states are only copied
   if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_recurrent_form(a->head_dim, p, s);
-  return launch_chunked(a->head_dim, p, s);
+  return launch_chunked(a->head_dim, p, workspace, s);
 }
 
 int memt_linear_attention_status(memt_stream_t stream, int32_t* status_out) {

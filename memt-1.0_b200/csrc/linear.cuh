@@ -33,6 +33,13 @@ struct LinearParams {
   const int32_t* slots_in;
   const int32_t* slots_out;
   int32_t num_in, num_out;
+  // Chunked form of few long samples: 0, or 64-token chunks per segment, and the segments' states
+  // [segment][H][D][D] (first their own sums, then the state before each) and decays [segment][H].
+  int32_t seg_chunks;
+  int32_t max_segments;
+  int32_t by_length;  // whole samples, the longest first
+  float* seg_states;
+  float2* seg_decays;
 };
 
 // tokens [bos, eos) of sample n, clamped to the packed rows
@@ -41,6 +48,66 @@ __device__ __forceinline__ void sample_range(const LinearParams& p, int n, int64
   eos = p.cu[n + 1];
   bos = bos < 0 ? 0 : (bos > p.L ? p.L : bos);
   eos = eos < bos ? bos : (eos > p.L ? p.L : eos);
+}
+
+// Segments of a sample: runs of seg_chunks chunks of 64 tokens, at least one.
+__device__ __forceinline__ int segments_of(const LinearParams& p, int64_t tokens) {
+  const int64_t run = (int64_t)p.seg_chunks * kTile;
+  return tokens > run ? static_cast<int>((tokens + run - 1) / run) : 1;
+}
+
+// Sample n, segment s of its `count`, of the call's segment number `unit` (samples in order), found by
+// a converged warp; false when there are fewer segments.
+__device__ __forceinline__ bool find_segment(const LinearParams& p, int unit, int& n, int& s, int& count) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    int own = 0;
+    if (n0 + lane < p.N) {
+      int64_t bos, eos;
+      sample_range(p, n0 + lane, bos, eos);
+      own = segments_of(p, eos - bos);
+    }
+    int incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const uint32_t past = __ballot_sync(~0u, base + incl > unit);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      n = n0 + l;
+      count = __shfl_sync(~0u, own, l);
+      s = unit - (base + __shfl_sync(~0u, incl, l) - count);
+      return true;
+    }
+    base += __shfl_sync(~0u, incl, 31);
+  }
+  return false;
+}
+
+// The sample with the rank-th longest token range (ties: the lower index first), found by a converged
+// warp. N is small: every lane ranks its samples against all.
+__device__ __forceinline__ int sample_by_length(const LinearParams& p, int rank) {
+  const int lane = threadIdx.x & 31;
+  int found = 0;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    const int n = n0 + lane;
+    int64_t bos, eos, len = -1;
+    if (n < p.N) {
+      sample_range(p, n, bos, eos);
+      len = eos - bos;
+    }
+    int ahead = 0;
+    for (int m = 0; m < p.N; ++m) {
+      sample_range(p, m, bos, eos);
+      ahead += eos - bos > len || (eos - bos == len && m < n);
+    }
+    const uint32_t hit = __ballot_sync(~0u, n < p.N && ahead == rank);
+    if (hit != 0) found = n0 + __ffs(hit) - 1;
+  }
+  return found;
 }
 
 __device__ __forceinline__ float log_decay(const LinearParams& p, int64_t t, int h) {
@@ -53,6 +120,48 @@ __device__ __forceinline__ bool slot_taken(const int32_t* slots, int n, int64_t 
   if (slots != nullptr)
     for (int i = tid; i < n; i += threads) taken |= slots[i] == static_cast<int32_t>(slot);
   return taken;
+}
+
+// Between the two passes over segments: the state before each one. A thread owns four values of one
+// (sample, head) state and walks over its segments; the segments' own sums are replaced in place.
+__global__ void __launch_bounds__(256) linear_segments_kernel(const LinearParams p, int D) {
+  const int per_state = D * D / 4, blocks = (per_state + 255) / 256;
+  const int at = (blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int nh = blockIdx.x / blocks, h = nh % p.H, n = nh / p.H;
+  int64_t bos, eos;
+  int first = 0, count = 1;
+  {  // this sample's first segment: every warp sums the samples before it
+    const int lane = threadIdx.x & 31;
+    for (int m = lane; m < n; m += 32) {
+      sample_range(p, m, bos, eos);
+      first += segments_of(p, eos - bos);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
+    sample_range(p, n, bos, eos);
+    count = segments_of(p, eos - bos);
+  }
+  if (count == 1 || at >= per_state) return;  // one segment starts from the sample's own state
+  const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n);
+  float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.h0 != nullptr && in_slot >= 0)
+    S = reinterpret_cast<const float4*>(p.h0 + (in_slot * p.H + h) * D * D)[at];
+  // (offsets that overlap, which no packed batch has, could make more segments than there is room for)
+  for (int s = 0; s < count && first + s < p.max_segments; ++s) {
+    const int64_t seg = (int64_t)(first + s) * p.H + h;
+    float4* state = reinterpret_cast<float4*>(p.seg_states + seg * D * D) + at;
+    float4 own = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 a = make_float2(0.f, 0.f);
+    if (s + 1 < count) {  // the last one's sum is not made: the second pass ends with it
+      own = *state;
+      a = p.seg_decays[seg];
+    }
+    *state = S;
+    S.x = fmaf(a.x, S.x, fmaf(a.y, S.x, own.x));
+    S.y = fmaf(a.x, S.y, fmaf(a.y, S.y, own.y));
+    S.z = fmaf(a.x, S.z, fmaf(a.y, S.z, own.z));
+    S.w = fmaf(a.x, S.w, fmaf(a.y, S.w, own.w));
+  }
 }
 
 struct LinearRecurrentCfg {

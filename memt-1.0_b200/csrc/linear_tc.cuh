@@ -146,8 +146,16 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
                                                        ~static_cast<uintptr_t>(1023));
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(~0u, tid >> 5, 0), quad = warp & 3;  // uniform: so are the roles' branches
-  const int vblk = blockIdx.x % Cfg::kBlocks, nh = blockIdx.x / Cfg::kBlocks;
-  const int h = nh % p.H, n = nh / p.H, hk = h / (p.H / p.Hk);
+  const int vblk = blockIdx.x % Cfg::kBlocks, unit = blockIdx.x / Cfg::kBlocks / p.H;
+  const int h = blockIdx.x / Cfg::kBlocks % p.H, hk = h / (p.H / p.Hk);
+  // a unit is a sample, or with segments one of a sample's `segs`
+  int n = unit, seg = 0, segs = 1;
+  if (p.seg_chunks > 0) {
+    if (!find_segment(p, unit, n, seg, segs)) return;
+    if (!OUT && seg + 1 == segs) return;  // the first pass sums what later segments start from
+  } else if (p.by_length) {
+    n = sample_by_length(p, unit);
+  }
 
   // barriers: Q, K, V tiles landed (QF, KF, VF) and free again (QE, KE, VE); decay table written /
   // read (TF, TE); V's operand written (VW); U of a unit ready (BU) and read (UE); scores ready (SC),
@@ -186,6 +194,11 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
 
   int64_t bos, eos;
   sample_range(p, n, bos, eos);
+  if (segs > 1) {
+    bos += (int64_t)seg * p.seg_chunks * kTile;
+    if (eos > bos + (int64_t)p.seg_chunks * kTile) eos = bos + (int64_t)p.seg_chunks * kTile;
+  }
+  const int64_t seg_state = ((int64_t)unit * p.H + h) * D * D;  // of seg_states
   const int nchunks = static_cast<int>((eos - bos + kTile - 1) / kTile);
   auto chunk_len = [&](int c) {
     const int64_t left = eos - bos - (int64_t)c * kTile;
@@ -548,9 +561,11 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
     // two of columns) that one stmatrix writes
     const int r0 = 16 * quad + (lane >> 2), pair = 2 * (lane & 3);
     const int prow = 16 * quad + 8 * ((lane >> 3) & 1) + (lane & 7), pcol = lane >> 4;
+    float2 seg_a = make_float2(1.f, 0.f);
     uint64_t S[KT / 2];  // pairs of fp32: keys KT half + 2 i, + 2 i + 1 of value vr
-    if (p.h0 != nullptr && in_slot >= 0) {
-      const float* src = p.h0 + (in_slot * p.H + h) * D * D + col_off;
+    const bool given = OUT && (segs > 1 || (p.h0 != nullptr && in_slot >= 0));
+    if (given) {
+      const float* src = (segs > 1 ? p.seg_states + seg_state : p.h0 + (in_slot * p.H + h) * D * D) + col_off;
 #pragma unroll
       for (int i = 0; i < KT; i += 2) S[i / 2] = f32x2_pack(src[i * D], src[(i + 1) * D]);
     } else {
@@ -625,8 +640,14 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
       // S = a S + U; a unit is both halves' keys, or at D = 256 this half's
       const int u = NP == 2 ? half : 0;
       const uint32_t col = tU + (NP == 2 ? 0 : KT * half);
-      const uint64_t ah = f32x2_splat(t.a_hi), al = f32x2_splat(t.a_lo);
+      const float a_hi = t.a_hi, a_lo = t.a_lo;
+      const uint64_t ah = f32x2_splat(a_hi), al = f32x2_splat(a_lo);
       arrive(TE + c % NT);
+      if constexpr (!OUT) {  // the segment's decay, a pair of fp32 numbers too
+        const float hi = seg_a.x * a_hi;
+        seg_a.y = fmaf(seg_a.x, a_hi, -hi) + fmaf(seg_a.x, a_lo, seg_a.y * a_hi);
+        seg_a.x = hi;
+      }
       wait(BU + u, c);
       __syncwarp();
       tc::fence_after();
@@ -643,9 +664,11 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
       tc::fence_before();
       arrive(UE + u);
     }
-    const bool taken = __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
-    if (__all_sync(~0u, alive) && writes && out_slot >= 0 && !taken) {
-      float* dst = p.ht + (out_slot * p.H + h) * D * D + col_off;
+    if (!OUT && tid == 12 * 32 && vblk == 0) p.seg_decays[(int64_t)unit * p.H + h] = seg_a;
+    const bool last = seg + 1 == segs;  // of its sample: its state is the final one
+    const bool taken = OUT && last && __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
+    if (__all_sync(~0u, alive) && writes && (OUT ? last && out_slot >= 0 && !taken : true)) {
+      float* dst = (OUT ? p.ht + (out_slot * p.H + h) * D * D : p.seg_states + seg_state) + col_off;
 #pragma unroll
       for (int i = 0; i < KT; i += 2) {
         dst[i * D] = f32x2_lo(S[i / 2]);

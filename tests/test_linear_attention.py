@@ -68,6 +68,9 @@ def test_linear_attention_refuses_workspace():
     assert lib.memt_linear_attention(ctypes.byref(a), 256, 0, None) == _lib.MEMT_ERR_WORKSPACE
     assert lib.memt_linear_attention(ctypes.byref(a), 264, 1 << 40, None) == _lib.MEMT_ERR_WORKSPACE
     f = lib.memt_linear_attention_workspace_size
+    assert f(8, 65536, 16, 128, _lib.MEMT_BF16) == 256  # enough samples and heads: no segments
+    assert f(1, 65536, 16, 128, _lib.MEMT_BF16) >= 9 * 16 * 128 * 128 * 4
+    assert f(1, 65536, 16, 128, _lib.MEMT_F32) == 256
     assert f(1, 0, 1, 64, _lib.MEMT_BF16) >= 256 and f(1, 100, 1, 96, _lib.MEMT_BF16) == 0
     assert f(0, 100, 1, 64, _lib.MEMT_BF16) == 0 and f(1, 100, 1, 64, 9) == 0
 
@@ -213,6 +216,29 @@ def test_linear_attention_many_chunks(cuda, D):
 
 
 @gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths", [[2500], [1537, 0, 700, 3], [64 * 40, 64 * 20 + 1]])
+@pytest.mark.parametrize("decay", ["head", "token"])
+def test_few_long_samples_in_segments(cuda, D, lengths, decay):
+    """Few (sample, head) pairs: the tokens are split over segments. Every segment adds one join of its
+    state (4 u) to the chunks' own; states start in a pool, one tensor for both, shared key heads."""
+    Hk, H, N = 1, 2, len(lengths)
+    q, k, v, g, h0, cu = _inputs(D, lengths, Hk, H, D, torch.bfloat16, decay, 0.05)
+    ref = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    pool = torch.full((N + 2, H, D, D), 3.0)
+    slots = list(range(N + 1, 1, -1))
+    pool[slots] = h0
+    dq, dk, dv, dg, dpool, dcu = _dev(q, k, v, g, pool, cu)
+    ds = torch.tensor(slots, dtype=torch.int32, device="cuda")
+    o, final = M.linear_attention(dq, dk, dv, dg, dpool, dcu, initial_slots=ds, final_state=dpool, final_slots=ds)
+    torch.cuda.synchronize()
+    to, ts = _tolerances(ref, [2 * n for n in lengths], D, torch.bfloat16, g, H)
+    _check(final[slots], ref[1], ts, "state")
+    _check(o, ref[0], to, "output")
+    assert bool((final[:2] == 3.0).all())
+
+
+@gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strong_decays_and_resets(cuda, dtype):
     """Decays from none to a full reset (g = -inf forgets everything before the token)."""
@@ -331,6 +357,11 @@ def test_bad_offsets_are_clamped(cuda):
         o, final = M.linear_attention(q, k, v, g, h0, torch.tensor(bad, dtype=torch.int32, device="cuda"))
         torch.cuda.synchronize()
         assert bool(torch.isfinite(final).all())
+    # in segments: samples that overlap add up to more tokens than there are
+    q, k, v, g, h0, _ = _dev(*_inputs(11, [1500, 1500, 10], 1, 1, 64, torch.bfloat16, "token"))
+    for bad in ([0, 3010, 0, 3010], [0, 3010, -1, 1 << 30]):
+        M.linear_attention(q, k, v, g, h0, torch.tensor(bad, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
 
 
 @gpu
