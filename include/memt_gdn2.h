@@ -412,7 +412,8 @@ typedef struct memt_linear_attention_args {
   int32_t num_final_slots;
 } memt_linear_attention_args;
 
-/* Workspace bytes for these sizes (0 on invalid sizes). */
+/* Workspace bytes for these sizes (0 on invalid sizes). 256 or less: nothing is kept there and the call
+ * takes a NULL workspace. */
 size_t memt_linear_attention_workspace_size(int32_t num_samples, int64_t total_tokens, int32_t num_heads,
                                             int32_t head_dim, int32_t dtype);
 

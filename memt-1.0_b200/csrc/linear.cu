@@ -151,7 +151,9 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   if (st != MEMT_OK) return st;
   const size_t need =
       memt_linear_attention_workspace_size(a->num_samples, a->total_tokens, a->num_heads, a->head_dim, a->dtype);
-  if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+  // (256 stands for none)
+  if (need > 256 &&
+      (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return MEMT_ERR_WORKSPACE;
   LinearParams p{};
   p.N = a->num_samples;

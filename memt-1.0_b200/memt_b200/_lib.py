@@ -7,6 +7,7 @@ importing an operator without the library raises immediately.
 from __future__ import annotations
 
 import ctypes
+import struct
 from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
@@ -130,6 +131,29 @@ class RotaryArgs(_SizedArgs):
         ("k_out", c_void_p), ("k_out_stride", c_int64), ("positions", c_void_p), ("positions_int64", c_int32),
         ("interleaved", c_int32), ("inv_freq", c_void_p), ("attention_scale", c_float), ("inverse", c_int32),
     ]
+
+
+class Packed:
+    """A struct of this module as bytes, packed from its fields' values in order (``struct_size`` is
+    added): for operators small enough that filling a ctypes structure by name shows."""
+
+    _FORMAT = {c_uint32: "I", c_int32: "i", c_int64: "q", c_void_p: "P", c_float: "f"}
+
+    def __init__(self, cls):
+        self.size = ctypes.sizeof(cls)
+        self._struct = struct.Struct("@" + "".join(self._FORMAT[t] for _, t in cls._fields_) + "0q")
+        if self._struct.size != self.size:
+            raise RuntimeError(f"{cls.__name__}: packed size {self._struct.size} is not {self.size}")
+
+    def __call__(self, *values):
+        return self._struct.pack(self.size, *values)
+
+
+def packed_entry(name, *rest):
+    """The entry point ``name`` for a struct given as bytes (``Packed``); ``rest``: its other argument types."""
+    fn = load()[name]
+    fn.restype, fn.argtypes = c_int, [c_char_p, *rest]
+    return fn
 
 
 # name -> (restype, argtypes): every symbol include/memt_gdn2.h declares

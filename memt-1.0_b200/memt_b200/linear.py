@@ -17,7 +17,7 @@ launch. They compute no gradients.
 
 from __future__ import annotations
 
-import ctypes
+from ctypes import c_size_t, c_void_p
 
 import torch
 
@@ -26,36 +26,48 @@ from .ops import _DTYPE, _pool, _states, _tokens_unchecked
 
 __all__ = ["linear_attention", "linear_attention_step", "gdn2_step"]
 
-_byref = ctypes.byref
+_current_device = torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_entries: dict = {}
 
 
-def _raw_stream(index):
-    return torch.cuda.current_stream(index).cuda_stream
-
-
-def _call(fn, name, dev, *args):
-    """fn(*args, stream) with the tensors' device current."""
-    if torch.cuda.current_device() == dev.index:
-        status = fn(*args, _raw_stream(dev.index))
+def _call(name, dev, *args):
+    """The entry point ``name`` on ``dev``'s current stream, with ``dev`` current; args: its packed
+    struct, then (pointer, size) of a workspace where it takes one."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = _lib.packed_entry(name, *((c_void_p, c_size_t) if len(args) == 3 else ()), c_void_p)
+    stream = _raw_stream(dev.index)
+    if _current_device() == dev.index:
+        status = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, _raw_stream(dev.index))
+            status = fn(*args, stream)
     if status != _lib.MEMT_OK:
         _lib.check(status, name)
+
+
+def _ptr(x):
+    return 0 if x is None else x.data_ptr()
+
+
+_linear_args = _lib.Packed(_lib.LinearAttentionArgs)
+_step_args = _lib.Packed(_lib.RecurrentStepArgs)
 
 
 def _rows(x, name, vec):
     """[1, L, H, D] or [L, H, D] -> ([L, H, D], elements per token row). Token rows whose heads are
     contiguous and whose starts are 16-byte aligned (a split view of a wider projection) are used
     in place; anything else is copied."""
-    x = _tokens_unchecked(x, name)
+    if x.dim() != 3 or not x.is_cuda:
+        x = _tokens_unchecked(x, name)
     L, H, D = x.shape
-    s = x.stride()
-    if s[2] == 1 and s[1] == D and x.data_ptr() % 16 == 0:
+    row, head, one = x.stride()
+    if one == 1 and head == D and x.data_ptr() % 16 == 0:
         if L <= 1:
             return x, H * D
-        if s[0] >= H * D and s[0] % vec == 0:
-            return x, s[0]
+        if row >= H * D and row % vec == 0:
+            return x, row
     return x.contiguous(), H * D
 
 
@@ -96,13 +108,15 @@ def _out_rows(out, like, inputs, vec, name="out"):
 
 def _qkv(q, k, v):
     """Checked token rows of q, k [L, Hk, D] and v [L, H, D]: ((q, stride), (k, ...), (v, ...), vec)."""
-    vec = 8 if v.dtype == torch.bfloat16 else 4
+    dtype = v.dtype
+    if dtype not in _DTYPE:
+        raise ValueError(f"unsupported dtype {dtype}")
+    vec = 8 if dtype is torch.bfloat16 else 4
     q, sq = _rows(q, "q", vec)
     k, sk = _rows(k, "k", vec)
     v, sv = _rows(v, "v", vec)
-    if v.dtype not in _DTYPE:
-        raise ValueError(f"unsupported dtype {v.dtype}")
-    if q.dtype != v.dtype or k.dtype != v.dtype or q.device != v.device or k.device != v.device:
+    dev = v.get_device()
+    if q.dtype is not dtype or k.dtype is not dtype or q.get_device() != dev or k.get_device() != dev:
         raise ValueError("q, k and v must share dtype and device")
     L, H, D = v.shape
     Hk = q.shape[1]
@@ -194,17 +208,12 @@ def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=N
     dtype = _DTYPE[v.dtype]
     need = lib.memt_linear_attention_workspace_size(N, L, H, D, dtype)
     # from the caching allocator, so that neither streams nor captured graphs share it
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    args = _lib.LinearAttentionArgs(
-        num_samples=N, num_heads=H, num_key_heads=q.shape[1], head_dim=D, dtype=dtype, total_tokens=L,
-        cu_seqlens=cu.data_ptr(), q=q.data_ptr(), q_stride=sq, k=k.data_ptr(), k_stride=sk, v=v.data_ptr(),
-        v_stride=sv, g=None if g is None else g.data_ptr(), g_layout=g_layout,
-        scale=D ** -0.5 if scale is None else scale, out=o.data_ptr(), out_stride=so,
-        initial_state=None if initial_state is None else initial_state.data_ptr(),
-        final_state=final_state.data_ptr(),
-        initial_slots=None if initial_slots is None else initial_slots.data_ptr(), num_initial_slots=n_in,
-        final_slots=None if final_slots is None else final_slots.data_ptr(), num_final_slots=n_out)
-    _call(lib.memt_linear_attention, "memt_linear_attention", dev, _byref(args), ws.data_ptr(), need)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+    args = _linear_args(
+        N, H, q.shape[1], D, dtype, L, cu.data_ptr(), q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _ptr(g),
+        g_layout, D ** -0.5 if scale is None else scale, o.data_ptr(), so, _ptr(initial_state), final_state.data_ptr(),
+        _ptr(initial_slots), n_in, _ptr(final_slots), n_out)
+    _call("memt_linear_attention", dev, args, _ptr(ws), need)
     return o, final_state
 
 
@@ -267,13 +276,9 @@ def _step(rule, q, k, v, g, states, beta, erase, write, scale, slots, read_incom
         o, so = _out_rows(out, v, ((q, sq), (k, sk), (v, sv)), vec)
     if N == 0:
         return o
-    args = _lib.RecurrentStepArgs(
-        rule=rule, num_samples=N, num_heads=H, num_key_heads=Hk, head_dim=D, dtype=_DTYPE[v.dtype],
-        read_incoming=1 if read_incoming else 0, q=q.data_ptr(), q_stride=sq, k=k.data_ptr(), k_stride=sk,
-        v=v.data_ptr(), v_stride=sv, g=None if g is None else g.data_ptr(), g_layout=g_layout,
-        beta_layout=beta_layout, beta=None if beta is None else beta.data_ptr(),
-        erase=None if erase is None else erase.data_ptr(), write=None if write is None else write.data_ptr(),
-        states=states.data_ptr(), slots=None if slots is None else slots.data_ptr(), num_slots=num_slots,
-        scale=D ** -0.5 if scale is None else scale, out=o.data_ptr(), out_stride=so)
-    _call(_lib.load().memt_recurrent_step, "memt_recurrent_step", dev, _byref(args))
+    args = _step_args(
+        rule, N, H, Hk, D, _DTYPE[v.dtype], 1 if read_incoming else 0, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(),
+        sv, _ptr(g), g_layout, beta_layout, _ptr(beta), _ptr(erase), _ptr(write), states.data_ptr(), _ptr(slots),
+        num_slots, D ** -0.5 if scale is None else scale, o.data_ptr(), so)
+    _call("memt_recurrent_step", dev, args)
     return o

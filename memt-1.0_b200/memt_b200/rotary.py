@@ -11,10 +11,12 @@ import math
 import torch
 
 from . import _lib
-from .linear import _byref, _call, _overlap
+from .linear import _call, _overlap, _ptr
 from .ops import _DTYPE, _tokens_unchecked
 
 __all__ = ["rotary", "rotary_frequencies"]
+
+_rotary_args = _lib.Packed(_lib.RotaryArgs)
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, trained_tokens=None, fast_turns=32.0,
@@ -57,14 +59,15 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
 
 def _head_rows(x, name):
     """[1, L, H, D] or [L, H, D] with contiguous heads -> ([L, H, D], elements per token row)."""
-    x = _tokens_unchecked(x, name)
+    if x.dim() != 3 or not x.is_cuda:
+        x = _tokens_unchecked(x, name)
     L, H, D = x.shape
-    s = x.stride()
-    if s[2] == 1 and (s[1] == D or H == 1):
+    row, head, one = x.stride()
+    if one == 1 and (head == D or H == 1):
         if L <= 1:
             return x, H * D
-        if s[0] >= H * D:
-            return x, s[0]
+        if row >= H * D:
+            return x, row
     return x.contiguous(), H * D
 
 
@@ -100,23 +103,18 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, inverse=False, atten
     if positions.device != dev or inv_freq.device != dev:
         raise ValueError(f"positions and inv_freq must be on {dev}")
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
-    given = q_out is not None or k_out is not None
     qo, sqo = _output(q, sq, q_out, "q_out")
     ko, sko = (None, 0) if k is None else _output(k, sk, k_out, "k_out")
-    if given and k is not None and (
-            (q_out is not None and _overlap(qo, sqo, k, sk)) or (k_out is not None and _overlap(ko, sko, q, sq))
-            or _overlap(qo, sqo, ko, sko)):
+    if k is not None and ((q_out is not None and _overlap(qo, sqo, k, sk))
+                          or (k_out is not None and (_overlap(ko, sko, q, sq) or _overlap(qo, sqo, ko, sko)))):
         raise ValueError("q_out and k_out must not overlap each other or the other input")
     if L == 0 or H == 0:
         return qo, ko
-    args = _lib.RotaryArgs(
-        num_heads=H, num_key_heads=Hk, head_dim=D, rotary_dim=2 * inv_freq.numel(), dtype=_DTYPE[q.dtype],
-        total_tokens=L, q=q.data_ptr(), q_stride=sq, k=None if k is None else k.data_ptr(), k_stride=sk,
-        q_out=qo.data_ptr(), q_out_stride=sqo, k_out=None if k is None else ko.data_ptr(), k_out_stride=sko,
-        positions=positions.data_ptr(), positions_int64=1 if positions.dtype == torch.int64 else 0,
-        interleaved=1 if interleaved else 0, inv_freq=inv_freq.data_ptr(), attention_scale=attention_scale,
-        inverse=1 if inverse else 0)
-    _call(_lib.load().memt_rotary, "memt_rotary", dev, _byref(args))
+    args = _rotary_args(
+        H, Hk, D, 2 * inv_freq.numel(), _DTYPE[q.dtype], L, q.data_ptr(), sq, _ptr(k), sk, qo.data_ptr(), sqo, _ptr(ko),
+        sko, positions.data_ptr(), 1 if positions.dtype is torch.int64 else 0, 1 if interleaved else 0,
+        inv_freq.data_ptr(), attention_scale, 1 if inverse else 0)
+    _call("memt_rotary", dev, args)
     return qo, ko
 
 
@@ -132,6 +130,6 @@ def _output(x, stride, out, name):
     if s[2] != 1 or (s[1] != D and H > 1) or (L > 1 and s[0] < H * D):
         raise ValueError(f"{name}: token rows must be contiguous heads")
     so = s[0] if L > 1 else H * D
-    if not (o.data_ptr() == x.data_ptr() and so == stride) and _overlap(o, so, x, stride):
+    if out is not x and not (o.data_ptr() == x.data_ptr() and so == stride) and _overlap(o, so, x, stride):
         raise ValueError(f"{name} must be the input itself or not overlap it")
     return o, so

@@ -62,7 +62,8 @@ def test_linear_attention_refuses(over, error):
 
 
 def test_linear_attention_refuses_workspace():
-    lib, a = _lib.load(), _linear_args()
+    # one long sample of few heads: its segments' states need memory
+    lib, a = _lib.load(), _linear_args(total_tokens=1 << 20)
     assert lib.memt_linear_attention(None, 256, 1 << 40, None) == _lib.MEMT_ERR_INVALID_ARGUMENT
     assert lib.memt_linear_attention(ctypes.byref(a), None, 1 << 40, None) == _lib.MEMT_ERR_WORKSPACE
     assert lib.memt_linear_attention(ctypes.byref(a), 256, 0, None) == _lib.MEMT_ERR_WORKSPACE
