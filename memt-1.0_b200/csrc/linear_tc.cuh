@@ -79,7 +79,7 @@ struct LinearTcCfg {
   static constexpr int kPanels = D < 128 ? 1 : D / 128;  // U and e^R K go in units of up to 128 keys
   static constexpr int kPanelKeys = D / kPanels;
   static constexpr int kKeys = D / 2;            // keys per state thread
-  static constexpr int kStages = D == 256 ? 2 : 4;
+  static constexpr int kStages = D == 256 ? 2 : (D == 128 ? 3 : 4);
   static constexpr int kTables = 4;
   static constexpr uint32_t kPanel = kTile * 128;  // 64 x 64 bf16: 8 KB
   static constexpr uint32_t kBytesQK = kTile * D * 2;
@@ -180,10 +180,6 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
     mbar_fence_init();
   }
   if (warp == 0) tc::alloc(smem_u32(tmem_slot), 512);
-  // blocks of P above the diagonal are zero in every chunk
-  for (int i = tid; i < int(Cfg::kPanel / 16); i += Cfg::kThreads)
-    reinterpret_cast<uint4*>(sm + Cfg::kOffP)[i] = make_uint4(0, 0, 0, 0);
-  tc::fence_smem_async();
   tc::fence_before();
   __syncthreads();
   tc::fence_after();
@@ -220,7 +216,6 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
       // ---------------- MMA issue ----------------
       constexpr uint32_t kIdSc = tc::idesc(tc::kBF16, 64, 64, false, false);
       constexpr uint32_t kIdX = tc::idesc(tc::kBF16, 128, 64, false, false);  // A in tensor memory, Q K-major
-      constexpr uint32_t kIdY = tc::idesc(tc::kBF16, 128, 64, true, false);   // V MN-major, P K-major
       constexpr uint32_t kIdU = tc::idesc(tc::kBF16, 128, Cfg::kPanelKeys, false, true);  // K MN-major
       auto go = [&]() {  // nothing more is issued after a wait ran out
         tc::fence_after();
@@ -279,8 +274,12 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         if (go()) {
         const uint64_t dv = tc::desc_mnmajor(base + Cfg::kOffV + s * Cfg::kBytesV, Cfg::kPanel, 0);
         const uint64_t dp = tc::desc_kmajor(base + Cfg::kOffP, 0);
+        // tokens 16 i .. 16 i + 15 are seen by the columns from 16 i on only: smaller products, and the blocks
+        // of P above the diagonal are never read
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i) tc::mma_bf16(tY, dv + 128 * i, dp + 2 * i, kIdY, i > 0);
+        for (int i = 0; i < kTile / 16; ++i)
+          tc::mma_bf16(tY + 16 * i, dv + 128 * i, dp + 128 * i + 2 * i, tc::idesc(tc::kBF16, 128, kTile - 16 * i, true, false),
+                       i > 0);
         tc::commit(B(XY));
         tc::commit(B(VE + s));
         }
@@ -403,7 +402,15 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
           t.between[lane] = fast_exp2(x);
         }
         if (lane == 0) {
-          const double a = exp(total);
+          // e^total = 2^n 2^f, |f| <= 1/2, by the Taylor series of 2^f in 64 bits (the first term left out is
+          // below 2^-37); e^total below 2^-900 is zero in fp32
+          const double y = total * 1.4426950408889634;
+          const double nr = rint(y), f = (y - nr) * 0.6931471805599453;
+          constexpr double kInvFact[9] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320};
+          double a = 1.0 / 362880;
+#pragma unroll
+          for (int i = 8; i >= 0; --i) a = fma(a, f, kInvFact[i]);
+          a = y < -900.0 ? 0.0 : a * __longlong_as_double((static_cast<long long>(nr) + 1023) << 52);
           t.a_hi = static_cast<float>(a);
           t.a_lo = static_cast<float>(a - static_cast<double>(t.a_hi));
         }
