@@ -11,8 +11,10 @@
 //
 // Bound by HBM: every element is read and written once, in 16-byte vectors. A thread owns one
 // vector of pairs of one token, evaluates its sines and cosines once and walks over heads with
-// them, so their cost is shared by the heads it walks. Few tokens leave SMs idle that way; the
-// heads of a token are then spread over more threads, which each evaluate the angles again.
+// them, four heads in flight, so their cost is shared by the heads it walks. Few tokens leave SMs idle
+// that way; the heads of a token are then spread over more threads, which each evaluate the angles
+// again. The vectors behind the rotary part are copied by threads of their own, behind all others
+// in the grid, so that no warp does both.
 #include "launch.h"
 
 namespace {
@@ -34,8 +36,20 @@ struct RotaryParams {
   int32_t inverse, interleaved;
   int32_t groups;     // threads a token's heads are spread over
   int32_t rot_units;  // vectors (pairs of vectors in the half layout) that turn, per head
-  int32_t units;      // ... plus the vectors behind the rotary part that are copied
+  int32_t copy_units;  // vectors behind the rotary part that are copied, per head
 };
+
+// Thread `idx` of `per_token` for each token -> (token, thread of it); 32-bit division where it suffices.
+__device__ __forceinline__ int64_t split(int64_t idx, int per_token, int& rest) {
+  if (idx <= 0xffffffffll) {
+    const uint32_t t = static_cast<uint32_t>(idx) / static_cast<uint32_t>(per_token);
+    rest = static_cast<int>(static_cast<uint32_t>(idx) - t * per_token);
+    return t;
+  }
+  const int64_t t = idx / per_token;
+  rest = static_cast<int>(idx - t * per_token);
+  return t;
+}
 
 __device__ __forceinline__ double position(const RotaryParams& p, int64_t t) {
   return p.pos64 ? static_cast<double>(static_cast<const int64_t*>(p.pos)[t])
@@ -102,23 +116,42 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   constexpr int V = Vec<T>::N;
   constexpr int kPairs = INTERLEAVED ? V / 2 : V;
   constexpr int kHeads = 4;
-  const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t per_token = (int64_t)p.units * p.groups;
-  const int64_t t = idx / per_token;
-  if (t >= p.L) return;
-  const int rest = static_cast<int>(idx - t * per_token);
-  const int group = rest / p.units, unit = rest - group * p.units;
+  int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int H = p.Hq + p.Hk;
-  if (unit >= p.rot_units) {  // behind the rotary part: copied
-    const int col = p.R + (unit - p.rot_units) * V;
-    for (int h = group; h < H; h += p.groups) {
-      const T* x;
-      T* y;
-      head_ptrs(p, t, h, x, y);
-      *reinterpret_cast<uint4*>(y + col) = *reinterpret_cast<const uint4*>(x + col);
+  const int64_t turning = p.L * p.rot_units * p.groups;
+  int rest;
+  if (idx >= turning) {  // behind the rotary part: copied
+    if (p.copy_units == 0) return;
+    const int64_t t = split(idx - turning, p.copy_units * p.groups, rest);
+    if (t >= p.L) return;
+    const int group = rest / p.copy_units, col = p.R + (rest - group * p.copy_units) * V;
+    for (int h0 = group; h0 < H; h0 += kHeads * p.groups) {
+      uint4 a[kHeads];
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j) {
+        const int h = h0 + j * p.groups;
+        const T* x;
+        T* y;
+        if (h < H) {
+          head_ptrs(p, t, h, x, y);
+          a[j] = *reinterpret_cast<const uint4*>(x + col);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j) {
+        const int h = h0 + j * p.groups;
+        const T* x;
+        T* y;
+        if (h < H) {
+          head_ptrs(p, t, h, x, y);
+          *reinterpret_cast<uint4*>(y + col) = a[j];
+        }
+      }
     }
     return;
   }
+  const int64_t t = split(idx, p.rot_units * p.groups, rest);
+  const int group = rest / p.rot_units, unit = rest - group * p.rot_units;
   float c[kPairs], s[kPairs];
   const double pos = position(p, t);
 #pragma unroll
@@ -175,29 +208,48 @@ __device__ __forceinline__ void store(__nv_bfloat16* y, float x) { *y = __float2
 // Rows or rotary parts that are not whole 16-byte vectors: one pair (or copied element) a thread.
 template <typename T>
 __global__ void __launch_bounds__(256) rotary_scalar_kernel(const RotaryParams p) {
+  constexpr int kHeads = 4;
   const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t per_token = (int64_t)p.units * p.groups;
-  const int64_t t = idx / per_token;
+  const int units = p.rot_units + p.copy_units;
+  int rest;
+  const int64_t t = split(idx, units * p.groups, rest);
   if (t >= p.L) return;
-  const int rest = static_cast<int>(idx - t * per_token);
-  const int group = rest / p.units, unit = rest - group * p.units;
+  const int group = rest / units, unit = rest - group * units;
   const int H = p.Hq + p.Hk, half = p.R >> 1;
   const bool turns = unit < p.rot_units;
   const int ia = turns ? (p.interleaved ? 2 * unit : unit) : p.R + unit - p.rot_units;
-  const int ib = p.interleaved ? ia + 1 : ia + half;
-  float c = 0.f, s = 0.f;
+  const int ib = turns ? (p.interleaved ? ia + 1 : ia + half) : ia;
+  float c = 1.f, s = 0.f;
   if (turns) angle(p, position(p, t), unit, c, s);
-  for (int h = group; h < H; h += p.groups) {
-    const T* x;
-    T* y;
-    head_ptrs(p, t, h, x, y);
-    if (!turns) {
-      y[ia] = x[ia];
-      continue;
+  for (int h0 = group; h0 < H; h0 += kHeads * p.groups) {
+    T a[kHeads], b[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = h0 + j * p.groups;
+      const T* x;
+      T* y;
+      if (h < H) {
+        head_ptrs(p, t, h, x, y);
+        a[j] = x[ia];
+        b[j] = x[ib];
+      }
     }
-    const float a = to_float(x[ia]), b = to_float(x[ib]);
-    store(y + ia, c * a - s * b);
-    store(y + ib, c * b + s * a);
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {
+      const int h = h0 + j * p.groups;
+      const T* x;
+      T* y;
+      if (h < H) {
+        head_ptrs(p, t, h, x, y);
+        if (turns) {
+          const float fa = to_float(a[j]), fb = to_float(b[j]);
+          store(y + ia, c * fa - s * fb);
+          store(y + ib, c * fb + s * fa);
+        } else {
+          y[ia] = a[j];
+        }
+      }
+    }
   }
 }
 
@@ -212,9 +264,9 @@ int launch_rotary(RotaryParams& p, bool copy_rest, int sms, cudaStream_t s) {
   vec = vec && aligned16(p.q) && aligned16(p.q_out) && aligned16(p.k) && aligned16(p.k_out);
   const int per_unit = vec ? (p.interleaved ? V : 2 * V) : 2;  // rotary elements per unit
   p.rot_units = p.R / per_unit;
-  p.units = p.rot_units + (copy_rest ? (p.D - p.R) / (vec ? V : 1) : 0);
+  p.copy_units = copy_rest ? (p.D - p.R) / (vec ? V : 1) : 0;
   // threads for two full waves at 1024 threads an SM, as far as there are heads to spread
-  const int64_t want = int64_t(sms) * 2048, have = p.L * p.units;
+  const int64_t want = int64_t(sms) * 2048, have = p.L * (p.rot_units + p.copy_units);
   const int H = p.Hq + p.Hk;
   int64_t groups = have > 0 ? (want + have - 1) / have : 1;
   if (groups > H) groups = H;

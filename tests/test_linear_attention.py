@@ -501,6 +501,36 @@ def test_gdn2_step(cuda, D, dtype, gates, incoming):
 
 
 @gpu
+@pytest.mark.parametrize("D,N,H", [(64, 120, 16), (64, 201, 9), (128, 47, 13), (128, 150, 8), (256, 37, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("gates", ["head", "channel"])
+@pytest.mark.parametrize("incoming", [False, True])
+def test_gdn2_step_of_many_sessions(cuda, D, N, H, dtype, gates, incoming):
+    """Many sessions, odd counts among them, in a pool with skipped and repeated slots."""
+    Hk = H if H % 2 else H // 2
+    gen, q, k, v, sig = _step_inputs(N, N, Hk, H, D, dtype)
+    g = -torch.rand(*((N, H) if gates == "head" else (N, H, D)), generator=gen)
+    beta = sig(N, Hk) if gates == "head" else sig(N, Hk, D)
+    erase, write = (None, None) if gates == "head" else (sig(N, Hk, D), sig(N, H, D))
+    pool = torch.randn(N + 3, H, D, D, generator=gen)
+    slots = torch.randperm(N + 3, generator=gen)[:N].to(torch.int32)
+    slots[5], slots[9], slots[20] = -1, N + 3, slots[2]
+    live = [i for i in range(N) if i not in (5, 9, 20)]
+    at = slots[live].long()
+    pick = lambda x: None if x is None else x[live]  # noqa: E731
+    ref = _step_reference(q[live], k[live], v[live], g[live], pool[at], pick(beta), pick(erase), pick(write), True,
+                          incoming, 0.25)
+    dq, dk, dv, dg, dp, ds, db, de, dw = _dev(q, k, v, g, pool, slots, beta, erase, write)
+    out = torch.full((N, H, D), 5.0, dtype=dtype, device="cuda")
+    o = M.gdn2_step(dq, dk, dv, dg, dp, beta=db, erase=de, write=dw, scale=0.25, slots=ds, read_incoming=incoming, out=out)
+    torch.cuda.synchronize()
+    _check_step(o[live], dp[at.cuda()], ref, D, dtype)
+    assert bool((o[[5, 9, 20]] == 5.0).all())
+    untouched = sorted(set(range(N + 3)) - set(at.tolist()))
+    assert torch.equal(dp[untouched].cpu(), pool[untouched])
+
+
+@gpu
 @pytest.mark.parametrize("rule", ["linear", "gdn2"])
 def test_step_pools_views_and_skipped_rows(cuda, rule):
     """Slots of a pool; a slot outside it and a slot named twice are skipped, with their rows of o;
