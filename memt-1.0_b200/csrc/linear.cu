@@ -31,16 +31,19 @@ int launch_recurrent_form(int D, const LinearParams& p, cudaStream_t s) {
 constexpr int kPlanSms = 148;
 
 // 64-token chunks per segment, or 0: one CTA per (sample, head, value block) walks a whole sample. Few of
-// them leave SMs idle for as long as a sample takes: 16 heads of one 65536-token sample 1.5 ms. Segments
+// them leave SMs idle for as long as a sample takes: 16 heads of one 65536-token sample 1.51 ms. Segments
 // fill the SMs once, at the price of a first pass that sums their states (k and v are read twice) and
-// a pass that joins them: 0.36 ms. A chunk takes about 1.7 us in one CTA, 1.1 us in the first pass, the
-// two further launches about 12 us, which decides whether the split pays.
+// a pass that joins them: 0.43 ms. A chunk takes 1.2 / 1.55 / 2.6 us in one CTA at D = 64 / 128 / 256,
+// 0.65 of that more in the first pass, and the launches about 18 us. Measured on either side, whole against
+// segments in us: 16 heads of one sample, D = 128: 512 tokens 19 / 27, 1024 31 / 30, 2048 55 / 36, 8192
+// 203 / 72; of two: 1024 31 / 33, 2048 55 / 45; two segments never pay (four samples: 8192 207 / 207).
 int plan_segment_chunks(int64_t N, int64_t L, int64_t H, int D) {
   const int64_t ctas = N * H * (D == 256 ? 2 : 1);
   const int64_t split = kPlanSms / ctas;
-  if (split < 2) return 0;
+  if (split < 3) return 0;
   const int64_t chunks = (L + kTile - 1) / kTile / N;  // of a mean sample
-  if (chunks * (1.7 - 2.8 / split) < 12.0) return 0;
+  const double chunk_us = D == 64 ? 1.2 : (D == 128 ? 1.55 : 2.6);
+  if (chunks * chunk_us * (1.0 - 1.65 / split) < 18.0) return 0;
   return static_cast<int>((chunks + split - 1) / split);
 }
 int64_t max_segments(int64_t N, int64_t L, int seg_chunks) { return L / (int64_t(seg_chunks) * kTile) + N; }
@@ -73,9 +76,10 @@ int launch_chunked(const LinearParams& p, void* workspace, cudaStream_t s) {
   if (e != cudaSuccess) return cuda_status(e);
   const int seg_chunks = plan_segment_chunks(p.N, p.L, p.H, D);
   if (seg_chunks == 0) {
-    // more CTAs than SMs: the longest samples first, so that no SM ends with one (16 samples of 1 to 16384
-    // tokens, 16 heads, d = 128: 617 us in order of the samples, 498 us by length)
-    P.p.by_length = p.N > 1 && p.N <= 256 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms;
+    // More CTAs than SMs: the longest samples first, so that no SM is left with one at the end (16 samples of
+    // 0 to 16384 tokens, 16 heads, d = 128: 617 us in order of the samples, 594 by length). Every CTA ranks
+    // the samples for itself, which short or many samples would not repay.
+    P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms && p.L / p.N >= 1024;
     return launch_pass<D, true>(P, p.N, s);
   }
   const int64_t units = max_segments(p.N, p.L, seg_chunks);

@@ -218,7 +218,7 @@ def test_linear_attention_many_chunks(cuda, D):
 
 @gpu
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("lengths", [[2500], [1537, 0, 700, 3], [64 * 40, 64 * 20 + 1]])
+@pytest.mark.parametrize("lengths", [[2500], [4000, 0, 2500, 3], [64 * 40, 64 * 20 + 1]])
 @pytest.mark.parametrize("decay", ["head", "token"])
 def test_few_long_samples_in_segments(cuda, D, lengths, decay):
     """Few (sample, head) pairs: the tokens are split over segments. Every segment adds one join of its
@@ -359,8 +359,8 @@ def test_bad_offsets_are_clamped(cuda):
         torch.cuda.synchronize()
         assert bool(torch.isfinite(final).all())
     # in segments: samples that overlap add up to more tokens than there are
-    q, k, v, g, h0, _ = _dev(*_inputs(11, [1500, 1500, 10], 1, 1, 64, torch.bfloat16, "token"))
-    for bad in ([0, 3010, 0, 3010], [0, 3010, -1, 1 << 30]):
+    q, k, v, g, h0, _ = _dev(*_inputs(11, [3000, 2000, 10], 1, 1, 64, torch.bfloat16, "token"))
+    for bad in ([0, 5010, 0, 5010], [0, 5010, -1, 1 << 30]):
         M.linear_attention(q, k, v, g, h0, torch.tensor(bad, dtype=torch.int32, device="cuda"))
         torch.cuda.synchronize()
 
