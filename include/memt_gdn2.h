@@ -77,7 +77,8 @@ typedef struct CUstream_st *memt_stream_t;
 /* Library version (major*10000 + minor*100 + patch).
  *   0.2.0  state pools by slot index (fields appended to the update, read and readout args)
  *   0.3.0  every argument struct starts with struct_size; the memory-block prologue; the
- *          DeepSeek grouped latent RMS norm; memt_gdn2_noalloc_status, memt_read_status */
+ *          DeepSeek grouped latent RMS norm; memt_gdn2_noalloc_status, memt_read_status; (entry points
+ *          added since, no struct changed:) linear attention, single-token steps, rotary positions */
 int memt_version(void);  /* 300 */
 
 /* Argument structs start with `uint32_t struct_size`, which the caller sets to

@@ -337,6 +337,54 @@ def test_no_initial_state_is_zeros_and_host_offsets(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_no_tokens_at_all(cuda, dtype):
+    """Only empty samples: the states are copied, in place or not; no decay, no output rows."""
+    h0 = torch.randn(3, 2, 64, 64, device="cuda")
+    x = torch.empty(0, 2, 64, dtype=dtype, device="cuda")
+    cu = torch.zeros(4, dtype=torch.int32, device="cuda")
+    for g in (None, torch.empty(0, 2, device="cuda"), torch.zeros(2, device="cuda")):
+        o, final = M.linear_attention(x, x, x, g, h0, cu)
+        assert o.shape == (0, 2, 64) and torch.equal(final, h0)
+    _, final = M.linear_attention(x, x, x, None, None, cu)
+    assert bool((final == 0).all())
+
+
+@gpu
+def test_pools_and_rows_beyond_32_bits(cuda):
+    """State pools of more than 2^32 bytes and 2^31 elements, and token rows of more than 2^31 elements."""
+    H, D = 16, 128
+    pool = torch.empty(8300, H, D, D, device="cuda")  # 2.18e9 elements
+    slots = torch.tensor([8299, 1], dtype=torch.int32, device="cuda")
+    gen, q, k, v, _ = _step_inputs(3, 2, H, H, D, torch.bfloat16)
+    S = torch.randn(2, H, D, D, generator=gen).cuda()
+    dq, dk, dv, dg = _dev(q, k, v, -torch.rand(2, H, generator=gen))
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    for run in (lambda s, sl: M.linear_attention_step(dq, dk, dv, dg, s, slots=sl),
+                lambda s, sl: M.gdn2_step(dq, dk, dv, dg, s, slots=sl),
+                lambda s, sl: M.linear_attention(dq, dk, dv, dg, s, cu, initial_slots=sl, final_state=s,
+                                                 final_slots=sl)[0]):
+        pool[slots.long()] = S
+        small = S.clone()
+        o, want = run(pool, slots), run(small, torch.arange(2, dtype=torch.int32, device="cuda"))
+        assert torch.equal(o, want) and torch.equal(pool[slots.long()], small)
+    del pool
+    # strong decays: a row depends on the last tokens alone, so a short run gives the last rows
+    L, H = 270000, 64
+    v = torch.randn(L, H, D, device="cuda", dtype=torch.bfloat16)
+    q, k = (torch.nn.functional.normalize(torch.randn(L, 1, D, device="cuda"), dim=-1).bfloat16() for _ in range(2))
+    g = torch.full((H,), -1.0, device="cuda")
+    o, final = M.linear_attention(q, k, v, g, None, torch.tensor([0, L]))
+    t = slice(L - 240 - L % 64, L)  # whole chunks behind its start
+    t = slice((t.start // 64) * 64, L)
+    o1, final1 = M.linear_attention(q[t], k[t], v[t], g, None, torch.tensor([0, L - t.start]))
+    torch.cuda.synchronize()
+    # what came before the short run has decayed to e^-200
+    assert torch.equal(o[-64:], o1[-64:])
+    assert float((final - final1).abs().max()) <= 1e-6 * float(final1.abs().max())
+
+
+@gpu
 def test_samples_are_independent_of_the_pack(cuda):
     """A sample's result does not depend on what it is packed with, bit for bit."""
     lengths = [130, 64, 300]
@@ -390,10 +438,11 @@ def test_linear_attention_refuses_arguments(cuda):
 
 
 @gpu
-def test_graphs_streams_and_replays(cuda):
+@pytest.mark.parametrize("lengths", [[700, 300], [3000]])
+def test_graphs_streams_and_replays(cuda, lengths):
     """Two captured graphs of one stream, replayed together on two streams, and an eager call give
-    the same results: no scratch is shared."""
-    cases = [_dev(*_inputs(20 + i, [700, 300], 2, 4, 128, torch.bfloat16, "token")) for i in range(2)]
+    the same results: no scratch is shared (one long sample: with segments' states in a workspace)."""
+    cases = [_dev(*_inputs(20 + i, lengths, 2, 4, 128, torch.bfloat16, "token")) for i in range(2)]
     eager = [M.linear_attention(*c) for c in cases]
     stream = torch.cuda.Stream()
     graphs, outs = [], []

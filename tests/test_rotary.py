@@ -136,6 +136,17 @@ def test_split_views_in_place(cuda, dtype):
 
 
 @gpu
+def test_rows_beyond_32_bits(cuda):
+    """More than 2^31 elements: the last rows equal those of a call of their own."""
+    L, H, D = 262200, 64, 128
+    q = torch.randn(L, H, D, device="cuda", dtype=torch.bfloat16)
+    pos, (inv, _) = torch.arange(L, device="cuda"), M.rotary_frequencies(64)
+    last, _ = M.rotary(q[-100:].clone(), None, pos[-100:], inv)
+    M.rotary(q, None, pos, inv, q_out=q)
+    assert torch.equal(q[-100:], last)
+
+
+@gpu
 def test_inverse_undoes_and_is_the_gradient(cuda):
     """<rotary(x), y> = <x, inverse(y)>: the inverse is the transpose, up to fp32 rounding."""
     gen = torch.Generator().manual_seed(2)
