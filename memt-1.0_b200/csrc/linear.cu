@@ -92,7 +92,7 @@ int launch_chunked(const LinearParams& p, void* workspace, cudaStream_t s) {
   if (st != MEMT_OK) return st;
   {
     ProfScope prof(kProfLinear, s);
-    const unsigned grid = static_cast<unsigned>(p.N * p.H * ((D * D / 4 + 255) / 256));  // fewer CTAs than SMs ran: small
+    const unsigned grid = static_cast<unsigned>(p.N * p.H * ((D * D / 4 + 255) / 256));  // N * H < kPlanSms: small
     linear_segments_kernel<<<grid, 256, 0, s>>>(P.p, D);
     st = cuda_status(cudaGetLastError());
     if (st != MEMT_OK) return st;
@@ -150,7 +150,7 @@ size_t memt_linear_attention_workspace_size(int32_t N, int64_t L, int32_t H, int
 }
 
 int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, size_t workspace_bytes,
-                          memt_stream_t stream) {
+                          memt_stream_t stream) try {
   const int st = check_linear(a);
   if (st != MEMT_OK) return st;
   const size_t need =
@@ -186,6 +186,8 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   // without tokens the states are only copied
   if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_recurrent_form(a->head_dim, p, s);
   return launch_chunked(a->head_dim, p, workspace, s);
+} catch (...) {  // the launch bookkeeping may run out of host memory
+  return MEMT_ERR_CUDA;
 }
 
 int memt_linear_attention_status(memt_stream_t stream, int32_t* status_out) {

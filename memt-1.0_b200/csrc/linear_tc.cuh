@@ -101,7 +101,7 @@ struct LinearTcCfg {
   static constexpr int kRegsControl = D == 256 ? 32 : 64, kRegsState = D == 256 ? 152 : 104,
                        kRegsWork = D == 256 ? 72 : 104;
   static constexpr int kOutTokens = D >= 128 ? kTile / 2 : kTile / 4;  // tokens of an output warp
-  static constexpr int kCols = D == 256 ? 8 : 16;  // columns of U that a state thread holds at a time
+  static constexpr int kCols = D == 256 ? 8 : 32;  // columns of U that a state thread holds at a time
   static_assert(kRegsControl + 2 * kRegsState + 2 * kRegsWork <= 5 * 96, "no more than the launch's registers");
   static_assert(kColSc + 64 <= 512 && kSmem <= 227 * 1024, "one CTA's resources");
 };
@@ -137,7 +137,8 @@ __device__ __forceinline__ void regs_dec() {
 }
 
 template <int D, bool OUT>
-__global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(const __grid_constant__ LinearTcParams P) {
+__global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
+    linear_tc_kernel(const __grid_constant__ LinearTcParams P) {
   using Cfg = LinearTcCfg<D>;
   constexpr int NS = Cfg::kStages, NP = Cfg::kPanels, NT = Cfg::kTables, KT = Cfg::kKeys, CW = Cfg::kCols;
   const LinearParams& p = P.p;
@@ -226,13 +227,13 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         wait(QF + s, c / NS);
         wait(KF + s, c / NS);
         if (go()) {
-        const uint64_t dq = tc::desc_kmajor(base + Cfg::kOffQ + s * Cfg::kBytesQK, 0);
-        const uint64_t dk = tc::desc_kmajor(base + Cfg::kOffK + s * Cfg::kBytesQK, 0);
+          const uint64_t dq = tc::desc_kmajor(base + Cfg::kOffQ + s * Cfg::kBytesQK, 0);
+          const uint64_t dk = tc::desc_kmajor(base + Cfg::kOffK + s * Cfg::kBytesQK, 0);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          tc::mma_bf16(tSc, dq + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2,
-                            dk + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2, kIdSc, i > 0);
-        tc::commit(B(SC));
+          for (int i = 0; i < D / 16; ++i)
+            tc::mma_bf16(tSc, dq + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2,
+                         dk + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2, kIdSc, i > 0);
+          tc::commit(B(SC));
         }
         __syncwarp();
       };
@@ -245,15 +246,15 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         if (u > 0) wait(UE, c);
         else if (c > 0) wait(UE + NP - 1, c - 1);
         if (go()) {
-        const uint64_t dk = tc::desc_mnmajor(
-            base + Cfg::kOffK + s * Cfg::kBytesQK + u * (Cfg::kPanelKeys / 64) * Cfg::kPanel, Cfg::kPanel, 0);
-        // smallest term first, so that the accumulator's truncations are those of small sums
+          const uint64_t dk = tc::desc_mnmajor(
+              base + Cfg::kOffK + s * Cfg::kBytesQK + u * (Cfg::kPanelKeys / 64) * Cfg::kPanel, Cfg::kPanel, 0);
+          // smallest term first, so that the accumulator's truncations are those of small sums
 #pragma unroll
-        for (int i = 0; i < 12; ++i)
-          tc::mma_bf16_ts(tU, tW + 8 * i, dk + 128 * (i & 3), kIdU, i > 0);
-        tc::commit(B(BU + u));
-        if (u == NP - 1) tc::commit(B(KE + s));
-        if (!OUT && u == NP - 1) tc::commit(B(VE + s));
+          for (int i = 0; i < 12; ++i)
+            tc::mma_bf16_ts(tU, tW + 8 * i, dk + 128 * (i & 3), kIdU, i > 0);
+          tc::commit(B(BU + u));
+          if (u == NP - 1) tc::commit(B(KE + s));
+          if (!OUT && u == NP - 1) tc::commit(B(VE + s));
         }
         __syncwarp();
       };
@@ -262,26 +263,26 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         wait(SB, c);
         if (!Cfg::kAlias && c > 0) wait(OE, c - 1);
         if (go()) {
-        const uint64_t dq = tc::desc_kmajor(base + Cfg::kOffQ + s * Cfg::kBytesQK, 0);
+          const uint64_t dq = tc::desc_kmajor(base + Cfg::kOffQ + s * Cfg::kBytesQK, 0);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          tc::mma_bf16_ts(tX, tSb + 8 * i, dq + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2, kIdX, i > 0);
-        tc::commit(B(XD));
-        tc::commit(B(QE + s));
+          for (int i = 0; i < D / 16; ++i)
+            tc::mma_bf16_ts(tX, tSb + 8 * i, dq + (i >> 2) * (Cfg::kPanel >> 4) + (i & 3) * 2, kIdX, i > 0);
+          tc::commit(B(XD));
+          tc::commit(B(QE + s));
         }
         __syncwarp();
         wait(BP, c);
         if (go()) {
-        const uint64_t dv = tc::desc_mnmajor(base + Cfg::kOffV + s * Cfg::kBytesV, Cfg::kPanel, 0);
-        const uint64_t dp = tc::desc_kmajor(base + Cfg::kOffP, 0);
-        // tokens 16 i .. 16 i + 15 are seen by the columns from 16 i on only: smaller products, and the blocks
-        // of P above the diagonal are never read
+          const uint64_t dv = tc::desc_mnmajor(base + Cfg::kOffV + s * Cfg::kBytesV, Cfg::kPanel, 0);
+          const uint64_t dp = tc::desc_kmajor(base + Cfg::kOffP, 0);
+          // tokens 16 i .. 16 i + 15 are seen by the columns from 16 i on only: smaller products, and the blocks
+          // of P above the diagonal are never read
 #pragma unroll
-        for (int i = 0; i < kTile / 16; ++i)
-          tc::mma_bf16(tY + 16 * i, dv + 128 * i, dp + 128 * i + 2 * i, tc::idesc(tc::kBF16, 128, kTile - 16 * i, true, false),
-                       i > 0);
-        tc::commit(B(XY));
-        tc::commit(B(VE + s));
+          for (int i = 0; i < kTile / 16; ++i)
+            tc::mma_bf16(tY + 16 * i, dv + 128 * i, dp + 128 * i + 2 * i,
+                         tc::idesc(tc::kBF16, 128, kTile - 16 * i, true, false), i > 0);
+          tc::commit(B(XY));
+          tc::commit(B(VE + s));
         }
         __syncwarp();
       };
@@ -406,7 +407,8 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
           // below 2^-37); e^total below 2^-900 is zero in fp32
           const double y = total * 1.4426950408889634;
           const double nr = rint(y), f = (y - nr) * 0.6931471805599453;
-          constexpr double kInvFact[9] = {1.0, 1.0, 1.0 / 2, 1.0 / 6, 1.0 / 24, 1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320};
+          constexpr double kInvFact[9] = {1.0,       1.0,       1.0 / 2,    1.0 / 6,    1.0 / 24,
+                                          1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320};
           double a = 1.0 / 362880;
 #pragma unroll
           for (int i = 8; i >= 0; --i) a = fma(a, f, kInvFact[i]);
@@ -444,11 +446,9 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
       }
       wait(TF + c % NT, c / NT);
       const DecayTable& t = tab[c % NT];
-      if (c > 0) {  // U has read the previous chunk's operand
-        wait(BU + NP - 1, c - 1);
-        __syncwarp();
-        tc::fence_after();
-      }
+      if (c > 0) wait(BU + NP - 1, c - 1);  // U has read the previous chunk's operand
+      __syncwarp();
+      tc::fence_after();
 #pragma unroll 1
       for (int e = 0; e < 2; ++e) {  // 16 values by 32 tokens
         const int val = (32 * quad + 16 * e) % Cfg::kVB + 8 * pval;
@@ -501,7 +501,8 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
 #pragma unroll 1
       for (int e = 0; e < 2; ++e) {
         uint32_t x[4 * kGroups], y[4 * kGroups];
-        tc::ld_frag2<kGroups>(tc::lane_addr(tX, 32 * quad + 16 * e, t0), tc::lane_addr(tY, 32 * quad + 16 * e, t0), x, y);
+        tc::ld_frag2<kGroups>(tc::lane_addr(tX, 32 * quad + 16 * e, t0), tc::lane_addr(tY, 32 * quad + 16 * e, t0), x,
+                              y);
         if (e == 1) {
           tc::fence_before();
           arrive(OE);
@@ -605,7 +606,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1) linear_tc_kernel(
         tc::fence_after();
         const float f0 = t.row[r0], f1 = t.row[r0 + 8];
 #pragma unroll 1
-        for (int J = half; J <= quad; J += 2) {  // 16 x 16 blocks up to the diagonal: decays, then bf16 into the operand
+        for (int J = half; J <= quad; J += 2) {  // 16 x 16 blocks up to the diagonal: decays, bf16 into the operand
           uint32_t x[8], z[4];  // x: columns 8 e + pair, + 1 of row r0, then of row r0 + 8, e = 0, 1
           tc::ld_frag<2>(tc::lane_addr(tSc, 32 * quad, 16 * J), x);
           if (J < quad) {

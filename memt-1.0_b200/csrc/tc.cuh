@@ -71,27 +71,6 @@ __device__ __forceinline__ void mma_bf16_ts(uint32_t d, uint32_t a, uint64_t b, 
       " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
       "r"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(acc)));
 }
-// The same for a whole converged warp, issued by the lane whose `lead` is set: no branch, so that
-// descriptors and addresses stay in uniform registers.
-__device__ __forceinline__ void mma_bf16_lead(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(acc)), "r"(lead));
-}
-__device__ __forceinline__ void mma_bf16_ts_lead(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
-  asm volatile(
-      "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
-      " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(id), "r"(static_cast<uint32_t>(acc)), "r"(lead));
-}
-__device__ __forceinline__ void commit_lead(uint32_t lead, uint32_t mbar) {
-  asm volatile(
-      "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
-      " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(mbar),
-      "r"(lead)
-      : "memory");
-}
 // arrive on the mbarrier once all previously issued MMAs of this thread have completed
 __device__ __forceinline__ void commit(uint32_t mbar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar)
@@ -159,9 +138,9 @@ __device__ __forceinline__ void ld8(uint32_t taddr, float (&v)[8]) {
 }
 template <int N>
 __device__ __forceinline__ void ldn(uint32_t taddr, float (&v)[N]) {
-  static_assert(N == 8 || N == 16, "columns");
+  static_assert(N == 8 || N == 32, "columns");
   if constexpr (N == 8) ld8(taddr, v);
-  else ld16(taddr, v);
+  else ld32(taddr, v);
 }
 
 // Fragment forms: 16 lanes from the address's lane, in the register layout of mma.sync fragments

@@ -105,9 +105,12 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, inverse=False, atten
     positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
     qo, sqo = _output(q, sq, q_out, "q_out")
     ko, sko = (None, 0) if k is None else _output(k, sk, k_out, "k_out")
-    if k is not None and ((q_out is not None and _overlap(qo, sqo, k, sk))
-                          or (k_out is not None and (_overlap(ko, sko, q, sq) or _overlap(qo, sqo, ko, sko)))):
-        raise ValueError("q_out and k_out must not overlap each other or the other input")
+    if k is not None and (q_out is not None or k_out is not None):
+        both = qo is q and ko is k  # in place: the outputs are the inputs
+        if (_overlap(qo, sqo, ko, sko)
+                or not both and (q_out is not None and _overlap(qo, sqo, k, sk)
+                                 or k_out is not None and _overlap(ko, sko, q, sq))):
+            raise ValueError("q_out and k_out must not overlap each other or the other input")
     if L == 0 or H == 0:
         return qo, ko
     args = _rotary_args(
@@ -122,6 +125,8 @@ def _output(x, stride, out, name):
     """A new tensor like x, or the given output's token rows (x itself, or rows apart from it)."""
     if out is None:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device), x.shape[1] * x.shape[2]
+    if out is x:
+        return x, stride
     o = _tokens_unchecked(out, name)
     L, H, D = x.shape
     if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device:
@@ -130,6 +135,6 @@ def _output(x, stride, out, name):
     if s[2] != 1 or (s[1] != D and H > 1) or (L > 1 and s[0] < H * D):
         raise ValueError(f"{name}: token rows must be contiguous heads")
     so = s[0] if L > 1 else H * D
-    if out is not x and not (o.data_ptr() == x.data_ptr() and so == stride) and _overlap(o, so, x, stride):
+    if not (o.data_ptr() == x.data_ptr() and so == stride) and _overlap(o, so, x, stride):
         raise ValueError(f"{name} must be the input itself or not overlap it")
     return o, so
