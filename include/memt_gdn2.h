@@ -380,8 +380,10 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  * final_state receives the last S (fp32). A sample without tokens keeps its initial state.
  *
  * dtype BF16: chunked on tensor cores. The fp32 state is kept exactly as the recurrence leaves it
- *   up to fp32 rounding (k is split into three bf16 terms); the output is made from bf16 scores
- *   and a bf16 copy of the state. dtype F32: exact fp32 token recurrence on CUDA cores.
+ *   up to fp32 rounding (the decayed v is split into three bf16 terms); the output is made from
+ *   bf16 scores and a bf16 copy of the state. In calls of up to 64 tokens a sample in the mean, samples
+ *   of at most 24 / 8 / 6 tokens (D = 64 / 128 / 256) go token by token in fp32 instead.
+ *   dtype F32: exact fp32 token recurrence on CUDA cores.
  * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] or
  * decreasing ones are clamped. The tensors are read as token rows of *_stride elements (a
  * multiple of 16 bytes), so split views of wider projections need no copy.

@@ -1,4 +1,6 @@
 // memt_linear_attention: argument checks and launch of the causal linear attention.
+#include <algorithm>
+
 #include "launch.h"
 #include "linear.cuh"
 #include "linear_tc.cuh"
@@ -9,21 +11,22 @@ using namespace memt;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int D>
-int launch_recurrent_form(const LinearParams& p, cudaStream_t s) {
-  constexpr int kBlocks = D / (LinearRecurrentCfg::kCols * LinearRecurrentCfg::kWarps);
-  const int64_t grid = int64_t(p.N) * p.H * kBlocks;
+template <int D, typename T>
+int launch_tokens(const LinearParams& p, cudaStream_t s) {
+  using Cfg = LinearTokensCfg<D>;
+  const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;
   if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   ProfScope prof(kProfLinear, s);
-  linear_recurrent_kernel<D><<<static_cast<unsigned>(grid), LinearRecurrentCfg::kWarps * 32, 0, s>>>(p);
+  linear_tokens_kernel<D, T><<<static_cast<unsigned>(grid), Cfg::kThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError());
 }
 
-int launch_recurrent_form(int D, const LinearParams& p, cudaStream_t s) {
+template <typename T>
+int launch_tokens(int D, const LinearParams& p, cudaStream_t s) {
   switch (D) {
-    case 64: return launch_recurrent_form<64>(p, s);
-    case 128: return launch_recurrent_form<128>(p, s);
-    default: return launch_recurrent_form<256>(p, s);
+    case 64: return launch_tokens<64, T>(p, s);
+    case 128: return launch_tokens<128, T>(p, s);
+    default: return launch_tokens<256, T>(p, s);
   }
 }
 
@@ -80,7 +83,13 @@ int launch_chunked(const LinearParams& p, void* workspace, cudaStream_t s) {
     // 0 to 16384 tokens, 16 heads, d = 128: 617 us in order of the samples, 594 by length). Every CTA ranks
     // the samples for itself, which short or many samples would not repay.
     P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms && p.L / p.N >= 1024;
-    return launch_pass<D, true>(P, p.N, s);
+    // With the short samples left to the other kernel, at most L / (few + 1) are longer. Where that is up to half
+    // of them, so many CTAs a head look for one each; otherwise every sample has its CTAs, and those of short ones
+    // end at once. 256 samples, 16 heads, D = 64: empty CTAs for all 31 us; CTAs that look and find none 7 us for
+    // 10 samples, 36 us for 122, 70 us for 248.
+    const int64_t most = p.few < 0 ? p.N : p.L / (p.few + 1);
+    P.p.only_long = most <= p.N / 2;
+    return launch_pass<D, true>(P, P.p.only_long ? std::max<int64_t>(most, 1) : p.N, s);
   }
   const int64_t units = max_segments(p.N, p.L, seg_chunks);
   P.p.seg_chunks = seg_chunks;
@@ -107,6 +116,12 @@ int launch_chunked(int D, const LinearParams& p, void* workspace, cudaStream_t s
     default: return launch_chunked<256>(p, workspace, s);
   }
 }
+
+// Tokens up to which a bf16 sample runs token by token. Measured, the token kernel alone against chunks alone,
+// 16 heads, us: 256 samples at D = 64: 1 token 24 / 149, 16 74 / 154, 24 104 / 152, 32 134 / 152; D = 128: 1 token
+// 83 / 201, 8 138 / 201, 12 182 / 203; 64 samples at D = 256: 1 token 96 / 168, 6 137 / 169, 8 156 / 170. The
+// chunks' launch that finds no sample costs up to 36 us more (D = 256, 64 samples: 19).
+int few_tokens(int D) { return D == 64 ? 24 : (D == 128 ? 8 : 6); }
 
 int check_linear(const memt_linear_attention_args* a) {
   if (a == nullptr || a->struct_size != sizeof(memt_linear_attention_args)) return MEMT_ERR_INVALID_ARGUMENT;
@@ -183,8 +198,20 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   p.slots_out = a->final_slots;
   p.num_out = a->num_final_slots;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // without tokens the states are only copied
-  if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_recurrent_form(a->head_dim, p, s);
+  // fp32, and calls without tokens, which only copy the states: all samples token by token
+  p.few = INT32_MAX;
+  if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_tokens<float>(a->head_dim, p, s);
+  // Up to 64 tokens a sample in the mean, both kernels run, each for its samples by their own lengths; where no
+  // sample is short, the idle launch costs 4 to 11 us of 136 to 206. Above, all samples run in chunks: a short
+  // sample's result may then differ in its last bits.
+  const int few = few_tokens(a->head_dim);
+  if (a->total_tokens <= few) return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+  p.few = -1;
+  if (a->num_samples > 1 && a->total_tokens <= int64_t(64) * a->num_samples) {
+    p.few = few;
+    const int st_few = launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+    if (st_few != MEMT_OK) return st_few;
+  }
   return launch_chunked(a->head_dim, p, workspace, s);
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;

@@ -3,13 +3,17 @@
 //
 //     S_t = e^{g_t} S_{t-1} + k_t v_t^T,    o_t = scale S_t^T q_t
 //
-// The token-by-token kernel is the definition in fp32 on CUDA cores. It serves fp32 inputs (as
-// the fp32 mode of the update does) and is bound by the latency of the token chain.
-// One warp owns kCols value columns of one (sample, head): the state's D rows are spread over the
-// lanes (D / 32 rows each), so a token costs D / 32 * kCols * 2 multiply-adds a lane and one
-// butterfly sum over the lanes, without any barrier between warps. The next token's vectors are
-// fetched while this one is folded in.
+// The token-by-token kernel is the definition in fp32 on CUDA cores. It serves fp32 inputs (as the
+// fp32 mode of the update does) and bf16 samples of few tokens, where the states are most of the
+// traffic and a 64-token chunk is mostly padding. The state is in registers as in the single-token
+// step (16-byte vectors of whole rows, 64 value columns a CTA); tokens come in batches of four, whose
+// vectors are fetched a batch ahead and whose outputs share one barrier. One token costs the states'
+// traffic (256 samples, 16 heads, D = 128: 83 us, the floor 83); each one more from 5 us to 11, the work
+// of folding it in. fp32 prompts (8 x 8192 tokens, 16 heads, D = 128): 4.4 ms, with four columns a warp and all
+// lanes on the rows 8.4.
 #pragma once
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "step.cuh"
@@ -33,11 +37,14 @@ struct LinearParams {
   const int32_t* slots_in;
   const int32_t* slots_out;
   int32_t num_in, num_out;
+  // Samples of up to `few` tokens go token by token, longer ones in chunks (fp32: all and none).
+  int32_t few;
   // Chunked form of few long samples: 0, or 64-token chunks per segment, and the segments' states
   // [segment][H][D][D] (first their own sums, then the state before each) and decays [segment][H].
   int32_t seg_chunks;
   int32_t max_segments;
-  int32_t by_length;  // whole samples, the longest first
+  int32_t by_length;   // whole samples, the longest first
+  int32_t only_long;   // fewer CTAs than samples: each finds one of more than `few` tokens
   float* seg_states;
   float2* seg_decays;
 };
@@ -110,6 +117,23 @@ __device__ __forceinline__ int sample_by_length(const LinearParams& p, int rank)
   return found;
 }
 
+// The unit-th sample of more than p.few tokens, found by a converged warp; -1 when there are fewer.
+__device__ __forceinline__ int find_long(const LinearParams& p, int unit) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    int64_t bos = 0, eos = 0;
+    const bool own = n0 + lane < p.N;
+    if (own) sample_range(p, n0 + lane, bos, eos);
+    const uint32_t longer = __ballot_sync(~0u, own && eos - bos > p.few);
+    const int rank = before + __popc(longer & ((1u << lane) - 1));
+    const uint32_t hit = __ballot_sync(~0u, rank == unit && (longer >> lane & 1));
+    if (hit != 0) return n0 + __ffs(hit) - 1;
+    before += __popc(longer);
+  }
+  return -1;
+}
+
 __device__ __forceinline__ float log_decay(const LinearParams& p, int64_t t, int h) {
   return p.g_layout == 1 ? p.g[t * p.H + h] : (p.g_layout == 3 ? p.g[h] : 0.f);
 }
@@ -164,70 +188,171 @@ __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearParams
   }
 }
 
-struct LinearRecurrentCfg {
-  static constexpr int kCols = 4;   // value columns per warp
-  static constexpr int kWarps = 4;  // warps per CTA, consecutive column groups
+// Token-by-token form: fp32 inputs, and bf16 samples of few tokens.
+template <int D>
+struct LinearTokensCfg {
+  static constexpr int kCols = 64, kBlocks = D / kCols;  // value columns per CTA, CTAs per (sample, head)
+  static constexpr int kRows = D == 64 ? 4 : 8;          // state rows per thread, 8 columns of each
+  static constexpr int kWarps = D / (4 * kRows);         // four row groups of eight lanes a warp
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kBatch = 4;                       // tokens between two barriers
+  static constexpr int kPer = (D + kThreads - 1) / kThreads;
+  static constexpr int kMinCtas = D == 256 ? 2 : (D == 128 ? 4 : 6);
 };
 
-template <int D>
-__global__ void __launch_bounds__(LinearRecurrentCfg::kWarps * 32) linear_recurrent_kernel(const LinearParams p) {
-  constexpr int C = LinearRecurrentCfg::kCols, W = LinearRecurrentCfg::kWarps, R = D / 32;
-  constexpr int kBlocks = D / (C * W);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int blk = blockIdx.x % kBlocks, nh = blockIdx.x / kBlocks;
+template <int D, typename T>
+__global__ void __launch_bounds__(LinearTokensCfg<D>::kThreads, LinearTokensCfg<D>::kMinCtas)
+    linear_tokens_kernel(const LinearParams p) {
+  using Cfg = LinearTokensCfg<D>;
+  constexpr int R = Cfg::kRows, W = Cfg::kWarps, TB = Cfg::kBatch, NT = Cfg::kThreads, C = Cfg::kCols, NP = Cfg::kPer;
+  __shared__ __align__(16) float s_k[2][TB][D], s_q[2][TB][D], s_v[2][TB][C];
+  __shared__ float s_a[2][TB];
+  __shared__ __align__(16) float s_o[2][W][TB][C];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int blk = blockIdx.x % Cfg::kBlocks, nh = blockIdx.x / Cfg::kBlocks;
   const int h = nh % p.H, n = nh / p.H, hk = h / (p.H / p.Hk);
-  const int col = (blk * W + warp) * C, row = lane * R;
+  // rows row0 + i, columns col .. col + 3 and col + 32 .. col + 35: a warp's load covers four rows' 128-byte
+  // lines, and a token costs two reads of shared memory for each of k, q and v
+  const int row0 = (4 * warp + (lane >> 3)) * R, col = 4 * (lane & 7);
   int64_t bos, eos;
   sample_range(p, n, bos, eos);
+  if (eos - bos > p.few) return;
   const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
-  float S[R][C];
-#pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int e = 0; e < C; ++e)
-      S[i][e] = p.h0 != nullptr && in_slot >= 0 ? p.h0[((in_slot * p.H + h) * D + row + i) * D + col + e] : 0.f;
-  float q[R], k[R], v[C], g = 0.f;
-  auto fetch = [&](int64_t t) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      q[i] = load_f32<float>(p.q, t * p.sq + (int64_t)hk * D + row + i);
-      k[i] = load_f32<float>(p.k, t * p.sk + (int64_t)hk * D + row + i);
-    }
-#pragma unroll
-    for (int e = 0; e < C; ++e) v[e] = load_f32<float>(p.v, t * p.sv + (int64_t)h * D + col + e);
-    g = log_decay(p, t, h);
-  };
-  if (bos < eos) fetch(bos);
-  // A decay that is the same for every token is a pair of fp32 numbers: the rounding of one, repeated
-  // for every token, would drift (7e-6 over 16384 tokens).
-  const double fixed = p.g_layout == 3 ? exp(static_cast<double>(p.g[h])) : 1.0;
-  const float fixed_hi = static_cast<float>(fixed), fixed_lo = static_cast<float>(fixed - fixed_hi);
-  for (int64_t t = bos; t < eos; ++t) {
-    float o[C] = {0.f, 0.f, 0.f, 0.f};
-    const float a = p.g_layout == 1 ? expf(g) : fixed_hi, a_lo = p.g_layout == 1 ? 0.f : fixed_lo;
+  const int64_t at = (int64_t)row0 * D + blk * C + col;
+  uint64_t S[R][4];  // fp32 pairs
+  if (p.h0 != nullptr && in_slot >= 0) {
+    const float* src = p.h0 + (in_slot * p.H + h) * D * D + at;
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int e = 0; e < C; ++e) {
-        S[i][e] = fmaf(a, S[i][e], fmaf(a_lo, S[i][e], k[i] * v[e]));
-        o[e] = fmaf(S[i][e], q[i], o[e]);
+      for (int e = 0; e < 2; ++e) {
+        const float4 x = __ldcs(reinterpret_cast<const float4*>(src + i * D + 32 * e));
+        S[i][2 * e] = f32x2_pack(x.x, x.y);
+        S[i][2 * e + 1] = f32x2_pack(x.z, x.w);
       }
-    if (t + 1 < eos) fetch(t + 1);
+  } else {
 #pragma unroll
-    for (int e = 0; e < C; ++e)
+    for (int i = 0; i < R; ++i) S[i][0] = S[i][1] = S[i][2] = S[i][3] = 0;
+  }
+  // A decay that is the same for every token is a pair of fp32 numbers: the rounding of one, repeated
+  // for every token, would drift (7e-6 over 16384 tokens).
+  const double fixed = p.g_layout == 3 ? exp(static_cast<double>(p.g[h])) : 1.0;
+  const float fixed_hi = static_cast<float>(fixed);
+  const uint64_t a_lo = f32x2_splat(p.g_layout == 3 ? static_cast<float>(fixed - fixed_hi) : 0.f);
+
+  // the next batch's vectors, as loaded: nothing waits for them before keep()
+  T xk[TB][NP], xq[TB][NP], xv[TB];
+  float xg = 0.f;
+  auto fetch = [&](int64_t t0) {
 #pragma unroll
-      for (int m = 16; m > 0; m >>= 1) o[e] += __shfl_xor_sync(0xffffffffu, o[e], m);
-    if (lane < C) {
-      const float x = lane == 0 ? o[0] : lane == 1 ? o[1] : lane == 2 ? o[2] : o[3];
-      store_f32(static_cast<float*>(p.out), t * p.so + (int64_t)h * D + col + lane, p.scale * x);
+    for (int t = 0; t < TB; ++t) {
+      const bool live = t0 + t < eos;
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int c = tid + i * NT;
+        xk[t][i] = xq[t][i] = T(0.f);
+        if (live && c < D) {
+          xk[t][i] = static_cast<const T*>(p.k)[(t0 + t) * p.sk + (int64_t)hk * D + c];
+          xq[t][i] = static_cast<const T*>(p.q)[(t0 + t) * p.sq + (int64_t)hk * D + c];
+        }
+      }
+      xv[t] = T(0.f);
+      if (live && tid < C) xv[t] = static_cast<const T*>(p.v)[(t0 + t) * p.sv + (int64_t)h * D + blk * C + tid];
+    }
+    xg = 0.f;
+    if (p.g_layout == 1 && tid < TB && t0 + tid < eos) xg = p.g[(t0 + tid) * p.H + h];
+  };
+  auto keep = [&](int buf) {
+#pragma unroll
+    for (int t = 0; t < TB; ++t) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const int c = tid + i * NT;
+        if (c < D) {
+          s_k[buf][t][c] = as_f32(xk[t][i]);
+          s_q[buf][t][c] = as_f32(xq[t][i]);
+        }
+      }
+      if (tid < C) s_v[buf][t][tid] = as_f32(xv[t]);
+    }
+    if (tid < TB) s_a[buf][tid] = p.g_layout == 1 ? expf(xg) : fixed_hi;
+  };
+  auto fold = [&](int buf, int t, uint64_t (&o)[4], auto pair) {  // one token into the state, its partial output
+    uint64_t v[4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float4 x = *reinterpret_cast<const float4*>(&s_v[buf][t][col + 32 * e]);
+      v[2 * e] = f32x2_pack(x.x, x.y);
+      v[2 * e + 1] = f32x2_pack(x.z, x.w);
+    }
+    const uint64_t a = f32x2_splat(s_a[buf][t]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = 0;
+#pragma unroll
+    for (int i0 = 0; i0 < R; i0 += 4) {
+      const float4 k4 = *reinterpret_cast<const float4*>(&s_k[buf][t][row0 + i0]);
+      const float4 q4 = *reinterpret_cast<const float4*>(&s_q[buf][t][row0 + i0]);
+      const float ks[4] = {k4.x, k4.y, k4.z, k4.w}, qs[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t k = f32x2_splat(ks[j]), q = f32x2_splat(qs[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint64_t x = mul_f32x2(k, v[e]);
+          if constexpr (decltype(pair)::value) x = fma_f32x2(a_lo, S[i0 + j][e], x);
+          S[i0 + j][e] = fma_f32x2(a, S[i0 + j][e], x);
+          o[e] = fma_f32x2(S[i0 + j][e], q, o[e]);
+        }
+      }
+    }
+  };
+  fetch(bos);
+  keep(0);
+  __syncthreads();
+  int b = 0;
+  for (int64_t t0 = bos; t0 < eos; t0 += TB, b ^= 1) {
+    fetch(t0 + TB);
+#pragma unroll 1
+    for (int t = 0; t < TB; ++t) {
+      if (t0 + t >= eos) break;
+      uint64_t o[4];
+      if (p.g_layout == 3) fold(b, t, o, std::true_type{});
+      else fold(b, t, o, std::false_type{});
+      // sums over the warp's four row groups: each exchange halves the columns a lane is left with
+      const bool hi = lane & 8, hi2 = lane & 16;
+      float z[4];  // columns of half `hi`
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint64_t mine = hi ? o[2 + e] : o[e], give = hi ? o[e] : o[2 + e];
+        z[2 * e] = f32x2_lo(mine) + __shfl_xor_sync(0xffffffffu, f32x2_lo(give), 8);
+        z[2 * e + 1] = f32x2_hi(mine) + __shfl_xor_sync(0xffffffffu, f32x2_hi(give), 8);
+      }
+      float2 y;  // columns 2 hi2, 2 hi2 + 1 of those
+      y.x = (hi2 ? z[2] : z[0]) + __shfl_xor_sync(0xffffffffu, hi2 ? z[0] : z[2], 16);
+      y.y = (hi2 ? z[3] : z[1]) + __shfl_xor_sync(0xffffffffu, hi2 ? z[1] : z[3], 16);
+      *reinterpret_cast<float2*>(&s_o[b][warp][t][col + (hi ? 32 : 0) + (hi2 ? 2 : 0)]) = y;
+    }
+    keep(b ^ 1);
+    __syncthreads();
+    for (int i = tid; i < TB * C; i += NT) {
+      const int t = i / C, c = i % C;
+      if (t0 + t >= eos) break;
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += s_o[b][w][t][c];
+      store_f32(static_cast<T*>(p.out), (t0 + t) * p.so + (int64_t)h * D + blk * C + c, p.scale * sum);
     }
   }
   const bool taken = __any_sync(0xffffffffu, slot_taken(p.slots_out, n, out_slot, lane, 32));
   if (out_slot < 0 || taken) return;
+  float* dst = p.ht + (out_slot * p.H + h) * D * D + at;
 #pragma unroll
   for (int i = 0; i < R; ++i)
 #pragma unroll
-    for (int e = 0; e < C; ++e) p.ht[((out_slot * p.H + h) * D + row + i) * D + col + e] = S[i][e];
+    for (int e = 0; e < 2; ++e)
+      __stcs(reinterpret_cast<float4*>(dst + i * D + 32 * e),
+             make_float4(f32x2_lo(S[i][2 * e]), f32x2_hi(S[i][2 * e]), f32x2_lo(S[i][2 * e + 1]),
+                         f32x2_hi(S[i][2 * e + 1])));
 }
 
 }  // namespace memt

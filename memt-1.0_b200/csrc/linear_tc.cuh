@@ -154,8 +154,18 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
   if (p.seg_chunks > 0) {
     if (!find_segment(p, unit, n, seg, segs)) return;
     if (!OUT && seg + 1 == segs) return;  // the first pass sums what later segments start from
+  } else if (p.only_long) {
+    n = find_long(p, unit);
+    if (n < 0) return;
   } else if (p.by_length) {
     n = sample_by_length(p, unit);
+  }
+  int64_t bos, eos;
+  sample_range(p, n, bos, eos);
+  if (eos - bos <= p.few) return;  // the token-by-token kernel's
+  if (segs > 1) {
+    bos += (int64_t)seg * p.seg_chunks * kTile;
+    if (eos > bos + (int64_t)p.seg_chunks * kTile) eos = bos + (int64_t)p.seg_chunks * kTile;
   }
 
   // barriers: Q, K, V tiles landed (QF, KF, VF) and free again (QE, KE, VE); decay table written /
@@ -189,12 +199,6 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
                  tX = tmem + Cfg::kColX, tY = tmem + Cfg::kColY, tSc = tmem + Cfg::kColSc;
   DecayTable* tab = reinterpret_cast<DecayTable*>(sm + Cfg::kOffTab);
 
-  int64_t bos, eos;
-  sample_range(p, n, bos, eos);
-  if (segs > 1) {
-    bos += (int64_t)seg * p.seg_chunks * kTile;
-    if (eos > bos + (int64_t)p.seg_chunks * kTile) eos = bos + (int64_t)p.seg_chunks * kTile;
-  }
   const int64_t seg_state = ((int64_t)unit * p.H + h) * D * D;  // of seg_states
   const int nchunks = static_cast<int>((eos - bos + kTile - 1) / kTile);
   auto chunk_len = [&](int c) {

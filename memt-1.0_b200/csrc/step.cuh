@@ -40,15 +40,11 @@ struct StepParams {
   void* out;
 };
 
+__device__ __forceinline__ float as_f32(float x) { return x; }
+__device__ __forceinline__ float as_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <typename T>
-__device__ __forceinline__ float load_f32(const void* base, int64_t i);
-template <>
-__device__ __forceinline__ float load_f32<float>(const void* base, int64_t i) {
-  return static_cast<const float*>(base)[i];
-}
-template <>
-__device__ __forceinline__ float load_f32<__nv_bfloat16>(const void* base, int64_t i) {
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[i]);
+__device__ __forceinline__ float load_f32(const void* base, int64_t i) {
+  return as_f32(static_cast<const T*>(base)[i]);
 }
 __device__ __forceinline__ void store_f32(float* base, int64_t i, float x) { base[i] = x; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16* base, int64_t i, float x) { base[i] = __float2bfloat16_rn(x); }

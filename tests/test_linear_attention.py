@@ -196,10 +196,34 @@ def _run_and_check(lengths, Hk, H, D, dtype, decay, seed=0, gscale=1.0):
 
 @gpu
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("lengths", [[1], [63], [64], [65], [128, 1, 0, 200], [0, 3, 130]])
+@pytest.mark.parametrize("lengths", [[1], [8], [13], [33], [63], [64], [65], [128, 1, 0, 200], [0, 3, 130],
+                                     [5, 0, 40, 12, 1, 9, 33, 2], [1] * 70 + [40, 0, 30] + [2] * 5])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_linear_attention_lengths(cuda, D, lengths, dtype):
     _run_and_check(lengths, 2, 2, D, dtype, "token", seed=D + len(lengths))
+
+
+@gpu
+@pytest.mark.parametrize("decay", ["token", "head", "none"])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_tokens_beside_prompts(cuda, D, decay):
+    """Short samples and prompts in one call, with shared key heads, in place in a pool: both kernels
+    write their own samples' slots and rows, and nothing else."""
+    lengths, Hk, H = [1, 4, 0, 5, 90, 2, 1, 33, 6, 3], 2, 4
+    q, k, v, g, h0, cu = _inputs(3, lengths, Hk, H, D, torch.bfloat16, decay)
+    at, others = torch.tensor([7, 2, 11, 0, 5, 9, 3, 1, 10, 4]), torch.tensor([6, 8])
+    ref = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    pool = torch.full((12, H, D, D), 3.0)
+    pool[at] = h0
+    dq, dk, dv, dg, dpool, dcu, slots = _dev(q, k, v, g, pool, cu, at.int())
+    out = torch.full((q.shape[0] + 2, H, D), 5.0, dtype=torch.bfloat16, device="cuda")
+    M.linear_attention(dq, dk, dv, dg, dpool, dcu, out=out[1:-1], final_state=dpool, initial_slots=slots,
+                       final_slots=slots)
+    torch.cuda.synchronize()
+    to, ts = _tolerances(ref, lengths, D, torch.bfloat16, g, H)
+    _check(out[1:-1], ref[0], to, "output")
+    _check(dpool[at.cuda()], ref[1], ts, "state")
+    assert bool((out[0] == 5).all()) and bool((out[-1] == 5).all()) and bool((dpool[others.cuda()] == 3).all())
 
 
 @gpu
@@ -385,10 +409,14 @@ def test_pools_and_rows_beyond_32_bits(cuda):
 
 
 @gpu
-def test_samples_are_independent_of_the_pack(cuda):
-    """A sample's result does not depend on what it is packed with, bit for bit."""
-    lengths = [130, 64, 300]
-    q, k, v, g, h0, cu = _dev(*_inputs(10, lengths, 2, 2, 128, torch.bfloat16, "token"))
+@pytest.mark.parametrize("D,lengths", [(128, [130, 64, 300]), (64, [3, 70, 0, 32, 33, 1]), (128, [12, 90, 13, 1, 2]),
+                                       (256, [8, 9, 100, 1, 30]), (64, [1] * 70 + [40, 0, 30, 2]),
+                                       (256, [1] * 70 + [40, 0, 30, 2])])
+def test_samples_are_independent_of_the_pack(cuda, D, lengths):
+    """A sample's result does not depend on what it is packed with, bit for bit, while the mean length
+    is at most 64 tokens (short samples run token by token, longer ones in chunks, each by its own
+    length) or no sample is short."""
+    q, k, v, g, h0, cu = _dev(*_inputs(10, lengths, 2, 2, D, torch.bfloat16, "token"))
     o, final = M.linear_attention(q, k, v, g, h0, cu)
     at = 0
     for n, T in enumerate(lengths):
