@@ -384,8 +384,9 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  *   bf16 scores and a bf16 copy of the state. In calls of up to 64 tokens a sample in the mean, samples
  *   of at most 24 / 8 / 6 tokens (D = 64 / 128 / 256) go token by token in fp32 instead.
  *   dtype F32: exact fp32 token recurrence on CUDA cores.
- * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] or
- * decreasing ones are clamped. The tensors are read as token rows of *_stride elements (a
+ * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] are clamped
+ * to it, and a sample whose end lies before its start is empty. Of samples that share rows each ends in
+ * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token rows of *_stride elements (a
  * multiple of 16 bytes), so split views of wider projections need no copy.
  */
 typedef struct memt_linear_attention_args {

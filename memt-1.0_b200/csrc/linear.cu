@@ -83,13 +83,7 @@ int launch_chunked(const LinearParams& p, void* workspace, cudaStream_t s) {
     // 0 to 16384 tokens, 16 heads, d = 128: 617 us in order of the samples, 594 by length). Every CTA ranks
     // the samples for itself, which short or many samples would not repay.
     P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms && p.L / p.N >= 1024;
-    // With the short samples left to the other kernel, at most L / (few + 1) are longer. Where that is up to half
-    // of them, so many CTAs a head look for one each; otherwise every sample has its CTAs, and those of short ones
-    // end at once. 256 samples, 16 heads, D = 64: empty CTAs for all 31 us; CTAs that look and find none 7 us for
-    // 10 samples, 36 us for 122, 70 us for 248.
-    const int64_t most = p.few < 0 ? p.N : p.L / (p.few + 1);
-    P.p.only_long = most <= p.N / 2;
-    return launch_pass<D, true>(P, P.p.only_long ? std::max<int64_t>(most, 1) : p.N, s);
+    return launch_pass<D, true>(P, p.only_long > 0 ? p.only_long : p.N, s);
   }
   const int64_t units = max_segments(p.N, p.L, seg_chunks);
   P.p.seg_chunks = seg_chunks;
@@ -209,6 +203,12 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   p.few = -1;
   if (a->num_samples > 1 && a->total_tokens <= int64_t(64) * a->num_samples) {
     p.few = few;
+    // No more than L / (few + 1) samples are longer. Where that is up to half of them, so many CTAs a head look for
+    // one each; otherwise every sample has its CTAs, and those of short ones end at once. 256 samples, 16 heads,
+    // D = 64: empty CTAs for all 31 us; CTAs that look and find none 7 us for 10 samples, 36 us for 122, 70 us
+    // for 248.
+    const int64_t most = p.L / (few + 1);
+    p.only_long = most <= p.N / 2 ? static_cast<int32_t>(most) : 0;
     const int st_few = launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
     if (st_few != MEMT_OK) return st_few;
   }

@@ -44,7 +44,7 @@ struct LinearParams {
   int32_t seg_chunks;
   int32_t max_segments;
   int32_t by_length;   // whole samples, the longest first
-  int32_t only_long;   // fewer CTAs than samples: each finds one of more than `few` tokens
+  int32_t only_long;   // 0, or the CTAs a head where each finds one of the samples of more than `few` tokens
   float* seg_states;
   float2* seg_decays;
 };
@@ -61,6 +61,14 @@ __device__ __forceinline__ void sample_range(const LinearParams& p, int n, int64
 __device__ __forceinline__ int segments_of(const LinearParams& p, int64_t tokens) {
   const int64_t run = (int64_t)p.seg_chunks * kTile;
   return tokens > run ? static_cast<int>((tokens + run - 1) / run) : 1;
+}
+
+// Segments of samples 0 .. n, of the `sum` that their lengths make: bounded such that the call's fit into
+// max_segments with at least one for each sample. Only offsets that overlap reach the bound; the last
+// segment of a sample then runs to its end.
+__device__ __forceinline__ int segments_up_to(const LinearParams& p, int n, int sum) {
+  const int room = p.max_segments - (p.N - 1 - n);
+  return sum < room ? sum : room;
 }
 
 // Sample n, segment s of its `count`, of the call's segment number `unit` (samples in order), found by
@@ -81,12 +89,15 @@ __device__ __forceinline__ bool find_segment(const LinearParams& p, int unit, in
       const int x = __shfl_up_sync(~0u, incl, o);
       if (lane >= o) incl += x;
     }
-    const uint32_t past = __ballot_sync(~0u, base + incl > unit);
+    const int last = segments_up_to(p, n0 + lane, base + incl);
+    const int first = n0 + lane == 0 ? 0 : segments_up_to(p, n0 + lane - 1, base + incl - own);
+    const uint32_t past = __ballot_sync(~0u, n0 + lane < p.N && last > unit);
     if (past != 0) {
       const int l = __ffs(past) - 1;
       n = n0 + l;
-      count = __shfl_sync(~0u, own, l);
-      s = unit - (base + __shfl_sync(~0u, incl, l) - count);
+      const int at = __shfl_sync(~0u, first, l);
+      count = __shfl_sync(~0u, last, l) - at;
+      s = unit - at;
       return true;
     }
     base += __shfl_sync(~0u, incl, 31);
@@ -134,6 +145,19 @@ __device__ __forceinline__ int find_long(const LinearParams& p, int unit) {
   return -1;
 }
 
+// Samples before n of more than p.few tokens, counted by a converged warp: offsets that overlap can make
+// more of them than there are CTAs to find them, and the token-by-token kernel takes the rest.
+__device__ __forceinline__ int long_before(const LinearParams& p, int n) {
+  int count = 0;
+  for (int n0 = 0; n0 < n; n0 += 32) {
+    const int m = n0 + (threadIdx.x & 31);
+    int64_t bos = 0, eos = 0;
+    if (m < n) sample_range(p, m, bos, eos);
+    count += __popc(__ballot_sync(~0u, m < n && eos - bos > p.few));
+  }
+  return count;
+}
+
 __device__ __forceinline__ float log_decay(const LinearParams& p, int64_t t, int h) {
   return p.g_layout == 1 ? p.g[t * p.H + h] : (p.g_layout == 3 ? p.g[h] : 0.f);
 }
@@ -163,15 +187,16 @@ __global__ void __launch_bounds__(256) linear_segments_kernel(const LinearParams
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
     sample_range(p, n, bos, eos);
-    count = segments_of(p, eos - bos);
+    count = segments_up_to(p, n, first + segments_of(p, eos - bos));
+    first = n == 0 ? 0 : segments_up_to(p, n - 1, first);
+    count -= first;
   }
   if (count == 1 || at >= per_state) return;  // one segment starts from the sample's own state
   const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n);
   float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
   if (p.h0 != nullptr && in_slot >= 0)
     S = reinterpret_cast<const float4*>(p.h0 + (in_slot * p.H + h) * D * D)[at];
-  // (offsets that overlap, which no packed batch has, could make more segments than there is room for)
-  for (int s = 0; s < count && first + s < p.max_segments; ++s) {
+  for (int s = 0; s < count; ++s) {
     const int64_t seg = (int64_t)(first + s) * p.H + h;
     float4* state = reinterpret_cast<float4*>(p.seg_states + seg * D * D) + at;
     float4 own = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -216,7 +241,7 @@ __global__ void __launch_bounds__(LinearTokensCfg<D>::kThreads, LinearTokensCfg<
   const int row0 = (4 * warp + (lane >> 3)) * R, col = 4 * (lane & 7);
   int64_t bos, eos;
   sample_range(p, n, bos, eos);
-  if (eos - bos > p.few) return;
+  if (eos - bos > p.few && (p.only_long == 0 || long_before(p, n) < p.only_long)) return;  // goes in chunks
   const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
   const int64_t at = (int64_t)row0 * D + blk * C + col;
   uint64_t S[R][4];  // fp32 pairs

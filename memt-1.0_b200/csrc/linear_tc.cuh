@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
   if (eos - bos <= p.few) return;  // the token-by-token kernel's
   if (segs > 1) {
     bos += (int64_t)seg * p.seg_chunks * kTile;
-    if (eos > bos + (int64_t)p.seg_chunks * kTile) eos = bos + (int64_t)p.seg_chunks * kTile;
+    if (seg + 1 < segs) eos = bos + (int64_t)p.seg_chunks * kTile;
   }
 
   // barriers: Q, K, V tiles landed (QF, KF, VF) and free again (QE, KE, VE); decay table written /

@@ -442,6 +442,28 @@ def test_bad_offsets_are_clamped(cuda):
 
 
 @gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("cu,L", [([0, 100] * 12, 100), ([0, 90, 40, 60, 60, 61] * 5, 90),   # chunks beside tokens
+                                  ([0, 5010, 0, 5010], 5010), ([0, 4000, 1, 3000, 0, 9], 4000)])  # segments
+def test_overlapping_samples_are_whole(cuda, D, cu, L):
+    """Samples whose offsets overlap add up to more tokens than there are; each still ends in the state
+    of its own tokens (rows of the output that two of them share belong to either)."""
+    q, k, v, g, _, _ = _inputs(17, [L], 1, 1, D, torch.bfloat16, "token")
+    h0 = 0.5 * torch.randn(len(cu) - 1, 1, D, D, generator=torch.Generator().manual_seed(2))
+    ranges = [(a, max(a, b)) for a, b in zip(cu[:-1], cu[1:])]
+    refs = []
+    for n, (a, b) in enumerate(ranges):
+        ref = _recurrence(q[a:b], k[a:b], v[a:b], g[a:b], h0[n:n + 1], torch.tensor([0, b - a]), 1.0)
+        refs.append((ref, _tolerances(ref, [max(b - a, 1)], D, torch.bfloat16, g, 1)[1]))
+    dq, dk, dv, dg, dh = _dev(q, k, v, g, h0)
+    final = torch.full_like(dh, float("nan"))
+    M.linear_attention(dq, dk, dv, dg, dh, torch.tensor(cu, dtype=torch.int32, device="cuda"), final_state=final)
+    torch.cuda.synchronize()
+    for n, (ref, tol) in enumerate(refs):
+        _check(final[n:n + 1], ref[1], tol, f"state {n}")
+
+
+@gpu
 def test_linear_attention_refuses_arguments(cuda):
     q, k, v, g, h0, cu = _dev(*_inputs(12, [20, 12], 2, 2, 64, torch.bfloat16, "token"))
     f = M.linear_attention
