@@ -386,8 +386,8 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  *   dtype F32: exact fp32 token recurrence on CUDA cores.
  * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] are clamped
  * to it, and a sample whose end lies before its start is empty. Of samples that share rows each ends in
- * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token rows of *_stride elements (a
- * multiple of 16 bytes), so split views of wider projections need no copy.
+ * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token
+ * rows of *_stride elements (a multiple of 16 bytes), so split views of wider projections need no copy.
  */
 typedef struct memt_linear_attention_args {
   uint32_t struct_size;    /* sizeof(memt_linear_attention_args)                */

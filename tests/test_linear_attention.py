@@ -227,6 +227,36 @@ def test_few_tokens_beside_prompts(cuda, D, decay):
 
 
 @gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_graph_replays_with_other_lengths(cuda, D):
+    """A captured call replayed with other offsets and tokens: short samples turn long and back."""
+    N, H, L = 40, 2, 200
+    packs = ([5] * N, [1] * 38 + [100, 62], [0] * 39 + [L], [L - 39] + [1] * 39, [0, 25, 9, 7] * 4 + [1] * 24)
+    q, k, v, g, h0, cu = _dev(*_inputs(23, packs[0], H, H, D, torch.bfloat16, "token"))
+    o, final = torch.zeros_like(v), torch.zeros_like(h0)
+    run = lambda: M.linear_attention(q, k, v, g, h0, cu, out=o, final_state=final)  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed, lengths in enumerate(packs):
+        new = _inputs(seed, [L], H, H, D, torch.bfloat16, "token")
+        for x, y in zip((q, k, v, g), new):
+            x.copy_(y)
+        cu.copy_(torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32))
+        o.fill_(3.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = _recurrence(*new[:4], h0.cpu(), cu.cpu(), D ** -0.5)
+        to, ts = _tolerances(ref, lengths, D, torch.bfloat16, new[3], H)
+        used = sum(lengths)
+        _check(final, ref[1], ts, f"state of pack {seed}")
+        _check(o[:used], ref[0][:used], to[:used], f"output of pack {seed}")
+        assert bool((o[used:] == 3).all())
+
+
+@gpu
 @pytest.mark.parametrize("decay", ["none", "head", "token"])
 @pytest.mark.parametrize("Hk,H", [(1, 3), (2, 4), (3, 3)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
