@@ -92,6 +92,8 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, inverse=False, atten
     if k is not None:
         k, sk = _head_rows(k, "k")
         Hk = k.shape[1]
+        if H == 0 and Hk > 0:
+            raise ValueError("k needs a q of at least one head")
         if k.shape[0] != L or k.shape[2] != D or k.dtype != q.dtype or k.device != dev:
             raise ValueError("k must be [L, key heads, D] in q's dtype and on its device")
     elif k_out is not None:

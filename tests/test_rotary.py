@@ -173,7 +173,7 @@ def test_rotary_refuses_arguments(cuda):
         lambda: f(q, k, pos[:3], inv), lambda: f(q, k, pos.float(), inv), lambda: f(q, k, pos.cpu(), inv),
         lambda: f(q, k, pos, inv.float()), lambda: f(q, k, pos, torch.ones(33, dtype=torch.float64, device="cuda")),
         lambda: f(q, k, pos, inv, q_out=q[:3]), lambda: f(q, k, pos, inv, q_out=q.bfloat16()),
-        lambda: f(q, None, pos, inv, k_out=k), lambda: f(buf[:4], None, pos, inv, q_out=buf[1:]),
+        lambda: f(q[:, :0], k, pos, inv), lambda: f(q, None, pos, inv, k_out=k), lambda: f(buf[:4], None, pos, inv, q_out=buf[1:]),
         lambda: f(q, k, pos, inv, k_out=q[:, :1]), lambda: f(q, k, pos, inv, q_out=q, k_out=q[:, 1:]),
     ]
     for i, call in enumerate(bad):
