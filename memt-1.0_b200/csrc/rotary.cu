@@ -287,7 +287,7 @@ int launch_rotary(RotaryParams& p, bool copy_rest, int sms, cudaStream_t s) {
 
 }  // namespace
 
-extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) {
+extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try {
   if (a == nullptr || a->struct_size != sizeof(memt_rotary_args)) return MEMT_ERR_INVALID_ARGUMENT;
   if (a->total_tokens < 0 || a->num_heads < 1 || a->num_key_heads < 0 || a->head_dim < 2 || a->rotary_dim < 2 ||
       a->rotary_dim % 2 != 0 || a->rotary_dim > a->head_dim || (a->dtype != MEMT_BF16 && a->dtype != MEMT_F32) ||
@@ -329,4 +329,6 @@ extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return a->dtype == MEMT_BF16 ? launch_rotary<__nv_bfloat16>(p, !in_place, sms, s)
                                : launch_rotary<float>(p, !in_place, sms, s);
+} catch (...) {  // the launch bookkeeping may run out of host memory
+  return MEMT_ERR_CUDA;
 }

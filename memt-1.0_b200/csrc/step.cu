@@ -26,7 +26,7 @@ int launch_step(const StepParams& p, bool delta, bool bf16, cudaStream_t s) {
 
 }  // namespace
 
-extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_stream_t stream) {
+extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_stream_t stream) try {
   if (a == nullptr || a->struct_size != sizeof(memt_recurrent_step_args)) return MEMT_ERR_INVALID_ARGUMENT;
   if (a->rule != MEMT_RULE_LINEAR && a->rule != MEMT_RULE_GDN2) return MEMT_ERR_INVALID_ARGUMENT;
   const bool delta = a->rule == MEMT_RULE_GDN2;
@@ -82,4 +82,6 @@ extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_strea
     case 128: return launch_step<128>(p, delta, bf16, s);
     default: return launch_step<256>(p, delta, bf16, s);
   }
+} catch (...) {  // the launch bookkeeping may run out of host memory
+  return MEMT_ERR_CUDA;
 }
