@@ -406,7 +406,7 @@ typedef struct memt_linear_attention_args {
   float scale;
   void *out;               int64_t out_stride; /* [L,H,D]                       */
   const float *initial_state; /* [N,H,D,D] fp32, or NULL: zero states           */
-  float *final_state;         /* [N,H,D,D] fp32, may alias initial_state        */
+  float *final_state;         /* [N,H,D,D] fp32: initial_state itself, or apart from it */
   /* Optional state pools, as in memt_gdn2_update_args. An input slot outside its pool starts
    * from a zero state; an output slot outside its pool, or one that an earlier sample of the call
    * writes, is not written. */

@@ -52,6 +52,9 @@ BAD_LINEAR = [
     (dict(out_stride=128), "INVALID_ARGUMENT"), (dict(k_stride=132), "MISALIGNED"), (dict(v=24), "MISALIGNED"),
     (dict(initial_slots=16, num_initial_slots=1), "INVALID_ARGUMENT"),
     (dict(final_slots=16, num_final_slots=0), "INVALID_ARGUMENT"),
+    # states of two samples (64 KB each) that overlap by one
+    (dict(num_samples=2, initial_state=16 + 65536), "INVALID_ARGUMENT"),
+    (dict(num_samples=2, initial_state=16, final_state=16 + 65536), "INVALID_ARGUMENT"),
 ]
 
 
