@@ -139,7 +139,8 @@ int check_linear(const memt_linear_attention_args* a) {
     return MEMT_ERR_INVALID_ARGUMENT;
   // without slots, states are one tensor or apart: a sample must not end where another one starts from
   if (a->initial_state != nullptr && a->initial_slots == nullptr && a->final_slots == nullptr) {
-    const uintptr_t in = reinterpret_cast<uintptr_t>(a->initial_state), fin = reinterpret_cast<uintptr_t>(a->final_state);
+    const uintptr_t in = reinterpret_cast<uintptr_t>(a->initial_state);
+    const uintptr_t fin = reinterpret_cast<uintptr_t>(a->final_state);
     const uint64_t bytes = uint64_t(a->num_samples) * a->num_heads * D * D * sizeof(float);
     if (in != fin && (in < fin ? fin - in : in - fin) < bytes) return MEMT_ERR_INVALID_ARGUMENT;
   }
