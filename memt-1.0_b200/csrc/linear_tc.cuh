@@ -679,6 +679,9 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
     if (!OUT && tid == 12 * 32 && vblk == 0) p.seg_decays[(int64_t)unit * p.H + h] = seg_a;
     const bool last = seg + 1 == segs;  // of its sample: its state is the final one
     const bool taken = OUT && last && __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
+    // In place at D = 64, quadrants 2 and 3 load the rows that 0 and 1 store: within a sample's only chunk
+    // nothing else keeps a late warp's loads before another warp's stores.
+    if constexpr (OUT && D < 128) asm volatile("bar.sync 2, 256;" ::: "memory");
     if (__all_sync(~0u, alive) && writes && (OUT ? last && out_slot >= 0 && !taken : true)) {
       float* dst = (OUT ? p.ht + (out_slot * p.H + h) * D * D : p.seg_states + seg_state) + col_off;
 #pragma unroll
