@@ -388,6 +388,8 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  * to it, and a sample whose end lies before its start is empty. Of samples that share rows each ends in
  * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token
  * rows of *_stride elements (a multiple of 16 bytes), so split views of wider projections need no copy.
+ * out, final_state and the workspace must overlap nothing else that the call reads or writes, except
+ * final_state the initial states as stated below; other overlaps are refused.
  */
 typedef struct memt_linear_attention_args {
   uint32_t struct_size;    /* sizeof(memt_linear_attention_args)                */
@@ -441,7 +443,8 @@ int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
  * with read_incoming the output reads the state before the update, as a commit does. Arithmetic
  * is fp32 whatever the dtype. beta and erase belong to key heads, g and write to value heads.
  * A sample whose slot lies outside the pool, or whose slot an earlier sample of the call names,
- * is skipped: neither its state nor its output row is written (pad a batch with slot -1). */
+ * is skipped: neither its state nor its output row is written (pad a batch with slot -1).
+ * Neither out nor the states may overlap anything else that the call reads or writes (refused). */
 #define MEMT_RULE_LINEAR 0
 #define MEMT_RULE_GDN2 1
 typedef struct memt_recurrent_step_args {
@@ -477,7 +480,8 @@ int memt_recurrent_step(const memt_recurrent_step_args *args, memt_stream_t stre
  * every head (elements i and i + rotary_dim/2, or 2i and 2i + 1 when interleaved) is turned by
  * position * inv_freq[i] (by its negative when inverse) and multiplied by attention_scale; the
  * elements behind rotary_dim are copied. Angles are formed in 64 bits, the rotation is fp32. The
- * outputs may be the inputs (in place); otherwise they must not overlap them. */
+ * outputs may be the inputs (in place); otherwise they must not overlap them, and never positions or
+ * inv_freq (refused). */
 typedef struct memt_rotary_args {
   uint32_t struct_size;    /* sizeof(memt_rotary_args)                          */
   int32_t num_heads;       /* query heads                                       */

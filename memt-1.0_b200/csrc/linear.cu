@@ -4,6 +4,7 @@
 #include "launch.h"
 #include "linear.cuh"
 #include "linear_tc.cuh"
+#include "overlap.h"
 
 namespace {
 
@@ -152,6 +153,24 @@ int check_linear(const memt_linear_attention_args* a) {
   return MEMT_OK;
 }
 
+// What the call writes, against all that it reads and the rest of what it writes (states may be one tensor).
+bool writes_overlap(const memt_linear_attention_args* a, const void* workspace, size_t workspace_bytes) {
+  const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4, L = a->total_tokens, N = a->num_samples;
+  const int64_t row = int64_t(a->num_heads) * a->head_dim * size, krow = int64_t(a->num_key_heads) * a->head_dim * size;
+  const int64_t state = int64_t(a->num_heads) * a->head_dim * a->head_dim * 4;
+  const Rows out(a->out, row, a->out_stride * size, L);
+  const Rows fin(a->final_state, state * (a->final_slots != nullptr ? a->num_final_slots : N));
+  const Rows ws(workspace, static_cast<int64_t>(workspace_bytes));
+  const Rows q(a->q, krow, a->q_stride * size, L), k(a->k, krow, a->k_stride * size, L);
+  const Rows v(a->v, row, a->v_stride * size, L);
+  const Rows g(a->g, int64_t(a->num_heads) * 4 * (a->g_layout == MEMT_GATE_PER_HEAD ? L : 1));
+  const Rows cu(a->cu_seqlens, (N + 1) * 4);
+  const Rows in(a->initial_state, state * (a->initial_slots != nullptr ? a->num_initial_slots : N));
+  const Rows from(a->initial_slots, N * 4), to(a->final_slots, N * 4);
+  return overlaps_any(out, {q, k, v, g, cu, in, from, to, fin, ws}) ||
+         overlaps_any(fin, {q, k, v, g, cu, from, to, ws}) || overlaps_any(ws, {q, k, v, g, cu, in, from, to});
+}
+
 }  // namespace
 
 extern "C" {
@@ -175,6 +194,7 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   if (need > 256 &&
       (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return MEMT_ERR_WORKSPACE;
+  if (writes_overlap(a, need > 256 ? workspace : nullptr, need)) return MEMT_ERR_INVALID_ARGUMENT;
   LinearParams p{};
   p.N = a->num_samples;
   p.H = a->num_heads;

@@ -16,6 +16,7 @@
 // again. The vectors behind the rotary part are copied by threads of their own, behind all others
 // in the grid, so that no warp does both.
 #include "launch.h"
+#include "overlap.h"
 
 namespace {
 
@@ -299,6 +300,13 @@ extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try 
       (a->k == nullptr || a->k_out == nullptr || a->k_stride < krow || a->k_out_stride < krow))
     return MEMT_ERR_INVALID_ARGUMENT;
   if (a->total_tokens == 0) return MEMT_OK;
+  {  // every thread reads positions and angles, other threads' outputs must not lie there
+    const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4, L = a->total_tokens;
+    const Rows pos(a->positions, L * (a->positions_int64 != 0 ? 8 : 4)), inv(a->inv_freq, int64_t(a->rotary_dim) * 4);
+    const Rows qo(a->q_out, qrow * size, a->q_out_stride * size, L);
+    const Rows ko(a->num_key_heads > 0 ? a->k_out : nullptr, krow * size, a->k_out_stride * size, L);
+    if (overlaps_any(qo, {pos, inv}) || overlaps_any(ko, {pos, inv})) return MEMT_ERR_INVALID_ARGUMENT;
+  }
   RotaryParams p{};
   p.L = a->total_tokens;
   p.Hq = a->num_heads;

@@ -1,5 +1,6 @@
 // memt_recurrent_step: argument checks and launch of the single-token recurrences (step.cuh).
 #include "launch.h"
+#include "overlap.h"
 #include "step.cuh"
 
 namespace {
@@ -22,6 +23,22 @@ template <int D>
 int launch_step(const StepParams& p, bool delta, bool bf16, cudaStream_t s) {
   if (delta) return bf16 ? launch<D, true, __nv_bfloat16>(p, s) : launch<D, true, float>(p, s);
   return bf16 ? launch<D, false, __nv_bfloat16>(p, s) : launch<D, false, float>(p, s);
+}
+
+// What the call writes (output rows, states), against all that it reads and each other: several CTAs share
+// a head, each reads whole rows of the gates and writes its columns of the output.
+bool writes_overlap(const memt_recurrent_step_args* a) {
+  const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4, N = a->num_samples, H = a->num_heads, Hk = a->num_key_heads;
+  const int64_t D = a->head_dim, row = H * D * size, krow = Hk * D * size;
+  const Rows out(a->out, row, a->out_stride * size, N);
+  const Rows states(a->states, H * D * D * 4 * (a->slots != nullptr ? a->num_slots : N));
+  const Rows q(a->q, krow, a->q_stride * size, N), k(a->k, krow, a->k_stride * size, N);
+  const Rows v(a->v, row, a->v_stride * size, N);
+  const Rows g(a->g, H * 4 * (a->g_layout == MEMT_GATE_CONSTANT ? 1 : N) * (a->g_layout == MEMT_GATE_PER_CHANNEL ? D : 1));
+  const Rows beta(a->beta, N * (a->beta_layout == MEMT_GATE_PER_CHANNEL ? krow : Hk * size));
+  const Rows erase(a->erase, N * krow), write(a->write, N * row), slots(a->slots, N * 4);
+  return overlaps_any(out, {q, k, v, g, beta, erase, write, slots, states}) ||
+         overlaps_any(states, {q, k, v, g, beta, erase, write, slots});
 }
 
 }  // namespace
@@ -52,6 +69,7 @@ extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_strea
   if (a->slots != nullptr && a->num_slots < 1) return MEMT_ERR_INVALID_ARGUMENT;
   if (!aligned16(a->states)) return MEMT_ERR_MISALIGNED;
   if (a->num_samples == 0) return MEMT_OK;
+  if (writes_overlap(a)) return MEMT_ERR_INVALID_ARGUMENT;
   StepParams p{};
   p.N = a->num_samples;
   p.H = a->num_heads;

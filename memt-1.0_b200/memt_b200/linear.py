@@ -176,7 +176,8 @@ def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=N
     [S, H, D, D], and sample n starts from initial_state[initial_slots[n]] and ends in
     final_state[final_slots[n]]. A slot outside its pool reads zeros, or is not written; of samples
     that name one final slot the first is written. The two pools may be one tensor if no sample starts
-    from a slot that another one ends in. ``out`` must not overlap q, k or v.
+    from a slot that another one ends in. ``out`` must not overlap any other argument, nor the final
+    states any but the initial ones.
     """
     q, sq, k, sk, v, sv, vec = _qkv(q, k, v)
     L, H, D = v.shape
@@ -223,7 +224,8 @@ def linear_attention_step(q, k, v, g, states, *, scale=None, slots=None, out=Non
     q, k: [N, Hk, D]; v: [N, H, D], bf16 or fp32; g: fp32 [N, H], [H] or None. states: fp32
     [N, H, D, D], or with slots (int32 [N] on the device) a pool [S, H, D, D] of which session n
     updates states[slots[n]]. A session whose slot lies outside the pool, or is an earlier session's,
-    is skipped: its state and its row of o are left as they were (pad a batch with slot -1).
+    is skipped: its state and its row of o are left as they were (pad a batch with slot -1). Neither
+    ``out`` nor the states may overlap any other argument.
     """
     return _step(_lib.RULE_LINEAR, q, k, v, g, states, None, None, None, scale, slots, False, out)
 
@@ -236,7 +238,7 @@ def gdn2_step(q, k, v, g, states, *, beta=None, erase=None, write=None, scale=No
     S = S~ + k' (write v - S~^T (erase k'))^T. o = scale S^T q reads the new state, or with
     ``read_incoming`` the state before the update, as a commit does. g: fp32 [N, H], [N, H, D], [H]
     or None; beta: [N, Hk] or [N, Hk, D]; erase: [N, Hk, D]; write: [N, H, D], in q's dtype. States,
-    slots and heads as in ``linear_attention_step``.
+    slots, heads and overlaps as in ``linear_attention_step``.
     """
     return _step(_lib.RULE_GDN2, q, k, v, g, states, beta, erase, write, scale, slots, read_incoming, out)
 

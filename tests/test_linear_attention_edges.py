@@ -37,3 +37,127 @@ def test_in_place_samples_of_one_chunk(cuda, dtype, pool):
         torch.cuda.synchronize()
         assert final is states and torch.equal(states, apart[1]) and torch.equal(o, apart[0])
     _check(final.flip(0) if pool else final, ref[1], ts, "state")
+
+
+# ---------------------------------------------------------------------------
+# outputs and states that overlap other arguments (refused before any launch)
+# ---------------------------------------------------------------------------
+
+P = 1 << 20  # addresses a MB apart: nothing is read there
+
+
+def _linear(**over):
+    """A valid call of 8 tokens, 4 heads on 2 key heads, D = 64, bf16; every argument apart."""
+    f = dict(num_samples=2, num_heads=4, num_key_heads=2, head_dim=64, dtype=_lib.MEMT_BF16, total_tokens=8,
+             cu_seqlens=P, q=2 * P, q_stride=128, k=3 * P, k_stride=128, v=4 * P, v_stride=256, g=5 * P,
+             g_layout=_lib.GATE_PER_HEAD, scale=1.0, out=6 * P, out_stride=256, initial_state=7 * P,
+             final_state=8 * P)
+    f.update(over)
+    a = _lib.LinearAttentionArgs(**f)
+    return _lib.load().memt_linear_attention(ctypes.byref(a), None, 0, None)
+
+
+def _step(**over):
+    """A valid step of 2 sessions with every gate, 2 heads, D = 128, bf16; every argument apart."""
+    f = dict(rule=_lib.RULE_GDN2, num_samples=2, num_heads=2, num_key_heads=2, head_dim=128, dtype=_lib.MEMT_BF16,
+             q=P, q_stride=256, k=2 * P, k_stride=256, v=3 * P, v_stride=256, g=4 * P,
+             g_layout=_lib.GATE_PER_CHANNEL, beta=5 * P, beta_layout=_lib.GATE_PER_CHANNEL, erase=6 * P, write=7 * P,
+             states=8 * P, scale=1.0, out=9 * P, out_stride=256)
+    f.update(over)
+    a = _lib.RecurrentStepArgs(**f)
+    return _lib.load().memt_recurrent_step(ctypes.byref(a), None)
+
+
+def _rotary(**over):
+    f = dict(num_heads=2, num_key_heads=1, head_dim=64, rotary_dim=32, dtype=_lib.MEMT_BF16, total_tokens=4, q=P,
+             q_stride=128, k=2 * P, k_stride=64, q_out=3 * P, q_out_stride=128, k_out=4 * P, k_out_stride=64,
+             positions=5 * P, positions_int64=1, inv_freq=6 * P, attention_scale=1.0)
+    f.update(over)
+    a = _lib.RotaryArgs(**f)
+    return _lib.load().memt_rotary(ctypes.byref(a), None)
+
+
+STATE64, STATE128 = 4 * 64 * 64 * 4, 2 * 128 * 128 * 4  # bytes of a sample's states above
+
+
+@pytest.mark.parametrize("over", [
+    dict(out=2 * P), dict(out=3 * P + 7 * 256 + 240), dict(out=4 * P - 7 * 512 - 16), dict(out=5 * P),
+    dict(out=5 * P + 8 * 16 - 16), dict(out=P), dict(out=7 * P), dict(out=7 * P + 2 * STATE64 - 16),
+    dict(out=8 * P + 16), dict(out=5 * P, g_layout=_lib.GATE_CONSTANT),
+    dict(dtype=_lib.MEMT_F32, q_stride=128, out=5 * P),
+    dict(final_state=2 * P), dict(final_state=4 * P + 8 * 512 - 16), dict(final_state=5 * P), dict(final_state=P),
+    dict(initial_slots=9 * P, num_initial_slots=3, out=9 * P), dict(final_slots=9 * P, num_final_slots=5, out=9 * P),
+    dict(final_slots=9 * P, num_final_slots=5, out=8 * P + 5 * STATE64 - 16),
+    dict(final_slots=8 * P, num_final_slots=5),
+    # columns of one wide buffer that share one element vector
+    dict(q=2 * P, q_stride=512, out=2 * P + 240, out_stride=512),
+    dict(v=4 * P, v_stride=640, out=4 * P + 1280 - 496, out_stride=640),
+    dict(v=4 * P, v_stride=640, out=4 * P - 1280 - 496, out_stride=640)])
+def test_linear_attention_refuses_overlaps(over):
+    assert _linear(**over) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("over", [
+    dict(out=P), dict(out=2 * P), dict(out=3 * P), dict(out=4 * P), dict(out=5 * P), dict(out=6 * P),
+    dict(out=7 * P), dict(out=7 * P + 256), dict(out=7 * P - 1008), dict(out=6 * P + 1008), dict(out=8 * P),
+    dict(out=8 * P + 2 * STATE128 - 16), dict(out=4 * P + 2 * 1024 - 16),
+    dict(out=5 * P, beta_layout=_lib.GATE_PER_HEAD), dict(out=4 * P, g_layout=_lib.GATE_CONSTANT),
+    dict(slots=10 * P, num_slots=4, out=10 * P), dict(slots=10 * P, num_slots=4, out=8 * P + 4 * STATE128 - 16),
+    dict(slots=8 * P, num_slots=4), dict(states=P), dict(states=4 * P), dict(states=5 * P), dict(states=6 * P),
+    dict(states=7 * P), dict(states=3 * P - 2 * STATE128 + 16)])
+def test_step_refuses_overlaps(over):
+    assert _step(**over) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("over", [
+    dict(q_out=5 * P), dict(k_out=5 * P + 16), dict(q_out=6 * P), dict(k_out=6 * P + 112),
+    dict(q_out=5 * P - 3 * 512 - 240, q_out_stride=256), dict(k_out=6 * P - 16)])
+def test_rotary_refuses_overlaps(over):
+    assert _rotary(**over) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_outputs_over_gates_are_refused_and_beside_them_are_not(cuda, D, dtype):
+    """Through the Python layer: out as one of the gates raises; gates, inputs and output as columns of one
+    wide buffer, the output between them, are apart and give what separate tensors give."""
+    N, H = 3, 2
+    gen = torch.Generator().manual_seed(D)
+    r = lambda *s: torch.randn(*s, generator=gen)  # noqa: E731
+    q, k, v = (0.1 * r(N, H, D) for _ in range(3))
+    erase, write, beta = (torch.sigmoid(r(N, H, D)) for _ in range(3))
+    S = r(N, H, D, D).cuda()
+    g = -torch.rand(N, H, D, generator=gen).cuda()
+    args = [x.to(dtype).cuda() for x in (q, k, v, erase, write, beta)]
+    q, k, v, erase, write, beta = args
+    kept = S.clone()
+    states = [S.view(-1)[-N * H * D:].view(N, H, D)] if dtype == torch.float32 else []
+    for out in [erase, write, beta, q, k, v] + ([g] if states else []) + states:
+        with pytest.raises(ValueError):
+            M.gdn2_step(q, k, v, g, S, beta=beta, erase=erase, write=write, out=out)
+    for out in [q, v] + states:
+        with pytest.raises(ValueError):
+            M.linear_attention_step(q, k, v, None, S, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(S, kept)
+    want = M.gdn2_step(q, k, v, g, S, beta=beta, erase=erase, write=write)
+    wide = torch.zeros(N, 4 * H * D, dtype=dtype, device="cuda")
+    cols = [wide[:, i * H * D:(i + 1) * H * D].view(N, H, D) for i in range(4)]
+    for c, x in zip(cols, (q, k, v)):
+        c.copy_(x)
+    got = M.gdn2_step(cols[0], cols[1], cols[2], g, kept, beta=beta, erase=erase, write=write, out=cols[3])
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(kept, S)
+
+
+@gpu
+def test_linear_attention_refuses_an_output_over_its_decay(cuda):
+    """fp32: the output over the states, and decays that lie inside the output's last row."""
+    q, k, v, g, h0, cu = _dev(*_inputs(3, [20, 12], 2, 2, 64, torch.float32, "token"))
+    buf = torch.zeros(v.numel(), device="cuda")
+    inside = buf[-g.numel():].view_as(g)
+    for decay, places in ((inside, dict(out=buf.view_as(v))), (g, dict(out=h0.view(-1)[:v.numel()].view_as(v))),
+                          (g, dict(out=h0.view(-1)[-v.numel():].view_as(v), final_state=h0))):
+        with pytest.raises(ValueError):
+            M.linear_attention(q, k, v, decay, h0, cu, **places)
