@@ -130,8 +130,9 @@ int check_linear(const memt_linear_attention_args* a) {
     return MEMT_ERR_INVALID_ARGUMENT;
   if (a->g_layout != MEMT_GATE_NONE && a->g_layout != MEMT_GATE_PER_HEAD && a->g_layout != MEMT_GATE_CONSTANT)
     return MEMT_ERR_INVALID_ARGUMENT;
-  if (a->g_layout == MEMT_GATE_NONE ? a->g != nullptr : a->g == nullptr && a->total_tokens > 0)
-    return MEMT_ERR_INVALID_ARGUMENT;
+  // (an [L, H] tensor without tokens has no address; a constant decay is read whatever the tokens are)
+  const bool no_g = a->g_layout == MEMT_GATE_NONE || (a->g_layout == MEMT_GATE_PER_HEAD && a->total_tokens == 0);
+  if (a->g == nullptr ? !no_g : a->g_layout == MEMT_GATE_NONE) return MEMT_ERR_INVALID_ARGUMENT;
   const int64_t row = int64_t(a->num_heads) * D, krow = int64_t(a->num_key_heads) * D;
   if (a->q_stride < krow || a->k_stride < krow || a->v_stride < row || a->out_stride < row)
     return MEMT_ERR_INVALID_ARGUMENT;

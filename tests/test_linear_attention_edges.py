@@ -161,3 +161,11 @@ def test_linear_attention_refuses_an_output_over_its_decay(cuda):
                           (g, dict(out=h0.view(-1)[-v.numel():].view_as(v), final_state=h0))):
         with pytest.raises(ValueError):
             M.linear_attention(q, k, v, decay, h0, cu, **places)
+
+
+@pytest.mark.parametrize("tokens", [0, 8])
+@pytest.mark.parametrize("dtype", [_lib.MEMT_BF16, _lib.MEMT_F32])
+def test_linear_attention_refuses_a_missing_constant_decay(tokens, dtype):
+    """The [H] decays are read whatever the number of tokens."""
+    over = dict(g=None, g_layout=_lib.GATE_CONSTANT, dtype=dtype, total_tokens=tokens)
+    assert _linear(**over) == _lib.MEMT_ERR_INVALID_ARGUMENT
