@@ -159,11 +159,15 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
                                   fmaf(k, d[3], S[i].w)));
     }
     if (group == 0) {
-      // o = S~^T q + (k'.q) d for the new state
+      // o = S~^T q + (k'.q) d for the new state; the incoming one does not know d, which may not be finite
       float all = 0.f;
-      if (!p.incoming)
+      if (p.incoming) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = 0.f;
+      } else {
 #pragma unroll
         for (int j = 0; j < Cfg::kWarps; ++j) all += s_kq[j];
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float sum = 0.f;

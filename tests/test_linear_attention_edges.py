@@ -9,7 +9,8 @@ import torch
 
 import memt_b200 as M
 from memt_b200 import _lib
-from test_linear_attention import (_check, _dev, _inputs, _recurrence, _tolerances)
+from test_linear_attention import (HALF, U, _check, _dev, _inputs, _recurrence, _step_inputs, _step_reference,
+                                   _tolerances)
 
 gpu = pytest.mark.gpu
 
@@ -169,3 +170,26 @@ def test_linear_attention_refuses_a_missing_constant_decay(tokens, dtype):
     """The [H] decays are read whatever the number of tokens."""
     over = dict(g=None, g_layout=_lib.GATE_CONSTANT, dtype=dtype, total_tokens=tokens)
     assert _linear(**over) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+def test_incoming_read_does_not_know_the_token(cuda, D, dtype, value):
+    """read_incoming: a value of the token that is not finite enters the new state's column and leaves the
+    output, which reads the state before it, as it is."""
+    N, H = 3, 2
+    gen, q, k, v, _ = _step_inputs(7, N, H, H, D, dtype)
+    g, S = -torch.rand(N, H, generator=gen), torch.randn(N, H, D, D, generator=gen)
+    v[1, 0, 5] = value
+    ref = _step_reference(q, k, v, g, S, delta=True, incoming=True)
+    dq, dk, dv, dg, dS = _dev(q, k, v, g, S)
+    o = M.gdn2_step(dq, dk, dv, dg, dS, scale=1.0, read_incoming=True)
+    torch.cuda.synchronize()
+    clean = torch.ones(N, H, D, dtype=torch.bool)
+    clean[1, 0, 5] = False
+    at = clean[:, :, None, :].expand_as(S)
+    _check(o, ref[0], (2 * D + 24) * U * ref[2] + HALF[dtype] * ref[0].abs() * 1.01 + 1e-40, "output")
+    _check(dS.cpu()[at], ref[1][at], (D + 16) * U * ref[3][at] + 1e-40, "state")
+    assert not bool(torch.isfinite(dS[1, 0, :, 5]).any())
