@@ -384,6 +384,7 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  *   bf16 scores and a bf16 copy of the state. In calls of up to 64 tokens a sample in the mean, samples
  *   of at most 24 / 8 / 6 tokens (D = 64 / 128 / 256) go token by token in fp32 instead.
  *   dtype F32: exact fp32 token recurrence on CUDA cores.
+ * A token that is not finite changes no earlier token's output.
  * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] are clamped
  * to it, and a sample whose end lies before its start is empty. Of samples that share rows each ends in
  * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token

@@ -193,3 +193,76 @@ def test_incoming_read_does_not_know_the_token(cuda, D, dtype, value):
     _check(o, ref[0], (2 * D + 24) * U * ref[2] + HALF[dtype] * ref[0].abs() * 1.01 + 1e-40, "output")
     _check(dS.cpu()[at], ref[1][at], (D + 16) * U * ref[3][at] + 1e-40, "state")
     assert not bool(torch.isfinite(dS[1, 0, :, 5]).any())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("heads", [2, 32])
+@pytest.mark.parametrize("what", ["v", "k", "q", "g"])
+def test_a_token_that_is_not_finite_leaves_earlier_ones(cuda, D, dtype, heads, what):
+    """NaN or infinity in one token of a sample: outputs of earlier tokens of every 16-token block, of other
+    columns (v), heads and samples stay within their bounds; its own column is spoiled from it on."""
+    lengths, Hk, H = [5, 320, 64, 200], heads // 2, heads
+    q, k, v, g, h0, cu = _inputs(D + heads, lengths, Hk, H, D, dtype, "token")
+    clean = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    to, ts = _tolerances(clean, lengths, D, dtype, g, H)
+    values = [float("nan"), float("inf"), -float("inf")]
+    # row, value head, column (of v): first and last tokens of blocks and chunks, two in a column of one chunk
+    marks = [(5 + 17, 0, 3), (5 + 31, 1, 40), (5 + 64, 0, 63), (5 + 50, 0, 9), (5 + 20, 0, 9), (5 + 255, 1, D - 1),
+             (325, 1, 0), (325 + 63, 0, 33), (389 + 199, 0, 1), (389 + 128 + 7, 1, D // 2)]
+    spoiled = torch.zeros(v.shape, dtype=torch.bool)
+    ends = {n: (int(cu[n]), int(cu[n + 1])) for n in range(4)}
+    for i, (t, h, c) in enumerate(marks):
+        end = next(e for s, e in ends.values() if s <= t < e)
+        value = values[i % 3]
+        if what == "v":
+            v[t, h, c] = value
+            spoiled[t:end, h, c] = True
+        elif what == "k":
+            k[t, 0, c] = value
+            spoiled[t:end, :2] = True  # both value heads of key head 0
+        elif what == "q":
+            q[t, 0, c] = value
+            spoiled[t, :2] = True
+        else:
+            g[t, h] = float("nan")
+            spoiled[t:end, h] = True
+    o, final = M.linear_attention(*_dev(q, k, v, g, h0, cu))
+    torch.cuda.synchronize()
+    o, final = o.float().cpu(), final.cpu()
+    _check(o[~spoiled], clean[0][~spoiled], to[~spoiled], "output")
+    assert not bool(torch.isfinite(o[spoiled]).any())
+    last = torch.stack([spoiled[e - 1] for _, e in ends.values()])  # [N, H, D]: columns of the final states
+    if what == "q":
+        last.zero_()
+    at = last[:, :, None, :].expand_as(final)
+    _check(final[~at], clean[1][~at], ts[~at], "state")
+    if what in ("v", "g"):
+        assert not bool(torch.isfinite(final[at]).any())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_values_that_are_not_finite_in_segments(cuda, D, in_place):
+    """The same where a sample is split: later segments start from a state that is not finite, the outputs of
+    the token's block are made from its own segment's start."""
+    L, H = 2500, 2
+    q, k, v, g, h0, cu = _inputs(D, [L], 1, H, D, torch.bfloat16, "token", 0.05)
+    assert _lib.load().memt_linear_attention_workspace_size(1, L, H, D, _lib.MEMT_BF16) > 256
+    clean = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    to, ts = _tolerances(clean, [2 * L], D, torch.bfloat16, g, H)
+    spoiled = torch.zeros(v.shape, dtype=torch.bool)
+    for t, h, c, value in ((1003, 0, 5, "nan"), (2, 1, 6, "inf"), (L - 1, 0, D - 1, "nan"), (1500, 0, 5, "inf")):
+        v[t, h, c] = float(value)
+        spoiled[t:, h, c] = True
+    dq, dk, dv, dg, dh, dcu = _dev(q, k, v, g, h0, cu)
+    o, final = M.linear_attention(dq, dk, dv, dg, dh, dcu, final_state=dh if in_place else None)
+    torch.cuda.synchronize()
+    o, final = o.float().cpu(), final.cpu()
+    _check(o[~spoiled], clean[0][~spoiled], to[~spoiled], "output")
+    assert not bool(torch.isfinite(o[spoiled]).any())
+    at = spoiled[-1][None, :, None, :].expand_as(final)
+    _check(final[~at], clean[1][~at], ts[~at], "state")
+    assert not bool(torch.isfinite(final[at]).any())
