@@ -158,6 +158,14 @@ __device__ __forceinline__ int long_before(const LinearParams& p, int n) {
   return count;
 }
 
+// A decay as a pair of fp32 numbers, hi + lo. Neither is negative, and lo is above zero where hi is, so that
+// an infinite state stays infinite with its sign: hi inf + (lo inf + u). (2^-149 of a state changes no sum.)
+__device__ __forceinline__ float low_half(float hi, float lo) { return hi > 0.f ? fmaxf(lo, 1.4e-45f) : lo; }
+__device__ __forceinline__ void split_decay(double a, float& hi, float& lo) {
+  hi = __double2float_rd(a);
+  lo = low_half(hi, static_cast<float>(a - static_cast<double>(hi)));
+}
+
 __device__ __forceinline__ float log_decay(const LinearParams& p, int64_t t, int h) {
   return p.g_layout == 1 ? p.g[t * p.H + h] : (p.g_layout == 3 ? p.g[h] : 0.f);
 }
@@ -261,9 +269,9 @@ __global__ void __launch_bounds__(LinearTokensCfg<D>::kThreads, LinearTokensCfg<
   }
   // A decay that is the same for every token is a pair of fp32 numbers: the rounding of one, repeated
   // for every token, would drift (7e-6 over 16384 tokens).
-  const double fixed = p.g_layout == 3 ? exp(static_cast<double>(p.g[h])) : 1.0;
-  const float fixed_hi = static_cast<float>(fixed);
-  const uint64_t a_lo = f32x2_splat(p.g_layout == 3 ? static_cast<float>(fixed - fixed_hi) : 0.f);
+  float fixed_hi, fixed_lo;
+  split_decay(p.g_layout == 3 ? exp(static_cast<double>(p.g[h])) : 1.0, fixed_hi, fixed_lo);
+  const uint64_t a_lo = f32x2_splat(fixed_lo);
 
   // the next batch's vectors, as loaded: nothing waits for them before keep()
   T xk[TB][NP], xq[TB][NP], xv[TB];

@@ -20,7 +20,8 @@
 // terms (8 bits each), so that the sum over a chunk is an fp32 sum and the final state is what the
 // fp32 recurrence gives (measured 1e-7 relative; one bf16 term leaves 1e-3, two 2e-6). The chunk's
 // decay is applied as a pair of fp32 numbers: one number, its rounding repeated for every chunk of a
-// constant decay, would drift by 2^-25 a chunk. Scores P and the copy of the state that X reads are
+// constant decay, would drift by 2^-25 a chunk. Neither of the pair is negative, so that an infinite state
+// stays one. Scores P and the copy of the state that X reads are
 // bf16 (2^-9 relative each), as is the output; no other value is rounded below fp32.
 // Decay weights never come from differences of long sums: P's weight is the product of the decay from
 // its row's 16-token block start, of whole blocks between, and to its column's block end; inside a
@@ -460,8 +461,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
 #pragma unroll
           for (int i = 8; i >= 0; --i) a = fma(a, f, kInvFact[i]);
           a = y < -900.0 ? 0.0 : a * __longlong_as_double((static_cast<long long>(nr) + 1023) << 52);
-          t.a_hi = static_cast<float>(a);
-          t.a_lo = static_cast<float>(a - static_cast<double>(t.a_hi));
+          split_decay(a, t.a_hi, t.a_lo);
         }
         arrive(TF + ts);
       }
@@ -730,8 +730,8 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
       const uint64_t ah = f32x2_splat(a_hi), al = f32x2_splat(a_lo);
       arrive(TE + c % NT);
       if constexpr (!OUT) {  // the segment's decay, a pair of fp32 numbers too
-        const float hi = seg_a.x * a_hi;
-        seg_a.y = fmaf(seg_a.x, a_hi, -hi) + fmaf(seg_a.x, a_lo, seg_a.y * a_hi);
+        const float hi = __fmul_rd(seg_a.x, a_hi);
+        seg_a.y = low_half(hi, fmaf(seg_a.x, a_hi, -hi) + fmaf(seg_a.x, a_lo, seg_a.y * a_hi));
         seg_a.x = hi;
       }
       wait(BU + u, c);

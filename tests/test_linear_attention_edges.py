@@ -266,3 +266,31 @@ def test_values_that_are_not_finite_in_segments(cuda, D, in_place):
     at = spoiled[-1][None, :, None, :].expand_as(final)
     _check(final[~at], clean[1][~at], ts[~at], "state")
     assert not bool(torch.isfinite(final[at]).any())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("decay", ["none", "head", "token"])
+@pytest.mark.parametrize("lengths,H", [([70, 3], 2), ([1500], 2), ([300, 200], 2)])
+def test_infinite_states_stay_infinite(cuda, D, dtype, decay, lengths, H):
+    """An infinite element of the initial state keeps its sign through any decay above zero, and the outputs
+    of its column are infinite with q's sign; everything else is within its bound."""
+    q, k, v, g, h0, cu = _inputs(D, lengths, H, H, D, dtype, decay, 0.05)
+    clean = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    to, ts = _tolerances(clean, [2 * n for n in lengths], D, dtype, g, H)
+    places = [(0, 0, 5, 7, 1.0), (0, 1, 0, D - 1, -1.0), (len(lengths) - 1, 1, D - 1, 40, 1.0)]
+    at, spoiled = torch.zeros(h0.shape, dtype=torch.bool), torch.zeros(v.shape, dtype=torch.bool)
+    for n, h, d, c, sign in places:
+        h0[n, h, d, c] = sign * float("inf")
+        at[n, h, d, c] = True
+        spoiled[int(cu[n]):int(cu[n + 1]), h, c] = True
+    o, final = M.linear_attention(*_dev(q, k, v, g, h0, cu))
+    torch.cuda.synchronize()
+    o, final = o.float().cpu(), final.cpu()
+    assert torch.equal(final[at], h0[at])
+    _check(final[~at], clean[1][~at], ts[~at], "state")
+    _check(o[~spoiled], clean[0][~spoiled], to[~spoiled], "output")
+    for n, h, d, c, sign in places:
+        rows = slice(int(cu[n]), int(cu[n + 1]))
+        assert torch.equal(o[rows, h, c], sign * torch.sign(q[rows, h, d].float()) * float("inf"))
