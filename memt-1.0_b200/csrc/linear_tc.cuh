@@ -38,9 +38,10 @@
 // The last chunk of a sample is padded with whatever the TMA brings (the next sample's rows, or
 // zeros past the last row): those columns of P are masked by selection, those rows of K's and V's
 // tiles are set to zero (0 x NaN would not be), and those tokens' outputs are not stored.
-// A v that is not finite meets the zero weights of up to 15 earlier tokens in Y. A sample whose final state
-// is not finite therefore looks for such values once its chunks are done and makes those outputs again, token
-// by token (8 x 8192 tokens, 16 heads, D = 128: 249 us, 351 with one NaN; 16384 tokens before the NaN 4.9 ms).
+// A v that is not finite meets the zero weights of up to 15 earlier tokens in Y, and its three terms would be
+// a difference of infinities. A sample whose final state is not finite therefore looks for such values once
+// its chunks are done and makes what they spoil again, token by token (8 x 8192 tokens, 16 heads, D = 128:
+// 255 us, 360 with one NaN; 16384 tokens before the NaN 4.9 ms).
 // Looking for them in every chunk, in the split or in the table warps, cost 4 to 16 % of every call.
 // At D = 64 the 64 values fill half of the 128 lanes; V's tile is loaded twice so that lanes 64-127
 // repeat lanes 0-63 and take half of the output rows.
@@ -142,36 +143,43 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R));
 }
 
-// The outputs of value column `col` for the tokens of a block of 16 before its token t1 (from bos), by a warp in
-// fp32, token by token from the state `seg_start`, or the sample's own.
-template <int D>
-__device__ __forceinline__ void tokens_before(const LinearParams& p, int n, int h, int col, int64_t bos, int t1,
-                                           const float* seg_start) {
+// Value column `col` again, by a warp in fp32, token by token from the state `start` (null: zeros): the outputs
+// from the block of 16 of its token t1 (from bos) on, the first whose v is not finite. A NaN there ends it, the
+// state and the outputs behind are NaN already; otherwise the last state goes to `end` (null: nowhere).
+template <int D, bool OUT>
+__device__ __forceinline__ void column_again(const LinearParams& p, int h, int col, int64_t bos, int tokens, int t1,
+                                             const float* start, float* end) {
   constexpr int R = D / 32;
-  const int lane = threadIdx.x & 31, t0 = t1 & ~15, hk = h / (p.H / p.Hk);
-  if (t0 == t1) return;
-  const int64_t slot = pool_slot(p.slots_in, p.num_in, n);
-  const float* src = seg_start != nullptr ? seg_start
-                                          : (p.h0 != nullptr && slot >= 0 ? p.h0 + (slot * p.H + h) * D * D : nullptr);
+  const int lane = threadIdx.x & 31, hk = h / (p.H / p.Hk);
+  const int64_t vcol = (int64_t)h * D + col, krow = (int64_t)hk * D + R * lane;
+  if (isnan(load_f32<__nv_bfloat16>(p.v, (bos + t1) * p.sv + vcol))) {
+    tokens = t1;
+    end = nullptr;
+    if (!OUT || (t1 & 15) == 0) return;
+  }
   float S[R];
 #pragma unroll
-  for (int i = 0; i < R; ++i) S[i] = src != nullptr ? src[(R * lane + i) * D + col] : 0.f;
-  for (int t = 0; t < t1; ++t) {
+  for (int i = 0; i < R; ++i) S[i] = start != nullptr ? start[(R * lane + i) * D + col] : 0.f;
+  for (int t = 0; t < tokens; ++t) {
     const int64_t row = bos + t;
     const float a = expf(log_decay(p, row, h));
-    const float v = load_f32<__nv_bfloat16>(p.v, row * p.sv + (int64_t)h * D + col);
+    const float v = load_f32<__nv_bfloat16>(p.v, row * p.sv + vcol);
+    const bool out = OUT && t >= (t1 & ~15);
     float o = 0.f;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int64_t at = (int64_t)hk * D + R * lane + i;
-      S[i] = fmaf(a, S[i], load_f32<__nv_bfloat16>(p.k, row * p.sk + at) * v);
-      if (t >= t0) o = fmaf(load_f32<__nv_bfloat16>(p.q, row * p.sq + at), S[i], o);
+      S[i] = fmaf(a, S[i], load_f32<__nv_bfloat16>(p.k, row * p.sk + krow + i) * v);
+      if (out) o = fmaf(load_f32<__nv_bfloat16>(p.q, row * p.sq + krow + i), S[i], o);
     }
-    if (t >= t0) {
+    if (out) {
 #pragma unroll
       for (int x = 16; x > 0; x >>= 1) o += __shfl_xor_sync(~0u, o, x);
-      if (lane == 0) store_f32(static_cast<__nv_bfloat16*>(p.out), row * p.so + (int64_t)h * D + col, p.scale * o);
+      if (lane == 0) store_f32(static_cast<__nv_bfloat16*>(p.out), row * p.so + vcol, p.scale * o);
     }
+  }
+  if (end != nullptr) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) end[(R * lane + i) * D + col] = S[i];
   }
 }
 
@@ -232,7 +240,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
   // of each value the first token whose v is not finite, and whether some value's state is not
   int32_t* spoiled_at = reinterpret_cast<int32_t*>(sm + Cfg::kOffSpoiled);
   int32_t* any_spoiled = spoiled_at + Cfg::kVB;
-  if (OUT && tid <= Cfg::kVB) spoiled_at[tid] = tid < Cfg::kVB ? INT32_MAX : 0;
+  if (tid <= Cfg::kVB) spoiled_at[tid] = tid < Cfg::kVB ? INT32_MAX : 0;
   if (warp == 0) tc::alloc(smem_u32(tmem_slot), 512);
   tc::fence_before();
   __syncthreads();
@@ -243,7 +251,6 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
   DecayTable* tab = reinterpret_cast<DecayTable*>(sm + Cfg::kOffTab);
 
   const int64_t seg_state = ((int64_t)unit * p.H + h) * D * D;  // of seg_states
-  const float* seg_start = segs > 1 ? p.seg_states + seg_state : nullptr;
   const int nchunks = static_cast<int>((eos - bos + kTile - 1) / kTile);
   auto chunk_len = [&](int c) {
     const int64_t left = eos - bos - (int64_t)c * kTile;
@@ -604,36 +611,47 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
     }
     if (OUT && !Cfg::kAlias && nchunks > 0) write_out(nchunks - 1);
     if (lane == 0) bulk_wait_all();
-    if constexpr (OUT) {
-      __syncwarp();
-      asm volatile("bar.sync 2, 512;" ::: "memory");
-      if (*any_spoiled) {
-        // A v that is not finite: Y has weighed it by zero for earlier tokens of its block of 16, which
-        // leaves them NaN. Find the first one of every value, and make those outputs token by token.
-        constexpr int kLanes = Cfg::kVB / 8, kStep = 8 * 32 / kLanes;  // lanes a token, tokens of all warps' loads
-        const int T = static_cast<int>(eos - bos), val = 8 * (lane % kLanes);
-        const __nv_bfloat16* v =
-            static_cast<const __nv_bfloat16*>(p.v) + bos * p.sv + (int64_t)h * D + vblk * Cfg::kVB + val;
-        for (int t0 = (warp - 4) * (32 / kLanes) + lane / kLanes; t0 < T; t0 += 4 * kStep) {
-          uint4 x[4];
+    __syncwarp();
+    asm volatile("bar.sync 2, 512;" ::: "memory");
+    if (*any_spoiled) {
+      // A v that is not finite: Y has weighed it by zero for earlier tokens of its block of 16, which leaves
+      // them NaN, and its three terms are a difference of infinities. Find the first one of every value.
+      constexpr int kLanes = Cfg::kVB / 8, kStep = 8 * 32 / kLanes;  // lanes a token, tokens of all warps' loads
+      const int T = static_cast<int>(eos - bos), val = 8 * (lane % kLanes);
+      const __nv_bfloat16* v =
+          static_cast<const __nv_bfloat16*>(p.v) + bos * p.sv + (int64_t)h * D + vblk * Cfg::kVB + val;
+      for (int t0 = (warp - 4) * (32 / kLanes) + lane / kLanes; t0 < T; t0 += 4 * kStep) {
+        uint4 x[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            x[j] = t0 + j * kStep < T ? *reinterpret_cast<const uint4*>(v + (t0 + j * kStep) * p.sv)
-                                      : make_uint4(0, 0, 0, 0);
+        for (int j = 0; j < 4; ++j)
+          x[j] = t0 + j * kStep < T ? *reinterpret_cast<const uint4*>(v + (t0 + j * kStep) * p.sv)
+                                    : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if ((w[e >> 1] >> (16 * (e & 1)) & 0x7f80) == 0x7f80 && t0 + j * kStep < spoiled_at[val + e])
-                atomicMin(spoiled_at + val + e, t0 + j * kStep);
-          }
+          for (int e = 0; e < 8; ++e)
+            if ((w[e >> 1] >> (16 * (e & 1)) & 0x7f80) == 0x7f80 && t0 + j * kStep < spoiled_at[val + e])
+              atomicMin(spoiled_at + val + e, t0 + j * kStep);
         }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        for (int c = warp - 4; c < Cfg::kVB; c += 8)
-          if (spoiled_at[c] != INT32_MAX) tokens_before<D>(p, n, h, vblk * Cfg::kVB + c, bos, spoiled_at[c], seg_start);
-        asm volatile("bar.sync 2, 512;" ::: "memory");
       }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
+      const bool taken = __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
+      const float* start = p.h0 != nullptr && in_slot >= 0 ? p.h0 + (in_slot * p.H + h) * D * D : nullptr;
+      float* end = seg + 1 == segs && out_slot >= 0 && !taken ? p.ht + (out_slot * p.H + h) * D * D : nullptr;
+      if (segs > 1) start = OUT ? p.seg_states + seg_state : nullptr;
+      if (!OUT) end = p.seg_states + seg_state;
+      for (int c = warp - 4; c < Cfg::kVB; c += 8) {
+        const int t1 = spoiled_at[c];
+        if (t1 == INT32_MAX) continue;
+        const int64_t col = vblk * Cfg::kVB + c;
+        column_again<D, OUT>(p, h, static_cast<int>(col), bos, T, t1, start, end);
+        const bool stored = !isnan(load_f32<__nv_bfloat16>(p.v, (bos + t1) * p.sv + (int64_t)h * D + col));
+        __syncwarp();
+        if (lane == 0 && stored) spoiled_at[c] = -1;
+      }
+      asm volatile("bar.sync 2, 512;" ::: "memory");
     }
   } else {
     // ---------------- the state: value row of this lane, keys KT half .. ----------------
@@ -754,16 +772,15 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
     const bool last = seg + 1 == segs;  // of its sample: its state is the final one
     const bool taken = OUT && last && __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
     // No state is stored before the first one's loads are done (in place at D = 64 quadrants 2 and 3 load the
-    // rows that 0 and 1 store), and, where one is not finite, before outputs have been made from them again.
-    if constexpr (OUT) {
-      uint64_t seen = 0;  // two zeros; NaN once a state is not finite
+    // rows that 0 and 1 store), and, where one is not finite, before columns have been made from them again
+    // (those with a state of their own are marked as stored).
+    uint64_t seen = 0;  // two zeros; NaN once a state is not finite
 #pragma unroll
-      for (int i = 0; i < KT / 2; ++i) seen = fma_f32x2(S[i], 0, seen);
-      if (f32x2_lo(seen) != 0.f || f32x2_hi(seen) != 0.f) *any_spoiled = 1;
-      asm volatile("bar.sync 2, 512;" ::: "memory");
-      if (*any_spoiled) asm volatile("bar.sync 2, 512;" ::: "memory");
-    }
-    if (__all_sync(~0u, alive) && writes && (OUT ? last && out_slot >= 0 && !taken : true)) {
+    for (int i = 0; i < KT / 2; ++i) seen = fma_f32x2(S[i], 0, seen);
+    if (f32x2_lo(seen) != 0.f || f32x2_hi(seen) != 0.f) *any_spoiled = 1;
+    asm volatile("bar.sync 2, 512;" ::: "memory");
+    if (*any_spoiled) asm volatile("bar.sync 2, 512;" ::: "memory");
+    if (__all_sync(~0u, alive) && writes && spoiled_at[vr] >= 0 && (OUT ? last && out_slot >= 0 && !taken : true)) {
       float* dst = (OUT ? p.ht + (out_slot * p.H + h) * D * D : p.seg_states + seg_state) + col_off;
 #pragma unroll
       for (int i = 0; i < KT; i += 2) {

@@ -294,3 +294,25 @@ def test_infinite_states_stay_infinite(cuda, D, dtype, decay, lengths, H):
     for n, h, d, c, sign in places:
         rows = slice(int(cu[n]), int(cu[n + 1]))
         assert torch.equal(o[rows, h, c], sign * torch.sign(q[rows, h, d].float()) * float("inf"))
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,H", [([70, 3], 2), ([1500], 2), ([300, 200], 2)])
+def test_infinite_values_make_infinite_states(cuda, D, dtype, lengths, H):
+    """An infinite v makes its column of the state infinite with k's signs, as k v^T is."""
+    q, k, v, g, h0, cu = _inputs(D, lengths, H, H, D, dtype, "token", 0.05)
+    clean = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    _, ts = _tolerances(clean, [2 * n for n in lengths], D, dtype, g, H)
+    k[33, 0], k[lengths[0] - 1, 1] = (torch.where(k[t, h] == 0, 0.125, k[t, h].float()).to(dtype)
+                                      for t, h in ((33, 0), (lengths[0] - 1, 1)))
+    v[33, 0, 7], v[lengths[0] - 1, 1, 40] = float("inf"), -float("inf")
+    o, final = M.linear_attention(*_dev(q, k, v, g, h0, cu))
+    torch.cuda.synchronize()
+    final = final.cpu()
+    assert torch.equal(final[0, 0, :, 7], torch.sign(k[33, 0].float()) * float("inf"))
+    assert torch.equal(final[0, 1, :, 40], -torch.sign(k[lengths[0] - 1, 1].float()) * float("inf"))
+    at = torch.zeros(h0.shape, dtype=torch.bool)
+    at[0, 0, :, 7] = at[0, 1, :, 40] = True
+    _check(final[~at], clean[1][~at], ts[~at], "state")
