@@ -68,7 +68,10 @@ def _rows(x, name, vec):
             return x, H * D
         if row >= H * D and row % vec == 0:
             return x, row
-    return x.contiguous(), H * D
+    x = x.contiguous()
+    if x.data_ptr() % 16 != 0:  # a whole tensor at an odd address
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x, H * D
 
 
 def _overlap(a, sa, b, sb):

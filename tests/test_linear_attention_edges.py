@@ -316,3 +316,31 @@ def test_infinite_values_make_infinite_states(cuda, D, dtype, lengths, H):
     at = torch.zeros(h0.shape, dtype=torch.bool)
     at[0, 0, :, 7] = at[0, 1, :, 40] = True
     _check(final[~at], clean[1][~at], ts[~at], "state")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("L", [1, 5, 70])
+def test_rows_at_any_address(cuda, dtype, L):
+    """Inputs off the 16-byte grid, whole tensors and columns of a wider buffer: the same bits as aligned ones."""
+    Hk, H, D = 1, 2, 64
+    q, k, v, g, h0, cu = _dev(*_inputs(L, [L], Hk, H, D, dtype, "token"))
+    want, state = M.linear_attention(q, k, v, g, h0, cu)
+    s1 = h0.expand(L, H, D, D).clone()
+    s2 = s1.clone()
+    step = M.linear_attention_step(q, k, v, g, s1)
+
+    def shifted(x):
+        buf = torch.zeros(x.numel() + 1, dtype=x.dtype, device="cuda")
+        buf[1:] = x.reshape(-1)
+        return buf[1:].view_as(x)
+
+    wide = torch.zeros(L, (2 * Hk + H) * D + 8, dtype=dtype, device="cuda")
+    cols = (wide[:, 3:3 + D].view(L, Hk, D), wide[:, 3 + D:3 + 2 * D].view(L, Hk, D),
+            wide[:, 3 + 2 * D:3 + 4 * D].view(L, H, D))
+    for c, x in zip(cols, (q, k, v)):
+        c.copy_(x)
+    for args in ((shifted(q), shifted(k), shifted(v)), cols):
+        o, f = M.linear_attention(*args, shifted(g), h0, cu)
+        assert torch.equal(o, want) and torch.equal(f, state)
+    assert torch.equal(M.linear_attention_step(*cols, shifted(g), s2), step) and torch.equal(s1, s2)
