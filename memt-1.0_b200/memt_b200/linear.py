@@ -152,13 +152,18 @@ def _head_decay(g, L, H, dev, channels=None):
 
 
 def _offsets(cu_seqlens, L, dev):
-    """Device int32 offsets; host offsets are validated first."""
+    """Device int32 offsets. Host offsets are validated and copied in stream order, from memory of their own."""
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 or cu_seqlens.dtype not in (torch.int32, torch.int64):
         raise ValueError("cu_seqlens must hold at least two integer offsets")
     if not cu_seqlens.is_cuda:
         cu = cu_seqlens.to(torch.int64)
         if int(cu[0]) < 0 or int(cu[-1]) > L or bool((cu[1:] < cu[:-1]).any()):
             raise ValueError("cu_seqlens must be nondecreasing offsets within the token rows")
+        with torch.cuda.device(dev):
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError("cu_seqlens must be on the device while a graph is captured")
+        cu_seqlens = cu_seqlens.to(torch.int32, copy=True).contiguous()
+        return cu_seqlens.to(dev, non_blocking=True)  # pageable: staged before the call returns
     elif cu_seqlens.device != dev:
         raise ValueError(f"cu_seqlens must be on {dev}")
     return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous()
@@ -172,8 +177,8 @@ def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=N
     q, k: [L, Hk, D]; v: [L, H, D], bf16 (tensor cores) or fp32 (exact token recurrence), D 64, 128 or
     256; a leading 1 and split views are accepted. g: fp32 natural-log decay <= 0, [L, H] for each
     token or [H] for all, or None (no decay). initial_state: fp32 [N, H, D, D], or None for zeros.
-    cu_seqlens: N + 1 offsets, int32 on the device (int64 or host offsets are converted); rows of o
-    outside every sample are left as they were. scale defaults to D ** -0.5.
+    cu_seqlens: N + 1 offsets, int32 on the device (int64 or host offsets are converted, host ones not
+    while a graph is captured); rows of o outside every sample are left as they were. scale defaults to D ** -0.5.
 
     initial_slots / final_slots (int32 [N] on the device): initial_state / final_state are then pools
     [S, H, D, D], and sample n starts from initial_state[initial_slots[n]] and ends in

@@ -344,3 +344,36 @@ def test_rows_at_any_address(cuda, dtype, L):
         o, f = M.linear_attention(*args, shifted(g), h0, cu)
         assert torch.equal(o, want) and torch.equal(f, state)
     assert torch.equal(M.linear_attention_step(*cols, shifted(g), s2), step) and torch.equal(s1, s2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("pinned", [False, True])
+def test_host_offsets_do_not_block_the_host(cuda, dtype, pinned):
+    """Offsets on the host are copied in stream order: nothing synchronises, later changes of the host tensor
+    are not seen, and a capture, which could only keep their address, refuses them."""
+    q, k, v, g, h0, cu = _inputs(9, [50, 90], 2, 2, 64, torch.bfloat16, "token")
+    dq, dk, dv, dg, dh, dcu = _dev(q, k, v, g, h0, cu)
+    want = M.linear_attention(dq, dk, dv, dg, dh, dcu)
+    busy = torch.randn(4096, 4096, device="cuda")
+    host = cu.to(dtype)
+    host = host.pin_memory() if pinned else host
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(20):
+            busy = busy @ busy * 1e-4
+        o, f = M.linear_attention(dq, dk, dv, dg, dh, host)
+        host.zero_()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    torch.cuda.synchronize()
+    assert torch.equal(o, want[0]) and torch.equal(f, want[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError):
+            M.linear_attention(dq, dk, dv, dg, dh, host)
+        busy.add_(1)
+    graph.replay()
+    torch.cuda.synchronize()
