@@ -166,7 +166,9 @@ def _offsets(cu_seqlens, L, dev):
         return cu_seqlens.to(dev, non_blocking=True)  # pageable: staged before the call returns
     elif cu_seqlens.device != dev:
         raise ValueError(f"cu_seqlens must be on {dev}")
-    return cu_seqlens.to(device=dev, dtype=torch.int32).contiguous()
+    if cu_seqlens.dtype is torch.int64:  # clamped as the kernels clamp, before 32 bits lose what is outside
+        cu_seqlens = cu_seqlens.clamp(0, L).to(torch.int32)
+    return cu_seqlens.contiguous()
 
 
 def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=None, final_state=None,

@@ -377,3 +377,14 @@ def test_host_offsets_do_not_block_the_host(cuda, dtype, pinned):
         busy.add_(1)
     graph.replay()
     torch.cuda.synchronize()
+
+
+@gpu
+def test_offsets_beyond_32_bits_are_clamped(cuda):
+    """int64 device offsets outside int32 are clamped to the rows like any other."""
+    q, k, v, g, h0, _ = _dev(*_inputs(13, [40, 60], 2, 2, 64, torch.bfloat16, "token"))
+    for wide, cu in (([0, 40, 2 ** 32 + 50], [0, 40, 100]), ([-2 ** 32 + 40, 40, 100], [0, 40, 100]),
+                     ([0, 2 ** 33, 2 ** 40], [0, 100, 100])):
+        o, f = M.linear_attention(q, k, v, g, h0, torch.tensor(wide, device="cuda"))
+        want = M.linear_attention(q, k, v, g, h0, torch.tensor(cu, dtype=torch.int32, device="cuda"))
+        assert torch.equal(o, want[0]) and torch.equal(f, want[1])
