@@ -63,7 +63,7 @@ def _rows(x, name, vec):
         x = _tokens_unchecked(x, name)
     L, H, D = x.shape
     row, head, one = x.stride()
-    if one == 1 and head == D and x.data_ptr() % 16 == 0:
+    if one == 1 and (head == D or H == 1) and x.data_ptr() % 16 == 0:
         if L <= 1:
             return x, H * D
         if row >= H * D and row % vec == 0:
@@ -100,7 +100,7 @@ def _out_rows(out, like, inputs, vec, name="out"):
     if o.shape != like.shape or o.dtype != like.dtype or o.device != like.device:
         raise ValueError(f"{name}: expected {tuple(like.shape)} {like.dtype} on {like.device}")
     s = o.stride()
-    if s[2] != 1 or s[1] != D or o.data_ptr() % 16 != 0 or (L > 1 and (s[0] < H * D or s[0] % vec != 0)):
+    if s[2] != 1 or (s[1] != D and H > 1) or o.data_ptr() % 16 != 0 or (L > 1 and (s[0] < H * D or s[0] % vec != 0)):
         raise ValueError(f"{name}: token rows must be contiguous heads on 16-byte boundaries")
     stride = s[0] if L > 1 else H * D
     for x, sx in inputs:

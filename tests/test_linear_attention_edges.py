@@ -388,3 +388,18 @@ def test_offsets_beyond_32_bits_are_clamped(cuda):
         o, f = M.linear_attention(q, k, v, g, h0, torch.tensor(wide, device="cuda"))
         want = M.linear_attention(q, k, v, g, h0, torch.tensor(cu, dtype=torch.int32, device="cuda"))
         assert torch.equal(o, want[0]) and torch.equal(f, want[1])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_outputs_of_one_head(cuda, dtype):
+    """With one head its stride says nothing: an output that is a transposed [1, L, D] buffer is rows."""
+    q, k, v, g, h0, cu = _dev(*_inputs(14, [40, 60], 1, 1, 64, dtype, "token"))
+    want, _ = M.linear_attention(q, k, v, g, h0, cu)
+    out = torch.zeros(1, 100, 64, dtype=dtype, device="cuda").transpose(0, 1)
+    o, _ = M.linear_attention(q, k, v, g, h0, cu, out=out)
+    assert torch.equal(out, want) and o.data_ptr() == out.data_ptr()
+    states = torch.zeros(100, 1, 64, 64, device="cuda")
+    same = states.clone()
+    want = M.linear_attention_step(q, k, v, g, states)
+    assert torch.equal(M.linear_attention_step(q, k, v, g, same, out=out), want) and torch.equal(same, states)
