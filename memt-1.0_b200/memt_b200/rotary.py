@@ -43,6 +43,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
     elif scaling == "yarn":
         if trained_tokens is None or trained_tokens < 1:
             raise ValueError("yarn scaling needs trained_tokens")
+        if not 0.0 < slow_turns <= fast_turns:
+            raise ValueError("slow_turns must be above 0 and at most fast_turns")
 
         def pair_of(turns):  # the pair that makes this many turns over the trained context
             return rotary_dim * math.log(trained_tokens / (2 * math.pi * turns)) / (2 * math.log(base))
@@ -50,6 +52,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
         low = max(math.floor(pair_of(fast_turns)), 0)
         high = min(math.ceil(pair_of(slow_turns)), rotary_dim - 1)
         ramp = ((pair - low) / max(high - low, 1e-3)).clamp(0.0, 1.0)
+        if pair_of(slow_turns) < 0:  # not even the first pair makes as many
+            ramp = torch.ones_like(pair)
         inv = inv / factor * ramp + inv * (1.0 - ramp)
         attention_scale = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):
