@@ -429,8 +429,8 @@ int memt_linear_attention(const memt_linear_attention_args *args, void *workspac
                           memt_stream_t stream);
 
 /* Status of the bf16 calls on the current device since the last call, then cleared: bit 0 = a
- * bounded wait inside the kernel ran out (results of that call are incomplete). Synchronises the
- * stream; intended for tests and debugging. */
+ * bounded wait inside the kernel ran out (outputs of that call are incomplete, the final states that it
+ * concerns NaN). Synchronises the stream; intended for tests and debugging. */
 int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
 
 /* ---- one token of a recurrence, states in place --------------------------

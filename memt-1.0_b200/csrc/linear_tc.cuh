@@ -46,7 +46,7 @@
 // At D = 64 the 64 values fill half of the 128 lanes; V's tile is loaded twice so that lanes 64-127
 // repeat lanes 0-63 and take half of the output rows.
 // Every wait is bounded: a thread whose wait runs out flags it and stops waiting, the control warps
-// drain what they have in flight, and the final state stays unwritten.
+// drain what they have in flight, and the final state is NaN.
 #pragma once
 
 #include "linear.cuh"
@@ -96,7 +96,7 @@ struct LinearTcCfg {
   static constexpr uint32_t kOffP = kOffV + kStages * kBytesV;
   static constexpr uint32_t kOffOut = kOffP + kPanel;           // 2 KB per output warp
   static constexpr uint32_t kOffTab = kOffOut + 8 * 2048;
-  static constexpr uint32_t kOffSpoiled = kOffTab + kTables * sizeof(DecayTable);  // kVB tokens and a flag
+  static constexpr uint32_t kOffSpoiled = kOffTab + kTables * sizeof(DecayTable);  // kVB tokens, two flags
   static constexpr uint32_t kOffBar = kOffSpoiled + 1024;
   static constexpr size_t kSmem = kOffBar + 512 + 1024;
   // tensor memory columns: U^T of one unit, the three terms of (e^R V)^T, bf16(S)^T, X^T, Y^T, Sc
@@ -237,10 +237,12 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
     }
     mbar_fence_init();
   }
-  // of each value the first token whose v is not finite, and whether some value's state is not
+  // of each value the first token whose v is not finite, whether some value's state is not, whether a wait
+  // ran out
   int32_t* spoiled_at = reinterpret_cast<int32_t*>(sm + Cfg::kOffSpoiled);
   int32_t* any_spoiled = spoiled_at + Cfg::kVB;
-  if (tid <= Cfg::kVB) spoiled_at[tid] = tid < Cfg::kVB ? INT32_MAX : 0;
+  int32_t* stalled = any_spoiled + 1;
+  if (tid < Cfg::kVB + 2) spoiled_at[tid] = tid < Cfg::kVB ? INT32_MAX : 0;
   if (warp == 0) tc::alloc(smem_u32(tmem_slot), 512);
   tc::fence_before();
   __syncthreads();
@@ -611,6 +613,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
     }
     if (OUT && !Cfg::kAlias && nchunks > 0) write_out(nchunks - 1);
     if (lane == 0) bulk_wait_all();
+    if (!alive) *stalled = 1;
     __syncwarp();
     asm volatile("bar.sync 2, 512;" ::: "memory");
     if (*any_spoiled) {
@@ -778,9 +781,14 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
 #pragma unroll
     for (int i = 0; i < KT / 2; ++i) seen = fma_f32x2(S[i], 0, seen);
     if (f32x2_lo(seen) != 0.f || f32x2_hi(seen) != 0.f) *any_spoiled = 1;
+    if (!alive) *stalled = 1;
     asm volatile("bar.sync 2, 512;" ::: "memory");
     if (*any_spoiled) asm volatile("bar.sync 2, 512;" ::: "memory");
-    if (__all_sync(~0u, alive) && writes && spoiled_at[vr] >= 0 && (OUT ? last && out_slot >= 0 && !taken : true)) {
+    if (*stalled) {  // the caller sees it in the state
+#pragma unroll
+      for (int i = 0; i < KT / 2; ++i) S[i] = f32x2_splat(__int_as_float(0x7fffffff));
+    }
+    if (writes && (spoiled_at[vr] >= 0 || *stalled) && (OUT ? last && out_slot >= 0 && !taken : true)) {
       float* dst = (OUT ? p.ht + (out_slot * p.H + h) * D * D : p.seg_states + seg_state) + col_off;
 #pragma unroll
       for (int i = 0; i < KT; i += 2) {

@@ -403,3 +403,22 @@ def test_outputs_of_one_head(cuda, dtype):
     same = states.clone()
     want = M.linear_attention_step(q, k, v, g, states)
     assert torch.equal(M.linear_attention_step(q, k, v, g, same, out=out), want) and torch.equal(same, states)
+
+
+def test_status_needs_a_place():
+    assert _lib.load().memt_linear_attention_status(None, None) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+@gpu
+def test_status_after_calls_of_every_kind(cuda):
+    """No wait of the chunked kernel runs out: whole samples, segments, empty ones, values that are not finite."""
+    lib, status = _lib.load(), ctypes.c_int32(-1)
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for D in (64, 128, 256):
+        for lengths, H in (([100], 1), ([3000], 2), ([64, 0, 1, 300], 64)):
+            args = _dev(*_inputs(D, lengths, 1, H, D, torch.bfloat16, "token"))
+            M.linear_attention(*args)
+            args[2][7, 0, 3] = float("nan")
+            M.linear_attention(*args)
+    for _ in range(2):
+        assert lib.memt_linear_attention_status(stream, ctypes.byref(status)) == _lib.MEMT_OK and status.value == 0
