@@ -9,8 +9,8 @@ import torch
 
 import memt_b200 as M
 from memt_b200 import _lib
-from test_linear_attention import (HALF, U, _check, _dev, _inputs, _recurrence, _step_inputs, _step_reference,
-                                   _tolerances)
+from test_linear_attention import (HALF, U, _check, _dev, _inputs, _recurrence, _run_and_check, _step_inputs,
+                                   _step_reference, _tolerances)
 
 gpu = pytest.mark.gpu
 
@@ -422,3 +422,67 @@ def test_status_after_calls_of_every_kind(cuda):
             M.linear_attention(*args)
     for _ in range(2):
         assert lib.memt_linear_attention_status(stream, ctypes.byref(status)) == _lib.MEMT_OK and status.value == 0
+
+
+# ---------------------------------------------------------------------------
+# whole samples of many chunks
+# ---------------------------------------------------------------------------
+
+def _whole(N, L, H, D):
+    """The call keeps no segments: a CTA walks a sample's chunks from the first to the last."""
+    assert _lib.load().memt_linear_attention_workspace_size(N, L, H, D, _lib.MEMT_BF16) == 256
+
+
+@gpu
+@pytest.mark.parametrize("D,H", [(64, 32), (128, 32), (256, 16)])
+@pytest.mark.parametrize("decay", ["head", "token"])
+def test_chains_of_chunks(cuda, D, H, decay):
+    """17 and 11 chunks a CTA: every stage of the tiles and every decay table is used several times."""
+    lengths = [1100, 700]
+    _whole(2, sum(lengths), H, D)
+    _run_and_check(lengths, H // 2, H, D, torch.bfloat16, decay, seed=D, gscale=0.05)
+
+
+RAGGED = [1500, 900, 0, 1500, 1280, 1, 2000, 900, 1700, 1300]  # more than 148 CTAs, above 1024 tokens in the mean
+
+
+@gpu
+def test_longest_samples_first(cuda):
+    """The order by length, with equal lengths, an empty sample and one of one token, in place in a pool."""
+    H, D, N = 16, 64, len(RAGGED)
+    _whole(N, sum(RAGGED), H, D)
+    q, k, v, g, h0, cu = _inputs(19, RAGGED, 4, H, D, torch.bfloat16, "token", 0.05)
+    ref = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    to, ts = _tolerances(ref, RAGGED, D, torch.bfloat16, g, H)
+    slots = torch.tensor([3, 11, 0, 7, 5, 2, 9, 1, 10, 4])
+    pool = torch.full((12, H, D, D), 3.0)
+    pool[slots] = h0
+    dq, dk, dv, dg, dpool, dcu, ds = _dev(q, k, v, g, pool, cu, slots.int())
+    o, _ = M.linear_attention(dq, dk, dv, dg, dpool, dcu, initial_slots=ds, final_state=dpool, final_slots=ds)
+    torch.cuda.synchronize()
+    _check(o, ref[0], to, "output")
+    _check(dpool[slots.cuda()], ref[1], ts, "state")
+    assert bool((dpool[[6, 8]] == 3.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("D,H", [(128, 64), (256, 32)])
+def test_longest_samples_first_equal_each_alone(cuda, D, H):
+    """Bit for bit what each sample gives in a call of its own (whole as well)."""
+    _whole(len(RAGGED), sum(RAGGED), H, D)
+    gen = torch.Generator(device="cuda").manual_seed(D)
+    L = sum(RAGGED)
+    q, k = (torch.nn.functional.normalize(torch.randn(L, H // 4, D, generator=gen, device="cuda"), dim=-1).bfloat16()
+            for _ in range(2))
+    v = torch.randn(L, H, D, generator=gen, device="cuda").bfloat16()
+    g = 0.05 * torch.nn.functional.logsigmoid(2 + torch.randn(L, H, generator=gen, device="cuda"))
+    h0 = torch.randn(len(RAGGED), H, D, D, generator=gen, device="cuda")
+    cu = [sum(RAGGED[:i]) for i in range(len(RAGGED) + 1)]
+    o, final = M.linear_attention(q, k, v, g, h0, torch.tensor(cu))
+    for n, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        if b - a > 24:  # (few tokens alone run token by token)
+            _whole(1, b - a, H, D)
+            o1, f1 = M.linear_attention(q[a:b], k[a:b], v[a:b], g[a:b], h0[n:n + 1], torch.tensor([0, b - a]))
+            assert torch.equal(o[a:b], o1) and torch.equal(final[n], f1[0])
+        elif a == b:
+            assert torch.equal(final[n], h0[n])
