@@ -412,7 +412,8 @@ typedef struct memt_linear_attention_args {
   float *final_state;         /* [N,H,D,D] fp32: initial_state itself, or apart from it */
   /* Optional state pools, as in memt_gdn2_update_args. An input slot outside its pool starts
    * from a zero state; an output slot outside its pool, or one that an earlier sample of the call
-   * writes, is not written. */
+   * writes, is not written. The pools may share whole states (never parts of one), of which no sample
+   * may end in one that another sample starts from. */
   const int32_t *initial_slots;
   int32_t num_initial_slots;
   const int32_t *final_slots;

@@ -139,12 +139,17 @@ int check_linear(const memt_linear_attention_args* a) {
   if ((a->initial_slots != nullptr && (a->num_initial_slots < 1 || a->initial_state == nullptr)) ||
       (a->final_slots != nullptr && a->num_final_slots < 1))
     return MEMT_ERR_INVALID_ARGUMENT;
-  // without slots, states are one tensor or apart: a sample must not end where another one starts from
-  if (a->initial_state != nullptr && a->initial_slots == nullptr && a->final_slots == nullptr) {
+  // A sample must not end where another one starts from. Without slots, states are one tensor or apart; pools may
+  // share whole states, which the slots then tell apart.
+  if (a->initial_state != nullptr) {
     const uintptr_t in = reinterpret_cast<uintptr_t>(a->initial_state);
     const uintptr_t fin = reinterpret_cast<uintptr_t>(a->final_state);
-    const uint64_t bytes = uint64_t(a->num_samples) * a->num_heads * D * D * sizeof(float);
-    if (in != fin && (in < fin ? fin - in : in - fin) < bytes) return MEMT_ERR_INVALID_ARGUMENT;
+    const uint64_t state = uint64_t(a->num_heads) * D * D * sizeof(float), off = in < fin ? fin - in : in - fin;
+    const uint64_t n_in = a->initial_slots != nullptr ? a->num_initial_slots : a->num_samples;
+    const uint64_t n_fin = a->final_slots != nullptr ? a->num_final_slots : a->num_samples;
+    const bool shared = off < state * (in < fin ? n_in : n_fin);
+    const bool pools = a->initial_slots != nullptr || a->final_slots != nullptr;
+    if (shared && (pools ? off % state != 0 : off != 0)) return MEMT_ERR_INVALID_ARGUMENT;
   }
   const int64_t vec = a->dtype == MEMT_BF16 ? 8 : 4;
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||

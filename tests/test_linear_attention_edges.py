@@ -486,3 +486,30 @@ def test_longest_samples_first_equal_each_alone(cuda, D, H):
             assert torch.equal(o[a:b], o1) and torch.equal(final[n], f1[0])
         elif a == b:
             assert torch.equal(final[n], h0[n])
+
+
+@pytest.mark.parametrize("over", [
+    dict(initial_slots=9 * P, num_initial_slots=4, initial_state=7 * P, final_state=7 * P + STATE64 // 4),
+    dict(final_slots=9 * P, num_final_slots=4, initial_state=7 * P + 3 * STATE64 + 16, final_state=7 * P),
+    dict(initial_slots=9 * P, num_initial_slots=4, final_slots=10 * P, num_final_slots=4, initial_state=7 * P,
+         final_state=7 * P - STATE64 // 2)])
+def test_linear_attention_refuses_pools_that_share_parts_of_states(over):
+    assert _linear(**over) == _lib.MEMT_ERR_INVALID_ARGUMENT
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_pools_that_share_whole_states(cuda, dtype):
+    """Views of one pool, shifted by two states; slots keep the samples apart, or in place."""
+    q, k, v, g, h0, cu = _dev(*_inputs(15, [40, 60], 2, 2, 64, dtype, "token"))
+    want, state = M.linear_attention(q, k, v, g, h0, cu)
+    pool = torch.full((6, 2, 64, 64), 3.0, device="cuda")
+    pool[1], pool[4] = h0[0], h0[1]
+    slots = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    o, _ = M.linear_attention(q, k, v, g, pool[:5], cu, initial_slots=slots(1, 4), final_state=pool[2:],
+                              final_slots=slots(3, 2))  # states 5 and 4
+    assert torch.equal(o, want) and torch.equal(pool[5], state[0]) and torch.equal(pool[4], state[1])
+    assert bool((pool[[0, 2, 3]] == 3.0).all()) and torch.equal(pool[1], h0[0])
+    with pytest.raises(ValueError):
+        M.linear_attention(q, k, v, g, pool.view(-1)[64 * 64:64 * 64 + 4 * 2 * 64 * 64].view(4, 2, 64, 64), cu,
+                           initial_slots=slots(0, 1), final_state=pool, final_slots=slots(2, 3))
