@@ -41,7 +41,7 @@
 // A v that is not finite meets the zero weights of up to 15 earlier tokens in Y, and its three terms would be
 // a difference of infinities. A sample whose final state is not finite therefore looks for such values once
 // its chunks are done and makes what they spoil again, token by token (8 x 8192 tokens, 16 heads, D = 128:
-// 255 us, 360 with one NaN; 16384 tokens before the NaN 4.9 ms).
+// 264 us, 360 with one NaN; a column of 16384 tokens 2.1 ms).
 // Looking for them in every chunk, in the split or in the table warps, cost 4 to 16 % of every call.
 // At D = 64 the 64 values fill half of the 128 lanes; V's tile is loaded twice so that lanes 64-127
 // repeat lanes 0-63 and take half of the output rows.
@@ -160,21 +160,33 @@ __device__ __forceinline__ void column_again(const LinearParams& p, int h, int c
   float S[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) S[i] = start != nullptr ? start[(R * lane + i) * D + col] : 0.f;
-  for (int t = 0; t < tokens; ++t) {
-    const int64_t row = bos + t;
-    const float a = expf(log_decay(p, row, h));
-    const float v = load_f32<__nv_bfloat16>(p.v, row * p.sv + vcol);
-    const bool out = OUT && t >= (t1 & ~15);
-    float o = 0.f;
+  // tokens whose loads are in flight together: 16384 tokens 2.1 ms where one by one 4.7; more than one at D = 256
+  // spills in the chunks' loops as well (4 % of every call)
+  constexpr int B = D == 256 ? 1 : 4;
+  for (int tb = 0; tb < tokens; tb += B) {
+    float a[B], v[B], k[B][R];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      S[i] = fmaf(a, S[i], load_f32<__nv_bfloat16>(p.k, row * p.sk + krow + i) * v);
-      if (out) o = fmaf(load_f32<__nv_bfloat16>(p.q, row * p.sq + krow + i), S[i], o);
+    for (int j = 0; j < B; ++j) {
+      const bool live = tb + j < tokens;  // behind the last one: e^0 S + 0
+      const int64_t row = bos + tb + (live ? j : 0);
+      a[j] = live ? log_decay(p, row, h) : 0.f;
+      v[j] = live ? load_f32<__nv_bfloat16>(p.v, row * p.sv + vcol) : 0.f;
+#pragma unroll
+      for (int i = 0; i < R; ++i) k[j][i] = live ? load_f32<__nv_bfloat16>(p.k, row * p.sk + krow + i) : 0.f;
     }
-    if (out) {
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) o += __shfl_xor_sync(~0u, o, x);
-      if (lane == 0) store_f32(static_cast<__nv_bfloat16*>(p.out), row * p.so + vcol, p.scale * o);
+    for (int j = 0; j < B; ++j) {
+      const int64_t row = bos + tb + j;
+#pragma unroll
+      for (int i = 0; i < R; ++i) S[i] = fmaf(expf(a[j]), S[i], k[j][i] * v[j]);
+      if (OUT && tb + j >= (t1 & ~15) && tb + j < tokens) {
+        float o = 0.f;
+#pragma unroll
+        for (int i = 0; i < R; ++i) o = fmaf(load_f32<__nv_bfloat16>(p.q, row * p.sq + krow + i), S[i], o);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) o += __shfl_xor_sync(~0u, o, x);
+        if (lane == 0) store_f32(static_cast<__nv_bfloat16*>(p.out), row * p.so + vcol, p.scale * o);
+      }
     }
   }
   if (end != nullptr) {
