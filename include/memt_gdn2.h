@@ -384,7 +384,8 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  *   bf16 scores and a bf16 copy of the state. In calls of up to 64 tokens a sample in the mean, samples
  *   of at most 24 / 8 / 6 tokens (D = 64 / 128 / 256) go token by token in fp32 instead.
  *   dtype F32: exact fp32 token recurrence on CUDA cores.
- * A token that is not finite changes no earlier token's output.
+ * A token that is not finite changes no earlier token's output. An infinite state, or the column of one that
+ * an infinite v makes, keeps its sign under any decay above zero.
  * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] are clamped
  * to it, and a sample whose end lies before its start is empty. Of samples that share rows each ends in
  * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token
@@ -404,7 +405,8 @@ typedef struct memt_linear_attention_args {
   const void *q;           int64_t q_stride;   /* [L,Hk,D]                      */
   const void *k;           int64_t k_stride;   /* [L,Hk,D]                      */
   const void *v;           int64_t v_stride;   /* [L,H,D]                       */
-  const float *g;          /* natural-log decay (<= 0): NONE, PER_HEAD [L,H], CONSTANT [H] */
+  const float *g;          /* natural-log decay (<= 0): NONE, PER_HEAD [L,H] (may be NULL without
+                            * tokens), CONSTANT [H]                             */
   int32_t g_layout;
   float scale;
   void *out;               int64_t out_stride; /* [L,H,D]                       */

@@ -35,9 +35,11 @@ int launch_tokens(int D, const LinearParams& p, cudaStream_t s) {
 constexpr int kPlanSms = 148;
 
 // 64-token chunks per segment, or 0: one CTA per (sample, head, value block) walks a whole sample. Few of
-// them leave SMs idle for as long as a sample takes: 16 heads of one 65536-token sample 1.51 ms. Segments
-// fill the SMs once, at the price of a first pass that sums their states (k and v are read twice) and
-// a pass that joins them: 0.43 ms. A chunk takes 1.2 / 1.55 / 2.6 us in one CTA at D = 64 / 128 / 256,
+// them leave SMs idle for as long as a sample takes: 16 heads of one 65536-token sample 1.51 ms. Segments of a
+// mean sample's chunks over the free SMs fill them once (samples of unequal length can make one more each,
+// and the second pass then takes a second wave), at the price of a first pass that sums their states (k and
+// v are read twice) and a pass that joins them: 0.43 ms. The rule counts samples, not tokens: short samples
+// beside a long one can leave it whole. A chunk takes 1.2 / 1.55 / 2.6 us in one CTA at D = 64 / 128 / 256,
 // 0.65 of that more in the first pass, and the launches about 18 us. Measured on either side, whole against
 // segments in us: 16 heads of one sample, D = 128: 512 tokens 19 / 27, 1024 31 / 30, 2048 55 / 36, 8192
 // 203 / 72; of two: 1024 31 / 33, 2048 55 / 45; two segments never pay (four samples: 8192 207 / 207).

@@ -21,8 +21,8 @@
 // fp32 recurrence gives (measured 1e-7 relative; one bf16 term leaves 1e-3, two 2e-6). The chunk's
 // decay is applied as a pair of fp32 numbers: one number, its rounding repeated for every chunk of a
 // constant decay, would drift by 2^-25 a chunk. Neither of the pair is negative, so that an infinite state
-// stays one. Scores P and the copy of the state that X reads are
-// bf16 (2^-9 relative each), as is the output; no other value is rounded below fp32.
+// stays one. Scores P and the copy of the state that X reads are bf16 (at most 2^-8 relative each), as is
+// the output; no other value is rounded below fp32.
 // Decay weights never come from differences of long sums: P's weight is the product of the decay from
 // its row's 16-token block start, of whole blocks between, and to its column's block end; inside a
 // block of 16 it is one difference. So every factor is <= 1 for any decay, a reset (e^g = 0) included.
