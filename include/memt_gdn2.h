@@ -385,7 +385,8 @@ int memt_latent_rms_norm(const memt_latent_norm_args *args, memt_stream_t stream
  *   of at most 24 / 8 / 6 tokens (D = 64 / 128 / 256) go token by token in fp32 instead.
  *   dtype F32: exact fp32 token recurrence on CUDA cores.
  * A token that is not finite changes no earlier token's output. An infinite state, or the column of one that
- * an infinite v makes, keeps its sign under any decay above zero.
+ * an infinite v makes, keeps its sign under any decay above zero; an infinite k makes NaN in bf16 (its
+ * products with v's three terms differ in sign).
  * Rows of out that belong to no sample are not written. Offsets outside [0, total_tokens] are clamped
  * to it, and a sample whose end lies before its start is empty. Of samples that share rows each ends in
  * the state of its own tokens; the shared rows of out hold either's. The tensors are read as token
