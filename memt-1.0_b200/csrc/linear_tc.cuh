@@ -41,7 +41,7 @@
 // A v that is not finite meets the zero weights of up to 15 earlier tokens in Y, and its three terms would be
 // a difference of infinities. A sample whose final state is not finite therefore looks for such values once
 // its chunks are done and makes what they spoil again, token by token (8 x 8192 tokens, 16 heads, D = 128:
-// 264 us, 360 with one NaN; a column of 16384 tokens 2.1 ms).
+// 220 us in a short run, 350 with a NaN near a sample's start, 2.2 ms near its end).
 // Looking for them in every chunk, in the split or in the table warps, cost 4 to 16 % of every call.
 // At D = 64 the 64 values fill half of the 128 lanes; V's tile is loaded twice so that lanes 64-127
 // repeat lanes 0-63 and take half of the output rows.
@@ -143,31 +143,31 @@ __device__ __forceinline__ void regs_dec() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R));
 }
 
-// Value column `col` again, by a warp in fp32, token by token from the state `start` (null: zeros): the outputs
-// from the block of 16 of its token t1 (from bos) on, the first whose v is not finite. A NaN there ends it, the
-// state and the outputs behind are NaN already; otherwise the last state goes to `end` (null: nowhere).
+// Value column `col` again, by a warp in fp32, token by token from the state `start` (null: zeros) up to its
+// token t1 (from bos), the first whose v is not finite: the outputs of t1's block of 16 before it. Behind a NaN the
+// state and the outputs are NaN already. An infinity makes the whole column infinite (or NaN), which only other
+// such tokens and full resets change; the last state goes to `end` (null: nowhere). The outputs behind stay NaN.
 template <int D, bool OUT>
 __device__ __forceinline__ void column_again(const LinearParams& p, int h, int col, int64_t bos, int tokens, int t1,
                                              const float* start, float* end) {
   constexpr int R = D / 32;
   const int lane = threadIdx.x & 31, hk = h / (p.H / p.Hk);
   const int64_t vcol = (int64_t)h * D + col, krow = (int64_t)hk * D + R * lane;
-  if (isnan(load_f32<__nv_bfloat16>(p.v, (bos + t1) * p.sv + vcol))) {
-    tokens = t1;
-    end = nullptr;
-    if (!OUT || (t1 & 15) == 0) return;
-  }
+  if (isnan(load_f32<__nv_bfloat16>(p.v, (bos + t1) * p.sv + vcol))) end = nullptr;
+  const bool outputs = OUT && (t1 & 15) != 0;
+  if (!outputs && end == nullptr) return;
+  const int upto = t1 + (end != nullptr);
   float S[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) S[i] = start != nullptr ? start[(R * lane + i) * D + col] : 0.f;
-  // tokens whose loads are in flight together: 16384 tokens 2.1 ms where one by one 4.7; more than one at D = 256
+  // tokens whose loads are in flight together: a long column 2.1 ms where one by one 4.7; more than one at D = 256
   // spills in the chunks' loops as well (4 % of every call)
   constexpr int B = D == 256 ? 1 : 4;
-  for (int tb = 0; tb < tokens; tb += B) {
+  for (int tb = 0; tb < upto; tb += B) {
     float a[B], v[B], k[B][R];
 #pragma unroll
     for (int j = 0; j < B; ++j) {
-      const bool live = tb + j < tokens;  // behind the last one: e^0 S + 0
+      const bool live = tb + j < upto;  // behind the last one: e^0 S + 0
       const int64_t row = bos + tb + (live ? j : 0);
       a[j] = live ? log_decay(p, row, h) : 0.f;
       v[j] = live ? load_f32<__nv_bfloat16>(p.v, row * p.sv + vcol) : 0.f;
@@ -179,7 +179,7 @@ __device__ __forceinline__ void column_again(const LinearParams& p, int h, int c
       const int64_t row = bos + tb + j;
 #pragma unroll
       for (int i = 0; i < R; ++i) S[i] = fmaf(expf(a[j]), S[i], k[j][i] * v[j]);
-      if (OUT && tb + j >= (t1 & ~15) && tb + j < tokens) {
+      if (outputs && tb + j >= (t1 & ~15) && tb + j < t1) {
         float o = 0.f;
 #pragma unroll
         for (int i = 0; i < R; ++i) o = fmaf(load_f32<__nv_bfloat16>(p.q, row * p.sq + krow + i), S[i], o);
@@ -190,6 +190,24 @@ __device__ __forceinline__ void column_again(const LinearParams& p, int h, int c
     }
   }
   if (end != nullptr) {
+    for (int tb = upto; tb < tokens; tb += 32) {
+      const int64_t at = bos + tb + lane;
+      const bool mine = tb + lane < tokens && (!isfinite(load_f32<__nv_bfloat16>(p.v, at * p.sv + vcol)) ||
+                                               expf(log_decay(p, at, h)) == 0.f);
+      uint32_t hits = __ballot_sync(~0u, mine);
+      if (hits != 0) {
+        bool all_nan = true;
+#pragma unroll
+        for (int i = 0; i < R; ++i) all_nan &= isnan(S[i]);
+        if (__all_sync(~0u, all_nan)) break;
+      }
+      for (; hits != 0; hits &= hits - 1) {
+        const int64_t row = bos + tb + __ffs(hits) - 1;
+        const float a = expf(log_decay(p, row, h)), v = load_f32<__nv_bfloat16>(p.v, row * p.sv + vcol);
+#pragma unroll
+        for (int i = 0; i < R; ++i) S[i] = fmaf(a, S[i], load_f32<__nv_bfloat16>(p.k, row * p.sk + krow + i) * v);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < R; ++i) end[(R * lane + i) * D + col] = S[i];
   }

@@ -513,3 +513,34 @@ def test_pools_that_share_whole_states(cuda, dtype):
     with pytest.raises(ValueError):
         M.linear_attention(q, k, v, g, pool.view(-1)[64 * 64:64 * 64 + 4 * 2 * 64 * 64].view(4, 2, 64, 64), cu,
                            initial_slots=slots(0, 1), final_state=pool, final_slots=slots(2, 3))
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("L", [300, 2500])
+def test_infinite_values_that_meet(cuda, D, dtype, L):
+    """Infinite columns of the state under further infinities of either sign and full resets, element by element
+    as the definition: the same infinities, NaN where two meet or a reset multiplies one by zero."""
+    H = 2
+    q, k, v, g, h0, cu = _inputs(D + L, [L], H, H, D, dtype, "token", 0.05)
+    rows = [40, 41, 100, 170, 171, L - 2]
+    for t in rows:
+        k[t] = torch.where(k[t] == 0, torch.full_like(k[t], 0.125), k[t])
+    inf = float("inf")
+    v[40, 0, 1], v[170, 0, 1] = inf, inf                       # two that agree where k's signs do
+    v[41, 0, 2], v[L - 2, 0, 2], k[L - 2, 0] = inf, inf, k[41, 0]  # two that agree everywhere
+    v[100, 1, 3], v[171, 1, 4] = -inf, inf                     # one before a reset, one behind it
+    v[40, 0, 5], v[100, 0, 5] = inf, float("nan")
+    g[150, 1] = -inf
+    ref = _recurrence(q, k, v, g, h0, cu, D ** -0.5)
+    o, final = M.linear_attention(*_dev(q, k, v, g, h0, cu))
+    torch.cuda.synchronize()
+    final, want = final.cpu()[0], ref[1][0]
+    for h, c in ((0, 1), (0, 2), (0, 5), (1, 3), (1, 4)):
+        assert not bool(torch.isfinite(want[h, :, c]).any())
+        assert torch.equal(final[h, :, c].double().nan_to_num(7.0), want[h, :, c].nan_to_num(7.0)), (h, c)
+    _, ts = _tolerances(_recurrence(q, k, v.nan_to_num(0.0, 0.0, 0.0), g, h0, cu, D ** -0.5), [2 * L], D, dtype,
+                        torch.tensor([1.0]), H)
+    clean = torch.isfinite(want)
+    _check(final[clean], want[clean], ts[0][clean] + 1e-20, "state")
