@@ -1,9 +1,10 @@
-"""The gated delta rule over prompts and rotary positions with several axes: what is timed.
+"""The gated delta rule over prompts and single tokens, and rotary positions with several axes: what is timed.
 
-Two operators, each beside its plain form in elementary torch operations:
+Three operators, each beside its plain form in elementary torch operations:
 
 * ``gated_delta``  packed prompts, S_t = a_t S_{t-1} + beta_t k_t (v_t - a_t S_{t-1}^T k_t)^T with a_t = exp(g_t),
                    o_t = scale S_t^T q_t: every token reads the state it has just written
+* ``gated_delta_step``  one token of it for each session, the states updated in place
 * ``rotary_axes``  rotary positions of queries and keys with several axes (time, height, width), each pair
                    of elements turned by the position on an axis of its own
 
@@ -49,6 +50,12 @@ def _prompts(name, sessions, tokens, key_heads, heads, dim, *, dtype="bf16", rag
     return {"name": name, **case} if name else case
 
 
+def _step(name, sessions, key_heads, heads, dim, *, dtype="bf16", decay="token", pool=True):
+    case = {"op": "gated_delta_step", "sessions": sessions, "tokens": 1, "key_heads": key_heads, "heads": heads,
+            "dim": dim, "dtype": dtype, "ragged": False, "decay": decay, "pool": pool}
+    return {"name": name, **case} if name else case
+
+
 def _axes(name, tokens, heads, key_heads, dim, rotary_dim, axes, *, dtype="bf16", cycled=False, interleaved=False,
           inverse=False, in_place=False, first=0):
     case = {"op": "rotary_axes", "tokens": tokens, "heads": heads, "key_heads": key_heads, "dim": dim,
@@ -73,6 +80,10 @@ def listed():
         _prompts("delta sessions few tokens", 256, 16, 16, 16, 128, ragged=True, pool=True),
         # two sessions of a small layer in fp32
         _prompts("delta prompts fp32", 2, 1000, 2, 4, 64, dtype="fp32", ragged=True),
+        # decode of 256 concurrent sessions, one layer
+        _step("delta step 256 sessions", 256, 16, 16, 128),
+        # decode of a single session of a small layer in fp32: latency
+        _step("delta step one fp32", 1, 4, 8, 64, dtype="fp32", decay="head", pool=False),
         # queries and keys of packed video prompts, whole heads, far positions in time
         _axes("axes prompts", 65536, 16, 16, 128, 128, 3, first=1000000),
         # a part of wide heads, the axes in turn, interleaved pairs, backward direction, odd token count
@@ -88,7 +99,7 @@ def _log_int(rng, low, high):
 
 
 def draw(rng):
-    op = rng.choice(["gated_delta", "gated_delta", "gated_delta", "rotary_axes"])
+    op = rng.choice(["gated_delta", "gated_delta", "gated_delta", "gated_delta_step", "rotary_axes"])
     dim = rng.choice([64, 128, 128, 256])
     key_heads = _log_int(rng, 1, 16)
     heads = key_heads * rng.choice([1, 1, 2, 4])
@@ -99,6 +110,9 @@ def draw(rng):
                      cycled=rng.random() < 0.5, interleaved=rng.random() < 0.5, inverse=rng.random() < 0.5,
                      in_place=rng.random() < 0.5, first=_log_int(rng, 1, 1000000))
     dtype = rng.choice(["bf16", "bf16", "bf16", "fp32"])
+    if op == "gated_delta_step":
+        return _step(None, _log_int(rng, 1, max(1, min(256, (1 << 26) // (heads * dim * dim)))), key_heads, heads, dim,
+                     dtype=rng.choice(["bf16", "fp32"]), decay=rng.choice(["head", "token"]), pool=rng.random() < 0.5)
     if rng.random() < 0.3:  # many sessions of few tokens
         sessions = _log_int(rng, 8, max(8, min(256, (1 << 26) // (heads * dim * dim))))
         tokens = _log_int(rng, 1, 64)
@@ -192,7 +206,7 @@ def _pair_axes(pairs, axes, cycled):
 # ---------------------------------------------------------------------------
 
 def run(s):
-    return _run_gated_delta(s) if s["op"] == "gated_delta" else _run_rotary_axes(s)
+    return _RUN[s["op"]](s)
 
 
 def _run_gated_delta(s):
@@ -260,6 +274,20 @@ def _plain_gated_delta(q, k, v, g, beta, states, slots, cu, longest, scale):
     return o[sample, token - cu.long()[sample]], s.contiguous()
 
 
+def _run_gated_delta_step(s):
+    if own:
+        return [_memt().gated_delta_step(s["q"], s["k"], s["v"], s["g"], s["beta"], s["states"], scale=s["scale"],
+                                         slots=s["slots"]), s["states"]]
+    rep = s["v"].shape[1] // s["q"].shape[1]
+    q, k = s["q"].float().repeat_interleave(rep, 1), s["k"].float().repeat_interleave(rep, 1)
+    at = slice(None) if s["slots"] is None else s["slots"].long()
+    state = s["states"][at] * s["g"].exp()[..., None, None]
+    delta = s["beta"].float()[..., None] * (s["v"].float() - (k[..., None, :] @ state).squeeze(-2))
+    state = state + k[..., :, None] * delta[..., None, :]
+    s["states"][at] = state
+    return [(s["scale"] * (q[..., None, :] @ state).squeeze(-2)).to(s["v"].dtype), s["states"]]
+
+
 def _run_rotary_axes(s):
     if own:
         place = {"q_out": s["q"], "k_out": s["k"]} if s["in_place"] else {}
@@ -285,6 +313,9 @@ def _plain_rotate(x, cos, sin, interleaved):
         a, b = part[..., :half], part[..., half:]
         y = torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
     return torch.cat((y.to(x.dtype), rest), -1)
+
+
+_RUN = {"gated_delta": _run_gated_delta, "gated_delta_step": _run_gated_delta_step, "rotary_axes": _run_rotary_axes}
 
 
 # ---------------------------------------------------------------------------
