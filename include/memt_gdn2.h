@@ -68,17 +68,20 @@ typedef struct CUstream_st *memt_stream_t;
  * PER_HEAD:    one value per (token, head): [L, H]          (BASELINE's g, beta)
  * PER_CHANNEL: one value per (token, head, channel): [L, H, D] (the reference's layout)
  * CONSTANT:    one value per head for all tokens: [H]
+ * PER_VALUE_HEAD: one value per (token, value head) where a gate is per key head otherwise
  */
 #define MEMT_GATE_NONE 0
 #define MEMT_GATE_PER_HEAD 1
 #define MEMT_GATE_PER_CHANNEL 2
 #define MEMT_GATE_CONSTANT 3 /* one value per head, the same for every token: [H] (linear attention, steps) */
+#define MEMT_GATE_PER_VALUE_HEAD 4 /* beta [L, H] of the gated delta rule and its step */
 
 /* Library version (major*10000 + minor*100 + patch).
  *   0.2.0  state pools by slot index (fields appended to the update, read and readout args)
  *   0.3.0  every argument struct starts with struct_size; the memory-block prologue; the
  *          DeepSeek grouped latent RMS norm; memt_gdn2_noalloc_status, memt_read_status; (entry points
- *          added since, no struct changed:) linear attention, single-token steps, rotary positions */
+ *          added since, no struct changed:) linear attention, single-token steps, rotary positions; the
+ *          gated delta rule over prompts, rotary positions with several axes */
 int memt_version(void);  /* 300 */
 
 /* Argument structs start with `uint32_t struct_size`, which the caller sets to
@@ -437,24 +440,74 @@ int memt_linear_attention(const memt_linear_attention_args *args, void *workspac
  * concerns NaN). Synchronises the stream; intended for tests and debugging. */
 int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
 
+/* ---- the gated delta rule over prompts -------------------------------------
+ *
+ * No counterpart in the reference (its reads see the incoming snapshot only): the recurrence of
+ * memt_gdn2_update with one decay for each head, in which every token reads the state it has just written.
+ * Per sample n and value head h, from initial_state (key head h / (num_heads / num_key_heads)):
+ *     S~  = exp(g_t) S_{t-1}
+ *     S_t = S~ + beta_t k_t (v_t - S~^T k_t)^T
+ *     out_t = cast(scale S_t^T q_t)
+ * final_state receives the last S. RULE_GATED_DELTA of memt_recurrent_step is its single-token form.
+ *
+ * dtype, rows, samples, states, pools and overlaps as in memt_linear_attention_args; beta is in q's dtype.
+ */
+typedef struct memt_gated_delta_args {
+  uint32_t struct_size;    /* sizeof(memt_gated_delta_args)                     */
+  int32_t num_samples;     /* N >= 1                                            */
+  int32_t num_heads;       /* H value heads                                     */
+  int32_t num_key_heads;   /* Hk query and key heads, a divisor of H            */
+  int32_t head_dim;        /* D: 64, 128 or 256                                 */
+  int32_t dtype;           /* MEMT_BF16 or MEMT_F32: q, k, v, beta and out      */
+  int64_t total_tokens;    /* rows L of q, k, v, out                            */
+  const int32_t *cu_seqlens; /* device [N+1]                                    */
+  const void *q;           int64_t q_stride;   /* [L,Hk,D]                      */
+  const void *k;           int64_t k_stride;   /* [L,Hk,D]                      */
+  const void *v;           int64_t v_stride;   /* [L,H,D]                       */
+  const float *g;          /* natural-log decay (<= 0): NONE, PER_HEAD [L,H], CONSTANT [H] */
+  int32_t g_layout;
+  int32_t beta_layout;     /* NONE (1), PER_HEAD [L,Hk], PER_VALUE_HEAD [L,H]   */
+  const void *beta;        /* g and beta [L,..] may be NULL without tokens      */
+  float scale;
+  void *out;               int64_t out_stride; /* [L,H,D]                       */
+  const float *initial_state; /* [N,H,D,D] fp32, or NULL: zero states           */
+  float *final_state;         /* [N,H,D,D] fp32: initial_state itself, or apart from it */
+  const int32_t *initial_slots; /* optional state pools                         */
+  int32_t num_initial_slots;
+  const int32_t *final_slots;
+  int32_t num_final_slots;
+} memt_gated_delta_args;
+
+/* Workspace bytes for these sizes (0 on invalid sizes). 256 or less: nothing is kept there and the call
+ * takes a NULL workspace. */
+size_t memt_gated_delta_workspace_size(int32_t num_samples, int64_t total_tokens, int32_t num_heads,
+                                       int32_t head_dim, int32_t dtype);
+
+/* workspace: device memory of at least the size above, 256-byte aligned. */
+int memt_gated_delta(const memt_gated_delta_args *args, void *workspace, size_t workspace_bytes,
+                     memt_stream_t stream);
+
 /* ---- one token of a recurrence, states in place --------------------------
  *
  * No counterpart in the reference (its executor commits through the chunked update): the
- * single-token form of the two recurrences, one pass over the fp32 states. For sample n and
+ * single-token form of the recurrences, one pass over the fp32 states. For sample n and
  * value head h, key head h / (num_heads / num_key_heads):
  *   RULE_LINEAR: S <- exp(g) S + k v^T,                        out = cast(scale S^T q)
  *   RULE_GDN2:   k' = sqrt(beta) k,  S~ = diag(exp(g)) S,  d = write*v - S~^T (erase*k'),
  *                S <- S~ + k' d^T,                             out = cast(scale S^T q)
- * with read_incoming the output reads the state before the update, as a commit does. Arithmetic
+ *   RULE_GATED_DELTA: S~ = exp(g) S,  S <- S~ + beta k (v - S~^T k)^T,   out = cast(scale S^T q)
+ *                (g NONE, PER_HEAD or CONSTANT, beta NONE, PER_HEAD or PER_VALUE_HEAD; no erase, no write)
+ * with read_incoming the output of RULE_GDN2 reads the state before the update, as a commit does. Arithmetic
  * is fp32 whatever the dtype. beta and erase belong to key heads, g and write to value heads.
  * A sample whose slot lies outside the pool, or whose slot an earlier sample of the call names,
  * is skipped: neither its state nor its output row is written (pad a batch with slot -1).
  * Neither out nor the states may overlap anything else that the call reads or writes (refused). */
 #define MEMT_RULE_LINEAR 0
 #define MEMT_RULE_GDN2 1
+#define MEMT_RULE_GATED_DELTA 3
 typedef struct memt_recurrent_step_args {
   uint32_t struct_size;    /* sizeof(memt_recurrent_step_args)                  */
-  int32_t rule;            /* MEMT_RULE_LINEAR or MEMT_RULE_GDN2                */
+  int32_t rule;            /* MEMT_RULE_LINEAR, MEMT_RULE_GDN2 or MEMT_RULE_GATED_DELTA */
   int32_t num_samples;     /* N tokens, one per sample                          */
   int32_t num_heads;       /* H value heads                                     */
   int32_t num_key_heads;   /* Hk, a divisor of H                                */
@@ -466,7 +519,7 @@ typedef struct memt_recurrent_step_args {
   const void *v;           int64_t v_stride;   /* [N,H,D]                       */
   const float *g;          /* NONE, PER_HEAD [N,H], CONSTANT [H]; GDN2 also PER_CHANNEL [N,H,D] */
   int32_t g_layout;
-  int32_t beta_layout;     /* NONE, PER_HEAD [N,Hk], PER_CHANNEL [N,Hk,D]       */
+  int32_t beta_layout;     /* NONE, PER_HEAD [N,Hk], PER_CHANNEL [N,Hk,D]; GATED_DELTA also PER_VALUE_HEAD [N,H] */
   const void *beta;
   const void *erase;       /* NULL or [N,Hk,D]                                  */
   const void *write;       /* NULL or [N,H,D]                                   */
@@ -509,14 +562,47 @@ typedef struct memt_rotary_args {
 
 int memt_rotary(const memt_rotary_args *args, memt_stream_t stream);
 
+/* ---- rotary positions with several axes ------------------------------------
+ *
+ * memt_rotary with num_axes positions for each token (time, height and width of an image's patches): pair i
+ * is turned by positions[pair_axes[i]][token] * inv_freq[i]. A pair whose axis lies outside [0, num_axes)
+ * stays at position 0. positions: num_axes rows of total_tokens, position_stride elements from one to the
+ * next. The outputs must overlap neither positions nor pair_axes nor inv_freq (refused); everything else as
+ * in memt_rotary_args.
+ */
+typedef struct memt_rotary_axes_args {
+  uint32_t struct_size;    /* sizeof(memt_rotary_axes_args)                     */
+  int32_t num_heads;       /* query heads                                       */
+  int32_t num_key_heads;   /* 0: no keys (k, k_out ignored)                     */
+  int32_t head_dim;
+  int32_t rotary_dim;      /* even, <= head_dim                                 */
+  int32_t dtype;           /* MEMT_BF16 or MEMT_F32                             */
+  int64_t total_tokens;
+  const void *q;           int64_t q_stride;   /* token rows of *_stride elements */
+  const void *k;           int64_t k_stride;
+  void *q_out;             int64_t q_out_stride;
+  void *k_out;             int64_t k_out_stride;
+  const void *positions;   /* int32 or int64 [num_axes][total_tokens]           */
+  int64_t position_stride; /* elements between axes, >= total_tokens (any for one axis) */
+  int32_t positions_int64;
+  int32_t num_axes;        /* >= 1                                              */
+  const int32_t *pair_axes; /* device [rotary_dim / 2]                          */
+  int32_t interleaved;     /* pairs 2i, 2i + 1 instead of i, i + rotary_dim / 2 */
+  int32_t inverse;
+  const double *inv_freq;  /* device fp64 [rotary_dim / 2], radians per position */
+  float attention_scale;
+} memt_rotary_axes_args;
+
+int memt_rotary_axes(const memt_rotary_axes_args *args, memt_stream_t stream);
+
 /* ---- kernel timing (benchmarks) ----------------------------------------
  *
  * No counterpart in the reference (its kernels are timed from Python). When enabled,
  * every kernel this library launches is bracketed by CUDA events on its own stream and
  * its device time is accumulated per kernel family; disabled (the default) it costs
  * nothing. Families: 0 plan, 1 intra (WY operands), 2 scan, 3 read (GEMV),
- * 4 read (tensor-core tiles), 5 fp32 recurrence, 6 prologue and latent norm, 7 linear attention,
- * 8 single-token steps, 9 rotary.
+ * 4 read (tensor-core tiles), 5 fp32 recurrence, 6 prologue and latent norm, 7 linear attention
+ * and the gated delta rule over prompts, 8 single-token steps, 9 rotary.
  */
 #define MEMT_PROF_FAMILIES 10
 int memt_profiler_enable(int on);

@@ -1,0 +1,98 @@
+// memt_gated_delta: argument checks and launch of the gated delta rule over prompts.
+#include "delta.cuh"
+#include "launch.h"
+#include "prompts.h"
+
+namespace {
+
+using namespace memt;
+
+template <int D, typename T>
+int launch_tokens(const DeltaParams& p, cudaStream_t s) {
+  using Cfg = DeltaTokensCfg<D>;
+  const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;
+  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  ProfScope prof(kProfLinear, s);
+  delta_tokens_kernel<D, T><<<static_cast<unsigned>(grid), Cfg::kThreads, 0, s>>>(p);
+  return cuda_status(cudaGetLastError());
+}
+
+template <typename T>
+int launch_tokens(int D, const DeltaParams& p, cudaStream_t s) {
+  switch (D) {
+    case 64: return launch_tokens<64, T>(p, s);
+    case 128: return launch_tokens<128, T>(p, s);
+    default: return launch_tokens<256, T>(p, s);
+  }
+}
+
+int check_delta(const memt_gated_delta_args* a) {
+  const int st = check_prompts(a);
+  if (st != MEMT_OK) return st;
+  if (a->beta_layout != MEMT_GATE_NONE && a->beta_layout != MEMT_GATE_PER_HEAD &&
+      a->beta_layout != MEMT_GATE_PER_VALUE_HEAD)
+    return MEMT_ERR_INVALID_ARGUMENT;
+  // (a tensor without tokens has no address)
+  if (a->beta == nullptr ? a->beta_layout != MEMT_GATE_NONE && a->total_tokens > 0 : a->beta_layout == MEMT_GATE_NONE)
+    return MEMT_ERR_INVALID_ARGUMENT;
+  return MEMT_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t memt_gated_delta_workspace_size(int32_t N, int64_t L, int32_t H, int32_t D, int32_t dtype) {
+  if (N < 1 || L < 0 || H < 1 || (D != 64 && D != 128 && D != 256)) return 0;
+  if (dtype != MEMT_F32 && dtype != MEMT_BF16) return 0;
+  return 256;
+}
+
+int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t workspace_bytes,
+                     memt_stream_t stream) try {
+  const int st = check_delta(a);
+  if (st != MEMT_OK) return st;
+  const size_t need =
+      memt_gated_delta_workspace_size(a->num_samples, a->total_tokens, a->num_heads, a->head_dim, a->dtype);
+  // (256 stands for none)
+  if (need > 256 &&
+      (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
+    return MEMT_ERR_WORKSPACE;
+  const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4;
+  const int64_t gates = a->beta_layout == MEMT_GATE_PER_HEAD ? a->num_key_heads : a->num_heads;
+  if (prompts_overlap(a, need > 256 ? workspace : nullptr, need, Rows(a->beta, a->total_tokens * gates * size)))
+    return MEMT_ERR_INVALID_ARGUMENT;
+  DeltaParams p{};
+  p.N = a->num_samples;
+  p.H = a->num_heads;
+  p.Hk = a->num_key_heads;
+  p.L = a->total_tokens;
+  p.cu = a->cu_seqlens;
+  p.q = a->q;
+  p.k = a->k;
+  p.v = a->v;
+  p.sq = a->q_stride;
+  p.sk = a->k_stride;
+  p.sv = a->v_stride;
+  p.so = a->out_stride;
+  p.g = a->g;
+  p.g_layout = a->g_layout;
+  p.beta = a->beta;
+  p.beta_layout = a->beta_layout;
+  p.scale = a->scale;
+  p.out = a->out;
+  p.h0 = a->initial_state;
+  p.ht = a->final_state;
+  p.slots_in = a->initial_slots;
+  p.num_in = a->num_initial_slots;
+  p.slots_out = a->final_slots;
+  p.num_out = a->num_final_slots;
+  p.few = INT32_MAX;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (a->dtype == MEMT_F32) return launch_tokens<float>(a->head_dim, p, s);
+  return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+} catch (...) {  // the launch bookkeeping may run out of host memory
+  return MEMT_ERR_CUDA;
+}
+
+}  // extern "C"

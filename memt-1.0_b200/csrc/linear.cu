@@ -4,13 +4,11 @@
 #include "launch.h"
 #include "linear.cuh"
 #include "linear_tc.cuh"
-#include "overlap.h"
+#include "prompts.h"
 
 namespace {
 
 using namespace memt;
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 template <int D, typename T>
 int launch_tokens(const LinearParams& p, cudaStream_t s) {
@@ -120,65 +118,6 @@ int launch_chunked(int D, const LinearParams& p, void* workspace, cudaStream_t s
 // chunks' launch that finds no sample costs up to 36 us more (D = 256, 64 samples: 19).
 int few_tokens(int D) { return D == 64 ? 24 : (D == 128 ? 8 : 6); }
 
-int check_linear(const memt_linear_attention_args* a) {
-  if (a == nullptr || a->struct_size != sizeof(memt_linear_attention_args)) return MEMT_ERR_INVALID_ARGUMENT;
-  if (a->num_samples < 1 || a->num_heads < 1 || a->num_key_heads < 1 || a->num_heads % a->num_key_heads != 0 ||
-      a->total_tokens < 0 || a->total_tokens > INT32_MAX - 1 || (a->dtype != MEMT_BF16 && a->dtype != MEMT_F32))
-    return MEMT_ERR_INVALID_ARGUMENT;
-  const int D = a->head_dim;
-  if (D != 64 && D != 128 && D != 256) return MEMT_ERR_UNSUPPORTED;
-  if (a->cu_seqlens == nullptr || a->final_state == nullptr) return MEMT_ERR_INVALID_ARGUMENT;
-  if (a->total_tokens > 0 && (a->q == nullptr || a->k == nullptr || a->v == nullptr || a->out == nullptr))
-    return MEMT_ERR_INVALID_ARGUMENT;
-  if (a->g_layout != MEMT_GATE_NONE && a->g_layout != MEMT_GATE_PER_HEAD && a->g_layout != MEMT_GATE_CONSTANT)
-    return MEMT_ERR_INVALID_ARGUMENT;
-  // (an [L, H] tensor without tokens has no address; a constant decay is read whatever the tokens are)
-  const bool no_g = a->g_layout == MEMT_GATE_NONE || (a->g_layout == MEMT_GATE_PER_HEAD && a->total_tokens == 0);
-  if (a->g == nullptr ? !no_g : a->g_layout == MEMT_GATE_NONE) return MEMT_ERR_INVALID_ARGUMENT;
-  const int64_t row = int64_t(a->num_heads) * D, krow = int64_t(a->num_key_heads) * D;
-  if (a->q_stride < krow || a->k_stride < krow || a->v_stride < row || a->out_stride < row)
-    return MEMT_ERR_INVALID_ARGUMENT;
-  if ((a->initial_slots != nullptr && (a->num_initial_slots < 1 || a->initial_state == nullptr)) ||
-      (a->final_slots != nullptr && a->num_final_slots < 1))
-    return MEMT_ERR_INVALID_ARGUMENT;
-  // A sample must not end where another one starts from. Without slots, states are one tensor or apart; pools may
-  // share whole states, which the slots then tell apart.
-  if (a->initial_state != nullptr) {
-    const uintptr_t in = reinterpret_cast<uintptr_t>(a->initial_state);
-    const uintptr_t fin = reinterpret_cast<uintptr_t>(a->final_state);
-    const uint64_t state = uint64_t(a->num_heads) * D * D * sizeof(float), off = in < fin ? fin - in : in - fin;
-    const uint64_t n_in = a->initial_slots != nullptr ? a->num_initial_slots : a->num_samples;
-    const uint64_t n_fin = a->final_slots != nullptr ? a->num_final_slots : a->num_samples;
-    const bool shared = off < state * (in < fin ? n_in : n_fin);
-    const bool pools = a->initial_slots != nullptr || a->final_slots != nullptr;
-    if (shared && (pools ? off % state != 0 : off != 0)) return MEMT_ERR_INVALID_ARGUMENT;
-  }
-  const int64_t vec = a->dtype == MEMT_BF16 ? 8 : 4;
-  if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->out) ||
-      !aligned16(a->initial_state) || !aligned16(a->final_state) || a->q_stride % vec != 0 ||
-      a->k_stride % vec != 0 || a->v_stride % vec != 0 || a->out_stride % vec != 0)
-    return MEMT_ERR_MISALIGNED;
-  return MEMT_OK;
-}
-
-// What the call writes, against all that it reads and the rest of what it writes (states may be one tensor).
-bool writes_overlap(const memt_linear_attention_args* a, const void* workspace, size_t workspace_bytes) {
-  const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4, L = a->total_tokens, N = a->num_samples;
-  const int64_t row = int64_t(a->num_heads) * a->head_dim * size, krow = int64_t(a->num_key_heads) * a->head_dim * size;
-  const int64_t state = int64_t(a->num_heads) * a->head_dim * a->head_dim * 4;
-  const Rows out(a->out, row, a->out_stride * size, L);
-  const Rows fin(a->final_state, state * (a->final_slots != nullptr ? a->num_final_slots : N));
-  const Rows ws(workspace, static_cast<int64_t>(workspace_bytes));
-  const Rows q(a->q, krow, a->q_stride * size, L), k(a->k, krow, a->k_stride * size, L);
-  const Rows v(a->v, row, a->v_stride * size, L);
-  const Rows g(a->g, int64_t(a->num_heads) * 4 * (a->g_layout == MEMT_GATE_PER_HEAD ? L : 1));
-  const Rows cu(a->cu_seqlens, (N + 1) * 4);
-  const Rows in(a->initial_state, state * (a->initial_slots != nullptr ? a->num_initial_slots : N));
-  const Rows from(a->initial_slots, N * 4), to(a->final_slots, N * 4);
-  return overlaps_any(out, {q, k, v, g, cu, in, from, to, fin, ws}) ||
-         overlaps_any(fin, {q, k, v, g, cu, from, to, ws}) || overlaps_any(ws, {q, k, v, g, cu, in, from, to});
-}
-
 }  // namespace
 
 extern "C" {
@@ -194,7 +133,7 @@ size_t memt_linear_attention_workspace_size(int32_t N, int64_t L, int32_t H, int
 
 int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, size_t workspace_bytes,
                           memt_stream_t stream) try {
-  const int st = check_linear(a);
+  const int st = check_prompts(a);
   if (st != MEMT_OK) return st;
   const size_t need =
       memt_linear_attention_workspace_size(a->num_samples, a->total_tokens, a->num_heads, a->head_dim, a->dtype);
@@ -202,7 +141,7 @@ int memt_linear_attention(const memt_linear_attention_args* a, void* workspace, 
   if (need > 256 &&
       (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255u)))
     return MEMT_ERR_WORKSPACE;
-  if (writes_overlap(a, need > 256 ? workspace : nullptr, need)) return MEMT_ERR_INVALID_ARGUMENT;
+  if (prompts_overlap(a, need > 256 ? workspace : nullptr, need)) return MEMT_ERR_INVALID_ARGUMENT;
   LinearParams p{};
   p.N = a->num_samples;
   p.H = a->num_heads;

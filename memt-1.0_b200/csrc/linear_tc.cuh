@@ -113,34 +113,47 @@ struct LinearTcCfg {
   static_assert(kColSc + 64 <= 512 && kSmem <= 227 * 1024, "one CTA's resources");
 };
 
-__device__ __forceinline__ bool mbar_try(uint32_t mbar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-      " selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(mbar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// Wait for the phase with the given parity for at most 2^30 clocks (half a second): a poll may
-// suspend the thread, so polls are no measure of time.
-__device__ __forceinline__ bool mbar_wait_clock(uint32_t mbar, uint32_t parity) {
-  if (mbar_try(mbar, parity)) return true;
-  const uint32_t begin = static_cast<uint32_t>(clock());
-#pragma unroll 1
-  while (!mbar_try(mbar, parity))
-    if (static_cast<uint32_t>(clock()) - begin > (1u << 30)) return false;
-  return true;
-}
-
-template <int R>
-__device__ __forceinline__ void regs_inc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R));
-}
-template <int R>
-__device__ __forceinline__ void regs_dec() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R));
+// Between the two passes over segments: the state before each one. A thread owns four values of one
+// (sample, head) state and walks over its segments; the segments' own sums are replaced in place.
+__global__ void __launch_bounds__(256) linear_segments_kernel(const LinearParams p, int D) {
+  const int per_state = D * D / 4, blocks = (per_state + 255) / 256;
+  const int at = (blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int nh = blockIdx.x / blocks, h = nh % p.H, n = nh / p.H;
+  int64_t bos, eos;
+  int first = 0, count = 1;
+  {  // this sample's first segment: every warp sums the samples before it
+    const int lane = threadIdx.x & 31;
+    for (int m = lane; m < n; m += 32) {
+      sample_range(p, m, bos, eos);
+      first += segments_of(p, eos - bos);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
+    sample_range(p, n, bos, eos);
+    count = segments_up_to(p, n, first + segments_of(p, eos - bos));
+    first = n == 0 ? 0 : segments_up_to(p, n - 1, first);
+    count -= first;
+  }
+  if (count == 1 || at >= per_state) return;  // one segment starts from the sample's own state
+  const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n);
+  float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.h0 != nullptr && in_slot >= 0)
+    S = reinterpret_cast<const float4*>(p.h0 + (in_slot * p.H + h) * D * D)[at];
+  for (int s = 0; s < count; ++s) {
+    const int64_t seg = (int64_t)(first + s) * p.H + h;
+    float4* state = reinterpret_cast<float4*>(p.seg_states + seg * D * D) + at;
+    float4 own = make_float4(0.f, 0.f, 0.f, 0.f);
+    float2 a = make_float2(0.f, 0.f);
+    if (s + 1 < count) {  // the last one's sum is not made: the second pass ends with it
+      own = *state;
+      a = p.seg_decays[seg];
+    }
+    *state = S;
+    S.x = fmaf(a.x, S.x, fmaf(a.y, S.x, own.x));
+    S.y = fmaf(a.x, S.y, fmaf(a.y, S.y, own.y));
+    S.z = fmaf(a.x, S.z, fmaf(a.y, S.z, own.z));
+    S.w = fmaf(a.x, S.w, fmaf(a.y, S.w, own.w));
+  }
 }
 
 // Value column `col` again, by a warp in fp32, token by token from the state `start` (null: zeros) up to its

@@ -1,9 +1,10 @@
-// memt_rotary: rotary positions of queries and keys, both in one launch.
+// memt_rotary, memt_rotary_axes: rotary positions of queries and keys, both in one launch.
 //
 // Pair i of a head (elements i and i + R/2 in the half layout, 2i and 2i + 1 in the interleaved
 // one) at position p is turned by the angle p * inv_freq[i]:
 //     y_a = c x_a - s x_b,   y_b = c x_b + s x_a,   (c, s) = scale * (cos, sin)(p * inv_freq[i])
-// and the inverse (the operator's own backward pass) turns by the negative angle.
+// and the inverse (the operator's own backward pass) turns by the negative angle. With several axes (AXES)
+// a token has a position on each and pair i takes that of its axis.
 //
 // The angle is formed and reduced to a fraction of a turn in 64 bits: at position 10^6 an fp32
 // product is off by 0.03 radians. Sine and cosine of the fraction, and the rotation, are fp32;
@@ -32,6 +33,9 @@ struct RotaryParams {
   int64_t sq, sk, sqo, sko;  // elements per token row
   const void* pos;
   int32_t pos64;
+  int32_t axes;              // AXES: rows of pos, pos_stride elements apart
+  int64_t pos_stride;
+  const int32_t* pair_axes;  // row of each pair; a pair outside of them stays at position 0
   const double* inv_freq;
   float scale;
   int32_t inverse, interleaved;
@@ -64,6 +68,14 @@ __device__ __forceinline__ void angle(const RotaryParams& p, double pos, int pai
   sincospif(2.0f * static_cast<float>(turns), &s, &c);
   c *= p.scale;
   s *= p.inverse ? -p.scale : p.scale;
+}
+
+// the position that turns `pair` of token t (`pos`: the token's only one, without axes)
+template <bool AXES>
+__device__ __forceinline__ double pair_position(const RotaryParams& p, double pos, int64_t t, int pair) {
+  if constexpr (!AXES) return pos;
+  const int axis = p.pair_axes[pair];
+  return axis >= 0 && axis < p.axes ? position(p, axis * p.pos_stride + t) : 0.0;
 }
 
 // one 16-byte vector as fp32 values, and back
@@ -112,7 +124,7 @@ __device__ __forceinline__ void head_ptrs(const RotaryParams& p, int64_t t, int 
 }
 
 // 16-byte vectors. kHeads heads are in flight per thread at a time.
-template <typename T, bool INTERLEAVED>
+template <typename T, bool INTERLEAVED, bool AXES>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   constexpr int V = Vec<T>::N;
   constexpr int kPairs = INTERLEAVED ? V / 2 : V;
@@ -154,9 +166,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const int64_t t = split(idx, p.rot_units * p.groups, rest);
   const int group = rest / p.rot_units, unit = rest - group * p.rot_units;
   float c[kPairs], s[kPairs];
-  const double pos = position(p, t);
+  const double pos = AXES ? 0.0 : position(p, t);
 #pragma unroll
-  for (int i = 0; i < kPairs; ++i) angle(p, pos, unit * kPairs + i, c[i], s[i]);
+  for (int i = 0; i < kPairs; ++i)
+    angle(p, pair_position<AXES>(p, pos, t, unit * kPairs + i), unit * kPairs + i, c[i], s[i]);
   const int col = unit * V, half = p.R >> 1;
   for (int h0 = group; h0 < H; h0 += kHeads * p.groups) {
     uint4 a[kHeads], b[kHeads];
@@ -207,7 +220,7 @@ __device__ __forceinline__ void store(float* y, float x) { *y = x; }
 __device__ __forceinline__ void store(__nv_bfloat16* y, float x) { *y = __float2bfloat16_rn(x); }
 
 // Rows or rotary parts that are not whole 16-byte vectors: one pair (or copied element) a thread.
-template <typename T>
+template <typename T, bool AXES>
 __global__ void __launch_bounds__(256) rotary_scalar_kernel(const RotaryParams p) {
   constexpr int kHeads = 4;
   const int64_t idx = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -221,7 +234,7 @@ __global__ void __launch_bounds__(256) rotary_scalar_kernel(const RotaryParams p
   const int ia = turns ? (p.interleaved ? 2 * unit : unit) : p.R + unit - p.rot_units;
   const int ib = turns ? (p.interleaved ? ia + 1 : ia + half) : ia;
   float c = 1.f, s = 0.f;
-  if (turns) angle(p, position(p, t), unit, c, s);
+  if (turns) angle(p, pair_position<AXES>(p, AXES ? 0.0 : position(p, t), t, unit), unit, c, s);
   for (int h0 = group; h0 < H; h0 += kHeads * p.groups) {
     T a[kHeads], b[kHeads];
 #pragma unroll
@@ -256,7 +269,7 @@ __global__ void __launch_bounds__(256) rotary_scalar_kernel(const RotaryParams p
 
 bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15u) == 0; }
 
-template <typename T>
+template <typename T, bool AXES>
 int launch_rotary(RotaryParams& p, bool copy_rest, int sms, cudaStream_t s) {
   constexpr int V = Vec<T>::N;
   bool vec = p.D % V == 0 && (p.interleaved ? p.R % V == 0 : p.R % (2 * V) == 0);
@@ -278,18 +291,16 @@ int launch_rotary(RotaryParams& p, bool copy_rest, int sms, cudaStream_t s) {
   ProfScope prof(kProfRotary, s);
   const unsigned grid = static_cast<unsigned>(blocks);
   if (!vec)
-    rotary_scalar_kernel<T><<<grid, 256, 0, s>>>(p);
+    rotary_scalar_kernel<T, AXES><<<grid, 256, 0, s>>>(p);
   else if (p.interleaved)
-    rotary_kernel<T, true><<<grid, 256, 0, s>>>(p);
+    rotary_kernel<T, true, AXES><<<grid, 256, 0, s>>>(p);
   else
-    rotary_kernel<T, false><<<grid, 256, 0, s>>>(p);
+    rotary_kernel<T, false, AXES><<<grid, 256, 0, s>>>(p);
   return cuda_status(cudaGetLastError());
 }
 
-}  // namespace
-
-extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try {
-  if (a == nullptr || a->struct_size != sizeof(memt_rotary_args)) return MEMT_ERR_INVALID_ARGUMENT;
+// Both entry points: `a` without its struct_size; axes 0: one position a token, else as in memt_rotary_axes_args.
+int rotary(const memt_rotary_args* a, int axes, const int32_t* pair_axes, int64_t pos_stride, cudaStream_t s) {
   if (a->total_tokens < 0 || a->num_heads < 1 || a->num_key_heads < 0 || a->head_dim < 2 || a->rotary_dim < 2 ||
       a->rotary_dim % 2 != 0 || a->rotary_dim > a->head_dim || (a->dtype != MEMT_BF16 && a->dtype != MEMT_F32) ||
       a->inv_freq == nullptr || a->positions == nullptr || a->q == nullptr || a->q_out == nullptr)
@@ -301,11 +312,12 @@ extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try 
     return MEMT_ERR_INVALID_ARGUMENT;
   if (a->total_tokens == 0) return MEMT_OK;
   {  // every thread reads positions and angles, other threads' outputs must not lie there
-    const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4, L = a->total_tokens;
-    const Rows pos(a->positions, L * (a->positions_int64 != 0 ? 8 : 4)), inv(a->inv_freq, int64_t(a->rotary_dim) * 4);
+    const int64_t size = a->dtype == MEMT_BF16 ? 2 : 4, L = a->total_tokens, each = a->positions_int64 != 0 ? 8 : 4;
+    const Rows pos(a->positions, L * each, axes > 1 ? pos_stride * each : L * each, axes > 1 ? axes : 1);
+    const Rows inv(a->inv_freq, int64_t(a->rotary_dim) * 4), pairs(pair_axes, int64_t(a->rotary_dim) * 2);
     const Rows qo(a->q_out, qrow * size, a->q_out_stride * size, L);
     const Rows ko(a->num_key_heads > 0 ? a->k_out : nullptr, krow * size, a->k_out_stride * size, L);
-    if (overlaps_any(qo, {pos, inv}) || overlaps_any(ko, {pos, inv})) return MEMT_ERR_INVALID_ARGUMENT;
+    if (overlaps_any(qo, {pos, inv, pairs}) || overlaps_any(ko, {pos, inv, pairs})) return MEMT_ERR_INVALID_ARGUMENT;
   }
   RotaryParams p{};
   p.L = a->total_tokens;
@@ -325,6 +337,9 @@ extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try 
   }
   p.pos = a->positions;
   p.pos64 = a->positions_int64 != 0;
+  p.axes = axes;
+  p.pos_stride = pos_stride;
+  p.pair_axes = pair_axes;
   p.inv_freq = a->inv_freq;
   p.scale = a->attention_scale;
   p.inverse = a->inverse != 0;
@@ -334,9 +349,35 @@ extern "C" int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try 
   if (st != MEMT_OK) return st;
   // in place, the elements behind the rotary part stay where they are
   const bool in_place = p.q == p.q_out && (p.Hk == 0 || p.k == p.k_out);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return a->dtype == MEMT_BF16 ? launch_rotary<__nv_bfloat16>(p, !in_place, sms, s)
-                               : launch_rotary<float>(p, !in_place, sms, s);
+  if (axes > 0)
+    return a->dtype == MEMT_BF16 ? launch_rotary<__nv_bfloat16, true>(p, !in_place, sms, s)
+                                 : launch_rotary<float, true>(p, !in_place, sms, s);
+  return a->dtype == MEMT_BF16 ? launch_rotary<__nv_bfloat16, false>(p, !in_place, sms, s)
+                               : launch_rotary<float, false>(p, !in_place, sms, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int memt_rotary(const memt_rotary_args* a, memt_stream_t stream) try {
+  if (a == nullptr || a->struct_size != sizeof(memt_rotary_args)) return MEMT_ERR_INVALID_ARGUMENT;
+  return rotary(a, 0, nullptr, 0, reinterpret_cast<cudaStream_t>(stream));
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;
 }
+
+int memt_rotary_axes(const memt_rotary_axes_args* a, memt_stream_t stream) try {
+  if (a == nullptr || a->struct_size != sizeof(memt_rotary_axes_args)) return MEMT_ERR_INVALID_ARGUMENT;
+  if (a->num_axes < 1 || a->pair_axes == nullptr || (a->num_axes > 1 && a->position_stride < a->total_tokens))
+    return MEMT_ERR_INVALID_ARGUMENT;
+  const memt_rotary_args one = {sizeof(memt_rotary_args), a->num_heads, a->num_key_heads, a->head_dim, a->rotary_dim,
+                                a->dtype, a->total_tokens, a->q, a->q_stride, a->k, a->k_stride, a->q_out,
+                                a->q_out_stride, a->k_out, a->k_out_stride, a->positions, a->positions_int64,
+                                a->interleaved, a->inv_freq, a->attention_scale, a->inverse};
+  return rotary(&one, a->num_axes, a->pair_axes, a->position_stride, reinterpret_cast<cudaStream_t>(stream));
+} catch (...) {
+  return MEMT_ERR_CUDA;
+}
+
+}  // extern "C"

@@ -35,7 +35,8 @@ bool writes_overlap(const memt_recurrent_step_args* a) {
   const Rows q(a->q, krow, a->q_stride * size, N), k(a->k, krow, a->k_stride * size, N);
   const Rows v(a->v, row, a->v_stride * size, N);
   const Rows g(a->g, H * 4 * (a->g_layout == MEMT_GATE_CONSTANT ? 1 : N) * (a->g_layout == MEMT_GATE_PER_CHANNEL ? D : 1));
-  const Rows beta(a->beta, N * (a->beta_layout == MEMT_GATE_PER_CHANNEL ? krow : Hk * size));
+  const Rows beta(a->beta, N * (a->beta_layout == MEMT_GATE_PER_CHANNEL ? krow
+                                : a->beta_layout == MEMT_GATE_PER_VALUE_HEAD ? H * size : Hk * size));
   const Rows erase(a->erase, N * krow), write(a->write, N * row), slots(a->slots, N * 4);
   return overlaps_any(out, {q, k, v, g, beta, erase, write, slots, states}) ||
          overlaps_any(states, {q, k, v, g, beta, erase, write, slots});
@@ -45,8 +46,8 @@ bool writes_overlap(const memt_recurrent_step_args* a) {
 
 extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_stream_t stream) try {
   if (a == nullptr || a->struct_size != sizeof(memt_recurrent_step_args)) return MEMT_ERR_INVALID_ARGUMENT;
-  if (a->rule != MEMT_RULE_LINEAR && a->rule != MEMT_RULE_GDN2) return MEMT_ERR_INVALID_ARGUMENT;
-  const bool delta = a->rule == MEMT_RULE_GDN2;
+  if (a->rule != MEMT_RULE_LINEAR && a->rule != MEMT_RULE_GDN2 && a->rule != MEMT_RULE_GATED_DELTA) return MEMT_ERR_INVALID_ARGUMENT;
+  const bool delta = a->rule != MEMT_RULE_LINEAR, gated = a->rule == MEMT_RULE_GATED_DELTA;
   if (a->num_samples < 0 || a->num_heads < 1 || a->num_key_heads < 1 || a->num_heads % a->num_key_heads != 0 ||
       (a->dtype != MEMT_BF16 && a->dtype != MEMT_F32))
     return MEMT_ERR_INVALID_ARGUMENT;
@@ -60,9 +61,14 @@ extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_strea
   if (!delta && (a->g_layout == MEMT_GATE_PER_CHANNEL || a->beta != nullptr || a->erase != nullptr ||
                  a->write != nullptr || a->read_incoming != 0))
     return MEMT_ERR_UNSUPPORTED;
-  if (a->beta_layout < MEMT_GATE_NONE || a->beta_layout > MEMT_GATE_PER_CHANNEL ||
+  if (a->beta_layout < MEMT_GATE_NONE || a->beta_layout > MEMT_GATE_PER_VALUE_HEAD ||
+      a->beta_layout == MEMT_GATE_CONSTANT ||
       (a->beta_layout == MEMT_GATE_NONE) != (a->beta == nullptr))
     return MEMT_ERR_INVALID_ARGUMENT;
+  if (gated ? a->g_layout == MEMT_GATE_PER_CHANNEL || a->beta_layout == MEMT_GATE_PER_CHANNEL ||
+                  a->erase != nullptr || a->write != nullptr || a->read_incoming != 0
+            : a->beta_layout == MEMT_GATE_PER_VALUE_HEAD)
+    return MEMT_ERR_UNSUPPORTED;
   const int64_t row = int64_t(a->num_heads) * D, krow = int64_t(a->num_key_heads) * D;
   if (a->q_stride < krow || a->k_stride < krow || a->v_stride < row || a->out_stride < row)
     return MEMT_ERR_INVALID_ARGUMENT;
@@ -92,6 +98,7 @@ extern "C" int memt_recurrent_step(const memt_recurrent_step_args* a, memt_strea
   p.slots = a->slots;
   p.num_slots = a->num_slots;
   p.incoming = a->read_incoming != 0;
+  p.gated = gated;
   p.out = a->out;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const bool bf16 = a->dtype == MEMT_BF16;

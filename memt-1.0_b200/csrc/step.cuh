@@ -1,8 +1,9 @@
 // One token of a matrix-state recurrence for each session, the states updated in place.
 //
 //   linear attention   S <- e^g S + k v^T,                               o = scale S^T q
-//   gated delta rule   S~ = diag(e^g) S,  d = w v - S~^T (b k'),  S <- S~ + k' d^T,
+//   stable GDN-2       S~ = diag(e^g) S,  d = w v - S~^T (b k'),  S <- S~ + k' d^T,
 //                      o = scale S^T q, with the new state or the incoming one
+//   gated delta rule   S~ = e^g S,  d = beta (v - S~^T k),  S <- S~ + k d^T,     o = scale S^T q
 // with k' = sqrt(beta) k. All arithmetic is fp32 on the fp32 state; the output is rounded once.
 //
 // Bound by HBM: the state is read and written once, 8 D^2 bytes for each (session, head), every
@@ -37,6 +38,7 @@ struct StepParams {
   const int32_t* slots;
   int32_t num_slots;
   int32_t incoming;
+  int32_t gated;  // DELTA: the gated delta rule, beta on the correction instead of the key
   void* out;
 };
 
@@ -49,6 +51,13 @@ __device__ __forceinline__ float load_f32(const void* base, int64_t i) {
 __device__ __forceinline__ void store_f32(float* base, int64_t i, float x) { base[i] = x; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16* base, int64_t i, float x) { base[i] = __float2bfloat16_rn(x); }
 
+// beta of a token and value head, given for each value head or its key head; none: 1
+template <typename T, typename P>
+__device__ __forceinline__ float load_beta(const P& p, int64_t t, int h) {
+  if (p.beta_layout == 0) return 1.f;
+  return p.beta_layout == 4 ? load_f32<T>(p.beta, t * p.H + h) : load_f32<T>(p.beta, t * p.Hk + h / (p.H / p.Hk));
+}
+
 template <int D>
 struct StepCfg {
   static constexpr int kCols = 64;  // value columns per CTA
@@ -60,7 +69,7 @@ struct StepCfg {
   static constexpr int kThreads = 32 * kWarps;
 };
 
-// DELTA: the gated delta rule. T: type of q, k, v, the gates and the output.
+// DELTA: the rules with a correction. T: type of q, k, v, the gates and the output.
 template <int D, bool DELTA, typename T>
 __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepParams p) {
   using Cfg = StepCfg<D>;
@@ -89,6 +98,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
   if (p.slots != nullptr)
     for (int i = tid; i < n; i += NT) taken |= p.slots[i] == static_cast<int32_t>(slot);
   const int64_t qrow = (int64_t)n * p.sq + (int64_t)hk * D, krow = (int64_t)n * p.sk + (int64_t)hk * D;
+  const float beta = DELTA && p.gated ? load_beta<T>(p, n, h) : 1.f;
   for (int i = tid; i < D; i += NT) {
     s_q[i] = load_f32<T>(p.q, qrow + i);
     float k = load_f32<T>(p.k, krow + i);
@@ -98,7 +108,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
     if (p.g_layout == 3) a = expf(p.g[h]);
     s_a[i] = a;
     if constexpr (DELTA) {
-      if (p.beta_layout == 1) k *= sqrtf(load_f32<T>(p.beta, (int64_t)n * p.Hk + hk));
+      if (!p.gated && p.beta_layout == 1) k *= sqrtf(load_f32<T>(p.beta, (int64_t)n * p.Hk + hk));
       if (p.beta_layout == 2) k *= sqrtf(load_f32<T>(p.beta, ((int64_t)n * p.Hk + hk) * D + i));
       s_kb[i] = p.erase != nullptr ? k * load_f32<T>(p.erase, ((int64_t)n * p.Hk + hk) * D + i) : k;
     }
@@ -151,6 +161,10 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
       d[1] -= x.y;
       d[2] -= x.z;
       d[3] -= x.w;
+    }
+    if (p.gated) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) d[e] *= beta;
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {

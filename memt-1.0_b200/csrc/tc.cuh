@@ -239,4 +239,36 @@ __device__ __forceinline__ uint32_t lane_addr(uint32_t base, int lane0, int col)
 }
 
 }  // namespace tc
+
+// Waits and register shares of kernels whose warps have roles of their own.
+__device__ __forceinline__ bool mbar_try(uint32_t mbar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(mbar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// Wait for the phase with the given parity for at most 2^30 clocks (half a second): a poll may
+// suspend the thread, so polls are no measure of time.
+__device__ __forceinline__ bool mbar_wait_clock(uint32_t mbar, uint32_t parity) {
+  if (mbar_try(mbar, parity)) return true;
+  const uint32_t begin = static_cast<uint32_t>(clock());
+#pragma unroll 1
+  while (!mbar_try(mbar, parity))
+    if (static_cast<uint32_t>(clock()) - begin > (1u << 30)) return false;
+  return true;
+}
+
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(R));
+}
+
 }  // namespace memt

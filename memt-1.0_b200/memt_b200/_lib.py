@@ -27,9 +27,11 @@ GATE_NONE = 0
 GATE_PER_HEAD = 1
 GATE_PER_CHANNEL = 2
 GATE_CONSTANT = 3
+GATE_PER_VALUE_HEAD = 4
 
 RULE_LINEAR = 0
 RULE_GDN2 = 1
+RULE_GATED_DELTA = 3
 
 
 class _SizedArgs(ctypes.Structure):
@@ -110,6 +112,19 @@ class LinearAttentionArgs(_SizedArgs):
     ]
 
 
+class GatedDeltaArgs(_SizedArgs):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("num_samples", c_int32), ("num_heads", c_int32), ("num_key_heads", c_int32), ("head_dim", c_int32),
+        ("dtype", c_int32), ("total_tokens", c_int64), ("cu_seqlens", c_void_p),
+        ("q", c_void_p), ("q_stride", c_int64), ("k", c_void_p), ("k_stride", c_int64),
+        ("v", c_void_p), ("v_stride", c_int64), ("g", c_void_p), ("g_layout", c_int32), ("beta_layout", c_int32),
+        ("beta", c_void_p), ("scale", c_float), ("out", c_void_p), ("out_stride", c_int64),
+        ("initial_state", c_void_p), ("final_state", c_void_p), ("initial_slots", c_void_p),
+        ("num_initial_slots", c_int32), ("final_slots", c_void_p), ("num_final_slots", c_int32),
+    ]
+
+
 class RecurrentStepArgs(_SizedArgs):
     _fields_ = [
         ("struct_size", c_uint32),
@@ -130,6 +145,18 @@ class RotaryArgs(_SizedArgs):
         ("k", c_void_p), ("k_stride", c_int64), ("q_out", c_void_p), ("q_out_stride", c_int64),
         ("k_out", c_void_p), ("k_out_stride", c_int64), ("positions", c_void_p), ("positions_int64", c_int32),
         ("interleaved", c_int32), ("inv_freq", c_void_p), ("attention_scale", c_float), ("inverse", c_int32),
+    ]
+
+
+class RotaryAxesArgs(_SizedArgs):
+    _fields_ = [
+        ("struct_size", c_uint32),
+        ("num_heads", c_int32), ("num_key_heads", c_int32), ("head_dim", c_int32), ("rotary_dim", c_int32),
+        ("dtype", c_int32), ("total_tokens", c_int64), ("q", c_void_p), ("q_stride", c_int64),
+        ("k", c_void_p), ("k_stride", c_int64), ("q_out", c_void_p), ("q_out_stride", c_int64),
+        ("k_out", c_void_p), ("k_out_stride", c_int64), ("positions", c_void_p), ("position_stride", c_int64),
+        ("positions_int64", c_int32), ("num_axes", c_int32), ("pair_axes", c_void_p), ("interleaved", c_int32),
+        ("inverse", c_int32), ("inv_freq", c_void_p), ("attention_scale", c_float),
     ]
 
 
@@ -176,8 +203,11 @@ SIGNATURES = {
     "memt_linear_attention_workspace_size": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32]),
     "memt_linear_attention": (c_int, [POINTER(LinearAttentionArgs), c_void_p, c_size_t, c_void_p]),
     "memt_linear_attention_status": (c_int, [c_void_p, POINTER(c_int32)]),
+    "memt_gated_delta_workspace_size": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32]),
+    "memt_gated_delta": (c_int, [POINTER(GatedDeltaArgs), c_void_p, c_size_t, c_void_p]),
     "memt_recurrent_step": (c_int, [POINTER(RecurrentStepArgs), c_void_p]),
     "memt_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
+    "memt_rotary_axes": (c_int, [POINTER(RotaryAxesArgs), c_void_p]),
     "memt_profiler_enable": (c_int, [c_int]),
     "memt_profiler_reset": (c_int, []),
     "memt_profiler_read": (c_int, [POINTER(ctypes.c_double), POINTER(c_int64), c_int]),

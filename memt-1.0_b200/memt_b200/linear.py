@@ -1,10 +1,13 @@
-"""Causal linear attention with a decay for each head, and single-token recurrent steps.
+"""Causal linear attention with a decay for each head, the gated delta rule, and single-token recurrent steps.
 
 * ``linear_attention``       S_t = exp(g_t) S_{t-1} + k_t v_t^T, o_t = scale S_t^T q_t over packed
                              prompts (``memt_linear_attention``)
-* ``linear_attention_step``  the same recurrence for one token of each session, in place
+* ``gated_delta``            S~ = exp(g_t) S_{t-1}, S_t = S~ + beta_t k_t (v_t - S~^T k_t)^T, o_t = scale S_t^T q_t
+                             over packed prompts (``memt_gated_delta``)
+* ``linear_attention_step``  the recurrence of ``linear_attention`` for one token of each session, in place
+* ``gated_delta_step``       the recurrence of ``gated_delta`` for one token of each session, in place
 * ``gdn2_step``              one token of the stable GDN-2 rule (the recurrence of ``gdn2_update``)
-                             for each session, in place (both ``memt_recurrent_step``)
+                             for each session, in place (all three ``memt_recurrent_step``)
 
 States are the framework's fp32 [N, H, K, V] tensors or pools of them addressed by int32 slots, so
 one pool serves ``gdn2_update``, the reads and these operators. Queries and keys may have fewer
@@ -24,7 +27,7 @@ import torch
 from . import _lib
 from .ops import _DTYPE, _pool, _states, _tokens_unchecked
 
-__all__ = ["linear_attention", "linear_attention_step", "gdn2_step"]
+__all__ = ["linear_attention", "gated_delta", "linear_attention_step", "gated_delta_step", "gdn2_step"]
 
 _current_device = torch.cuda.current_device
 _raw_stream = torch._C._cuda_getCurrentRawStream
@@ -52,6 +55,7 @@ def _ptr(x):
 
 
 _linear_args = _lib.Packed(_lib.LinearAttentionArgs)
+_delta_args = _lib.Packed(_lib.GatedDeltaArgs)
 _step_args = _lib.Packed(_lib.RecurrentStepArgs)
 
 
@@ -171,6 +175,34 @@ def _offsets(cu_seqlens, L, dev):
     return cu_seqlens.contiguous()
 
 
+def _prompt_states(initial_state, initial_slots, final_state, final_slots, N, H, D, dev):
+    """Checked states of packed prompts: (initial_state, its slots, their pool's size, final_state, ...)."""
+    n_in = n_out = 0
+    if initial_state is None:
+        if initial_slots is not None:
+            raise ValueError("initial_slots index into initial_state, which must then be given")
+    else:
+        initial_state, initial_slots, n_in = _pool(initial_state, initial_slots, N, H, D, D, dev, "initial_state")
+    if final_state is None:
+        if final_slots is not None:
+            raise ValueError("final_slots index into final_state, which must then be given")
+        final_state = torch.empty(N, H, D, D, device=dev, dtype=torch.float32)
+    elif final_slots is not None:
+        _, final_slots, n_out = _pool(final_state, final_slots, N, H, D, D, dev, "final_state")
+    else:
+        _states(final_state, N, H, D, D, dev, "final_state")
+        if not final_state.is_contiguous():
+            raise ValueError("final_state must be contiguous")
+    return initial_state, initial_slots, n_in, final_state, final_slots, n_out
+
+
+def _prompt_out(out, q, sq, k, sk, v, sv, vec):
+    """(o, elements per token row): the given output's rows or a new tensor like v."""
+    if out is None:
+        return torch.empty(v.shape, device=v.device, dtype=v.dtype), v.shape[1] * v.shape[2]
+    return _out_rows(out, v, ((q, sq), (k, sk), (v, sv)), vec)
+
+
 def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=None, final_state=None,
                      initial_slots=None, final_slots=None):
     """Causal linear attention over packed samples -> (o [L, H, D] in v's dtype, final_state).
@@ -195,26 +227,9 @@ def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=N
     g, g_layout = _head_decay(g, L, H, dev)
     cu = _offsets(cu_seqlens, L, dev)
     N = cu.numel() - 1
-    n_in = n_out = 0
-    if initial_state is None:
-        if initial_slots is not None:
-            raise ValueError("initial_slots index into initial_state, which must then be given")
-    else:
-        initial_state, initial_slots, n_in = _pool(initial_state, initial_slots, N, H, D, D, dev, "initial_state")
-    if final_state is None:
-        if final_slots is not None:
-            raise ValueError("final_slots index into final_state, which must then be given")
-        final_state = torch.empty(N, H, D, D, device=dev, dtype=torch.float32)
-    elif final_slots is not None:
-        _, final_slots, n_out = _pool(final_state, final_slots, N, H, D, D, dev, "final_state")
-    else:
-        _states(final_state, N, H, D, D, dev, "final_state")
-        if not final_state.is_contiguous():
-            raise ValueError("final_state must be contiguous")
-    if out is None:
-        o, so = torch.empty(L, H, D, device=dev, dtype=v.dtype), H * D
-    else:
-        o, so = _out_rows(out, v, ((q, sq), (k, sk), (v, sv)), vec)
+    initial_state, initial_slots, n_in, final_state, final_slots, n_out = _prompt_states(
+        initial_state, initial_slots, final_state, final_slots, N, H, D, dev)
+    o, so = _prompt_out(out, q, sq, k, sk, v, sv, vec)
     lib = _lib.load()
     dtype = _DTYPE[v.dtype]
     need = lib.memt_linear_attention_workspace_size(N, L, H, D, dtype)
@@ -228,6 +243,43 @@ def linear_attention(q, k, v, g, initial_state, cu_seqlens, *, scale=None, out=N
     return o, final_state
 
 
+def gated_delta(q, k, v, g, beta, initial_state, cu_seqlens, *, scale=None, out=None, final_state=None,
+                initial_slots=None, final_slots=None):
+    """The gated delta rule over packed samples, every token reading the state it has just written
+    -> (o [L, H, D] in v's dtype, final_state).
+
+    Per sample, from ``initial_state``: S~ = exp(g_t) S_{t-1}, S_t = S~ + beta_t k_t (v_t - S~^T k_t)^T,
+    o_t = scale S_t^T q_t. q, k: [L, Hk, D]; v: [L, H, D], bf16 or fp32, D 64, 128 or 256 (keys are meant to be of
+    unit length, as ``qwen_prologue`` makes them: beta |k|^2 above 2 lets the state grow). g: fp32 natural-log
+    decay <= 0, [L, H], [H] or None. beta: in v's dtype, [L, H] for each value head or [L, Hk] for each key head, or
+    None (1). ``gated_delta_step`` continues a sample token by token.
+
+    States, slots, offsets, scale and ``out`` as in ``linear_attention``, their rules on overlaps too.
+    """
+    q, sq, k, sk, v, sv, vec = _qkv(q, k, v)
+    L, H, D = v.shape
+    Hk = q.shape[1]
+    dev = v.device
+    g, g_layout = _head_decay(g, L, H, dev)
+    beta, beta_layout = _head_beta(beta, L, Hk, H, v)
+    cu = _offsets(cu_seqlens, L, dev)
+    N = cu.numel() - 1
+    initial_state, initial_slots, n_in, final_state, final_slots, n_out = _prompt_states(
+        initial_state, initial_slots, final_state, final_slots, N, H, D, dev)
+    o, so = _prompt_out(out, q, sq, k, sk, v, sv, vec)
+    lib = _lib.load()
+    dtype = _DTYPE[v.dtype]
+    need = lib.memt_gated_delta_workspace_size(N, L, H, D, dtype)
+    # from the caching allocator, so that neither streams nor captured graphs share it
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need > 256 else None
+    args = _delta_args(
+        N, H, Hk, D, dtype, L, cu.data_ptr(), q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _ptr(g), g_layout,
+        beta_layout, _ptr(beta), D ** -0.5 if scale is None else scale, o.data_ptr(), so, _ptr(initial_state),
+        final_state.data_ptr(), _ptr(initial_slots), n_in, _ptr(final_slots), n_out)
+    _call("memt_gated_delta", dev, args, _ptr(ws), need)
+    return o, final_state
+
+
 def linear_attention_step(q, k, v, g, states, *, scale=None, slots=None, out=None):
     """One token of ``linear_attention`` for each of N sessions -> o [N, H, D]; states in place.
 
@@ -238,6 +290,15 @@ def linear_attention_step(q, k, v, g, states, *, scale=None, slots=None, out=Non
     ``out`` nor the states may overlap any other argument.
     """
     return _step(_lib.RULE_LINEAR, q, k, v, g, states, None, None, None, scale, slots, False, out)
+
+
+def gated_delta_step(q, k, v, g, beta, states, *, scale=None, slots=None, out=None):
+    """One token of ``gated_delta`` for each of N sessions -> o [N, H, D]; states in place.
+
+    S~ = exp(g) S, S = S~ + beta k (v - S~^T k)^T, o = scale S^T q in fp32 arithmetic. g: fp32 [N, H], [H] or None;
+    beta: in v's dtype [N, H] or [N, Hk], or None. States, slots, heads and overlaps as in ``linear_attention_step``.
+    """
+    return _step(_lib.RULE_GATED_DELTA, q, k, v, g, states, beta, None, None, scale, slots, False, out)
 
 
 def gdn2_step(q, k, v, g, states, *, beta=None, erase=None, write=None, scale=None, slots=None, read_incoming=False,
@@ -265,6 +326,14 @@ def _gate_rows(x, shapes, like, name):
     return x.contiguous()
 
 
+def _head_beta(beta, L, Hk, H, like):
+    """beta None, [L, Hk] or [L, H] -> (tensor, layout)."""
+    if beta is None:
+        return None, _lib.GATE_NONE
+    beta = _gate_rows(beta, ((L, Hk), (L, H)), like, "beta")
+    return beta, _lib.GATE_PER_HEAD if beta.shape[1] == Hk else _lib.GATE_PER_VALUE_HEAD
+
+
 def _step(rule, q, k, v, g, states, beta, erase, write, scale, slots, read_incoming, out):
     q, sq, k, sk, v, sv, vec = _qkv(q, k, v)
     N, H, D = v.shape
@@ -272,7 +341,9 @@ def _step(rule, q, k, v, g, states, beta, erase, write, scale, slots, read_incom
     dev = v.device
     g, g_layout = _head_decay(g, N, H, dev, D if rule == _lib.RULE_GDN2 else None)
     beta_layout = _lib.GATE_NONE
-    if beta is not None:
+    if rule == _lib.RULE_GATED_DELTA:
+        beta, beta_layout = _head_beta(beta, N, Hk, H, v)
+    elif beta is not None:
         beta = _gate_rows(beta, ((N, Hk), (N, Hk, D)), v, "beta")
         beta_layout = _lib.GATE_PER_HEAD if beta.dim() == 2 else _lib.GATE_PER_CHANNEL
     if erase is not None:

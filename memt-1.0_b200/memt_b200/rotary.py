@@ -1,7 +1,9 @@
 """Rotary positions of queries and keys (``memt_rotary``), and the frequencies they turn by.
 
-``rotary`` prepares q and k for ``linear_attention`` and its step; ``rotary_frequencies`` builds the
-angles per position, also stretched for contexts longer than the trained one.
+``rotary`` prepares q and k for ``linear_attention``, ``gated_delta`` and their steps; ``rotary_axes``
+(``memt_rotary_axes``) does so for tokens that have a position on several axes, as the patches of images and
+video do. ``rotary_frequencies`` builds the angles per position, also stretched for contexts longer than the
+trained one; ``rotary_sections`` says which axis turns which pair.
 """
 
 from __future__ import annotations
@@ -14,9 +16,10 @@ from . import _lib
 from .linear import _call, _overlap, _ptr
 from .ops import _DTYPE, _tokens_unchecked
 
-__all__ = ["rotary", "rotary_frequencies"]
+__all__ = ["rotary", "rotary_axes", "rotary_frequencies", "rotary_sections"]
 
 _rotary_args = _lib.Packed(_lib.RotaryArgs)
+_axes_args = _lib.Packed(_lib.RotaryAxesArgs)
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, trained_tokens=None, fast_turns=32.0,
@@ -61,6 +64,21 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
     return inv.to(device), attention_scale
 
 
+def rotary_sections(sections, *, cycled=False, device="cuda"):
+    """The axis of every pair (int32 [sum(sections)] on ``device``) for ``rotary_axes``: axis a turns
+    ``sections[a]`` pairs, one run of pairs after another, or with ``cycled`` the axes take turns for as long as
+    each has pairs left.
+    """
+    sections = [int(n) for n in sections]
+    if not sections or min(sections) < 0 or sum(sections) < 1:
+        raise ValueError("sections must hold a count of pairs for each axis, one pair at least")
+    if cycled:
+        axes = [a for turn in range(max(sections)) for a, n in enumerate(sections) if turn < n]
+    else:
+        axes = [a for a, n in enumerate(sections) for _ in range(n)]
+    return torch.tensor(axes, dtype=torch.int32).to(device)
+
+
 def _head_rows(x, name):
     """[1, L, H, D] or [L, H, D] with contiguous heads -> ([L, H, D], elements per token row)."""
     if x.dim() != 3 or not x.is_cuda:
@@ -87,6 +105,22 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, inverse=False, atten
     [L]. inv_freq: fp64 on the device (``rotary_frequencies``). ``q_out`` / ``k_out`` may be q / k
     themselves (in place); other overlaps of an output with an input or output are refused.
     """
+    return _rotary(q, k, positions, inv_freq, None, interleaved, inverse, attention_scale, q_out, k_out)
+
+
+def rotary_axes(q, k, positions, inv_freq, pair_axes, *, interleaved=False, inverse=False, attention_scale=1.0,
+                q_out=None, k_out=None):
+    """``rotary`` for tokens with a position on each of several axes -> (q_out [L, H, D], k_out [L, Hk, D]).
+
+    Pair i is turned by positions[pair_axes[i], token] * inv_freq[i]. positions: int32 or int64 [axes, L] (or
+    [axes, 1, L]; rows may be strided, as a slice of a longer buffer is). pair_axes: int32 on the device, one for
+    each of inv_freq's pairs (``rotary_sections``); a pair whose axis is none of positions' stays at position 0.
+    Everything else as in ``rotary``: ``inverse`` with the same scale is the backward pass.
+    """
+    return _rotary(q, k, positions, inv_freq, pair_axes, interleaved, inverse, attention_scale, q_out, k_out)
+
+
+def _rotary(q, k, positions, inv_freq, axes, interleaved, inverse, attention_scale, q_out, k_out):
     q, sq = _head_rows(q, "q")
     L, H, D = q.shape
     dev = q.device
@@ -102,13 +136,28 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, inverse=False, atten
             raise ValueError("k must be [L, key heads, D] in q's dtype and on its device")
     elif k_out is not None:
         raise ValueError("k_out needs k")
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((L,), (1, L)):
-        raise ValueError(f"positions must be int32 or int64 [{L}]")
+    if axes is None:
+        if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((L,), (1, L)):
+            raise ValueError(f"positions must be int32 or int64 [{L}]")
+    else:
+        if positions.dim() == 3 and positions.shape[1] == 1:
+            positions = positions[:, 0]
+        if positions.dtype not in (torch.int32, torch.int64) or positions.dim() != 2 or positions.shape[0] < 1 \
+                or positions.shape[1] != L:
+            raise ValueError(f"positions must be int32 or int64 [axes, {L}]")
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 2 <= 2 * inv_freq.numel() <= D:
         raise ValueError(f"inv_freq must be fp64 with at most {D // 2} angles")
     if positions.device != dev or inv_freq.device != dev:
         raise ValueError(f"positions and inv_freq must be on {dev}")
-    positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+    inv_freq = inv_freq.contiguous()
+    if axes is None:
+        positions = positions.contiguous()
+    else:
+        if axes.dtype != torch.int32 or axes.device != dev or axes.shape != inv_freq.shape:
+            raise ValueError(f"pair_axes must be int32 [{inv_freq.numel()}] on {dev}")
+        axes = axes.contiguous()
+        if L > 1 and positions.stride(1) != 1 or positions.shape[0] > 1 and positions.stride(0) < L:
+            positions = positions.contiguous()
     qo, sqo = _output(q, sq, q_out, "q_out")
     ko, sko = (None, 0) if k is None else _output(k, sk, k_out, "k_out")
     if k is not None and (q_out is not None or k_out is not None):
@@ -119,11 +168,19 @@ def rotary(q, k, positions, inv_freq, *, interleaved=False, inverse=False, atten
             raise ValueError("q_out and k_out must not overlap each other or the other input")
     if L == 0 or H == 0:
         return qo, ko
-    args = _rotary_args(
-        H, Hk, D, 2 * inv_freq.numel(), _DTYPE[q.dtype], L, q.data_ptr(), sq, _ptr(k), sk, qo.data_ptr(), sqo, _ptr(ko),
-        sko, positions.data_ptr(), 1 if positions.dtype is torch.int64 else 0, 1 if interleaved else 0,
-        inv_freq.data_ptr(), attention_scale, 1 if inverse else 0)
-    _call("memt_rotary", dev, args)
+    if axes is None:
+        args = _rotary_args(
+            H, Hk, D, 2 * inv_freq.numel(), _DTYPE[q.dtype], L, q.data_ptr(), sq, _ptr(k), sk, qo.data_ptr(), sqo,
+            _ptr(ko), sko, positions.data_ptr(), 1 if positions.dtype is torch.int64 else 0, 1 if interleaved else 0,
+            inv_freq.data_ptr(), attention_scale, 1 if inverse else 0)
+        _call("memt_rotary", dev, args)
+    else:
+        args = _axes_args(
+            H, Hk, D, 2 * inv_freq.numel(), _DTYPE[q.dtype], L, q.data_ptr(), sq, _ptr(k), sk, qo.data_ptr(), sqo,
+            _ptr(ko), sko, positions.data_ptr(), positions.stride(0), 1 if positions.dtype is torch.int64 else 0,
+            positions.shape[0], axes.data_ptr(), 1 if interleaved else 0, 1 if inverse else 0, inv_freq.data_ptr(),
+            attention_scale)
+        _call("memt_rotary_axes", dev, args)
     return qo, ko
 
 
