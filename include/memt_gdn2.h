@@ -487,6 +487,9 @@ size_t memt_gated_delta_workspace_size(int32_t num_samples, int64_t total_tokens
 int memt_gated_delta(const memt_gated_delta_args *args, void *workspace, size_t workspace_bytes,
                      memt_stream_t stream);
 
+/* As memt_linear_attention_status, of the bf16 calls of memt_gated_delta. */
+int memt_gated_delta_status(memt_stream_t stream, int32_t *status_out);
+
 /* ---- one token of a recurrence, states in place --------------------------
  *
  * No counterpart in the reference (its executor commits through the chunked update): the

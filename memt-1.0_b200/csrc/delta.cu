@@ -1,5 +1,6 @@
 // memt_gated_delta: argument checks and launch of the gated delta rule over prompts.
 #include "delta.cuh"
+#include "delta_tc.cuh"
 #include "launch.h"
 #include "prompts.h"
 
@@ -25,6 +26,40 @@ int launch_tokens(int D, const DeltaParams& p, cudaStream_t s) {
     default: return launch_tokens<256, T>(p, s);
   }
 }
+
+// Multiprocessors the order of samples is planned for.
+constexpr int kPlanSms = 148;
+
+template <int D>
+int launch_chunked(const DeltaParams& p, cudaStream_t s) {
+  using Cfg = DeltaTcCfg<D>;
+  DeltaTcParams P;
+  P.p = p;
+  const uint64_t rows = static_cast<uint64_t>(p.L);
+  cudaError_t e = make_tmap_bf16_2d(&P.q_map, p.q, uint64_t(p.Hk) * D, rows, uint64_t(p.sq) * 2, 64, kTile);
+  if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.k_map, p.k, uint64_t(p.Hk) * D, rows, uint64_t(p.sk) * 2, 64, kTile);
+  if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.v_map, p.v, uint64_t(p.H) * D, rows, uint64_t(p.sv) * 2, 64, kTile);
+  if (e == cudaSuccess) e = make_tmap_bf16_2d_sw64(&P.o_map, p.out, uint64_t(p.H) * D, rows, uint64_t(p.so) * 2, 32);
+  if (e == cudaSuccess) e = ensure_smem(delta_tc_kernel<D>, Cfg::kSmem);
+  if (e != cudaSuccess) return cuda_status(e);
+  // More CTAs than SMs: the longest samples first, so that no SM is left with one at the end.
+  P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms && p.L / p.N >= 1024;
+  const int64_t grid = int64_t(p.only_long > 0 ? p.only_long : p.N) * p.H * Cfg::kBlocks;
+  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  ProfScope prof(kProfLinear, s);
+  delta_tc_kernel<D><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
+  return cuda_status(cudaGetLastError());
+}
+
+int launch_chunked(int D, const DeltaParams& p, cudaStream_t s) {
+  switch (D) {
+    case 64: return launch_chunked<64>(p, s);
+    default: return launch_chunked<128>(p, s);
+  }
+}
+
+// Tokens up to which a bf16 sample runs token by token.
+int few_tokens(int D) { return D == 64 ? 24 : 8; }
 
 int check_delta(const memt_gated_delta_args* a) {
   const int st = check_prompts(a);
@@ -87,12 +122,36 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
   p.num_in = a->num_initial_slots;
   p.slots_out = a->final_slots;
   p.num_out = a->num_final_slots;
-  p.few = INT32_MAX;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (a->dtype == MEMT_F32) return launch_tokens<float>(a->head_dim, p, s);
-  return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+  // fp32, and calls without tokens, which only copy the states: all samples token by token
+  p.few = INT32_MAX;
+  if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_tokens<float>(a->head_dim, p, s);
+  const int few = few_tokens(a->head_dim);
+  if (a->head_dim == 256 || a->total_tokens <= few) return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+  p.few = -1;
+  if (a->num_samples > 1 && a->total_tokens <= int64_t(64) * a->num_samples) {
+    p.few = few;
+    const int64_t most = p.L / (few + 1);
+    p.only_long = most <= p.N / 2 ? static_cast<int32_t>(most) : 0;
+    const int st_few = launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+    if (st_few != MEMT_OK) return st_few;
+  }
+  return launch_chunked(a->head_dim, p, s);
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;
+}
+
+int memt_gated_delta_status(memt_stream_t stream, int32_t* status_out) {
+  if (status_out == nullptr) return MEMT_ERR_INVALID_ARGUMENT;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int zero = 0;
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&v, g_delta_status, sizeof(v), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_delta_status, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  if (e != cudaSuccess) return cuda_status(e);
+  *status_out = v;
+  return MEMT_OK;
 }
 
 }  // extern "C"

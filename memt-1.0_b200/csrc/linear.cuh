@@ -166,6 +166,19 @@ __device__ __forceinline__ void split_decay(double a, float& hi, float& lo) {
   lo = low_half(hi, static_cast<float>(a - static_cast<double>(hi)));
 }
 
+// 2^y as such a pair. 2^y = 2^n 2^f, |f| <= 1/2, by the Taylor series of 2^f in 64 bits (the first term left out is
+// below 2^-37); below 2^-900 it is zero in fp32.
+__device__ __forceinline__ void chunk_decay(double y, float& hi, float& lo) {
+  const double nr = rint(y), f = (y - nr) * 0.6931471805599453;
+  constexpr double kInvFact[9] = {1.0,       1.0,       1.0 / 2,    1.0 / 6,    1.0 / 24,
+                                  1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320};
+  double a = 1.0 / 362880;
+#pragma unroll
+  for (int i = 8; i >= 0; --i) a = fma(a, f, kInvFact[i]);
+  a = y < -900.0 ? 0.0 : a * __longlong_as_double((static_cast<long long>(nr) + 1023) << 52);
+  split_decay(a, hi, lo);
+}
+
 __device__ __forceinline__ float log_decay(const LinearParams& p, int64_t t, int h) {
   return p.g_layout == 1 ? p.g[t * p.H + h] : (p.g_layout == 3 ? p.g[h] : 0.f);
 }

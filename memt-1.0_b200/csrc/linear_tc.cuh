@@ -503,17 +503,7 @@ __global__ void __launch_bounds__(LinearTcCfg<D>::kThreads, 1)
           t.between[lane] = fast_exp2(x);
         }
         if (lane == 0) {
-          // e^total = 2^n 2^f, |f| <= 1/2, by the Taylor series of 2^f in 64 bits (the first term left out is
-          // below 2^-37); e^total below 2^-900 is zero in fp32
-          const double y = total * 1.4426950408889634;
-          const double nr = rint(y), f = (y - nr) * 0.6931471805599453;
-          constexpr double kInvFact[9] = {1.0,       1.0,       1.0 / 2,    1.0 / 6,    1.0 / 24,
-                                          1.0 / 120, 1.0 / 720, 1.0 / 5040, 1.0 / 40320};
-          double a = 1.0 / 362880;
-#pragma unroll
-          for (int i = 8; i >= 0; --i) a = fma(a, f, kInvFact[i]);
-          a = y < -900.0 ? 0.0 : a * __longlong_as_double((static_cast<long long>(nr) + 1023) << 52);
-          split_decay(a, t.a_hi, t.a_lo);
+          chunk_decay(total * 1.4426950408889634, t.a_hi, t.a_lo);
         }
         arrive(TF + ts);
       }

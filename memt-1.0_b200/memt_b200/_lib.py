@@ -205,6 +205,7 @@ SIGNATURES = {
     "memt_linear_attention_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "memt_gated_delta_workspace_size": (c_size_t, [c_int32, c_int64, c_int32, c_int32, c_int32]),
     "memt_gated_delta": (c_int, [POINTER(GatedDeltaArgs), c_void_p, c_size_t, c_void_p]),
+    "memt_gated_delta_status": (c_int, [c_void_p, POINTER(c_int32)]),
     "memt_recurrent_step": (c_int, [POINTER(RecurrentStepArgs), c_void_p]),
     "memt_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
     "memt_rotary_axes": (c_int, [POINTER(RotaryAxesArgs), c_void_p]),
