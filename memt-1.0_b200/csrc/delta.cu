@@ -30,9 +30,13 @@ int launch_tokens(int D, const DeltaParams& p, cudaStream_t s) {
 // Multiprocessors the order of samples is planned for.
 constexpr int kPlanSms = 148;
 
+// chunks of 64 tokens that N samples of L tokens can have between them, one at least for each
+int64_t max_units(int64_t N, int64_t L) { return L / kTile + N; }
+
 template <int D>
 int launch_chunked(const DeltaParams& p, cudaStream_t s) {
   using Cfg = DeltaTcCfg<D>;
+  using Pre = DeltaChunksCfg<D>;
   DeltaTcParams P;
   P.p = p;
   const uint64_t rows = static_cast<uint64_t>(p.L);
@@ -40,12 +44,20 @@ int launch_chunked(const DeltaParams& p, cudaStream_t s) {
   if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.k_map, p.k, uint64_t(p.Hk) * D, rows, uint64_t(p.sk) * 2, 64, kTile);
   if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.v_map, p.v, uint64_t(p.H) * D, rows, uint64_t(p.sv) * 2, 64, kTile);
   if (e == cudaSuccess) e = make_tmap_bf16_2d_sw64(&P.o_map, p.out, uint64_t(p.H) * D, rows, uint64_t(p.so) * 2, 32);
+  if (e == cudaSuccess) e = ensure_smem(delta_chunks_kernel<D>, Pre::kSmem);
   if (e == cudaSuccess) e = ensure_smem(delta_tc_kernel<D>, Cfg::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
+  const int64_t units = p.max_segments * int64_t(p.H);
+  const int64_t grid = int64_t(p.only_long > 0 ? p.only_long : p.N) * p.H * Cfg::kBlocks;
+  if (units > INT32_MAX || grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  {
+    ProfScope prof(kProfLinear, s);
+    delta_chunks_kernel<D><<<static_cast<unsigned>(units), Pre::kThreads, Pre::kSmem, s>>>(P);
+    const int st = cuda_status(cudaGetLastError());
+    if (st != MEMT_OK) return st;
+  }
   // More CTAs than SMs: the longest samples first, so that no SM is left with one at the end.
   P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms && p.L / p.N >= 1024;
-  const int64_t grid = int64_t(p.only_long > 0 ? p.only_long : p.N) * p.H * Cfg::kBlocks;
-  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   ProfScope prof(kProfLinear, s);
   delta_tc_kernel<D><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
   return cuda_status(cudaGetLastError());
@@ -54,7 +66,8 @@ int launch_chunked(const DeltaParams& p, cudaStream_t s) {
 int launch_chunked(int D, const DeltaParams& p, cudaStream_t s) {
   switch (D) {
     case 64: return launch_chunked<64>(p, s);
-    default: return launch_chunked<128>(p, s);
+    case 128: return launch_chunked<128>(p, s);
+    default: return launch_chunked<256>(p, s);
   }
 }
 
@@ -80,7 +93,8 @@ extern "C" {
 size_t memt_gated_delta_workspace_size(int32_t N, int64_t L, int32_t H, int32_t D, int32_t dtype) {
   if (N < 1 || L < 0 || H < 1 || (D != 64 && D != 128 && D != 256)) return 0;
   if (dtype != MEMT_F32 && dtype != MEMT_BF16) return 0;
-  return 256;
+  if (dtype == MEMT_F32 || L <= few_tokens(D)) return 256;  // token by token
+  return (size_t(max_units(N, L)) * H * DeltaChunks::kBytes + 255) & ~size_t(255);
 }
 
 int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t workspace_bytes,
@@ -127,7 +141,7 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
   p.few = INT32_MAX;
   if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_tokens<float>(a->head_dim, p, s);
   const int few = few_tokens(a->head_dim);
-  if (a->head_dim == 256 || a->total_tokens <= few) return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+  if (a->total_tokens <= few) return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
   p.few = -1;
   if (a->num_samples > 1 && a->total_tokens <= int64_t(64) * a->num_samples) {
     p.few = few;
@@ -136,6 +150,9 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
     const int st_few = launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
     if (st_few != MEMT_OK) return st_few;
   }
+  p.chunks = workspace;
+  p.seg_chunks = 1;
+  p.max_segments = static_cast<int32_t>(max_units(p.N, p.L));
   return launch_chunked(a->head_dim, p, s);
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;

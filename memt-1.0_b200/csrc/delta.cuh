@@ -22,7 +22,27 @@ namespace memt {
 struct DeltaParams : LinearParams {
   const void* beta;
   int32_t beta_layout;  // MEMT_GATE_NONE / PER_HEAD (key heads) / PER_VALUE_HEAD
+  // Chunked form (delta_chunks.cuh, delta_tc.cuh): what each chunk needs of its keys, queries and gates, [unit][H] of
+  // DeltaChunks::kBytes. The units are the segments of linear.cuh, of one chunk each (seg_chunks 1).
+  void* chunks;
 };
+
+// The units of sample n, by a converged warp: the first one's number and how many; fewer than the sample has
+// chunks only where offsets overlap (segments_up_to).
+__device__ __forceinline__ void sample_units(const DeltaParams& p, int n, int& first, int& count) {
+  int64_t bos, eos;
+  first = 0;
+  for (int m = threadIdx.x & 31; m < n; m += 32) {
+    sample_range(p, m, bos, eos);
+    first += segments_of(p, eos - bos);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
+  sample_range(p, n, bos, eos);
+  count = segments_up_to(p, n, first + segments_of(p, eos - bos));
+  first = n == 0 ? 0 : segments_up_to(p, n - 1, first);
+  count -= first;
+}
 
 // A warp's columns of one state, four to a lane, and a token's step on them.
 template <int D>

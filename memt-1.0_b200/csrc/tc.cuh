@@ -43,6 +43,13 @@ __device__ __forceinline__ uint64_t desc_mnmajor(uint32_t tile, uint32_t panel_b
   return desc_sw128(tile + static_cast<uint32_t>(ks) * 2048u, panel_bytes, 1024);
 }
 
+// K-major operand tile without a swizzle: core matrices of 8 rows by 16 bytes, the two of a K step lbo bytes apart,
+// those of the next 8 rows sbo
+__device__ __forceinline__ uint64_t desc_plain(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 |
+         static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32 | static_cast<uint64_t>(1) << 46;
+}
+
 enum : int { kF16 = 0, kBF16 = 1, kTF32 = 2 };
 // instruction descriptor: fp32 accumulator, dense, no negation
 __host__ __device__ constexpr uint32_t idesc(int fmt, int M, int N, bool a_mn, bool b_mn) {
@@ -138,8 +145,9 @@ __device__ __forceinline__ void ld8(uint32_t taddr, float (&v)[8]) {
 }
 template <int N>
 __device__ __forceinline__ void ldn(uint32_t taddr, float (&v)[N]) {
-  static_assert(N == 8 || N == 32, "columns");
+  static_assert(N == 8 || N == 16 || N == 32, "columns");
   if constexpr (N == 8) ld8(taddr, v);
+  else if constexpr (N == 16) ld16(taddr, v);
   else ld32(taddr, v);
 }
 
@@ -158,16 +166,6 @@ __device__ __forceinline__ void ld_frag<2>(uint32_t taddr, uint32_t (&r)[8]) {
       "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
       "tcgen05.wait::ld.sync.aligned;"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-      : "r"(taddr)
-      : "memory");
-}
-template <>
-__device__ __forceinline__ void ld_frag<4>(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
 }
@@ -192,6 +190,12 @@ __device__ __forceinline__ void ld_frag2<2>(uint32_t a0, uint32_t a1, uint32_t (
         "=r"(q[0]), "=r"(q[1]), "=r"(q[2]), "=r"(q[3]), "=r"(q[4]), "=r"(q[5]), "=r"(q[6]), "=r"(q[7])
       : "r"(a0), "r"(a1)
       : "memory");
+}
+// 8 columns of 16 lanes
+__device__ __forceinline__ void st_frag8(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
 }
 // 16 columns of 16 lanes
 __device__ __forceinline__ void st_frag16(uint32_t taddr, const uint32_t (&r)[8]) {
@@ -268,6 +272,29 @@ __device__ __forceinline__ bool mbar_wait_clock(uint32_t mbar, uint32_t parity) 
   const uint32_t begin = static_cast<uint32_t>(clock());
 #pragma unroll 1
   while (!mbar_try(mbar, parity))
+    if (static_cast<uint32_t>(clock()) - begin > (1u << 30)) return false;
+  return true;
+}
+
+// The same in three instructions a poll, the clock read once in 64: where many warps wait at once, their polls
+// take issue slots from those that work.
+__device__ __forceinline__ bool mbar_polls(uint32_t mbar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 64;\n"
+      "LOOP_%=:\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      " @p bra DONE_%=;\n sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra LOOP_%=;\n"
+      "DONE_%=:\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(mbar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool mbar_wait_polls(uint32_t mbar, uint32_t parity) {
+  if (mbar_polls(mbar, parity)) return true;
+  const uint32_t begin = static_cast<uint32_t>(clock());
+#pragma unroll 1
+  while (!mbar_polls(mbar, parity))
     if (static_cast<uint32_t>(clock()) - begin > (1u << 30)) return false;
   return true;
 }

@@ -12,9 +12,9 @@ import random
 
 import pytest
 
-STAGES, TABLES = {64: 4, 128: 3}, 4
-READERS = {"KQ": 1, "V": 8, "table": 12, "scores": 4, "A": 4, "T": 1, "B": 1, "S": 1, "X": 8, "R": 1, "U": 8, "W": 1,
-           "P": 8, "out": 4}
+TABLES = 4
+READERS = {"KQ": 1, "V": 16, "TB": 1, "table": 20, "S": 1, "X": 8, "R": 1, "U": 8, "W": 1, "P": 8, "out": 4,
+           "xq": 4, "over": 4}
 
 
 class _Barrier:
@@ -29,29 +29,34 @@ class _Barrier:
             self.pending = self.count
 
 
-def _roles(D, n):
-    """(barriers, role name -> generator) of one CTA with n chunks. The names are the kernel's."""
-    ns, bars = STAGES[D], {}
+def _roles(ns, n, alias):
+    """(barriers, role name -> generator) of one CTA with n chunks, ns stages; alias: O lies on
+    U (D = 256). The names are the kernel's."""
+    bars = {}
 
     def add(names, number, count):
         for name in names.split():
             for i in range(number):
                 bars[name, i] = _Barrier(count)
 
-    add("KF VF KE", ns, 1)
-    add("VE", ns, 8)
+    add("LF LE", ns, 1)
     add("TF", TABLES, 1)
-    add("TE", TABLES, 12)
-    add("SC XD UD PD OD", 1, 1)
-    add("SR AE TW OE", 1, 4)
-    add("AW BW", 1, 2)
-    add("SB RW WW", 1, 8)
+    add("TE", TABLES, 20)
+    add("XD UD PD", 2, 1)
+    add("OD", 1, 1)
+    add("OE", 1, 4)
+    # named barriers, in warps; those in pairs are of the chain's halves
+    add("barS barR barW", 2, 9)
+    add("barEnd", 1, 20)
 
     def wait(name, phase, i=0):
         return "wait", (name, i), phase
 
     def arrive(name, i=0):
         return "arrive", (name, i), None
+
+    def sync(name, i=0):
+        return "sync", (name, i), None
 
     def issue(reads, writes, *barriers):  # a batch of MMAs: what it reads and writes, the barriers it arrives on
         return "issue", barriers, (reads, writes)
@@ -63,38 +68,33 @@ def _roles(D, n):
         return "writes", what, None
 
     def mma():
-        def scores(c):
-            yield wait("KF", c // ns, c % ns)
-            if c > 0:
-                yield wait("SR", c - 1)
-            yield issue([("KQ", c % ns, c, 0)], [("scores", 0, c)], ("SC", 0))
-
-        if n:
-            yield from scores(0)
         for c in range(n):
             s = c % ns
-            yield wait("SB", c)
-            yield issue([("KQ", s, c, 0), ("S", 0, c, 0)], [("X", 0, c)], ("XD", 0))
-            if c + 1 < n:
-                yield from scores(c + 1)
-            yield wait("RW", c)
-            yield wait("TW", c)
-            yield issue([("R", 0, c, 1), ("T", 0, c, 1)], [("U", 0, c)], ("UD", 0))
-            if c > 0:
+            yield wait("LF", c // ns, s)
+            yield sync("barS", 0)
+            yield issue([("KQ", s, c, 0), ("S", 0, c, 0)], [])
+            yield sync("barS", 1)
+            yield issue([("KQ", s, c, 0), ("S", 1, c, 0)], [("X", 0, c), ("X", 1, c)], ("XD", 0), ("XD", 1))
+            if alias and c > 0:
                 yield wait("OE", c - 1)
-            yield issue([("KQ", s, c, 0), ("S", 0, c, 1)], [("out", 0, c)])
-            yield wait("WW", c)
-            yield issue([("KQ", s, c, 1), ("W", 0, c, 0)], [("P", 0, c)], ("PD", 0), ("KE", s))
-            yield wait("BW", c)
-            yield issue([("B", 0, c, 1), ("W", 0, c, 1)], [], ("OD", 0))
+            yield issue([("KQ", s, c, 0), ("S", 0, c, 1), ("S", 1, c, 1)], [("xq", 0 if alias else c & 1, c)])
+            yield sync("barR", 0)
+            yield issue([("R", 0, c, 0), ("TB", s, c, 0)], [("U", 0, c)] + [("over", 0, c)] * alias, ("UD", 0))
+            yield sync("barR", 1)
+            yield issue([("R", 0, c, 1), ("R", 1, c, 1), ("TB", s, c, 0)], [("U", 1, c)], ("UD", 1))
+            yield sync("barW", 0)
+            yield issue([("KQ", s, c, 0), ("W", 0, c, 0)], [])
+            yield sync("barW", 1)
+            yield issue([("KQ", s, c, 1), ("W", 1, c, 0)], [("P", 0, c), ("P", 1, c)], ("PD", 0), ("PD", 1))
+            if not alias and c > 0:
+                yield wait("OE", c - 1)
+            yield issue([("TB", s, c, 1), ("W", 0, c, 1), ("W", 1, c, 1)], [("out", 0, c)], ("OD", 0), ("LE", s))
 
     def loads():
         for c in range(n):
-            s = c % ns
-            for full, free, what in (("KF", "KE", "KQ"), ("VF", "VE", "V")):
-                if c >= ns:
-                    yield wait(free, c // ns - 1, s)
-                yield "load", (full, s), (what, s, c)
+            if c >= ns:
+                yield wait("LE", c // ns - 1, c % ns)
+            yield "load", ("LF", c % ns), [(what, c % ns, c) for what in ("KQ", "V", "TB")]
 
     def table(first):
         for c in range(first, n, 2):
@@ -103,76 +103,54 @@ def _roles(D, n):
             yield writes(("table", c % TABLES, c))
             yield arrive("TF", c % TABLES)
 
-    def invert(i):
+    def outputs(i):
         for c in range(n):
-            yield wait("AW", c)
-            yield reads(("A", 0, c, 1))
-            if c > 0:
-                yield wait("UD", c - 1)
-            if i == 0:
-                yield writes(("T", 0, c))
-            yield arrive("TW")
-            yield arrive("AE")
-
-    def outputs(quad):
-        b = quad >= 2
-
-        def prepare(c):
             yield wait("TF", c // TABLES, c % TABLES)
-            yield wait("SC", c)
-            if c > 0:
-                yield wait("OD" if b else "AE", c - 1)
-            yield reads(("scores", 0, c, 1))
-            if quad == 1 or quad == 3:
-                yield writes(("B" if b else "A", 0, c))
-            yield arrive("SR")
-            yield arrive("BW" if b else "AW")
-
-        def write_out(c):
             yield wait("OD", c)
-            yield reads(("out", 0, c, 1))
+            for _ in range(30):  # (they take their time)
+                yield reads()
+            yield reads(("out", 0, c, 1), ("xq", 0 if alias else c & 1, c, 1), *[("over", 0, c, 1)] * alias)
             yield arrive("OE")
             yield reads(("table", c % TABLES, c, 1))
             yield arrive("TE", c % TABLES)
-
-        for c in range(n):
-            yield from prepare(c)
-            if c > 0:
-                yield from write_out(c - 1)
-        if n:
-            yield from write_out(n - 1)
+        yield sync("barEnd")
 
     def chain(i):
-        for c in range(n):
-            s = c % ns
-            if c > 0:
-                yield reads(("P", 0, c - 1, 1))
-            if i == 0:
-                yield writes(("S", 0, c))
-            yield arrive("SB")
-            yield wait("VF", c // ns, s)
+        half = i // 8
+
+        def fetch(c):
+            yield wait("LF", c // ns, c % ns)
             yield wait("TF", c // TABLES, c % TABLES)
-            yield reads(("V", s, c, 1))
-            yield arrive("VE", s)
-            yield wait("XD", c)
-            yield reads(("X", 0, c, 1))
-            if i == 0:
-                yield writes(("R", 0, c))
-            yield arrive("RW")
-            yield wait("UD", c)
-            yield reads(("U", 0, c, 1), ("table", c % TABLES, c, 1))
-            if i == 0:
-                yield writes(("W", 0, c))
-            yield arrive("WW")
-            yield arrive("TE", c % TABLES)
-            yield wait("PD", c)
+            yield reads(("V", c % ns, c, 1), ("table", c % TABLES, c, 0))
+
         if n:
-            yield reads(("P", 0, n - 1, 1))
+            yield from fetch(0)
+        for c in range(n):
+            if i % 8 == 0:
+                yield writes(("S", half, c))
+            yield arrive("barS", half)
+            yield wait("XD", c, half)
+            yield reads(("X", half, c, 1))
+            if i % 8 == 0:
+                yield writes(("R", half, c))
+            yield arrive("barR", half)
+            yield reads(("table", c % TABLES, c, 0))
+            yield wait("UD", c, half)
+            yield reads(("U", half, c, 1))
+            if i % 8 == 0:
+                yield writes(("W", half, c))
+            yield arrive("barW", half)
+            yield reads(("table", c % TABLES, c, 1))
+            yield arrive("TE", c % TABLES)
+            if c + 1 < n:
+                yield from fetch(c + 1)
+            yield wait("PD", c, half)
+            yield reads(("P", half, c, 1))
+        yield sync("barEnd")
 
     roles = {"mma": mma(), "loads": loads(), "table 0": table(0), "table 1": table(1)}
-    roles.update({f"invert {i}": invert(i) for i in range(4)})
     roles.update({f"outputs {i}": outputs(i) for i in range(4)})
-    roles.update({f"chain {i}": chain(i) for i in range(8)})
+    roles.update({f"chain {i}": chain(i) for i in range(16)})
     return bars, roles
 
 
@@ -189,15 +167,13 @@ class _Buffers:
 
     def read(self, name, place, chunk, last):
         old = self.held.get((name, place))
-        if name == "W" and old is None and chunk == 0:
-            return
         assert old is not None and old[0] == chunk, f"{name} {place}: chunk {old and old[0]} read as {chunk}"
         old[1] -= last
 
 
-def _run(D, n, seed, edit=None):
+def _run(ns, n, seed, edit=None, alias=False):
     rng = random.Random(seed)
-    bars, roles = _roles(D, n)
+    bars, roles = _roles(ns, n, alias)
     if edit is not None:
         edit(bars, roles)
     buffers = _Buffers()
@@ -215,6 +191,8 @@ def _run(D, n, seed, edit=None):
                 assert done >= op[2], f"underrun: {name} waits for phase {op[2]} of {op[1]}, {done} are done"
                 if done == op[2]:
                     continue
+            if op[0] == "joined" and bars[op[1]].done == op[2]:
+                continue
             ready.append(name)
         ready += ["tensor pipe"] * bool(batches) + ["tma"] * bool(tiles)
         if not ready:
@@ -232,10 +210,15 @@ def _run(D, n, seed, edit=None):
                 bars[b].arrive()
         elif name == "tma":
             barrier, what = tiles.pop(rng.randrange(len(tiles)))
-            buffers.write(*what)
+            for w in what:
+                buffers.write(*w)
             bars[barrier].arrive()
         else:
             kind, what, more = at[name]
+            if kind == "sync":  # arrives, and waits for the others
+                at[name] = "joined", what, bars[what].done
+                bars[what].arrive()
+                continue
             if kind == "arrive":
                 bars[what].arrive()
             elif kind == "issue":
@@ -251,20 +234,22 @@ def _run(D, n, seed, edit=None):
             at[name] = next(roles[name], None)
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("stages,alias", [(3, False), (2, True)])
 @pytest.mark.parametrize("chunks", [0, 1, 2, 3, 4, 5, 9, 14])
-def test_no_order_stalls_or_overtakes(D, chunks):
-    for seed in range(12):
-        _run(D, chunks, seed)
+def test_no_order_stalls_or_overtakes(stages, alias, chunks):
+    for seed in range(20):
+        _run(stages, chunks, seed, alias=alias)
 
 
-@pytest.mark.parametrize("name,role", [("UD", "invert"), ("OD", "outputs"), ("KE", "loads"), ("TE", "table"),
-                                       ("SR", "mma"), ("AE", "outputs"), ("RW", "mma"), ("SB", "mma"), ("PD", "chain")])
+@pytest.mark.parametrize("name,role", [("LE", "loads"), ("TE", "table"), ("barR", "mma"),
+                                       ("barS", "mma"), ("PD", "chain"), ("OD", "outputs"),
+                                       ("OE", "mma")])
 def test_a_wait_left_out_is_seen(name, role):
     def edit(bars, roles):
         for r in [r for r in roles if r.startswith(role)]:
-            roles[r] = (op for op in list(roles[r]) if not (op[0] == "wait" and op[1][0] == name))
+            roles[r] = (op for op in list(roles[r]) if not (op[0] in ("wait", "sync") and op[1][0] == name))
 
-    with pytest.raises(AssertionError):
-        for seed in range(40):
-            _run(128, 9, seed, edit)
+    for alias in (False, True):
+        with pytest.raises(AssertionError):
+            for seed in range(40):
+                _run(3, 9, seed, edit, alias)
