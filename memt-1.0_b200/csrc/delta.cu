@@ -1,4 +1,6 @@
 // memt_gated_delta: argument checks and launch of the gated delta rule over prompts.
+#include <algorithm>
+
 #include "delta.cuh"
 #include "delta_tc.cuh"
 #include "launch.h"
@@ -30,8 +32,20 @@ int launch_tokens(int D, const DeltaParams& p, cudaStream_t s) {
 // Multiprocessors the order of samples is planned for.
 constexpr int kPlanSms = 148;
 
-// chunks of 64 tokens that N samples of L tokens can have between them, one at least for each
-int64_t max_units(int64_t N, int64_t L) { return L / kTile + N; }
+// Tokens up to which a bf16 sample runs token by token. Measured, the token kernel alone against chunks alone, 16 heads,
+// us: 256 samples at D = 64: 8 tokens 95 / 342, 32 264 / 356, 48 349 / 363; D = 128: 8 tokens 211 / 455, 20 427 / 459, 24
+// 498 / 459; 64 samples at D = 256: 6 tokens 209 / 351, 12 298 / 355, 16 361 / 356. (The token kernel's times include some
+// 30 us of the chunks' launches that find no sample.)
+int few_tokens(int D) { return D == 64 ? 40 : (D == 128 ? 20 : 14); }
+
+// Whether both forms run, each for its samples by their own lengths: up to 64 tokens a sample in the mean.
+bool mixed(int64_t N, int64_t L) { return N > 1 && L <= 64 * N; }
+
+// chunks of 64 tokens that the samples that go in chunks can have between them
+int64_t max_units(int64_t N, int64_t L, int D) {
+  const int64_t samples = mixed(N, L) ? std::min(N, L / (few_tokens(D) + 1)) : N;
+  return L / kTile + samples;
+}
 
 template <int D>
 int launch_chunked(const DeltaParams& p, cudaStream_t s) {
@@ -47,7 +61,7 @@ int launch_chunked(const DeltaParams& p, cudaStream_t s) {
   if (e == cudaSuccess) e = ensure_smem(delta_chunks_kernel<D>, Pre::kSmem);
   if (e == cudaSuccess) e = ensure_smem(delta_tc_kernel<D>, Cfg::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
-  const int64_t units = p.max_segments * int64_t(p.H);
+  const int64_t units = p.max_units * int64_t(p.H);
   const int64_t grid = int64_t(p.only_long > 0 ? p.only_long : p.N) * p.H * Cfg::kBlocks;
   if (units > INT32_MAX || grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   {
@@ -71,9 +85,6 @@ int launch_chunked(int D, const DeltaParams& p, cudaStream_t s) {
   }
 }
 
-// Tokens up to which a bf16 sample runs token by token.
-int few_tokens(int D) { return D == 64 ? 24 : 8; }
-
 int check_delta(const memt_gated_delta_args* a) {
   const int st = check_prompts(a);
   if (st != MEMT_OK) return st;
@@ -94,7 +105,7 @@ size_t memt_gated_delta_workspace_size(int32_t N, int64_t L, int32_t H, int32_t 
   if (N < 1 || L < 0 || H < 1 || (D != 64 && D != 128 && D != 256)) return 0;
   if (dtype != MEMT_F32 && dtype != MEMT_BF16) return 0;
   if (dtype == MEMT_F32 || L <= few_tokens(D)) return 256;  // token by token
-  return (size_t(max_units(N, L)) * H * DeltaChunks::kBytes + 255) & ~size_t(255);
+  return (size_t(max_units(N, L, D)) * H * DeltaChunks::kBytes + 255) & ~size_t(255);
 }
 
 int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t workspace_bytes,
@@ -143,7 +154,7 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
   const int few = few_tokens(a->head_dim);
   if (a->total_tokens <= few) return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
   p.few = -1;
-  if (a->num_samples > 1 && a->total_tokens <= int64_t(64) * a->num_samples) {
+  if (mixed(p.N, p.L)) {
     p.few = few;
     const int64_t most = p.L / (few + 1);
     p.only_long = most <= p.N / 2 ? static_cast<int32_t>(most) : 0;
@@ -151,8 +162,7 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
     if (st_few != MEMT_OK) return st_few;
   }
   p.chunks = workspace;
-  p.seg_chunks = 1;
-  p.max_segments = static_cast<int32_t>(max_units(p.N, p.L));
+  p.max_units = static_cast<int32_t>(max_units(p.N, p.L, a->head_dim));
   return launch_chunked(a->head_dim, p, s);
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;

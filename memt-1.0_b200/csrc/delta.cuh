@@ -23,25 +23,51 @@ struct DeltaParams : LinearParams {
   const void* beta;
   int32_t beta_layout;  // MEMT_GATE_NONE / PER_HEAD (key heads) / PER_VALUE_HEAD
   // Chunked form (delta_chunks.cuh, delta_tc.cuh): what each chunk needs of its keys, queries and gates, [unit][H] of
-  // DeltaChunks::kBytes. The units are the segments of linear.cuh, of one chunk each (seg_chunks 1).
+  // DeltaChunks::kBytes. Units are the chunks of the samples of more than `few` tokens, in order; max_units of them fit,
+  // as many as there can be unless offsets overlap.
+  int32_t max_units;
   void* chunks;
 };
 
-// The units of sample n, by a converged warp: the first one's number and how many; fewer than the sample has
-// chunks only where offsets overlap (segments_up_to).
-__device__ __forceinline__ void sample_units(const DeltaParams& p, int n, int& first, int& count) {
+__device__ __forceinline__ int units_of(const DeltaParams& p, int n) {
   int64_t bos, eos;
-  first = 0;
-  for (int m = threadIdx.x & 31; m < n; m += 32) {
-    sample_range(p, m, bos, eos);
-    first += segments_of(p, eos - bos);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
   sample_range(p, n, bos, eos);
-  count = segments_up_to(p, n, first + segments_of(p, eos - bos));
-  first = n == 0 ? 0 : segments_up_to(p, n - 1, first);
-  count -= first;
+  return eos - bos > p.few ? static_cast<int>((eos - bos + kTile - 1) / kTile) : 0;
+}
+
+// The units of sample n, by a converged warp: the first one's number and how many.
+__device__ __forceinline__ void sample_units(const DeltaParams& p, int n, int& first, int& count) {
+  int64_t before = 0;
+  for (int m = threadIdx.x & 31; m < n; m += 32) before += units_of(p, m);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(~0u, before, o);
+  const int64_t end = before + units_of(p, n);
+  first = static_cast<int>(before < p.max_units ? before : p.max_units);
+  count = static_cast<int>(end < p.max_units ? end : p.max_units) - first;
+}
+
+// Chunk c of sample n, unit number `unit`, found by a converged warp; false when there are fewer.
+__device__ __forceinline__ bool find_unit(const DeltaParams& p, int unit, int& n, int& c) {
+  const int lane = threadIdx.x & 31;
+  int64_t base = 0;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    const int64_t own = n0 + lane < p.N ? units_of(p, n0 + lane) : 0;
+    int64_t incl = base + own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(~0u, incl - base, o);
+      if (lane >= o) incl += x;
+    }
+    const uint32_t past = __ballot_sync(~0u, incl > unit);
+    if (past != 0) {
+      const int l = __ffs(past) - 1;
+      n = n0 + l;
+      c = static_cast<int>(unit - __shfl_sync(~0u, incl - own, l));
+      return true;
+    }
+    base = __shfl_sync(~0u, incl, 31);
+  }
+  return false;
 }
 
 // A warp's columns of one state, four to a lane, and a token's step on them.

@@ -76,13 +76,11 @@ __global__ void __launch_bounds__(128, D == 256 ? 3 : 5) delta_chunks_kernel(con
   unsigned char* sm = smem_delta_chunks + ((1024u - (smem_u32(smem_delta_chunks) & 1023u)) & 1023u);
   const int tid = threadIdx.x, lane = tid & 31, iw = __shfl_sync(~0u, tid >> 5, 0);
   const int unit = blockIdx.x / p.H, h = blockIdx.x % p.H, hk = h / (p.H / p.Hk);
-  int n, c, count;
-  if (!find_segment(p, unit, n, c, count)) return;
+  int n, c;
+  if (!find_unit(p, unit, n, c)) return;
   int64_t bos, eos;
   sample_range(p, n, bos, eos);
-  if (eos - bos <= p.few) return;  // goes token by token
   bos += (int64_t)c * kTile;
-  if (bos >= eos) return;
   const int len = eos - bos < kTile ? static_cast<int>(eos - bos) : kTile;
 
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Cfg::kOffG + 3 * kTile * 4);
