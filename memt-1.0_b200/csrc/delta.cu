@@ -29,8 +29,35 @@ int launch_tokens(int D, const DeltaParams& p, cudaStream_t s) {
   }
 }
 
-// Multiprocessors the order of samples is planned for.
+// Multiprocessors the calls are planned for (the workspace size is known without a device).
 constexpr int kPlanSms = 148;
+
+// 64-token chunks per segment, or 0: one CTA per (sample, head, value block) walks a whole sample. Few of them leave
+// SMs idle for as long as a sample takes. With S segments a sample, a first pass goes over all but the last of them twice
+// (once for what they add to a zero state, once for what they make of an identity), a kernel joins them, and a second
+// pass over all makes the outputs: (0.9 w1 + w2) / S of the time of whole samples, for w1 and w2 waves of CTAs.
+// Samples of unequal length can make one segment more each. The rule counts samples, not tokens: short samples beside
+// a long one can leave it whole. A chunk takes some 1.9 / 2.4 / 3.9 us in one CTA at D = 64 / 128 / 256, the launches and the join
+// about 40 us.
+int plan_segment_chunks(int64_t N, int64_t L, int64_t H, int D) {
+  const int64_t ctas = N * H * (D == 256 ? 2 : 1), chunks = (L + kTile - 1) / kTile / N;  // of a mean sample
+  if (ctas * 2 > kPlanSms) return 0;
+  const double chunk_us = D == 64 ? 1.9 : (D == 128 ? 2.4 : 3.9);
+  int64_t best = 1;
+  double best_us = chunks * chunk_us;
+  for (int64_t S = 2; S <= 32 && S <= chunks; ++S) {
+    const int64_t w1 = (2 * ctas * (S - 1) + kPlanSms - 1) / kPlanSms, w2 = (ctas * S + kPlanSms - 1) / kPlanSms;
+    const double us = (0.9 * w1 + w2) * ((chunks + S - 1) / S) * chunk_us + 40.0;
+    if (us < 0.95 * best_us) {
+      best_us = us;
+      best = S;
+    }
+  }
+  return best == 1 ? 0 : static_cast<int>((chunks + best - 1) / best);
+}
+int64_t max_segments(int64_t N, int64_t L, int seg_chunks) { return L / (int64_t(seg_chunks) * kTile) + N; }
+
+size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Tokens up to which a bf16 sample runs token by token. Measured, the token kernel alone against chunks alone, 16 heads,
 // us: 256 samples at D = 64: 8 tokens 95 / 342, 32 264 / 356, 48 349 / 363; D = 128: 8 tokens 211 / 455, 20 427 / 459, 24
@@ -47,9 +74,24 @@ int64_t max_units(int64_t N, int64_t L, int D) {
   return L / kTile + samples;
 }
 
+size_t units_bytes(int64_t N, int64_t L, int64_t H, int D) {
+  return align256(size_t(max_units(N, L, D)) * H * DeltaChunks::kBytes);
+}
+
+template <int D, bool OUT>
+int launch_pass(const DeltaTcParams& P, int64_t units, cudaStream_t s) {
+  using Cfg = DeltaTcCfg<D>;
+  const cudaError_t e = ensure_smem(delta_tc_kernel<D, OUT>, Cfg::kSmem);
+  if (e != cudaSuccess) return cuda_status(e);
+  const int64_t grid = units * P.p.H * Cfg::kBlocks * (OUT ? 1 : 2);
+  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  ProfScope prof(kProfLinear, s);
+  delta_tc_kernel<D, OUT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
+  return cuda_status(cudaGetLastError());
+}
+
 template <int D>
 int launch_chunked(const DeltaParams& p, cudaStream_t s) {
-  using Cfg = DeltaTcCfg<D>;
   using Pre = DeltaChunksCfg<D>;
   DeltaTcParams P;
   P.p = p;
@@ -59,22 +101,29 @@ int launch_chunked(const DeltaParams& p, cudaStream_t s) {
   if (e == cudaSuccess) e = make_tmap_bf16_2d(&P.v_map, p.v, uint64_t(p.H) * D, rows, uint64_t(p.sv) * 2, 64, kTile);
   if (e == cudaSuccess) e = make_tmap_bf16_2d_sw64(&P.o_map, p.out, uint64_t(p.H) * D, rows, uint64_t(p.so) * 2, 32);
   if (e == cudaSuccess) e = ensure_smem(delta_chunks_kernel<D>, Pre::kSmem);
-  if (e == cudaSuccess) e = ensure_smem(delta_tc_kernel<D>, Cfg::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   const int64_t units = p.max_units * int64_t(p.H);
-  const int64_t grid = int64_t(p.only_long > 0 ? p.only_long : p.N) * p.H * Cfg::kBlocks;
-  if (units > INT32_MAX || grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
+  if (units > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   {
     ProfScope prof(kProfLinear, s);
     delta_chunks_kernel<D><<<static_cast<unsigned>(units), Pre::kThreads, Pre::kSmem, s>>>(P);
     const int st = cuda_status(cudaGetLastError());
     if (st != MEMT_OK) return st;
   }
-  // More CTAs than SMs: the longest samples first, so that no SM is left with one at the end.
-  P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * Cfg::kBlocks > kPlanSms && p.L / p.N >= 1024;
-  ProfScope prof(kProfLinear, s);
-  delta_tc_kernel<D><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
-  return cuda_status(cudaGetLastError());
+  if (p.seg_chunks == 0) {
+    // More CTAs than SMs: the longest samples first, so that no SM is left with one at the end.
+    P.p.by_length = p.N > 1 && p.N <= 32 && int64_t(p.N) * p.H * DeltaTcCfg<D>::kBlocks > kPlanSms && p.L / p.N >= 1024;
+    return launch_pass<D, true>(P, p.only_long > 0 ? p.only_long : p.N, s);
+  }
+  int st = launch_pass<D, false>(P, p.max_segments, s);
+  if (st != MEMT_OK) return st;
+  {
+    ProfScope prof(kProfLinear, s);
+    delta_join_kernel<D><<<static_cast<unsigned>(p.N * p.H * (D / 16)), D, 0, s>>>(P.p);  // N * H < kPlanSms: small
+    st = cuda_status(cudaGetLastError());
+    if (st != MEMT_OK) return st;
+  }
+  return launch_pass<D, true>(P, p.max_segments, s);
 }
 
 int launch_chunked(int D, const DeltaParams& p, cudaStream_t s) {
@@ -105,7 +154,10 @@ size_t memt_gated_delta_workspace_size(int32_t N, int64_t L, int32_t H, int32_t 
   if (N < 1 || L < 0 || H < 1 || (D != 64 && D != 128 && D != 256)) return 0;
   if (dtype != MEMT_F32 && dtype != MEMT_BF16) return 0;
   if (dtype == MEMT_F32 || L <= few_tokens(D)) return 256;  // token by token
-  return (size_t(max_units(N, L, D)) * H * DeltaChunks::kBytes + 255) & ~size_t(255);
+  const int seg_chunks = mixed(N, L) ? 0 : plan_segment_chunks(N, L, H, D);
+  const size_t states =
+      seg_chunks == 0 ? 0 : align256(size_t(max_segments(N, L, seg_chunks)) * H * D * D * sizeof(float));
+  return units_bytes(N, L, H, D) + 2 * states;
 }
 
 int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t workspace_bytes,
@@ -161,8 +213,17 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
     const int st_few = launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
     if (st_few != MEMT_OK) return st_few;
   }
+  const int D = a->head_dim;
   p.chunks = workspace;
-  p.max_units = static_cast<int32_t>(max_units(p.N, p.L, a->head_dim));
+  p.max_units = static_cast<int32_t>(max_units(p.N, p.L, D));
+  p.seg_chunks = mixed(p.N, p.L) ? 0 : plan_segment_chunks(p.N, p.L, p.H, D);
+  if (p.seg_chunks > 0) {
+    const int64_t segments = max_segments(p.N, p.L, p.seg_chunks);
+    p.max_segments = static_cast<int32_t>(segments);
+    p.seg_states = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + units_bytes(p.N, p.L, p.H, D));
+    p.seg_moves = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(p.seg_states) +
+                                           align256(size_t(segments) * p.H * D * D * sizeof(float)));
+  }
   return launch_chunked(a->head_dim, p, s);
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;

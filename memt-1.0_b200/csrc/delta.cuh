@@ -27,6 +27,8 @@ struct DeltaParams : LinearParams {
   // as many as there can be unless offsets overlap.
   int32_t max_units;
   void* chunks;
+  // Segments of few long samples (linear.cuh): seg_states and, as large, what each makes of an identity.
+  float* seg_moves;
 };
 
 __device__ __forceinline__ int units_of(const DeltaParams& p, int n) {

@@ -154,7 +154,9 @@ __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h,
   if (end != nullptr) cols.store(end + col);
 }
 
-template <int D>
+// OUT: outputs and final states. Otherwise the first pass over segments: what a segment adds to a zero state
+// (seg_states) and makes of an identity without values (seg_moves), in a CTA each.
+template <int D, bool OUT>
 __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(const __grid_constant__ DeltaTcParams P) {
   using Cfg = DeltaTcCfg<D>;
   constexpr int NS = Cfg::kStages, NT = Cfg::kTables, KT = Cfg::kKeys;
@@ -164,10 +166,15 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   unsigned char* sm = smem_delta_tc + ((1024u - (smem_u32(smem_delta_tc) & 1023u)) & 1023u);
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(~0u, tid >> 5, 0), quad = warp & 3;  // uniform: so are the roles' branches
-  const int vblk = blockIdx.x % Cfg::kBlocks, unit = blockIdx.x / Cfg::kBlocks / p.H;
-  const int h = blockIdx.x / Cfg::kBlocks % p.H, hk = h / (p.H / p.Hk);
-  int n = unit;
-  if (p.only_long) {
+  const int vblk = blockIdx.x % Cfg::kBlocks;
+  const int rest = blockIdx.x / Cfg::kBlocks / (OUT ? 1 : 2), unit = rest / p.H, h = rest % p.H, hk = h / (p.H / p.Hk);
+  const bool moves = !OUT && blockIdx.x / Cfg::kBlocks % 2;
+  // a unit is a sample, or with segments one of a sample's `segs`
+  int n = unit, seg = 0, segs = 1;
+  if (p.seg_chunks > 0) {
+    if (!find_segment(p, unit, n, seg, segs)) return;
+    if (!OUT && seg + 1 == segs) return;  // the first pass is for what later segments start from
+  } else if (p.only_long) {
     n = find_long(p, unit);
     if (n < 0) return;
   } else if (p.by_length) {
@@ -176,6 +183,20 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   int64_t bos, eos;
   sample_range(p, n, bos, eos);
   if (eos - bos <= p.few) return;  // the token-by-token kernel's
+  int first, units;
+  sample_units(p, n, first, units);
+  // Offsets that overlap can leave a sample without units for all of its chunks: it goes token by token, whole.
+  const bool tokenwise = units < (eos - bos + kTile - 1) / kTile;
+  if (tokenwise) {
+    if (!OUT || seg > 0) return;
+    segs = 1;
+  }
+  if (segs > 1) {
+    first += seg * p.seg_chunks;
+    bos += (int64_t)seg * p.seg_chunks * kTile;
+    if (seg + 1 < segs) eos = bos + (int64_t)p.seg_chunks * kTile;
+  }
+  const int nchunks = tokenwise ? 0 : static_cast<int>((eos - bos + kTile - 1) / kTile);
 
   // mbarriers: a chunk's tiles landed (LF) and free again (LE); table written / read (TF, TE); both halves of X (XD), U
   // (UD) and P (PD) and O (OD) ready; outputs read (OE); drained (DR)
@@ -191,7 +212,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   if (tid == 0) {
     for (int i = 0; i < NBAR; ++i) {
       uint32_t count = 1;  // TMA, tcgen05.commit or one thread
-      if (i >= TE && i < XD) count = 20;  // the chain's and the outputs' warps
+      if (i >= TE && i < XD) count = OUT ? 20 : 16;  // the chain's and the outputs' warps
       if (i == OE) count = 4;
       mbar_init(B(i), count);
     }
@@ -208,10 +229,6 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
                  tU = tmem + Cfg::kColU, tO = tmem + Cfg::kColO;
   auto tXQ = [&](int c) { return tmem + Cfg::kColXQ + (Cfg::kAlias ? 0 : 64 * (c & 1)); };
   DeltaTable* tab = reinterpret_cast<DeltaTable*>(sm + Cfg::kOffTab);
-  int first, units, nchunks = static_cast<int>((eos - bos + kTile - 1) / kTile);
-  sample_units(p, n, first, units);
-  const bool tokenwise = units < nchunks;  // offsets that overlap can leave a sample without units for all of its chunks
-  if (tokenwise) nchunks = 0;
   auto chunk_len = [&](int c) {
     const int64_t left = eos - bos - (int64_t)c * kTile;
     return static_cast<int>(left < kTile ? left : kTile);
@@ -219,9 +236,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
 
   bool alive = true;
   auto wait = [&](int b, uint32_t phase) {  // a wait that ran out is known to all before anything follows it
-    if (alive) {
-      alive = mbar_wait_polls(B(b), phase & 1);
-      }
+    if (alive) alive = mbar_wait_polls(B(b), phase & 1);
   };
   auto wait_long = [&](int b, uint32_t phase) {  // by a warp that is ahead of the others and need not hurry
     for (int i = 0; i < 64 && alive && !mbar_try(B(b), phase & 1); ++i) __nanosleep(100);
@@ -286,8 +301,8 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
           }
         }
         __syncwarp();
-        if (Cfg::kAlias && c > 0) wait(OE, c - 1);
-        if (go()) {
+        if (OUT && Cfg::kAlias && c > 0) wait(OE, c - 1);
+        if (OUT && go()) {
 #pragma unroll
           for (int i = 0; i < D / 16; ++i)
             tc::mma_bf16_ts(tXQ(c), state(0, i), dk + (kq(i) + (Cfg::kPanel >> 4)),
@@ -341,16 +356,20 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
           if constexpr (kParts == 1) tc::commit(B(PD + 1));
         }
         __syncwarp();
-        if (!Cfg::kAlias && c > 0) wait(OE, c - 1);
+        if (OUT && !Cfg::kAlias && c > 0) wait(OE, c - 1);
         if (go()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
+          for (int j = 0; OUT && j < 4; ++j)
             tc::mma_bf16_ts(tO + 16 * j, tX + 8 * j, dt + (2 * kTerm + rows(j, 16 * j)),
                             tc::idesc(tc::kBF16, 128, 64 - 16 * j, false, false), j > 0);
           tc::commit(B(OD));
           tc::commit(B(LE + s));
         }
         __syncwarp();
+      }
+      if (nchunks > 0) {  // the last arrivals land before the barriers go
+        wait(OD, nchunks - 1);
+        wait(LE + (nchunks - 1) % NS, (nchunks - 1) / NS);
       }
       // a wait that ran out: nothing of this warp may still run when tensor memory is freed
       if (!__all_sync(~0u, alive)) {
@@ -365,11 +384,11 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         const int y = static_cast<int>(bos) + c * kTile, s = c % NS;
         if (c >= NS) wait_long(LE + s, c / NS - 1);
         if (__all_sync(~0u, alive) && tc::elect_one()) {
-          mbar_expect_tx(B(LF + s), Cfg::kBytesKQ + Cfg::kBytesV + Cfg::kBytesTB);
+          mbar_expect_tx(B(LF + s), Cfg::kBytesKQ / (OUT ? 1 : 2) + Cfg::kBytesV + Cfg::kBytesTB);
           for (int i = 0; i < D / 64; ++i) {
             const uint32_t at = base + Cfg::kOffKQ + s * Cfg::kBytesKQ + i * Cfg::kPair;
             tma_load_2d(at, &P.k_map, hk * D + 64 * i, y, B(LF + s));
-            tma_load_2d(at + Cfg::kPanel, &P.q_map, hk * D + 64 * i, y, B(LF + s));
+            if (OUT) tma_load_2d(at + Cfg::kPanel, &P.q_map, hk * D + 64 * i, y, B(LF + s));
           }
           for (int i = 0; i < Cfg::kVB / 64; ++i)
             tma_load_2d(base + Cfg::kOffV + s * Cfg::kBytesV + i * Cfg::kPanel, &P.v_map,
@@ -442,7 +461,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     const int prow = 8 * (lane >> 4) + (lane & 7), pval = (lane >> 3) & 1;  // row of an stmatrix piece
     const int col = h * D + vblk * Cfg::kVB + 32 * quad % Cfg::kVB;
     constexpr int kPieces = D >= 128 ? 2 : 1;  // of 32 tokens
-    for (int c = 0; c < nchunks; ++c) {
+    for (int c = 0; OUT && c < nchunks; ++c) {
       const DeltaTable& t = tab[c % NT];
       const int len = chunk_len(c);
       wait(TF + c % NT, c / NT);
@@ -519,15 +538,18 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     const int prow = 8 * (lane >> 4) + (lane & 7), pval = (lane >> 3) & 1;  // row of an ldmatrix piece
     const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
     const int64_t head = (int64_t)D * D, col_off = (int64_t)(KT * part) * D + vblk * Cfg::kVB + vr;
+    const int64_t seg_state = ((int64_t)unit * p.H + h) * head;
     const float* start = p.h0 != nullptr && in_slot >= 0 ? p.h0 + (in_slot * p.H + h) * head : nullptr;
+    if (segs > 1) start = OUT ? p.seg_states + seg_state : nullptr;
     uint64_t S[KT / 2];  // pairs of fp32: keys KT part + 2 i, + 2 i + 1 of value vr
     if (start != nullptr) {
       const float* src = start + col_off;
 #pragma unroll
       for (int i = 0; i < KT; i += 2) S[i / 2] = f32x2_pack(src[i * D], src[(i + 1) * D]);
     } else {
+      const int one = moves ? vblk * Cfg::kVB + vr - KT * part : -1;
 #pragma unroll
-      for (int i = 0; i < KT / 2; ++i) S[i] = 0;
+      for (int i = 0; i < KT; i += 2) S[i / 2] = f32x2_pack(one == i ? 1.f : 0.f, one == i + 1 ? 1.f : 0.f);
     }
     const uint32_t own = tc::lane_addr(tS, 32 * quad, KT * part);  // of S's terms and of P
     const bool fixed = p.g_layout == 3;
@@ -557,7 +579,10 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         const float2 bf = *reinterpret_cast<const float2*>(&t.bf[16 * part + 8 * i + pair]);
         minus[i] = f32x2_pack(-bf.x, -bf.y);
       }
-      if (chunk_len(c) < kTile) {  // tokens behind the sample, whatever stands in their rows
+      if (!OUT && moves) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v[e][0] = v[e][1] = v[e][2] = v[e][3] = 0;
+      } else if (chunk_len(c) < kTile) {  // tokens behind the sample, whatever stands in their rows
         const int len = chunk_len(c) - 16 * part - pair;
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -652,7 +677,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         }
       }
     }
-    const bool taken = __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
+    const bool taken = OUT && __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
     // No state is stored before every thread has loaded its share of the first one and, where one is not finite,
     // before columns have been made from them again, their outputs over those stored above.
     constexpr int kGroup = DeltaColumns<D>::kCols;
@@ -662,7 +687,10 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     if (f32x2_lo(seen) != 0.f || f32x2_hi(seen) != 0.f) atomicOr(spoiled, 1u << (vr / kGroup));
     bar_sync<640>(kBarEnd);  // with the outputs' warps, once theirs have left
     float* end = out_slot >= 0 && !taken ? p.ht + (out_slot * p.H + h) * head : nullptr;
-    const uint32_t again = tokenwise ? ~0u : *spoiled;
+    if (OUT && seg + 1 < segs) end = nullptr;
+    if (!OUT) end = (moves ? p.seg_moves : p.seg_states) + seg_state;
+    // (what a segment that is not finite hands on is not made again: a column of it is spoiled as it is)
+    const uint32_t again = !OUT ? 0 : tokenwise ? ~0u : *spoiled;
     const bool lost = *stalled != 0;
     if (lost) {  // the caller sees it in the state
 #pragma unroll
@@ -676,7 +704,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         dst[(i + 1) * D] = f32x2_hi(S[i / 2]);
       }
     }
-    if (again != 0 && !lost) {
+    if (OUT && again != 0 && !lost) {
       for (int g = warp - 8; g < Cfg::kVB / kGroup; g += 16)
         if (again >> g & 1) delta_columns_again<D>(p, h, vblk * Cfg::kVB + g * kGroup, bos, eos, start, end);
     }
@@ -685,6 +713,83 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   tc::fence_before();
   __syncthreads();
   if (warp == 0) tc::dealloc(tmem, 512);
+}
+
+// Between the two passes over segments: the state before each one, S <- M S + H with what the first pass has made of an
+// identity and of a zero state, in fp32. A CTA has 16 value columns of one (sample, head) state and walks over its
+// segments, H replaced in place; a thread two rows of eight columns. A segment's product takes some 2000 cycles.
+template <int D>
+__global__ void __launch_bounds__(D) delta_join_kernel(const DeltaParams p) {
+  constexpr int C = 16;
+  __shared__ __align__(16) float s_S[2][D][C];
+  const int tid = threadIdx.x, blk = blockIdx.x % (D / C), nh = blockIdx.x / (D / C), h = nh % p.H, n = nh / p.H;
+  int64_t bos, eos;
+  int first = 0, count;
+  {  // this sample's first segment: every warp sums the samples before it
+    for (int m = tid & 31; m < n; m += 32) {
+      sample_range(p, m, bos, eos);
+      first += segments_of(p, eos - bos);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
+    sample_range(p, n, bos, eos);
+    count = segments_up_to(p, n, first + segments_of(p, eos - bos));
+    first = n == 0 ? 0 : segments_up_to(p, n - 1, first);
+    count -= first;
+  }
+  if (count == 1) return;  // one segment starts from the sample's own state
+  const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n);
+  const int r = tid >> 1 << 1, col = 8 * (tid & 1);
+  const int64_t at = (int64_t)r * D + blk * C + col;
+  auto read = [&](const float* x, float (&y)[2][8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 f = *reinterpret_cast<const float4*>(x + (e >> 1) * D + 4 * (e & 1));
+      y[e >> 1][4 * (e & 1)] = f.x;
+      y[e >> 1][4 * (e & 1) + 1] = f.y;
+      y[e >> 1][4 * (e & 1) + 2] = f.z;
+      y[e >> 1][4 * (e & 1) + 3] = f.w;
+    }
+  };
+  auto write = [&](float* x, int row, const float (&y)[2][8]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      *reinterpret_cast<float4*>(x + (e >> 1) * row + 4 * (e & 1)) =
+          make_float4(y[e >> 1][4 * (e & 1)], y[e >> 1][4 * (e & 1) + 1], y[e >> 1][4 * (e & 1) + 2],
+                      y[e >> 1][4 * (e & 1) + 3]);
+  };
+  float S[2][8] = {}, H[2][8];
+  if (p.h0 != nullptr && in_slot >= 0) read(p.h0 + (in_slot * p.H + h) * D * D + at, S);
+  for (int s = 0; s < count; ++s) {
+    const int64_t seg = ((int64_t)(first + s) * p.H + h) * D * D;
+    const bool last = s + 1 == count;  // its own sums are not made: the second pass ends with it
+    if (!last) read(p.seg_states + seg + at, H);
+    write(p.seg_states + seg + at, D, S);
+    if (last) break;
+    write(&s_S[s & 1][r][col], C, S);
+    __syncthreads();
+    const float* M = p.seg_moves + seg + (int64_t)r * D;
+#pragma unroll 2
+    for (int j = 0; j < D; j += 4) {
+      const float4 m[2] = {*reinterpret_cast<const float4*>(M + j), *reinterpret_cast<const float4*>(M + D + j)};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float4 a = *reinterpret_cast<const float4*>(&s_S[s & 1][j + e][col]);
+        const float4 b = *reinterpret_cast<const float4*>(&s_S[s & 1][j + e][col + 4]);
+        const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float x = e == 0 ? m[i].x : e == 1 ? m[i].y : e == 2 ? m[i].z : m[i].w;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) H[i][q] = fmaf(x, y[q], H[i][q]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) S[i][q] = H[i][q];
+  }
 }
 
 }  // namespace memt

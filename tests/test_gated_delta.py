@@ -14,6 +14,10 @@ the bounds are bounds of columns in the 2-norm (and of single outputs). With u =
     those of the chunk in hand. T is inverted in fp32: 64 u |T| (1 + |A|) of itself, and A carries 2 D + 20 + 7 r
     roundings for decays that sum to r in log2 (beyond r = 30 the weight itself is below u). The carried
     state: 4 u.
+  * over segments a sample's state is M s + H with a matrix M and sums H that walks of their own have made. A column's
+    error in such a walk is a linear map's of that column; over the columns of M it adds up in the Frobenius norm, which for
+    columns of length <= 1 is sqrt(D) times the bound of one, against |s| then. Sums and matrix do not share r and u:
+    norms of their parts stand for those of the whole. The product itself: D additions on |M| |s| <= sqrt(D) |s|.
   * its outputs round the state's copy, the scores and U to bf16 (half a step: 2^-8 each, elementwise in the sums
     over absolute values) on top of the state's own error times |q|.
 Each output is rounded once more to its type.
@@ -147,8 +151,8 @@ def _recurrence(q, k, v, g, beta, h0, cu, scale):
     return o, S, A, E
 
 
-def _chunk_bounds(q, k, v, g, beta, h0, cu, scale):
-    """The same of the chunked form: (bound of o, of the columns of final)."""
+def _chunk_bounds(q, k, v, g, beta, h0, cu, scale, joined=0):
+    """The same of the chunked form: (bound of o, of the columns of final); joined: D, with segments."""
     L, H, D = v.shape
     q, k, v, a, b = _wide(q, k, v, g, beta)
     S = h0.double().clone()
@@ -172,11 +176,15 @@ def _chunk_bounds(q, k, v, g, beta, h0, cu, scale):
             total = min(float(G.abs().max()) * 1.4427, 30.0)
             cols = lambda x: x.norm(dim=1)                                       # noqa: E731  [H, C, D] -> [H, D]
             s, rn, un = cols(S[n]), cols(r), cols(u)
-            dr = nk * (2.0 ** -16 + 4 * D * U) * s + 4 * U * cols(vc) + (2.0 ** -16 + 4 * U) * rn
+            dr = nk * (2.0 ** -16 + 4 * D * U) * s * (1 + joined ** 0.5) + 4 * U * cols(vc) + (2.0 ** -16 + 4 * U) * rn
             dT = (2.0 ** -15 + 384 * U) * T.flatten(1).norm(dim=1)[:, None] + 64 * U * nT * (1 + nA) \
                 + (2 * D + 20 + 7 * total) * U * nT ** 2 * low.flatten(1).norm(dim=1)[:, None]
             du = nT * dr + dT * rn + nk * nT * E[n]
-            step = nw * (nT * dr + dT * rn + (2.0 ** -16 + 256 * U + 7 * total * U) * un)
+            ru, uu = rn, un
+            if joined:  # the segment's own sums and the matrix on s apart
+                ru = (1 + joined ** 0.5) * (cols(bc * vc) + nk * s)
+                uu = nT * ru
+            step = nw * (nT * dr + dT * ru + (2.0 ** -16 + 256 * U + 7 * total * U) * uu)
             inter = f * (qc.abs() @ S[n].abs())
             scores = (qc @ kc.transpose(1, 2)).abs() * weight
             A[t0:t1] = abs(scale) * ((3 * bf * (inter + scores @ u.abs()) + 2 * bf * bf * inter)
@@ -184,7 +192,9 @@ def _chunk_bounds(q, k, v, g, beta, h0, cu, scale):
                                      + scores.norm(dim=2, keepdim=True) * du[:, None]).transpose(0, 1)
             keep = G[:, -1].exp()[:, None]
             S[n] = keep[..., None] * S[n] + (w * kc).transpose(1, 2) @ u
-            E[n] = keep * E[n] + step + 4 * U * cols(S[n])
+            E[n] = keep * E[n] + step + (4 + 3 * joined) * U * cols(S[n])
+            if joined:  # (a product with each segment's matrix at most a chunk, |M| <= 1)
+                E[n] += joined ** 1.5 * U * s
     return A, E
 
 
@@ -205,12 +215,12 @@ def _inputs(seed, lengths, Hk, H, D, dtype, decay="token", gscale=1.0, beta="val
     return tuple(None if x is None else x.cuda() for x in (q, k, v, g, b, h0)) + (cu,)
 
 
-def _check(o, final, x, dtype, scale):
-    """Outputs and final states against the definition; `x` as from _inputs."""
+def _check(o, final, x, dtype, scale, joined=False):
+    """Outputs and final states against the definition; `x` as from _inputs. joined: samples walked in segments."""
     q, k, v, g, b, h0, cu = x
     ref_o, ref_s, A, E = _recurrence(q, k, v, g, b, h0, cu, scale)
     if dtype is torch.bfloat16:  # either form
-        Ac, Ec = _chunk_bounds(q, k, v, g, b, h0, cu, scale)
+        Ac, Ec = _chunk_bounds(q, k, v, g, b, h0, cu, scale, v.shape[2] if joined else 0)
         A, E = torch.maximum(A, Ac), torch.maximum(E, Ec)
     eo, es = (o.double() - ref_o).abs(), (final.double() - ref_s).norm(dim=2)
     to = A * 1.01 + HALF[dtype] * (ref_o.abs() + A) + 1e-40
@@ -284,6 +294,45 @@ def test_heads_and_gates(cuda, decay, beta, Hk, H, dtype):
 @pytest.mark.parametrize("decay", ["none", "head", "token"])
 def test_many_chunks(cuda, D, decay):
     _run_and_check([64 * 9 + 5, 64 * 6], 2, 2, D, torch.bfloat16, decay=decay)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("lengths,decay", [([2900], "token"), ([2200], "none"), ([64 * 60, 7, 5000, 0], "head")])
+def test_segments(cuda, D, lengths, decay):
+    """Few long samples: walked in segments, each twice."""
+    Hk, H = (1, 2) if len(lengths) == 1 else (1, 1)
+    x = _inputs(4, lengths, Hk, H, D, torch.bfloat16, decay=decay)
+    need = _lib.load().memt_gated_delta_workspace_size
+    chunked = (sum(lengths) // 64 + len(lengths)) * H * 15360 + 256
+    assert need(len(lengths), sum(lengths), H, D, _lib.MEMT_BF16) > chunked  # (holds states of segments)
+    o, final = M.gated_delta(*x)
+    _check(o, final, x, torch.bfloat16, D ** -0.5, joined=True)
+    # without a first state, and in place
+    zero = torch.zeros_like(x[5])
+    ref = M.gated_delta(*x[:5], zero, x[6])
+    got = M.gated_delta(*x[:5], None, x[6])
+    assert torch.equal(ref[0], got[0]) and torch.equal(ref[1], got[1])
+    states = x[5].clone()
+    o2, _ = M.gated_delta(*x[:5], states, x[6], final_state=states)
+    assert torch.equal(o, o2) and torch.equal(states, final)
+
+
+@gpu
+@pytest.mark.parametrize("what", ["v", "k"])
+def test_segments_with_a_token_that_is_not_finite(cuda, what):
+    L, H, D, t = 2500, 1, 64, 1301
+    x = list(_inputs(6, [L], 1, H, D, torch.bfloat16))
+    o, final = M.gated_delta(*x)
+    x["k v".split().index(what) + 1][t, 0, 5] = float("inf")
+    o2, f2 = M.gated_delta(*x)
+    others = torch.arange(D, device="cuda") != 5
+    cols = others if what == "v" else torch.zeros_like(others)
+    near = 0.06 * float(o.float().abs().max())  # the column and its neighbours are made again, in the other form
+    assert bool(((o2[:t].float() - o[:t].float()).abs() <= near).all())
+    assert bool(((o2[:, :, cols].float() - o[:, :, cols].float()).abs() <= near).all())
+    assert bool(((f2[..., cols] - final[..., cols]).abs() <= 1e-3).all())
+    assert not bool(torch.isfinite(o2[t:, :, ~cols]).any()) and not bool(torch.isfinite(f2[..., ~cols]).any())
 
 
 @gpu

@@ -29,9 +29,9 @@ class _Barrier:
             self.pending = self.count
 
 
-def _roles(ns, n, alias):
+def _roles(ns, n, alias, out=True):
     """(barriers, role name -> generator) of one CTA with n chunks, ns stages; alias: O lies on
-    U (D = 256). The names are the kernel's."""
+    U (D = 256); out: outputs are made (not in a first pass over segments). The names are the kernel's."""
     bars = {}
 
     def add(names, number, count):
@@ -41,7 +41,7 @@ def _roles(ns, n, alias):
 
     add("LF LE", ns, 1)
     add("TF", TABLES, 1)
-    add("TE", TABLES, 20)
+    add("TE", TABLES, 20 if out else 16)
     add("XD UD PD", 2, 1)
     add("OD", 1, 1)
     add("OE", 1, 4)
@@ -72,23 +72,27 @@ def _roles(ns, n, alias):
             s = c % ns
             yield wait("LF", c // ns, s)
             yield sync("barS", 0)
-            yield issue([("KQ", s, c, 0), ("S", 0, c, 0)], [])
+            yield issue([("KQ", s, c, 0), ("S", 0, c, not out)], [])
             yield sync("barS", 1)
-            yield issue([("KQ", s, c, 0), ("S", 1, c, 0)], [("X", 0, c), ("X", 1, c)], ("XD", 0), ("XD", 1))
-            if alias and c > 0:
+            yield issue([("KQ", s, c, 0), ("S", 1, c, not out)], [("X", 0, c), ("X", 1, c)], ("XD", 0), ("XD", 1))
+            if out and alias and c > 0:
                 yield wait("OE", c - 1)
-            yield issue([("KQ", s, c, 0), ("S", 0, c, 1), ("S", 1, c, 1)], [("xq", 0 if alias else c & 1, c)])
+            if out:
+                yield issue([("KQ", s, c, 0), ("S", 0, c, 1), ("S", 1, c, 1)], [("xq", 0 if alias else c & 1, c)])
             yield sync("barR", 0)
-            yield issue([("R", 0, c, 0), ("TB", s, c, 0)], [("U", 0, c)] + [("over", 0, c)] * alias, ("UD", 0))
+            yield issue([("R", 0, c, 0), ("TB", s, c, 0)], [("U", 0, c)] + [("over", 0, c)] * (alias and out), ("UD", 0))
             yield sync("barR", 1)
             yield issue([("R", 0, c, 1), ("R", 1, c, 1), ("TB", s, c, 0)], [("U", 1, c)], ("UD", 1))
             yield sync("barW", 0)
             yield issue([("KQ", s, c, 0), ("W", 0, c, 0)], [])
             yield sync("barW", 1)
             yield issue([("KQ", s, c, 1), ("W", 1, c, 0)], [("P", 0, c), ("P", 1, c)], ("PD", 0), ("PD", 1))
-            if not alias and c > 0:
+            if out and not alias and c > 0:
                 yield wait("OE", c - 1)
-            yield issue([("TB", s, c, 1), ("W", 0, c, 1), ("W", 1, c, 1)], [("out", 0, c)], ("OD", 0), ("LE", s))
+            yield issue([("TB", s, c, 1), ("W", 0, c, 1), ("W", 1, c, 1)], [("out", 0, c)] * out, ("OD", 0), ("LE", s))
+        if n:
+            yield wait("OD", n - 1)
+            yield wait("LE", (n - 1) // ns, (n - 1) % ns)
 
     def loads():
         for c in range(n):
@@ -104,7 +108,7 @@ def _roles(ns, n, alias):
             yield arrive("TF", c % TABLES)
 
     def outputs(i):
-        for c in range(n):
+        for c in range(n if out else 0):
             yield wait("TF", c // TABLES, c % TABLES)
             yield wait("OD", c)
             for _ in range(30):  # (they take their time)
@@ -157,13 +161,13 @@ def _roles(ns, n, alias):
 class _Buffers:
     """name, place -> the chunk in it and how many last reads of it are still to come."""
 
-    def __init__(self):
-        self.held = {}
+    def __init__(self, readers):
+        self.held, self.readers = {}, readers
 
     def write(self, name, place, chunk):
         old = self.held.get((name, place))
         assert old is None or old[1] <= 0, f"{name} {place}: chunk {chunk} over {old[0]}, of which {old[1]} reads are open"
-        self.held[name, place] = [chunk, READERS[name]]
+        self.held[name, place] = [chunk, self.readers[name]]
 
     def read(self, name, place, chunk, last):
         old = self.held.get((name, place))
@@ -171,12 +175,12 @@ class _Buffers:
         old[1] -= last
 
 
-def _run(ns, n, seed, edit=None, alias=False):
+def _run(ns, n, seed, edit=None, alias=False, out=True):
     rng = random.Random(seed)
-    bars, roles = _roles(ns, n, alias)
+    bars, roles = _roles(ns, n, alias, out)
     if edit is not None:
         edit(bars, roles)
-    buffers = _Buffers()
+    buffers = _Buffers(READERS if out else {**READERS, "table": 16})
     at = {name: next(role, None) for name, role in roles.items()}
     batches, tiles = [], []
     weight = {name: rng.choice([1, 1, 5, 30]) for name in [*at, "tensor pipe", "tma"]}  # slow and fast ones
@@ -235,10 +239,11 @@ def _run(ns, n, seed, edit=None, alias=False):
 
 
 @pytest.mark.parametrize("stages,alias", [(3, False), (2, True)])
+@pytest.mark.parametrize("out", [True, False])
 @pytest.mark.parametrize("chunks", [0, 1, 2, 3, 4, 5, 9, 14])
-def test_no_order_stalls_or_overtakes(stages, alias, chunks):
+def test_no_order_stalls_or_overtakes(stages, alias, chunks, out):
     for seed in range(20):
-        _run(stages, chunks, seed, alias=alias)
+        _run(stages, chunks, seed, alias=alias, out=out)
 
 
 @pytest.mark.parametrize("name,role", [("LE", "loads"), ("TE", "table"), ("barR", "mma"),
