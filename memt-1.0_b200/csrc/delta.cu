@@ -2,7 +2,7 @@
 #include <algorithm>
 
 #include "delta.cuh"
-#include "delta_tc.cuh"
+#include "delta_join.cuh"
 #include "launch.h"
 #include "prompts.h"
 
@@ -34,20 +34,22 @@ constexpr int kPlanSms = 148;
 
 // 64-token chunks per segment, or 0: one CTA per (sample, head, value block) walks a whole sample. Few of them leave
 // SMs idle for as long as a sample takes. With S segments a sample, a first pass goes over all but the last of them twice
-// (once for what they add to a zero state, once for what they make of an identity), a kernel joins them, and a second
-// pass over all makes the outputs: (0.9 w1 + w2) / S of the time of whole samples, for w1 and w2 waves of CTAs.
-// Samples of unequal length can make one segment more each. The rule counts samples, not tokens: short samples beside
-// a long one can leave it whole. A chunk takes some 1.9 / 2.4 / 3.9 us in one CTA at D = 64 / 128 / 256, the launches and the join
-// about 40 us.
+// (once for what they add to a zero state, once for what they make of an identity), a kernel joins them one after the other,
+// and a second pass over all makes the outputs. Measured at D = 64 / 128 / 256: a chunk of a whole sample takes
+// 1.9 / 2.4 / 5.5 us, 0.85 of it in a wave of the first pass, 1.25 in a full wave of the second; a segment's join
+// 2.1 / 3.7 / 8 and more; a start of a wave some 6. Samples of unequal length can make one segment more each.
+// The rule counts samples, not tokens: short samples beside a long one can leave it whole.
 int plan_segment_chunks(int64_t N, int64_t L, int64_t H, int D) {
   const int64_t ctas = N * H * (D == 256 ? 2 : 1), chunks = (L + kTile - 1) / kTile / N;  // of a mean sample
   if (ctas * 2 > kPlanSms) return 0;
-  const double chunk_us = D == 64 ? 1.9 : (D == 128 ? 2.4 : 3.9);
+  const double chunk_us = D == 64 ? 1.9 : (D == 128 ? 2.4 : 5.5), join_us = D == 64 ? 2.1 : (D == 128 ? 3.7 : 8);
+  auto waves = [](int64_t n) { return static_cast<double>((n + kPlanSms - 1) / kPlanSms); };
+  const double joins = waves(N * H * (D / 16)) * join_us;
   int64_t best = 1;
-  double best_us = chunks * chunk_us;
+  double best_us = chunks * chunk_us + 6;
   for (int64_t S = 2; S <= 32 && S <= chunks; ++S) {
-    const int64_t w1 = (2 * ctas * (S - 1) + kPlanSms - 1) / kPlanSms, w2 = (ctas * S + kPlanSms - 1) / kPlanSms;
-    const double us = (0.9 * w1 + w2) * ((chunks + S - 1) / S) * chunk_us + 40.0;
+    const double run = ((chunks + S - 1) / S) * chunk_us + 6;
+    const double us = (0.85 * waves(2 * ctas * (S - 1)) + 1.25 * waves(ctas * S)) * run + S * joins + 15;
     if (us < 0.95 * best_us) {
       best_us = us;
       best = S;
@@ -118,8 +120,12 @@ int launch_chunked(const DeltaParams& p, cudaStream_t s) {
   int st = launch_pass<D, false>(P, p.max_segments, s);
   if (st != MEMT_OK) return st;
   {
+    using Join = DeltaJoinCfg<D>;
+    e = ensure_smem(delta_join_kernel<D>, Join::kSmem);
+    if (e != cudaSuccess) return cuda_status(e);
     ProfScope prof(kProfLinear, s);
-    delta_join_kernel<D><<<static_cast<unsigned>(p.N * p.H * (D / 16)), D, 0, s>>>(P.p);  // N * H < kPlanSms: small
+    const int grid = p.N * p.H * (D / Join::kCols);  // (N H <= kPlanSms)
+    delta_join_kernel<D><<<grid, D, Join::kSmem, s>>>(P.p);
     st = cuda_status(cudaGetLastError());
     if (st != MEMT_OK) return st;
   }

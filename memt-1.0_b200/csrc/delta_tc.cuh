@@ -155,7 +155,7 @@ __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h,
 }
 
 // OUT: outputs and final states. Otherwise the first pass over segments: what a segment adds to a zero state
-// (seg_states) and makes of an identity without values (seg_moves), in a CTA each.
+// (seg_states) and makes of an identity without values (seg_moves, transposed), in a CTA each.
 template <int D, bool OUT>
 __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(const __grid_constant__ DeltaTcParams P) {
   using Cfg = DeltaTcCfg<D>;
@@ -697,11 +697,17 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
       for (int i = 0; i < KT / 2; ++i) S[i] = f32x2_splat(__int_as_float(0x7fffffff));
     }
     if (writes && end != nullptr && (lost || !(again >> (vr / kGroup) & 1))) {
-      float* dst = end + col_off;
+      if (moves) {  // [value column][key], as the join reads it
+        ulonglong2* dst = reinterpret_cast<ulonglong2*>(end + (int64_t)(vblk * Cfg::kVB + vr) * D + KT * part);
 #pragma unroll
-      for (int i = 0; i < KT; i += 2) {
-        dst[i * D] = f32x2_lo(S[i / 2]);
-        dst[(i + 1) * D] = f32x2_hi(S[i / 2]);
+        for (int i = 0; i < KT / 4; ++i) dst[i] = make_ulonglong2(S[2 * i], S[2 * i + 1]);
+      } else {
+        float* dst = end + col_off;
+#pragma unroll
+        for (int i = 0; i < KT; i += 2) {
+          dst[i * D] = f32x2_lo(S[i / 2]);
+          dst[(i + 1) * D] = f32x2_hi(S[i / 2]);
+        }
       }
     }
     if (OUT && again != 0 && !lost) {
@@ -713,83 +719,6 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   tc::fence_before();
   __syncthreads();
   if (warp == 0) tc::dealloc(tmem, 512);
-}
-
-// Between the two passes over segments: the state before each one, S <- M S + H with what the first pass has made of an
-// identity and of a zero state, in fp32. A CTA has 16 value columns of one (sample, head) state and walks over its
-// segments, H replaced in place; a thread two rows of eight columns. A segment's product takes some 2000 cycles.
-template <int D>
-__global__ void __launch_bounds__(D) delta_join_kernel(const DeltaParams p) {
-  constexpr int C = 16;
-  __shared__ __align__(16) float s_S[2][D][C];
-  const int tid = threadIdx.x, blk = blockIdx.x % (D / C), nh = blockIdx.x / (D / C), h = nh % p.H, n = nh / p.H;
-  int64_t bos, eos;
-  int first = 0, count;
-  {  // this sample's first segment: every warp sums the samples before it
-    for (int m = tid & 31; m < n; m += 32) {
-      sample_range(p, m, bos, eos);
-      first += segments_of(p, eos - bos);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) first += __shfl_xor_sync(~0u, first, o);
-    sample_range(p, n, bos, eos);
-    count = segments_up_to(p, n, first + segments_of(p, eos - bos));
-    first = n == 0 ? 0 : segments_up_to(p, n - 1, first);
-    count -= first;
-  }
-  if (count == 1) return;  // one segment starts from the sample's own state
-  const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n);
-  const int r = tid >> 1 << 1, col = 8 * (tid & 1);
-  const int64_t at = (int64_t)r * D + blk * C + col;
-  auto read = [&](const float* x, float (&y)[2][8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4 f = *reinterpret_cast<const float4*>(x + (e >> 1) * D + 4 * (e & 1));
-      y[e >> 1][4 * (e & 1)] = f.x;
-      y[e >> 1][4 * (e & 1) + 1] = f.y;
-      y[e >> 1][4 * (e & 1) + 2] = f.z;
-      y[e >> 1][4 * (e & 1) + 3] = f.w;
-    }
-  };
-  auto write = [&](float* x, int row, const float (&y)[2][8]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      *reinterpret_cast<float4*>(x + (e >> 1) * row + 4 * (e & 1)) =
-          make_float4(y[e >> 1][4 * (e & 1)], y[e >> 1][4 * (e & 1) + 1], y[e >> 1][4 * (e & 1) + 2],
-                      y[e >> 1][4 * (e & 1) + 3]);
-  };
-  float S[2][8] = {}, H[2][8];
-  if (p.h0 != nullptr && in_slot >= 0) read(p.h0 + (in_slot * p.H + h) * D * D + at, S);
-  for (int s = 0; s < count; ++s) {
-    const int64_t seg = ((int64_t)(first + s) * p.H + h) * D * D;
-    const bool last = s + 1 == count;  // its own sums are not made: the second pass ends with it
-    if (!last) read(p.seg_states + seg + at, H);
-    write(p.seg_states + seg + at, D, S);
-    if (last) break;
-    write(&s_S[s & 1][r][col], C, S);
-    __syncthreads();
-    const float* M = p.seg_moves + seg + (int64_t)r * D;
-#pragma unroll 2
-    for (int j = 0; j < D; j += 4) {
-      const float4 m[2] = {*reinterpret_cast<const float4*>(M + j), *reinterpret_cast<const float4*>(M + D + j)};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 a = *reinterpret_cast<const float4*>(&s_S[s & 1][j + e][col]);
-        const float4 b = *reinterpret_cast<const float4*>(&s_S[s & 1][j + e][col + 4]);
-        const float y[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float x = e == 0 ? m[i].x : e == 1 ? m[i].y : e == 2 ? m[i].z : m[i].w;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) H[i][q] = fmaf(x, y[q], H[i][q]);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int q = 0; q < 8; ++q) S[i][q] = H[i][q];
-  }
 }
 
 }  // namespace memt
