@@ -58,15 +58,15 @@ struct DeltaChunksCfg {
   static constexpr int kRow = 72, kRowT = 40, kRowT2 = 24;
   static constexpr uint32_t kOffK = 0, kBytesK = kTile * D * 2;
   static constexpr uint32_t kOffQ = kOffK + kBytesK;
-  // A and the inverse's scratch lie over Q, which the scores are made of before
-  static constexpr uint32_t kOffA = kOffQ, kOffT = kOffA + kTile * kRow * 4;
+  // A and the inverse's scratch lie over K and Q, which the scores are made of before
+  static constexpr uint32_t kOffA = kOffK, kOffT = kOffA + kTile * kRow * 4;
   static constexpr uint32_t kBytesA = (kTile * kRow + 32 * kRowT + 16 * kRowT2) * 4;
-  static constexpr uint32_t kOffG = kOffQ + (kBytesA > kBytesK ? kBytesA : kBytesK);
+  static constexpr uint32_t kOffG = kBytesA > 2 * kBytesK ? (kBytesA + 15) / 16 * 16 : 2 * kBytesK;
   static constexpr size_t kSmem = kOffG + 3 * kTile * 4 + 16 + 1024;
 };
 
 template <int D>
-__global__ void __launch_bounds__(128, D == 256 ? 3 : 5) delta_chunks_kernel(const __grid_constant__ DeltaTcParams P) {
+__global__ void __launch_bounds__(128, D == 256 ? 3 : 6) delta_chunks_kernel(const __grid_constant__ DeltaTcParams P) {
   using Cfg = DeltaChunksCfg<D>;
   using T16 = __nv_bfloat16;
   constexpr int RL = Cfg::kRow, RT = Cfg::kRowT, RT2 = Cfg::kRowT2;
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(128, D == 256 ? 3 : 5) delta_chunks_kernel(con
       }
     }
   }
-  __syncthreads();  // A lies over Q
+  __syncthreads();  // A lies over K and Q
   float* A = reinterpret_cast<float*>(sm + Cfg::kOffA);
   float* TT = reinterpret_cast<float*>(sm + Cfg::kOffT);
   float* T2 = TT + 32 * RT;
