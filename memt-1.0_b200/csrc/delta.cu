@@ -10,14 +10,27 @@ namespace {
 
 using namespace memt;
 
-template <int D, typename T>
+// Columns (samples x heads x D) up to which a warp has 8 instead of 16 of them: half the work between the sums over rows,
+// which is what a token waits for, but more warps that load its row. 500 tokens, fp32, us with 8 / 16 columns:
+// D = 64: 8 heads 162 / 193, 192 218 / 242, 256 265 / 242; D = 128: 8 heads 201 / 275, 96 301 / 344, 128 377 / 347.
+constexpr int64_t kFewColumns = 12288;
+
+template <int D, typename T, int CG>
 int launch_tokens(const DeltaParams& p, cudaStream_t s) {
-  using Cfg = DeltaTokensCfg<D>;
+  using Cfg = DeltaTokensCfg<D, CG>;
   const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;
   if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   ProfScope prof(kProfLinear, s);
-  delta_tokens_kernel<D, T><<<static_cast<unsigned>(grid), Cfg::kThreads, 0, s>>>(p);
+  delta_tokens_kernel<D, T, CG><<<static_cast<unsigned>(grid), Cfg::kThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError());
+}
+
+template <int D, typename T>
+int launch_tokens(const DeltaParams& p, cudaStream_t s) {
+  if constexpr (D < 256) {
+    if (int64_t(p.N) * p.H * D <= kFewColumns) return launch_tokens<D, T, 2>(p, s);
+  }
+  return launch_tokens<D, T, D == 256 ? 2 : 4>(p, s);
 }
 
 template <typename T>

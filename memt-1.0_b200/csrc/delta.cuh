@@ -72,10 +72,10 @@ __device__ __forceinline__ bool find_unit(const DeltaParams& p, int unit, int& n
   return false;
 }
 
-// A warp's columns of one state, four to a lane, and a token's step on them.
-template <int D>
+// A warp's columns of one state, four to a lane, and a token's step on them; CG: lanes across the columns.
+template <int D, int CG = D == 256 ? 2 : 4>
 struct DeltaColumns {
-  static constexpr int kColGroups = D == 256 ? 2 : 4;  // lanes across the columns
+  static constexpr int kColGroups = CG;
   static constexpr int kRowGroups = 32 / kColGroups;
   static constexpr int kCols = 4 * kColGroups;         // columns of a warp
   static constexpr int kRows = D / kRowGroups;         // rows of a lane: 4 group + 4 kRowGroups m + 0 .. 3
@@ -201,17 +201,17 @@ struct DeltaColumns {
   }
 };
 
-template <int D>
+template <int D, int CG>
 struct DeltaTokensCfg {
   static constexpr int kWarps = 4, kThreads = 32 * kWarps;
-  static constexpr int kCols = kWarps * DeltaColumns<D>::kCols, kBlocks = D / kCols;  // of a CTA; CTAs per state
+  static constexpr int kCols = kWarps * DeltaColumns<D, CG>::kCols, kBlocks = D / kCols;  // of a CTA; CTAs per state
   static constexpr int kBatch = 4;  // tokens between two barriers
 };
 
-template <int D, typename T>
-__global__ void __launch_bounds__(DeltaTokensCfg<D>::kThreads, 4) delta_tokens_kernel(const DeltaParams p) {
-  using Cfg = DeltaTokensCfg<D>;
-  using Cols = DeltaColumns<D>;
+template <int D, typename T, int CG>
+__global__ void __launch_bounds__(DeltaTokensCfg<D, CG>::kThreads, 4) delta_tokens_kernel(const DeltaParams p) {
+  using Cfg = DeltaTokensCfg<D, CG>;
+  using Cols = DeltaColumns<D, CG>;
   constexpr int TB = Cfg::kBatch, NT = Cfg::kThreads, C = Cfg::kCols;
   constexpr int VE = 16 / sizeof(T), DV = D / VE, CV = C / VE;  // elements of a vector, vectors of a row
   constexpr int kVecs = TB * (2 * DV + CV), NV = (kVecs + NT - 1) / NT;
