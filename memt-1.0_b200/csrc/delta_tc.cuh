@@ -31,7 +31,7 @@
 //
 // Values that are not finite: the zeros of T and B meet them in tokens they must not reach. Whatever spoils a token
 // never leaves the state, so a CTA looks at its final state; a warp's columns of which one is not finite are made
-// again token by token (DeltaColumns) from the initial state, outputs too.
+// again token by token (DeltaAgain) from the initial state, outputs too.
 // Every wait is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, the control
 // warps drain what they have in flight, and the final state is NaN.
 #pragma once
@@ -112,34 +112,64 @@ __device__ __forceinline__ float exp2_pair(float h, float l) {
 
 // The warp's columns from `col` of one state, again, token by token from `start` (null: zeros) and with the outputs.
 // Once every value of the state is NaN, so is everything behind.
+// (At D = 64 and 128 with what the next token needs in registers, too, the chain itself comes out slower.)
+template <int D>
+using DeltaAgain = DeltaColumns<D, D == 64 ? 4 : 2>;
 template <int D>
 __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h, int col, int64_t bos, int64_t eos,
                                                  const float* start, float* end) {
-  using Cols = DeltaColumns<D>;
+  using Cols = DeltaAgain<D>;
   using T = __nv_bfloat16;
+  constexpr bool kAhead = D == 256;
+  constexpr int M = kAhead ? Cols::kRows / 4 : 1;
   Cols cols;
   cols.load(start != nullptr ? start + col : nullptr);
   const int hk = h / (p.H / p.Hk);
   float fixed_hi, fixed_lo;
   split_decay(p.g_layout == 3 ? exp(static_cast<double>(p.g[h])) : 1.0, fixed_hi, fixed_lo);
+  auto kt = [&](int64_t t) { return static_cast<const T*>(p.k) + t * p.sk + (int64_t)hk * D + Cols::row0(); };
+  auto qt = [&](int64_t t) { return static_cast<const T*>(p.q) + t * p.sq + (int64_t)hk * D + Cols::row0(); };
+  auto vt = [&](int64_t t) { return static_cast<const T*>(p.v) + t * p.sv + (int64_t)h * D + col; };
+  auto raw = [](const T* x, int m) { return *reinterpret_cast<const uint2*>(x + 4 * Cols::kRowGroups * m); };
+  auto four = [](uint2 u) {
+    const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  };
+  uint2 k2[M], q2[M];  // the next token's, as loaded
+  float v2 = 0.f, g2 = 0.f, b2 = 0.f;
+  auto fetch = [&](int64_t t) {
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      k2[m] = raw(kt(t), m);
+      q2[m] = raw(qt(t), m);
+    }
+    v2 = as_f32(vt(t)[Cols::col0() + Cols::own_col()]);
+    b2 = load_beta<T>(p, t, h);
+    if (p.g_layout == 1) g2 = p.g[t * p.H + h];
+  };
+  if (kAhead && bos < eos) fetch(bos);
   bool lost = false;
 #pragma unroll 1
   for (int64_t t = bos; t < eos; ++t) {
     float out = __int_as_float(0x7fffffff);
     if (!lost) {
-      const T* kt = static_cast<const T*>(p.k) + t * p.sk + (int64_t)hk * D + Cols::row0();
-      const T* qt = static_cast<const T*>(p.q) + t * p.sq + (int64_t)hk * D + Cols::row0();
-      const T* vt = static_cast<const T*>(p.v) + t * p.sv + (int64_t)h * D + col;
-      auto four = [](const T* x) {
-        const uint2 u = *reinterpret_cast<const uint2*>(x);
-        const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y);
-        return make_float4(a.x, a.y, b.x, b.y);
-      };
-      auto k = [&](int m) { return four(kt + 4 * Cols::kRowGroups * m); };
-      auto q = [&](int m) { return four(qt + 4 * Cols::kRowGroups * m); };
-      auto v = [&](int c) { return as_f32(vt[c]); };
-      const float beta = load_beta<T>(p, t, h);
-      const float a = p.g_layout == 1 ? expf(p.g[t * p.H + h]) : fixed_hi;
+      uint2 k1[M], q1[M];
+      float v1 = v2, beta = b2, g1 = g2;
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+          k1[m] = k2[m];
+          q1[m] = q2[m];
+        }
+        if (t + 1 < eos) fetch(t + 1);
+      } else {
+        beta = load_beta<T>(p, t, h);
+        if (p.g_layout == 1) g1 = p.g[t * p.H + h];
+      }
+      const float a = p.g_layout == 1 ? expf(g1) : fixed_hi;
+      auto k = [&](int m) { return four(kAhead ? k1[kAhead ? m : 0] : raw(kt(t), m)); };
+      auto q = [&](int m) { return four(kAhead ? q1[kAhead ? m : 0] : raw(qt(t), m)); };
+      auto v = [&](int c) { return kAhead ? v1 : as_f32(vt(t)[c]); };  // (c is this lane's own column)
       out = cols.template step<true>(k, q, v, a, p.g_layout == 1 ? 0.f : fixed_lo, beta);
       bool nan = true;
 #pragma unroll
@@ -205,7 +235,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   static_assert(NBAR * 8 + 24 <= 512, "barrier area");
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Cfg::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Cfg::kOffBar + NBAR * 8);
-  uint32_t* spoiled = tmem_slot + 1;  // bit c: some value of the CTA's columns 4 c .. 4 c + 3 is not finite
+  uint32_t* spoiled = tmem_slot + 1;  // bit c: some value of the CTA's c-th group of columns (DeltaAgain) is not finite
   uint32_t* stalled = tmem_slot + 2;  // a wait ran out
   const uint32_t base = smem_u32(sm), bars = smem_u32(bar);
   auto B = [&](int i) { return bars + 8 * i; };
@@ -680,7 +710,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     const bool taken = OUT && __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
     // No state is stored before every thread has loaded its share of the first one and, where one is not finite,
     // before columns have been made from them again, their outputs over those stored above.
-    constexpr int kGroup = DeltaColumns<D>::kCols;
+    constexpr int kGroup = DeltaAgain<D>::kCols;
     uint64_t seen = 0;  // two zeros; NaN once a state is not finite
 #pragma unroll
     for (int i = 0; i < KT / 2; ++i) seen = fma_f32x2(S[i], 0, seen);
