@@ -442,8 +442,8 @@ int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
 
 /* ---- the gated delta rule over prompts -------------------------------------
  *
- * No counterpart in the reference (its reads see the incoming snapshot only): the recurrence of
- * memt_gdn2_update with one decay for each head, in which every token reads the state it has just written.
+ * No counterpart in the reference (its reads see the incoming snapshot only): the gated delta rule with one
+ * decay and one beta for each head and token, in which every token reads the state it has just written.
  * Per sample n and value head h, from initial_state (key head h / (num_heads / num_key_heads)):
  *     S~  = exp(g_t) S_{t-1}
  *     S_t = S~ + beta_t k_t (v_t - S~^T k_t)^T
@@ -451,6 +451,13 @@ int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
  * final_state receives the last S. RULE_GATED_DELTA of memt_recurrent_step is its single-token form.
  *
  * dtype, rows, samples, states, pools and overlaps as in memt_linear_attention_args; beta is in q's dtype.
+ * Keys are meant to be of unit length: beta |k|^2 above 2 lets a state grow.
+ * fp32 goes token by token in fp32; bf16 in chunks of 64 tokens, with states exact to a few 1e-6 and scores, the
+ * state that queries read and corrections rounded to bf16 for the outputs. In bf16 calls of up to 64 tokens a sample
+ * in the mean, samples of at most 40 / 20 / 14 tokens (D = 64 / 128 / 256) go token by token; few long samples are
+ * split into segments. So results may differ within these roundings with what a sample is packed with.
+ * A token that is not finite changes nothing before it. A column of a bf16 state that is not finite at the end is
+ * made again token by token, its outputs too (2 us a token).
  */
 typedef struct memt_gated_delta_args {
   uint32_t struct_size;    /* sizeof(memt_gated_delta_args)                     */

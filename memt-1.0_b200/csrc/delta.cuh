@@ -10,7 +10,9 @@
 //     d = beta (v - a S^T k),   S <- a S + k d^T,   o = scale (a S^T q + (q.k) d)
 // k and q are staged in shared memory a batch of tokens ahead as 16-byte vectors, rows of a lane in groups of
 // four such that a warp reads them without bank conflicts and the packed arithmetic pairs rows.
-// Bound by the states' traffic for one token, by the latency of a token's chain of exchanges for many.
+// Bound by the states' traffic for one token, by the latency of a token's chain of exchanges for many: 0.31 us a token at
+// D = 64 (2 samples of up to 1000, 8 states), 0.40 at D = 128; 256 samples of up to 16 tokens, 16 heads, D = 128: 211 us
+// where the states' traffic alone takes 82.
 #pragma once
 
 #include <type_traits>

@@ -5,13 +5,16 @@
 // by: for each block of 16 columns j the rows from the diagonal block on, in core matrices of 8 rows by 16 bytes, the
 // two of 16 columns behind one another. What lies above the diagonal's blocks is neither made nor stored.
 //
-// One CTA of four warps a unit, five an SM. K and Q land by TMA. K K^T and Q K^T are on mma.sync (bf16 products, fp32
+// One CTA of four warps a unit, six an SM (D = 256: three). K and Q land by TMA. K K^T and Q K^T are on mma.sync (bf16 products, fp32
 // sums): two warps each, one the last 16 rows, one the rows before, columns up to the diagonal. The inverse of the unit
 // lower triangular I + A is fp32: 16 x 16 blocks by forward substitution, a lane a column, then two doublings
 // T_21 = -T_22 (A_21 T_11) with 3xTF32 products (both factors as two terms of 11 bits, 2^-21 of each left out; on
 // CUDA cores their reads of shared memory, 16 bytes for 16 additions, bound them). Sums of log decays are formed in 64
 // bits and kept as pairs of fp32 numbers, so that their differences are those of the tokens in between whatever
 // came before them.
+// Measured at 8 x 8192 tokens, 16 heads, D = 128 (16,384 units, 790 MB): 217 us, 3.6 TB/s. Some 7,300 warp instructions
+// a unit at 0.48 a cycle and scheduler; of ten resident warps four wait at a barrier between the steps, two for a fixed
+// latency. Five CTAs an SM (A beside K instead of over it) 229 us; one warp a unit, no barriers but 12 warps an SM, 300.
 #pragma once
 
 #include "delta.cuh"
