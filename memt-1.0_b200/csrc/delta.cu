@@ -19,7 +19,6 @@ template <int D, typename T, int CG>
 int launch_tokens(const DeltaParams& p, cudaStream_t s) {
   using Cfg = DeltaTokensCfg<D, CG>;
   const int64_t grid = int64_t(p.N) * p.H * Cfg::kBlocks;
-  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   ProfScope prof(kProfLinear, s);
   delta_tokens_kernel<D, T, CG><<<static_cast<unsigned>(grid), Cfg::kThreads, 0, s>>>(p);
   return cuda_status(cudaGetLastError());
@@ -93,13 +92,18 @@ size_t units_bytes(int64_t N, int64_t L, int64_t H, int D) {
   return align256(size_t(max_units(N, L, D)) * H * DeltaChunks::kBytes);
 }
 
+// Whether a launch of the call could have more CTAs than a grid holds (at most eight a unit or sample and head: some 10^10
+// tokens and heads, more than memory does).
+bool too_large(int64_t N, int64_t L, int64_t H, int D) {
+  return double(std::max(max_units(N, L, D), N)) * double(H) * 8 > INT32_MAX;
+}
+
 template <int D, bool OUT>
 int launch_pass(const DeltaTcParams& P, int64_t units, cudaStream_t s) {
   using Cfg = DeltaTcCfg<D>;
   const cudaError_t e = ensure_smem(delta_tc_kernel<D, OUT>, Cfg::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   const int64_t grid = units * P.p.H * Cfg::kBlocks * (OUT ? 1 : 2);
-  if (grid > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   ProfScope prof(kProfLinear, s);
   delta_tc_kernel<D, OUT><<<static_cast<unsigned>(grid), Cfg::kThreads, Cfg::kSmem, s>>>(P);
   return cuda_status(cudaGetLastError());
@@ -118,7 +122,6 @@ int launch_chunked(const DeltaParams& p, cudaStream_t s) {
   if (e == cudaSuccess) e = ensure_smem(delta_chunks_kernel<D>, Pre::kSmem);
   if (e != cudaSuccess) return cuda_status(e);
   const int64_t units = p.max_units * int64_t(p.H);
-  if (units > INT32_MAX) return MEMT_ERR_UNSUPPORTED;
   {
     ProfScope prof(kProfLinear, s);
     delta_chunks_kernel<D><<<static_cast<unsigned>(units), Pre::kThreads, Pre::kSmem, s>>>(P);
@@ -171,7 +174,7 @@ extern "C" {
 
 size_t memt_gated_delta_workspace_size(int32_t N, int64_t L, int32_t H, int32_t D, int32_t dtype) {
   if (N < 1 || L < 0 || H < 1 || (D != 64 && D != 128 && D != 256)) return 0;
-  if (dtype != MEMT_F32 && dtype != MEMT_BF16) return 0;
+  if ((dtype != MEMT_F32 && dtype != MEMT_BF16) || too_large(N, L, H, D)) return 0;
   if (dtype == MEMT_F32 || L <= few_tokens(D)) return 256;  // token by token
   const int seg_chunks = mixed(N, L) ? 0 : plan_segment_chunks(N, L, H, D);
   const size_t states =
@@ -183,6 +186,7 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
                      memt_stream_t stream) try {
   const int st = check_delta(a);
   if (st != MEMT_OK) return st;
+  if (too_large(a->num_samples, a->total_tokens, a->num_heads, a->head_dim)) return MEMT_ERR_UNSUPPORTED;
   const size_t need =
       memt_gated_delta_workspace_size(a->num_samples, a->total_tokens, a->num_heads, a->head_dim, a->dtype);
   // (256 stands for none)

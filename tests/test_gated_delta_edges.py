@@ -40,7 +40,13 @@ def test_workspace_grows_with_the_call():
         sizes = [f(200, t, 16, D, _lib.MEMT_BF16) for t in range(100, 40000, 321)]
         assert sizes == sorted(sizes)
         assert f(1, 2 ** 31 - 1, 1, D, _lib.MEMT_BF16) >= (2 ** 31 // 64) * 15360
-        assert f(2 ** 30, 2 ** 31 - 1, 64, D, _lib.MEMT_BF16) >= (2 ** 31 // 64) * 64 * 15360
+        assert f(2 ** 30, 2 ** 31 - 2, 64, D, _lib.MEMT_BF16) == 0 and f(2 ** 30, 1, 4, D, _lib.MEMT_F32) == 0
+        for n, tokens, heads in ((2 ** 30, 2 ** 31 - 2, 4), (2 ** 30, 1, 4), (1, 2 ** 31 - 2, 2 ** 20)):
+            far = [(i + 1) << 52 for i in range(8)]  # (nothing reads them: more CTAs than a grid holds)
+            a = _args(num_samples=n, total_tokens=tokens, num_heads=heads, num_key_heads=1, head_dim=D,
+                      q_stride=D, k_stride=D, v_stride=heads * D, out_stride=heads * D,
+                      **dict(zip(("q", "k", "v", "out", "g", "beta", "cu_seqlens", "final_state"), far)))
+            assert _lib.load().memt_gated_delta(ctypes.byref(a), 1 << 60, 2 ** 60, None) == _lib.MEMT_ERR_UNSUPPORTED
 
 
 @gpu
