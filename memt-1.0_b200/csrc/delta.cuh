@@ -50,28 +50,50 @@ __device__ __forceinline__ void sample_units(const DeltaParams& p, int n, int& f
   count = static_cast<int>(end < p.max_units ? end : p.max_units) - first;
 }
 
-// Chunk c of sample n, unit number `unit`, found by a converged warp; false when there are fewer.
-__device__ __forceinline__ bool find_unit(const DeltaParams& p, int unit, int& n, int& c) {
+// Chunk c of sample n, unit number `unit`, found by a converged warp; false when there are fewer. A lane counts E
+// samples side by side.
+template <int E>
+__device__ __forceinline__ bool find_unit_by(const DeltaParams& p, int unit, int& n, int& c) {
   const int lane = threadIdx.x & 31;
   int64_t base = 0;
-  for (int n0 = 0; n0 < p.N; n0 += 32) {
-    const int64_t own = n0 + lane < p.N ? units_of(p, n0 + lane) : 0;
-    int64_t incl = base + own;
+  for (int n0 = 0; n0 < p.N; n0 += 32 * E) {
+    int own[E];
+    int64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int m = n0 + E * lane + e;
+      own[e] = m < p.N ? units_of(p, m) : 0;
+      sum += own[e];
+    }
+    int64_t incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, incl - base, o);
+      const int64_t x = __shfl_up_sync(~0u, incl, o);
       if (lane >= o) incl += x;
     }
+    incl += base;
     const uint32_t past = __ballot_sync(~0u, incl > unit);
     if (past != 0) {
       const int l = __ffs(past) - 1;
-      n = n0 + l;
-      c = static_cast<int>(unit - __shfl_sync(~0u, incl - own, l));
+      int64_t at = unit - (incl - sum);  // (lane l's is a chunk of its own samples)
+      int e = 0;
+#pragma unroll
+      for (int i = 0; i + 1 < E; ++i) {
+        if (e == i && at >= own[i]) {
+          at -= own[i];
+          ++e;
+        }
+      }
+      n = __shfl_sync(~0u, n0 + E * lane + e, l);
+      c = __shfl_sync(~0u, static_cast<int>(at), l);
       return true;
     }
     base = __shfl_sync(~0u, incl, 31);
   }
   return false;
+}
+__device__ __forceinline__ bool find_unit(const DeltaParams& p, int unit, int& n, int& c) {
+  return p.N <= 32 ? find_unit_by<1>(p, unit, n, c) : find_unit_by<4>(p, unit, n, c);
 }
 
 // A warp's columns of one state, four to a lane, and a token's step on them; CG: lanes across the columns.
