@@ -1,7 +1,7 @@
 // What a chunk of the gated delta rule needs of its keys, queries and gates alone, for every (chunk of 64 tokens,
 // value head) at once: with G_i the sum of the log decays up to and including token i of the chunk
 //     A_ij = beta_i e^{G_i - G_j} k_i.k_j  (j < i),    T = (I + A)^-1,    B_ij = scale e^{G_i - G_j} q_i.k_j  (j <= i)
-// T leaves as two bf16 terms, B as one, in the layout of the operands that the chain of chunks (delta_tc.cuh) multiplies
+// T and B leave as two bf16 terms each, in the layout of the operands that the chain of chunks (delta_tc.cuh) multiplies
 // by: for each block of 16 columns j the rows from the diagonal block on, in core matrices of 8 rows by 16 bytes, the
 // two of 16 columns behind one another. What lies above the diagonal's blocks is neither made nor stored.
 //
@@ -12,9 +12,12 @@
 // CUDA cores their reads of shared memory, 16 bytes for 16 additions, bound them). Sums of log decays are formed in 64
 // bits and kept as pairs of fp32 numbers, so that their differences are those of the tokens in between whatever
 // came before them.
-// Measured at 8 x 8192 tokens, 16 heads, D = 128 (16,384 units, 790 MB): 217 us, 3.6 TB/s. Some 7,300 warp instructions
+// Measured at 8 x 8192 tokens, 16 heads, D = 128 (16,384 units, 870 MB): 226 us, 3.8 TB/s. Some 7,300 warp instructions
 // a unit at 0.48 a cycle and scheduler; of ten resident warps four wait at a barrier between the steps, two for a fixed
-// latency. Five CTAs an SM (A beside K instead of over it) 229 us; one warp a unit, no barriers but 12 warps an SM, 300.
+// latency. With one term of B
+// 219 us; five CTAs an SM (A beside K instead of over it) a twentieth more; one warp a unit, no barriers but 12 warps an
+// SM, 300; weights of blocks left of the diagonal as products of a row's and a column's 2 % less at D = 128, 3 % more
+// at 64.
 #pragma once
 
 #include "delta.cuh"
@@ -24,8 +27,8 @@
 namespace memt {
 
 struct DeltaChunks {
-  // bytes of a unit: T's two terms and B, each for its blocks of columns 64, 48, 32 and 16 rows of 32 bytes
-  static constexpr int kTerm = (64 + 48 + 32 + 16) * 32, kBytes = 3 * kTerm;
+  // bytes of a unit: T's two terms and B's, each for its blocks of columns 64, 48, 32 and 16 rows of 32 bytes
+  static constexpr int kTerm = (64 + 48 + 32 + 16) * 32, kBytes = 4 * kTerm;
   // first byte of column block j
   static __host__ __device__ constexpr int block(int j) { return 32 * (64 * j - 8 * j * (j - 1)); }
   // byte of row r, columns col .. col + 7 (col a multiple of 8)
@@ -210,8 +213,9 @@ __global__ void __launch_bounds__(128, D == 256 ? 3 : 6) delta_chunks_kernel(con
       if (of_q) {
         uint32_t* to = reinterpret_cast<uint32_t*>(out + 2 * DeltaChunks::kTerm + DeltaChunks::at(16 * m, 16 * J + 8 * e) +
                                                    fg * 16 + ft * 2);
-        to[0] = pack_bf16x2(x[0], x[1]);
-        to[64] = pack_bf16x2(x[2], x[3]);  // eight rows on
+        constexpr int kNext = DeltaChunks::kTerm / 4;
+        split2(f32x2_pack(x[0], x[1]), to[0], to[kNext]);
+        split2(f32x2_pack(x[2], x[3]), to[64], to[kNext + 64]);  // eight rows on
       } else {
         *reinterpret_cast<float2*>(A + r0 * RL + col) = make_float2(x[0], x[1]);
         *reinterpret_cast<float2*>(A + (r0 + 8) * RL + col) = make_float2(x[2], x[3]);

@@ -13,16 +13,18 @@
 //
 // Precision. The state is fp32 in registers. K and V are bf16 as given; every fp32 factor of a product that the state
 // depends on (S in S^T K^T, T, R, w U) is split into two bf16 terms, which leaves 2^-16 of each value at most and a few
-// 1e-6 of the state in all (one term would leave 1e-3). S^T Q^T reads the first term only, B and the U of O^T are bf16:
-// what only the output sees is rounded like the output. Sums of log decays are formed in 64 bits; the decay of a
+// 1e-6 of the state in all (one term would leave 1e-3). S^T Q^T reads the first term only, and
+// the U of O^T is bf16: what only the output sees is rounded like the output. (B has two terms: with one the outputs are
+// 2.9e-3 from the definition instead of 2.4e-3, where their own rounding is 1.7e-3. Two of U instead: the chain 9 to 16 %
+// slower.) Sums of log decays are formed in 64 bits; the decay of a
 // whole chunk is a pair of fp32 numbers where it is the same for every chunk.
 //
 // Roles (24 warps): warp 0 issues MMAs, warp 1 loads tiles, warps 2 and 3 make the decay tables of alternate chunks;
 // warps 4-7 make the outputs; warps 8-23 hold the state, a quarter of the keys each warpgroup, and walk the chain
 // X -> R -> U -> w U -> P -> S. What bounds a chunk is that chain: each of its three batches of MMAs has some 350
 // cycles from the first arrival to the threads that read the result, beside its own time and that of the threads
-// (8 x 8192 tokens, 16 heads, D = 128: 389 us, 3.0 us a chunk with 128 SMs at work and 2.4 with 16; tensor pipe 28 %,
-// 1.4 TB/s). So it goes in two halves, of the keys
+// (8 x 8192 tokens, 16 heads, D = 128: 368 to 390 us in different runs, 3.0 us a chunk with 128 SMs at work and 2.4
+// with 16; tensor pipe 28 %, 1.4 TB/s). So it goes in two halves, of the keys
 // for S and P and of the tokens for R and U (warps 8-15 and 16-23), one half's threads working while the other
 // half's products are made: X's sum over the first keys needs the first half of S only, U's first tokens only the first
 // half of R (T is lower triangular), P's sum over the first tokens only the first half of w U. V is fetched while P is
@@ -81,7 +83,8 @@ struct DeltaTcCfg {
   static constexpr bool kAlias = D == 256;
   static constexpr uint32_t kColS = 0, kColX = D, kColR = kColX + 64, kColU = kColR + 64, kColXQ = kColU + 64,
                             kColO = kAlias ? kColU : kColXQ + 128, kColEnd = kAlias ? kColXQ + 64 : kColO + 64;
-  // registers per thread after the split of the launch's 6 x 80 over the warpgroups
+  // registers per thread after the split of the launch's 6 x 80 over the warpgroups (40, 56, 96 at D = 128: the chain a sixth
+  // slower; more for the outputs, fewer for the state: the same)
   static constexpr int kRegsControl = D == 256 ? 40 : 56, kRegsOut = D == 256 ? 56 : 72,
                        kRegsState = D == 256 ? 96 : 88;
   static_assert(kRegsControl + kRegsOut + 4 * kRegsState <= 6 * 80, "no more than the launch's registers");
@@ -397,9 +400,11 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         if (OUT && !Cfg::kAlias && c > 0) wait(OE, c - 1);
         if (go()) {
 #pragma unroll
-          for (int j = 0; OUT && j < 4; ++j)
-            tc::mma_bf16_ts(tO + 16 * j, tX + 8 * j, dt + (2 * kTerm + rows(j, 16 * j)),
-                            tc::idesc(tc::kBF16, 128, 64 - 16 * j, false, false), j > 0);
+          for (int i = 0; OUT && i < 8; ++i) {  // B's second term, then its first
+            const int j = i & 3;
+            tc::mma_bf16_ts(tO + 16 * j, tX + 8 * j, dt + ((i < 4 ? 3 : 2) * kTerm + rows(j, 16 * j)),
+                            tc::idesc(tc::kBF16, 128, 64 - 16 * j, false, false), i > 0);
+          }
           tc::commit(B(OD));
           tc::commit(B(LE + s));
         }

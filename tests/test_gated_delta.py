@@ -304,7 +304,7 @@ def test_segments(cuda, D, lengths, decay):
     Hk, H = (1, 2) if len(lengths) == 1 else (1, 1)
     x = _inputs(4, lengths, Hk, H, D, torch.bfloat16, decay=decay)
     need = _lib.load().memt_gated_delta_workspace_size
-    chunked = (sum(lengths) // 64 + len(lengths)) * H * 15360 + 256
+    chunked = (sum(lengths) // 64 + len(lengths)) * H * 20480 + 256
     assert need(len(lengths), sum(lengths), H, D, _lib.MEMT_BF16) > chunked  # (holds states of segments)
     o, final = M.gated_delta(*x)
     _check(o, final, x, torch.bfloat16, D ** -0.5, joined=True)
