@@ -75,8 +75,8 @@ size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Tokens up to which a bf16 sample runs token by token. Measured, the token kernel alone against chunks alone, 16 heads,
 // us: 256 samples at D = 64: 8 tokens 95 / 342, 32 264 / 356, 48 349 / 363; D = 128: 8 tokens 211 / 455, 20 427 / 459, 24
-// 498 / 459; 64 samples at D = 256: 6 tokens 209 / 351, 12 298 / 355, 16 361 / 356. (The token kernel's times include some
-// 30 us of the chunks' launches that find no sample.)
+// 498 / 459; 64 samples at D = 256: 6 tokens 209 / 351, 12 298 / 355, 16 361 / 356. (The token kernel's times include
+// launches for chunks that find no sample.)
 int few_tokens(int D) { return D == 64 ? 40 : (D == 128 ? 20 : 14); }
 
 // Whether both forms run, each for its samples by their own lengths: up to 64 tokens a sample in the mean.
@@ -91,6 +91,18 @@ int64_t max_units(int64_t N, int64_t L, int D) {
 size_t units_bytes(int64_t N, int64_t L, int64_t H, int D) {
   return align256(size_t(max_units(N, L, D)) * H * DeltaChunks::kBytes);
 }
+
+// Tables of a call of many samples (delta_plan_kernel), behind the units: the bytes of all and of each.
+struct Tables {
+  size_t units, first, longs;
+  Tables(int64_t N, int64_t L, int D) : units(0), first(0), longs(0) {
+    if (N <= 32) return;  // a warp finds its sample at once
+    units = align256(size_t(max_units(N, L, D)) * sizeof(int2));
+    first = align256(size_t(N + 1) * sizeof(int32_t));
+    longs = align256(size_t(L / (few_tokens(D) + 1)) * sizeof(int32_t));
+  }
+  size_t bytes() const { return units + first + longs; }
+};
 
 // Whether a launch of the call could have more CTAs than a grid holds (at most eight a unit or sample and head: some 10^10
 // tokens and heads, more than memory does).
@@ -179,7 +191,7 @@ size_t memt_gated_delta_workspace_size(int32_t N, int64_t L, int32_t H, int32_t 
   const int seg_chunks = mixed(N, L) ? 0 : plan_segment_chunks(N, L, H, D);
   const size_t states =
       seg_chunks == 0 ? 0 : align256(size_t(max_segments(N, L, seg_chunks)) * H * D * D * sizeof(float));
-  return units_bytes(N, L, H, D) + 2 * states;
+  return units_bytes(N, L, H, D) + Tables(N, L, D).bytes() + 2 * states;
 }
 
 int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t workspace_bytes,
@@ -228,26 +240,38 @@ int memt_gated_delta(const memt_gated_delta_args* a, void* workspace, size_t wor
   if (a->dtype == MEMT_F32 || a->total_tokens == 0) return launch_tokens<float>(a->head_dim, p, s);
   const int few = few_tokens(a->head_dim);
   if (a->total_tokens <= few) return launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
-  p.few = -1;
-  if (mixed(p.N, p.L)) {
-    p.few = few;
-    const int64_t most = p.L / (few + 1);
-    p.only_long = most <= p.N / 2 ? static_cast<int32_t>(most) : 0;
-    const int st_few = launch_tokens<__nv_bfloat16>(a->head_dim, p, s);
+  const int D = a->head_dim;
+  const bool both = mixed(p.N, p.L);
+  const int64_t most = p.L / (few + 1);  // samples of more than `few` tokens, unless offsets overlap
+  p.few = both ? few : -1;
+  p.only_long = both && most <= p.N / 2 ? static_cast<int32_t>(most) : 0;
+  p.max_units = static_cast<int32_t>(max_units(p.N, p.L, D));
+  unsigned char* at = static_cast<unsigned char*>(workspace);
+  p.chunks = at;
+  at += units_bytes(p.N, p.L, p.H, D);
+  const Tables tables(p.N, p.L, D);
+  if (tables.bytes() > 0) {
+    p.unit_table = reinterpret_cast<int2*>(at);
+    p.first_unit = reinterpret_cast<int32_t*>(at + tables.units);
+    p.longs = reinterpret_cast<int32_t*>(at + tables.units + tables.first);
+    at += tables.bytes();
+    ProfScope prof(kProfLinear, s);
+    delta_plan_kernel<<<1, kPlanThreads, 0, s>>>(p, p.only_long);
+    const int st_plan = cuda_status(cudaGetLastError());
+    if (st_plan != MEMT_OK) return st_plan;
+  }
+  if (both) {
+    const int st_few = launch_tokens<__nv_bfloat16>(D, p, s);
     if (st_few != MEMT_OK) return st_few;
   }
-  const int D = a->head_dim;
-  p.chunks = workspace;
-  p.max_units = static_cast<int32_t>(max_units(p.N, p.L, D));
   p.seg_chunks = mixed(p.N, p.L) ? 0 : plan_segment_chunks(p.N, p.L, p.H, D);
   if (p.seg_chunks > 0) {
     const int64_t segments = max_segments(p.N, p.L, p.seg_chunks);
     p.max_segments = static_cast<int32_t>(segments);
-    p.seg_states = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + units_bytes(p.N, p.L, p.H, D));
-    p.seg_moves = reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(p.seg_states) +
-                                           align256(size_t(segments) * p.H * D * D * sizeof(float)));
+    p.seg_states = reinterpret_cast<float*>(at);
+    p.seg_moves = reinterpret_cast<float*>(at + align256(size_t(segments) * p.H * D * D * sizeof(float)));
   }
-  return launch_chunked(a->head_dim, p, s);
+  return launch_chunked(D, p, s);
 } catch (...) {  // the launch bookkeeping may run out of host memory
   return MEMT_ERR_CUDA;
 }

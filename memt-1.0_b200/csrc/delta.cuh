@@ -29,6 +29,11 @@ struct DeltaParams : LinearParams {
   // as many as there can be unless offsets overlap.
   int32_t max_units;
   void* chunks;
+  // Calls of many samples: where a unit's chunk is (sample, chunk; -1 behind the last), a sample's first unit [N + 1], and
+  // the samples of more than `few` tokens (-1 behind the last; only_long of them). Otherwise null: searched for.
+  int2* unit_table;
+  int32_t* first_unit;
+  int32_t* longs;
   // Segments of few long samples (linear.cuh): seg_states and, as large, what each makes of an identity.
   float* seg_moves;
 };
@@ -41,6 +46,11 @@ __device__ __forceinline__ int units_of(const DeltaParams& p, int n) {
 
 // The units of sample n, by a converged warp: the first one's number and how many.
 __device__ __forceinline__ void sample_units(const DeltaParams& p, int n, int& first, int& count) {
+  if (p.first_unit != nullptr) {
+    first = p.first_unit[n];
+    count = p.first_unit[n + 1] - first;
+    return;
+  }
   int64_t before = 0;
   for (int m = threadIdx.x & 31; m < n; m += 32) before += units_of(p, m);
 #pragma unroll
@@ -50,50 +60,85 @@ __device__ __forceinline__ void sample_units(const DeltaParams& p, int n, int& f
   count = static_cast<int>(end < p.max_units ? end : p.max_units) - first;
 }
 
-// Chunk c of sample n, unit number `unit`, found by a converged warp; false when there are fewer. A lane counts E
-// samples side by side.
-template <int E>
-__device__ __forceinline__ bool find_unit_by(const DeltaParams& p, int unit, int& n, int& c) {
+// Chunk c of sample n, unit number `unit`, found by a converged warp; false when there are fewer.
+__device__ __forceinline__ bool find_unit(const DeltaParams& p, int unit, int& n, int& c) {
+  if (p.unit_table != nullptr) {
+    const int2 x = p.unit_table[unit];
+    n = x.x;
+    c = x.y;
+    return n >= 0;
+  }
   const int lane = threadIdx.x & 31;
   int64_t base = 0;
-  for (int n0 = 0; n0 < p.N; n0 += 32 * E) {
-    int own[E];
-    int64_t sum = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int m = n0 + E * lane + e;
-      own[e] = m < p.N ? units_of(p, m) : 0;
-      sum += own[e];
-    }
-    int64_t incl = sum;
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    const int64_t own = n0 + lane < p.N ? units_of(p, n0 + lane) : 0;
+    int64_t incl = base + own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t x = __shfl_up_sync(~0u, incl, o);
+      const int64_t x = __shfl_up_sync(~0u, incl - base, o);
       if (lane >= o) incl += x;
     }
-    incl += base;
     const uint32_t past = __ballot_sync(~0u, incl > unit);
     if (past != 0) {
       const int l = __ffs(past) - 1;
-      int64_t at = unit - (incl - sum);  // (lane l's is a chunk of its own samples)
-      int e = 0;
-#pragma unroll
-      for (int i = 0; i + 1 < E; ++i) {
-        if (e == i && at >= own[i]) {
-          at -= own[i];
-          ++e;
-        }
-      }
-      n = __shfl_sync(~0u, n0 + E * lane + e, l);
-      c = __shfl_sync(~0u, static_cast<int>(at), l);
+      n = n0 + l;
+      c = static_cast<int>(unit - __shfl_sync(~0u, incl - own, l));
       return true;
     }
     base = __shfl_sync(~0u, incl, 31);
   }
   return false;
 }
-__device__ __forceinline__ bool find_unit(const DeltaParams& p, int unit, int& n, int& c) {
-  return p.N <= 32 ? find_unit_by<1>(p, unit, n, c) : find_unit_by<4>(p, unit, n, c);
+
+// The tables of a call of many samples, by one CTA: a search in every CTA of the others would take their number times
+// that of the samples (4096 samples of 8 tokens, 16 heads: half of the call). num_longs: entries of `longs`.
+constexpr int kPlanThreads = 1024;
+__global__ void __launch_bounds__(kPlanThreads) delta_plan_kernel(const DeltaParams p, int num_longs) {
+  __shared__ int64_t s_units[kPlanThreads / 32];
+  __shared__ int s_longs[kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto clamp = [&](int64_t u) { return static_cast<int>(u < p.max_units ? u : p.max_units); };
+  int64_t base = 0;
+  int long_base = 0;
+  for (int n0 = 0; n0 < p.N; n0 += kPlanThreads) {
+    const int n = n0 + tid;
+    const int own = n < p.N ? units_of(p, n) : 0;
+    int64_t incl = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(~0u, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const uint32_t longer = __ballot_sync(~0u, own > 0);
+    if (lane == 31) {
+      s_units[warp] = incl;
+      s_longs[warp] = __popc(longer);
+    }
+    __syncthreads();
+    int64_t first = base + incl - own;
+    int rank = long_base + __popc(longer & ((1u << lane) - 1));
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) {
+        first += s_units[w];
+        rank += s_longs[w];
+      }
+      base += s_units[w];
+      long_base += s_longs[w];
+    }
+    if (n < p.N) p.first_unit[n] = clamp(first);
+    if (own > 0 && rank < num_longs) p.longs[rank] = n;
+    for (uint32_t rest = longer; rest != 0; rest &= rest - 1) {  // a sample's units, by the warp
+      const int l = __ffs(rest) - 1;
+      const int64_t from = __shfl_sync(~0u, first, l);
+      const int to = clamp(from + __shfl_sync(~0u, own, l));
+      for (int64_t u = from + lane; u < to; u += 32)
+        p.unit_table[u] = make_int2(n0 + 32 * warp + l, static_cast<int>(u - from));
+    }
+    __syncthreads();
+  }
+  if (tid == 0) p.first_unit[p.N] = clamp(base);
+  for (int u = clamp(base) + tid; u < p.max_units; u += kPlanThreads) p.unit_table[u] = make_int2(-1, 0);
+  for (int i = long_base + tid; i < num_longs; i += kPlanThreads) p.longs[i] = -1;
 }
 
 // A warp's columns of one state, four to a lane, and a token's step on them; CG: lanes across the columns.

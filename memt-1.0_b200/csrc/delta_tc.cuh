@@ -208,16 +208,9 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   if (p.seg_chunks > 0) {
     if (!find_segment(p, unit, n, seg, segs)) return;
     if (!OUT && seg + 1 == segs) return;  // the first pass is for what later segments start from
-  } else if (p.only_long) {  // by one warp: most find none, and a search by all of them would take their time
-    int* found = reinterpret_cast<int*>(sm + Cfg::kOffBar);
-    if (warp == 0) {
-      const int x = find_long(p, unit);
-      if (lane == 0) *found = x;
-    }
-    __syncthreads();
-    n = *found;
+  } else if (p.only_long) {
+    n = p.longs != nullptr ? p.longs[unit] : find_long(p, unit);
     if (n < 0) return;
-    __syncthreads();
   } else if (p.by_length) {
     n = sample_by_length(p, unit);
   }

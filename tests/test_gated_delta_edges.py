@@ -166,3 +166,21 @@ def test_a_step_with_a_value_that_is_not_finite(cuda, dtype, value):
     o2[1, 1, 7] = o[1, 1, 7]
     states[1, 1, :, 7] = clean[1, 1, :, 7]
     assert torch.equal(o2, o) and torch.equal(states, clean)
+
+
+@gpu
+@pytest.mark.parametrize("N,most", [(1500, 12), (1030, 67), (33, 200)])
+def test_many_samples(cuda, N, most):
+    """Calls whose chunks are listed before (more than 32 samples, and more than one round of a CTA): few tokens each
+    with longer ones among them, all in chunks, and empty ones."""
+    gen = torch.Generator().manual_seed(N)
+    lengths = torch.randint(0 if most == 12 else most - 3, most + 1, (N,), generator=gen)
+    if most == 12:
+        longer = torch.randperm(N, generator=gen)[:40]
+        lengths[longer] = torch.randint(41, 300, (40,), generator=gen)
+    lengths[-1], lengths[5] = 0, 0
+    x = _inputs(37, lengths.tolist(), 1, 1, 64, torch.bfloat16)
+    o, final = M.gated_delta(*x)
+    _check(o, final, x, torch.bfloat16, 64 ** -0.5)
+    other = M.gated_delta(*x[:6], x[6].cuda())
+    assert torch.equal(o, other[0]) and torch.equal(final, other[1])
