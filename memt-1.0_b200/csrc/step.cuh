@@ -12,9 +12,10 @@
 // registers, then over warps through shared memory. All state loads are issued before the
 // token's vectors are fetched. A CTA takes 64 value columns, so that several on an SM are in different
 // phases, and marks its loads and stores as read and written once. 256 sessions x 16 heads x 128 x 128
-// (537 MB): 83.4 us linear, 87.1 us gated delta, 0.99 and 0.95 of the measured copy rate. Measured for the
-// gated delta: 128 columns 95 us (93 without the marks), 64 without the marks on loads 96, on stores 97;
-// states streamed through shared memory by bulk copies in a persistent CTA 104.
+// (537 MB): 83.4 us linear, 87.1 us stable GDN-2, 0.99 and 0.95 of the measured copy rate (per call 85.7, 93.3, and 90.0
+// with the gated delta rule's one decay and beta a head). Measured for GDN-2: 128 columns 95 us (93 without the
+// marks), 64 without the marks on loads 96, on stores 97; states streamed through shared memory by bulk copies in a
+// persistent CTA 104.
 #pragma once
 
 #include "common.cuh"

@@ -252,7 +252,8 @@ def gated_delta(q, k, v, g, beta, initial_state, cu_seqlens, *, scale=None, out=
     o_t = scale S_t^T q_t. q, k: [L, Hk, D]; v: [L, H, D], bf16 or fp32, D 64, 128 or 256 (keys are meant to be of
     unit length, as ``qwen_prologue`` makes them: beta |k|^2 above 2 lets the state grow). g: fp32 natural-log
     decay <= 0, [L, H], [H] or None. beta: in v's dtype, [L, H] for each value head or [L, Hk] for each key head, or
-    None (1). ``gated_delta_step`` continues a sample token by token.
+    None (1). ``gated_delta_step`` continues a sample token by token. Within the roundings of the forms (bf16 in chunks
+    or token by token, whole or in segments) a sample's result may differ with what it is packed with.
 
     States, slots, offsets, scale and ``out`` as in ``linear_attention``, their rules on overlaps too.
     """
