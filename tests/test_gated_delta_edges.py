@@ -184,3 +184,23 @@ def test_many_samples(cuda, N, most):
     _check(o, final, x, torch.bfloat16, 64 ** -0.5)
     other = M.gated_delta(*x[:6], x[6].cuda())
     assert torch.equal(o, other[0]) and torch.equal(final, other[1])
+
+
+@gpu
+@pytest.mark.parametrize("first,second", [([7, 60, 0, 130] * 10, [0, 41, 150, 6] * 10), ([5000, 1000], [900, 5100]),
+                                          ([9, 2, 33, 5] * 12, [1, 45, 0, 3] * 12)])
+def test_offsets_change_between_replays(cuda, first, second):
+    """The lengths are the device's: a captured call follows them."""
+    assert sum(first) == sum(second)
+    x = _inputs(38, first, 1, 1, 64, torch.bfloat16)
+    cu = x[6].cuda()
+    other = torch.tensor([0] + second).cumsum(0).to(torch.int32).cuda()
+    want = [M.gated_delta(*x[:6], c.clone()) for c in (cu, other)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = M.gated_delta(*x[:6], cu)
+    for offsets, (o, final) in ((other, want[1]), (x[6].cuda(), want[0]), (other, want[1])):
+        cu.copy_(offsets)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], o) and torch.equal(got[1], final)
