@@ -35,8 +35,10 @@
 // Values that are not finite: the zeros of T and B meet them in tokens they must not reach. Whatever spoils a token
 // never leaves the state, so a CTA looks at its final state; a warp's columns of which one is not finite are made
 // again token by token (DeltaAgain) from the initial state, outputs too (2 us a token).
-// Every wait is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, the control
-// warps drain what they have in flight, and the final state is NaN.
+// Every wait for an mbarrier is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, and the
+// control warps drain what they have in flight. Named barriers have no bound of their own: the MMA warp comes to all of
+// them, whatever it has given up, and so does each warp of the chain, once a phase: its waits keep it from arriving
+// twice, and where one of them has run out it joins the barrier instead of passing it (hand_over).
 #pragma once
 
 #include "delta_chunks.cuh"
@@ -279,6 +281,10 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   auto arrive = [&](int b) {  // one arrival per warp
     __syncwarp();
     if (lane == 0) mbar_arrive(B(b));
+  };
+  auto hand_over = [&](int id) {  // chain -> MMA, by a warp of which all or none have given up
+    if (alive) bar_arrive<288>(id);
+    else bar_sync<288>(id);
   };
 
   if (warp < 4) {
@@ -592,7 +598,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     const int half = part >> 1;  // of the chain
     auto ready = [&](int b, uint32_t phase) {
       wait(b + half, phase);
-      __syncwarp();
+      alive = __all_sync(~0u, alive);
       tc::fence_after();
     };
     // V of a chunk as fragments of 16 values by 16 tokens: a register holds two tokens of one value; and its gates
@@ -602,8 +608,8 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
       const int s = c % NS;
       wait(LF + s, c / NS);
       wait(TF + c % NT, c / NT);
+      alive = __all_sync(~0u, alive);
       const DeltaTable& t = tab[c % NT];
-      __syncwarp();
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int val = (32 * quad + 16 * e) % Cfg::kVB + 8 * pval, tok = 16 * part + prow;
@@ -639,7 +645,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
       }
       tc::wait_st();
       tc::fence_before();
-      bar_arrive<288>(kBarS + half);
+      hand_over(kBarS + half);
       const DeltaTable& t = tab[c % NT];
       {  // R = beta v - beta e^G X
         uint64_t y[2][4];
@@ -665,7 +671,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
       }
       tc::wait_st();
       tc::fence_before();
-      bar_arrive<288>(kBarR + half);
+      hand_over(kBarR + half);
       uint64_t ww[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -693,7 +699,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
       }
       tc::wait_st();
       tc::fence_before();
-      bar_arrive<288>(kBarW + half);
+      hand_over(kBarW + half);
       arrive(TE + c % NT);
       if (c + 1 < nchunks) fetch(c + 1);
       ready(PD, c);
