@@ -494,7 +494,9 @@ size_t memt_gated_delta_workspace_size(int32_t num_samples, int64_t total_tokens
 int memt_gated_delta(const memt_gated_delta_args *args, void *workspace, size_t workspace_bytes,
                      memt_stream_t stream);
 
-/* As memt_linear_attention_status, of the bf16 calls of memt_gated_delta. */
+/* As memt_linear_attention_status, of the bf16 calls of memt_gated_delta. What a thread block has stored is NaN where a
+ * wait of it ran out: its sample's outputs (with segments, its segment's) and final state in up to 128 value columns of a
+ * head, and all that starts from that state. */
 int memt_gated_delta_status(memt_stream_t stream, int32_t *status_out);
 
 /* ---- one token of a recurrence, states in place --------------------------

@@ -35,8 +35,8 @@
 // Values that are not finite: the zeros of T and B meet them in tokens they must not reach. Whatever spoils a token
 // never leaves the state, so a CTA looks at its final state; a warp's columns of which one is not finite are made
 // again token by token (DeltaAgain) from the initial state, outputs too (2 us a token).
-// Every wait for an mbarrier is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, and the
-// control warps drain what they have in flight. Named barriers have no bound of their own: the MMA warp comes to all of
+// Every wait for an mbarrier is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, the
+// control warps drain what they have in flight, and all that the CTA has stored becomes NaN (delta_lost). Named barriers have no bound of their own: the MMA warp comes to all of
 // them, whatever it has given up, and so does each warp of the chain, once a phase: its waits keep it from arriving
 // twice, and where one of them has run out it joins the barrier instead of passing it (hand_over).
 #pragma once
@@ -190,6 +190,29 @@ __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h,
   if (end != nullptr) cols.store(end + col);
 }
 
+// All that a CTA has stored becomes NaN: a wait of it ran out, in whichever role, and nothing of it can be relied on.
+template <int D, bool OUT>
+__device__ __forceinline__ void delta_lost(const DeltaParams& p, int n, int64_t bos, int64_t eos, bool last) {
+  constexpr int VB = DeltaTcCfg<D>::kVB, NT = DeltaTcCfg<D>::kThreads;
+  int cta;  // as in the kernel, which must not hold registers for this
+  asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(cta));
+  const int vblk = cta % (D / VB), rest = cta / (D / VB), h = rest / (OUT ? 1 : 2) % p.H;
+  const bool moves = !OUT && rest % 2;
+  const int64_t seg_state = (int64_t)(rest / (OUT ? 1 : 2)) * D * D;
+  const float nan = __int_as_float(0x7fffffff);
+  const int64_t out_slot = pool_slot(p.slots_out, p.num_out, n);
+  const bool taken = __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, threadIdx.x & 31, 32));
+  float* end = OUT ? (last && out_slot >= 0 && !taken ? p.ht + (out_slot * p.H + h) * D * D : nullptr)
+                   : (moves ? p.seg_moves : p.seg_states) + seg_state;
+  if (end != nullptr)
+    for (int i = threadIdx.x; i < D * VB; i += NT)
+      end[!OUT && moves ? vblk * VB * D + i : i / VB * D + vblk * VB + i % VB] = nan;
+  if constexpr (OUT) {
+    __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + (int64_t)h * D + vblk * VB;
+    for (int64_t i = threadIdx.x; i < (eos - bos) * VB; i += NT) store_f32(o, (bos + i / VB) * p.so + i % VB, nan);
+  }
+}
+
 // OUT: outputs and final states. Otherwise the first pass over segments: what a segment adds to a zero state
 // (seg_states) and makes of an identity without values (seg_moves, transposed), in a CTA each.
 template <int D, bool OUT>
@@ -238,11 +261,12 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   // (UD) and P (PD) and O (OD) ready; outputs read (OE); drained (DR)
   constexpr int LF = 0, LE = LF + NS, TF = LE + NS, TE = TF + NT, XD = TE + NT, UD = XD + 2, PD = UD + 2, OD = PD + 2,
                 OE = OD + 1, DR = OE + 1, NBAR = DR + 1;
-  static_assert(NBAR * 8 + 24 <= 512, "barrier area");
+  static_assert(NBAR * 8 + 40 <= 512, "barrier area");
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Cfg::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Cfg::kOffBar + NBAR * 8);
   uint32_t* spoiled = tmem_slot + 1;  // bit c: some value of the CTA's c-th group of columns (DeltaAgain) is not finite
   uint32_t* stalled = tmem_slot + 2;  // a wait ran out
+  int32_t* whose = reinterpret_cast<int32_t*>(tmem_slot + 3);  // sample, first and last token, whether the sample ends here
   const uint32_t base = smem_u32(sm), bars = smem_u32(bar);
   auto B = [&](int i) { return bars + 8 * i; };
   if (tid == 0) {
@@ -255,6 +279,10 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     mbar_fence_init();
     *spoiled = 0;
     *stalled = 0;
+    whose[0] = n;
+    whose[1] = static_cast<int>(bos);
+    whose[2] = static_cast<int>(eos);
+    whose[3] = seg + 1 == segs;
   }
   if (warp == 0) tc::alloc(smem_u32(tmem_slot), 512);
   tc::fence_before();
@@ -271,7 +299,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   };
 
   bool alive = true;
-  auto wait = [&](int b, uint32_t phase) {  // a wait that ran out is known to all before anything follows it
+  auto wait = [&](int b, uint32_t phase) {
     if (alive) alive = mbar_wait_polls(B(b), phase & 1);
   };
   auto wait_long = [&](int b, uint32_t phase) {  // by a warp that is ahead of the others and need not hurry
@@ -578,11 +606,14 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     const bool writes = D >= 128 || quad < 2;  // at D = 64 quadrants 2 and 3 repeat 0 and 1
     const int pair = 2 * (lane & 3);
     const int prow = 8 * (lane >> 4) + (lane & 7), pval = (lane >> 3) & 1;  // row of an ldmatrix piece
-    const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n), out_slot = pool_slot(p.slots_out, p.num_out, n);
     const int64_t head = (int64_t)D * D, col_off = (int64_t)(KT * part) * D + vblk * Cfg::kVB + vr;
     const int64_t seg_state = ((int64_t)unit * p.H + h) * head;
-    const float* start = p.h0 != nullptr && in_slot >= 0 ? p.h0 + (in_slot * p.H + h) * head : nullptr;
-    if (segs > 1) start = OUT ? p.seg_states + seg_state : nullptr;
+    auto first_state = [&](int n) -> const float* {
+      if (!OUT || segs > 1) return OUT ? p.seg_states + seg_state : nullptr;
+      const int64_t in_slot = pool_slot(p.slots_in, p.num_in, n);
+      return p.h0 != nullptr && in_slot >= 0 ? p.h0 + (in_slot * p.H + h) * head : nullptr;
+    };
+    const float* start = first_state(n);
     uint64_t S[KT / 2];  // pairs of fp32: keys KT part + 2 i, + 2 i + 1 of value vr
     if (start != nullptr) {
       const float* src = start + col_off;
@@ -719,7 +750,9 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         }
       }
     }
-    const bool taken = OUT && __any_sync(~0u, slot_taken(p.slots_out, n, out_slot, lane, 32));
+    const int sample = whose[0];  // (read back: registers held over the chain are few)
+    const int64_t out_slot = pool_slot(p.slots_out, p.num_out, sample);
+    const bool taken = OUT && __any_sync(~0u, slot_taken(p.slots_out, sample, out_slot, lane, 32));
     // No state is stored before every thread has loaded its share of the first one and, where one is not finite,
     // before columns have been made from them again, their outputs over those stored above.
     constexpr int kGroup = DeltaAgain<D>::kCols;
@@ -733,12 +766,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     if (!OUT) end = (moves ? p.seg_moves : p.seg_states) + seg_state;
     // (what a segment that is not finite hands on is not made again: a column of it is spoiled as it is)
     const uint32_t again = !OUT ? 0 : tokenwise ? ~0u : *spoiled;
-    const bool lost = *stalled != 0;
-    if (lost) {  // the caller sees it in the state
-#pragma unroll
-      for (int i = 0; i < KT / 2; ++i) S[i] = f32x2_splat(__int_as_float(0x7fffffff));
-    }
-    if (writes && end != nullptr && (lost || !(again >> (vr / kGroup) & 1))) {
+    if (writes && end != nullptr && !(again >> (vr / kGroup) & 1)) {
       if (moves) {  // [value column][key], as the join reads it
         ulonglong2* dst = reinterpret_cast<ulonglong2*>(end + (int64_t)(vblk * Cfg::kVB + vr) * D + KT * part);
 #pragma unroll
@@ -752,15 +780,20 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         }
       }
     }
-    if (OUT && again != 0 && !lost) {
+    if (OUT && again != 0 && alive) {
       for (int g = warp - 8; g < Cfg::kVB / kGroup; g += 16)
-        if (again >> g & 1) delta_columns_again<D>(p, h, vblk * Cfg::kVB + g * kGroup, bos, eos, start, end);
+        if (again >> g & 1)
+          delta_columns_again<D>(p, h, vblk * Cfg::kVB + g * kGroup, whose[1], whose[2], first_state(sample), end);
     }
   }
-  if (!alive) atomicOr(&g_delta_status, 1);
+  if (!alive) {
+    atomicOr(&g_delta_status, 1);
+    *stalled = 1;
+  }
   tc::fence_before();
-  __syncthreads();
+  __syncthreads();  // every wait of every role lies before
   if (warp == 0) tc::dealloc(tmem, 512);
+  if (*stalled != 0) delta_lost<D, OUT>(p, whose[0], whose[1], whose[2], whose[3] != 0);
 }
 
 }  // namespace memt

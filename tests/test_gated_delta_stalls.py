@@ -8,6 +8,7 @@ given up (``hand_over`` in the kernel).
 
 import random
 import re
+import subprocess
 from pathlib import Path
 
 import pytest
@@ -140,3 +141,109 @@ def test_the_chain_joins_named_barriers_once_it_has_given_up():
         assert f"hand_over({bar} + half)" in code and f"bar_sync<288>({bar})" in code
     # a warp of the chain has given up as a whole: behind both places where it waits
     assert code.count("alive = __all_sync(~0u, alive);") == 2
+
+
+# ---------------------------------------------------------------------------
+# what a CTA has stored, once one of its waits ran out
+# ---------------------------------------------------------------------------
+
+def test_a_wait_that_ran_out_is_seen_behind_the_last_barrier():
+    """Whichever role's it was: all join the barrier behind which the flag is read, and set it before."""
+    code = re.sub(r"\s+", " ", _code("delta_tc.cuh"))
+    tail = code[code.rindex("__syncthreads();"):]
+    before = code[:code.rindex("__syncthreads();")]
+    assert "if (*stalled != 0) delta_lost<D, OUT>(" in tail
+    assert before.rindex("*stalled = 1;") > before.rindex("hand_over(") > before.index("*stalled = 0;")
+    assert "if (!alive) { atomicOr(&g_delta_status, 1); *stalled = 1; }" in before
+
+
+_HOST = r"""
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <vector>
+#include <cmath>
+#define __device__
+#define __forceinline__ inline
+struct { unsigned x; } threadIdx;
+static int g_cta;
+struct bf16 { uint16_t x; };
+typedef bf16 __nv_bfloat16;
+static float __int_as_float(int i) { float f; memcpy(&f, &i, 4); return f; }
+static bool __any_sync(unsigned, bool x) { return x; }
+static void store_f32(bf16* p, int64_t i, float f) { uint32_t u; memcpy(&u, &f, 4); p[i].x = u >> 16; }
+struct DeltaParams { int H; float *ht, *seg_moves, *seg_states; const int32_t* slots_out; int num_out; void* out; int64_t so; };
+static int64_t pool_slot(const int32_t* s, int num, int n) {
+  if (s == nullptr) return n;
+  return s[n] < 0 || s[n] >= num ? -1 : s[n];
+}
+static bool slot_taken(const int32_t* s, int n, int64_t slot, int, int) {
+  bool t = false;
+  if (s != nullptr && slot >= 0) for (int m = 0; m < n; ++m) t |= s[m] == slot;
+  return t;
+}
+template <int D> struct DeltaTcCfg { static constexpr int kVB = D < 128 ? D : 128, kBlocks = D / kVB, kThreads = 768; };
+FUNCTION
+
+template <typename T> static bool nan_at(const T& x);
+template <> bool nan_at(const float& x) { return std::isnan(x); }
+template <> bool nan_at(const bf16& x) { return (x.x & 0x7f80) == 0x7f80 && (x.x & 0x7f); }
+
+template <int D, bool OUT> static int check() {
+  const int H = 3, N = 3, L = 23, VB = DeltaTcCfg<D>::kVB, B = D / VB;
+  const int32_t slots[N] = {1, 1, -1};
+  const int64_t so = H * D + 8, bos[N] = {2, 9, 9}, eos[N] = {9, 9, 20};
+  int bad = 0;
+  for (int pool = 0; pool < 2; ++pool)
+    for (int last = 0; last < 2; ++last)
+      for (g_cta = 0; g_cta < N * H * B * (OUT ? 1 : 2); ++g_cta) {
+        std::vector<float> ht(N * H * D * D), mv(ht), st(ht);
+        std::vector<bf16> out(L * so);
+        DeltaParams p{H, ht.data(), mv.data(), st.data(), pool ? slots : nullptr, N, out.data(), so};
+        const int vblk = g_cta % B, rest = g_cta / B / (OUT ? 1 : 2), unit = rest / H, h = rest % H;
+        const bool moves = !OUT && g_cta / B % 2;
+        for (threadIdx.x = 0; threadIdx.x < 768; ++threadIdx.x)
+          delta_lost<D, OUT>(p, unit, bos[unit], eos[unit], last);
+        const int slot = !pool ? unit : unit == 0 ? 1 : -1;  // (slot 1 is the first sample's)
+        for (int n = 0; n < N; ++n)
+          for (int g = 0; g < H; ++g)
+            for (int k = 0; k < D; ++k)
+              for (int v = 0; v < D; ++v) {
+                const size_t at = ((size_t)n * H + g) * D * D;
+                const bool cols = v / VB == vblk && g == h, own = cols && n == unit;
+                bad += nan_at(ht[at + k * D + v]) != (OUT && last && cols && n == slot);
+                bad += nan_at(st[at + k * D + v]) != (!OUT && !moves && own);
+                bad += nan_at(mv[at + v * D + k]) != (!OUT && moves && own);  // [value column][key]
+              }
+        for (int t = 0; t < L; ++t)
+          for (int c = 0; c < so; ++c)
+            bad += nan_at(out[t * so + c]) != (OUT && t >= bos[unit] && t < eos[unit] && c / D == h && c < H * D &&
+                                               c % D / VB == vblk);
+      }
+  return bad;
+}
+
+int main() {
+  const int bad[6] = {check<64, true>(), check<64, false>(), check<128, true>(), check<128, false>(),
+                      check<256, true>(), check<256, false>()};
+  int all = 0;
+  for (int b : bad) all += b;
+  printf("%d\n", all);
+  return all != 0;
+}
+"""
+
+
+def test_what_a_cta_has_stored_becomes_nan(tmp_path):
+    """The kernel's own function, compiled for the host: every element of the CTA's part and no other."""
+    code = (CSRC / "delta_tc.cuh").read_text()
+    begin = code.index("template <int D, bool OUT>\n__device__ __forceinline__ void delta_lost(")
+    function = code[begin:code.index("\n}\n", begin) + 3]
+    function, n = re.subn(r"asm volatile\([^;]*;\"[^;]*;", "cta = g_cta;", function)
+    assert n == 1
+    src = tmp_path / "lost.cpp"
+    src.write_text(_HOST.replace("FUNCTION", function))
+    exe = tmp_path / "lost"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
