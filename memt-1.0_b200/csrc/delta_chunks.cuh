@@ -90,7 +90,9 @@ __global__ void __launch_bounds__(128, D == 256 ? 3 : 6) delta_chunks_kernel(con
   const int len = eos - bos < kTile ? static_cast<int>(eos - bos) : kTile;
 
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Cfg::kOffG + 3 * kTile * 4);
+  uint32_t* late = reinterpret_cast<uint32_t*>(bar + 1);  // some thread has waited too long for the tiles
   if (tid == 0) {
+    *late = 0;
     mbar_init(smem_u32(bar), 1);
     mbar_fence_init();
     mbar_expect_tx(smem_u32(bar), 2 * Cfg::kBytesK);
@@ -129,11 +131,7 @@ __global__ void __launch_bounds__(128, D == 256 ? 3 : 6) delta_chunks_kernel(con
     }
   }
   __syncthreads();
-  if (!mbar_wait_clock(smem_u32(bar), 0)) {  // half a second without its tiles: the chain will read what it may
-    if (tid == 0) atomicOr(&g_delta_status, 1);
-    __syncthreads();
-    return;
-  }
+  if (!mbar_wait_clock(smem_u32(bar), 0)) *late = 1;  // half a second: goes on with what is there, up to the stores
   if (len < kTile) {  // rows of K behind the sample: zero (those of Q make rows of B that nothing reads)
     const int pieces = (kTile - len) * 8;
     for (int i = tid; i < D / 64 * pieces; i += 128)
@@ -332,6 +330,18 @@ __global__ void __launch_bounds__(128, D == 256 ? 3 : 6) delta_chunks_kernel(con
     put(A + (32 + m) * RL + n16 + 8, y[1], -1.f);
   }
   __syncthreads();
+  if (*late != 0) {
+    // T as NaN: every correction of the chunk and with them all columns of the state become NaN, which the chain makes again
+    // token by token, without T and B (in a first pass over segments the state stays NaN). The tiles land before
+    // shared memory is released.
+    const uint4 nan = make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);
+    for (int i = tid; i < 2 * DeltaChunks::kTerm / 16; i += Cfg::kThreads) reinterpret_cast<uint4*>(out)[i] = nan;
+    if (tid == 0) {
+      atomicOr(&g_delta_status, 1);
+      mbar_wait_clock(smem_u32(bar), 0);
+    }
+    return;
+  }
   // two bf16 terms, eight columns at a time: warp m the rows 16 m on, up to column 16 m + 15
 #pragma unroll 1
   for (int i = 0; i <= iw; ++i) {

@@ -36,9 +36,10 @@
 // never leaves the state, so a CTA looks at its final state; a warp's columns of which one is not finite are made
 // again token by token (DeltaAgain) from the initial state, outputs too (2 us a token).
 // Every wait for an mbarrier is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, the
-// control warps drain what they have in flight, and all that the CTA has stored becomes NaN (delta_lost). Named barriers have no bound of their own: the MMA warp comes to all of
-// them, whatever it has given up, and so does each warp of the chain, once a phase: its waits keep it from arriving
-// twice, and where one of them has run out it joins the barrier instead of passing it (hand_over).
+// control warps drain what they have in flight, and all that the CTA has stored becomes NaN (delta_lost). Named barriers
+// have no bound of their own: the MMA warp comes to all of them, whatever it has given up, and so does each warp of the
+// chain, once a phase: its waits keep it from arriving twice, and where one of them has run out it joins the barrier
+// instead of passing it (hand_over).
 #pragma once
 
 #include "delta_chunks.cuh"

@@ -247,3 +247,34 @@ def test_what_a_cta_has_stored_becomes_nan(tmp_path):
     subprocess.run(["g++", "-O2", "-std=c++17", "-o", str(exe), str(src)], check=True)
     r = subprocess.run([str(exe)], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout
+
+
+def test_a_chunk_whose_tiles_were_late_is_nan_for_the_chain():
+    """The operands' kernel: all of its threads learn of it behind a barrier, T becomes NaN in both terms, and the tiles are
+    waited for once more before the block ends."""
+    code = re.sub(r"\s+", " ", _code("delta_chunks.cuh"))
+    kernel = code[code.index("delta_chunks_kernel("):]
+    wait = kernel.index("if (!mbar_wait_clock(smem_u32(bar), 0)) *late = 1;")
+    branch = kernel.index("if (*late != 0) {")
+    assert kernel.index("*late = 0;") < kernel.index("__syncthreads();") < wait
+    between = kernel[wait:branch]
+    assert "return;" not in between and "__syncthreads();" in between
+    assert kernel.index("split2(f32x2_pack(lo4.x") > branch  # T is stored behind it
+    body = kernel[branch:kernel.index("return; }", branch)]
+    assert "0x7fff7fff" in body and "i < 2 * DeltaChunks::kTerm / 16; i += Cfg::kThreads" in body
+    assert "atomicOr(&g_delta_status, 1); mbar_wait_clock(smem_u32(bar), 0);" in body
+
+
+def test_a_nan_in_t_reaches_every_column_and_both_passes():
+    """In 64 bits, the zeros of T included: one chunk's T as NaN leaves no finite value in the state, whatever its tokens,
+    their gates and the states before are."""
+    import torch
+
+    gen = torch.Generator().manual_seed(1)
+    for beta, decay, before in ((0.5, 0.9, 1.0), (0.0, 0.0, 0.0), (1.0, 1.0, 0.0)):
+        k, v = torch.randn(64, 16, generator=gen).double(), torch.randn(64, 16, generator=gen).double()
+        S = before * torch.randn(16, 16, generator=gen).double()
+        T = torch.tril(torch.full((64, 64), float("nan"), dtype=torch.float64))  # stored up to the diagonal's blocks
+        r = beta * (v - decay * (k @ S))
+        u = T @ r
+        assert not bool(torch.isfinite(decay * S + k.T @ (0.5 * u)).any())
