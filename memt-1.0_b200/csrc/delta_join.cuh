@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(D) delta_join_kernel(const DeltaParams p) {
   if (p.h0 != nullptr && in_slot >= 0) read(p.h0 + (in_slot * p.H + h) * D * D + at, S);
   read(p.seg_states + ((int64_t)first * p.H + h) * D * D + at, H);
   bool alive = true;
-  int i = 0;
+  int i = 0, issued = pieces < Cfg::kStages ? pieces : Cfg::kStages;
   __syncthreads();
   for (int s = 0; s < count; ++s) {
     write(p.seg_states + ((int64_t)(first + s) * p.H + h) * D * D + at, D, S);
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(D) delta_join_kernel(const DeltaParams p) {
     if (s + 2 < count) read(p.seg_states + ((int64_t)(first + s + 1) * p.H + h) * D * D + at, H);
     for (int piece = 0; piece < kPieces; ++piece, ++i) {
       const int stage = i % Cfg::kStages;
-      if (!mbar_wait_clock(bars + 8 * stage, (i / Cfg::kStages) & 1)) alive = false;
+      if (alive) alive = mbar_wait_clock(bars + 8 * stage, (i / Cfg::kStages) & 1);
       const float* M = reinterpret_cast<const float*>(sm_join + stage * Cfg::kPiece) + r;
       const float* x = shared + piece * Cfg::kRows * C + col;
 #pragma unroll 8
@@ -109,14 +109,22 @@ __global__ void __launch_bounds__(D) delta_join_kernel(const DeltaParams p) {
         }
       }
       __syncthreads();
-      if (tid == 0 && i + Cfg::kStages < pieces) load(i + Cfg::kStages);
+      if (tid == 0 && alive && i + Cfg::kStages < pieces) {
+        load(i + Cfg::kStages);
+        issued = i + Cfg::kStages + 1;
+      }
     }
-    if (!alive) {  // a wait that ran out (each later piece is still waited for): the caller sees it in the state
+    if (!alive) {  // a wait that ran out: nothing more is waited for or loaded, and the caller sees it in the state
 #pragma unroll
       for (int e = 0; e < 8; ++e) S[e >> 2][e & 3] = f32x2_splat(__int_as_float(0x7fffffff));
     }
   }
-  if (!alive) atomicOr(&g_delta_status, 1);
+  if (!alive) {
+    atomicOr(&g_delta_status, 1);
+    if (tid == 0)  // what has been loaded lands before shared memory is released
+      for (int j = issued > Cfg::kStages ? issued - Cfg::kStages : 0; j < issued; ++j)
+        mbar_wait_clock(bars + 8 * (j % Cfg::kStages), (j / Cfg::kStages) & 1);
+  }
 }
 
 }  // namespace memt

@@ -278,3 +278,27 @@ def test_a_nan_in_t_reaches_every_column_and_both_passes():
         r = beta * (v - decay * (k @ S))
         u = T @ r
         assert not bool(torch.isfinite(decay * S + k.T @ (0.5 * u)).any())
+
+
+@pytest.mark.parametrize("pieces", [1, 4, 5, 64, 992])
+@pytest.mark.parametrize("lost", [0, 3, 63])
+def test_the_join_waits_a_few_times_at_most(pieces, lost):
+    """Between the passes over segments: a piece that never lands ends the waiting for later ones and their loads; what
+    has been loaded is waited for once more. Waits of half a second each, in the order of the kernel's code."""
+    code = re.sub(r"\s+", " ", _code("delta_join.cuh"))
+    assert "if (alive) alive = mbar_wait_clock(bars + 8 * stage, (i / Cfg::kStages) & 1);" in code
+    assert "if (tid == 0 && alive && i + Cfg::kStages < pieces) {" in code
+    assert code.count("mbar_wait_clock(") == 2 and "j = issued > Cfg::kStages ? issued - Cfg::kStages : 0; j < issued" in code
+    stages = int(re.search(r"kStages = (\d+)", code).group(1))
+    alive, issued, ran_out = True, min(stages, pieces), 0
+    landed = lambda i: i < lost  # noqa: E731  (in order, one after another, up to the lost one)
+    for i in range(pieces):
+        if alive and not landed(i):
+            alive, ran_out = False, ran_out + 1
+        if alive and i + stages < pieces:
+            issued = i + stages + 1
+    if not alive:
+        waited = list(range(max(issued - stages, 0), issued))
+        assert set(waited) >= {i for i in range(issued) if not landed(i)}  # nothing in flight is left out
+        ran_out += sum(not landed(j) for j in waited)
+    assert alive == (lost >= pieces) and ran_out <= 1 + stages
