@@ -128,28 +128,19 @@ __device__ __forceinline__ int sample_by_length(const LinearParams& p, int rank)
   return found;
 }
 
-// The unit-th sample of more than p.few tokens, found by a converged warp; -1 when there are fewer. Lengths of 128
-// samples are read at once: a CTA that finds none has waited for little else.
+// The unit-th sample of more than p.few tokens, found by a converged warp; -1 when there are fewer.
 __device__ __forceinline__ int find_long(const LinearParams& p, int unit) {
   const int lane = threadIdx.x & 31;
   int before = 0;
-  for (int n0 = 0; n0 < p.N; n0 += 128) {
-    bool longer[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      int64_t bos = 0, eos = 0;
-      const int n = n0 + 32 * e + lane;
-      if (n < p.N) sample_range(p, n, bos, eos);
-      longer[e] = n < p.N && eos - bos > p.few;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t all = __ballot_sync(~0u, longer[e]);
-      const int rank = before + __popc(all & ((1u << lane) - 1));
-      const uint32_t hit = __ballot_sync(~0u, rank == unit && longer[e]);
-      if (hit != 0) return n0 + 32 * e + __ffs(hit) - 1;
-      before += __popc(all);
-    }
+  for (int n0 = 0; n0 < p.N; n0 += 32) {
+    int64_t bos = 0, eos = 0;
+    const bool own = n0 + lane < p.N;
+    if (own) sample_range(p, n0 + lane, bos, eos);
+    const uint32_t longer = __ballot_sync(~0u, own && eos - bos > p.few);
+    const int rank = before + __popc(longer & ((1u << lane) - 1));
+    const uint32_t hit = __ballot_sync(~0u, rank == unit && (longer >> lane & 1));
+    if (hit != 0) return n0 + __ffs(hit) - 1;
+    before += __popc(longer);
   }
   return -1;
 }
