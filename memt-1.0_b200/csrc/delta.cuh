@@ -250,8 +250,9 @@ struct DeltaColumns {
         }
     }
     float out = fmaf(kq, d_own, aw);
-    // A correction that is not finite makes rows of either sign, which k.q would not show: the new state's sum.
-    if (__any_sync(~0u, !isfinite(d_own))) {
+    // What is not finite in the correction or the query makes terms of either sign, which k.q and S^T q would not show: the
+    // new state's sum.
+    if (__any_sync(~0u, !isfinite(out))) {
       uint64_t n2[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int m = 0; m < kRows / 4; ++m) {

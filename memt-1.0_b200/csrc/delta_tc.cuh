@@ -34,7 +34,9 @@
 //
 // Values that are not finite: the zeros of T and B meet them in tokens they must not reach. Whatever spoils a token
 // never leaves the state, so a CTA looks at its final state; a warp's columns of which one is not finite are made
-// again token by token (DeltaAgain) from the initial state, outputs too (2 us a token).
+// again token by token (DeltaAgain) from the initial state, outputs too (2 us a token). A query never enters the state: of
+// columns whose state is finite and some output is not, those outputs alone are made again (an infinite query's scores
+// differ in sign, and their second terms are differences of infinities), unless a NaN in the query settles them.
 // Every wait for an mbarrier is bounded as in linear_tc.cuh: a thread whose wait runs out flags it and stops waiting, the
 // control warps drain what they have in flight, and all that the CTA has stored becomes NaN (delta_lost). Named barriers
 // have no bound of their own: the MMA warp comes to all of them, whatever it has given up, and so does each warp of the
@@ -98,6 +100,7 @@ struct DeltaTcCfg {
 // pairs are of the chain's first and second half.
 enum DeltaBarrier {
   kBarEnd = 1,  // the chain's and the outputs' warps, once
+  kBarAgain = 8,  // the chain's, around columns that are made again
   kBarS = 2,    // the state's terms written: chain -> MMA
   kBarR = 4,    // R^T written: chain -> MMA
   kBarW = 6     // (w U)^T and U^T written: chain -> MMA
@@ -117,14 +120,21 @@ __device__ __forceinline__ float exp2_pair(float h, float l) {
   return fmaf(x, l * 0.69314718f, x);
 }
 
-// The warp's columns from `col` of one state, again, token by token from `start` (null: zeros) and with the outputs.
-// Once every value of the state is NaN, so is everything behind.
+// NaN in `seen` (zeros before) once a pair of bf16 numbers is not finite
+__device__ __forceinline__ uint32_t not_finite(uint32_t pair, uint32_t seen) {
+  uint32_t x;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(x) : "r"(pair), "r"(0u), "r"(seen));
+  return x;
+}
+
+// The warp's columns from `col` of one state, again, token by token from `start` (null: zeros) and with the outputs, or
+// with `odd` those of them that are not finite. Once every value of the state is NaN, so is everything behind.
 // (At D = 64 and 128 with what the next token needs in registers, too, the chain itself comes out slower.)
 template <int D>
 using DeltaAgain = DeltaColumns<D, D == 64 ? 4 : 2>;
 template <int D>
 __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h, int col, int64_t bos, int64_t eos,
-                                                 const float* start, float* end) {
+                                                    const float* start, float* end, bool odd) {
   using Cols = DeltaAgain<D>;
   using T = __nv_bfloat16;
   constexpr bool kAhead = D == 256;
@@ -185,10 +195,31 @@ __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h,
         for (int c = 0; c < 4; ++c) nan = nan && isnan(f32x2_lo(cols.S[i][c])) && isnan(f32x2_hi(cols.S[i][c]));
       lost = __all_sync(~0u, nan);
     }
-    if (Cols::writes())
-      store_f32(static_cast<T*>(p.out), t * p.so + (int64_t)h * D + col + Cols::col0() + Cols::own_col(), p.scale * out);
+    if (Cols::writes()) {
+      T* at = static_cast<T*>(p.out) + t * p.so + (int64_t)h * D + col + Cols::col0() + Cols::own_col();
+      if (!odd || !isfinite(as_f32(*at))) store_f32(at, 0, p.scale * out);
+    }
   }
   if (end != nullptr) cols.store(end + col);
+}
+
+// The end of the last token of the chunks odd[0] .. odd[1] whose output, in the CTA's columns from `col`, is not finite
+// although no NaN in its query makes it so, to odd[2]. By the chain's 16 warps.
+template <int D>
+__device__ __forceinline__ void odd_tokens(const DeltaParams& p, int h, int col, int64_t bos, int64_t eos, int32_t* odd,
+                                           int warp) {
+  constexpr int VB = DeltaTcCfg<D>::kVB;
+  const int lane = threadIdx.x & 31;
+  const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + (int64_t)(h / (p.H / p.Hk)) * D;
+  const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(p.out) + (int64_t)h * D + col;
+  const int64_t end = bos + (int64_t)(odd[1] + 1) * kTile;
+  for (int64_t t = bos + (int64_t)odd[0] * kTile + warp; t < end && t < eos; t += 16) {
+    bool nan = false, is_odd = false;
+    for (int i = lane; i < D; i += 32) nan = nan || isnan(as_f32(q[t * p.sq + i]));
+    for (int i = lane; i < VB; i += 32) is_odd = is_odd || !isfinite(as_f32(o[t * p.so + i]));
+    const bool some = __any_sync(~0u, is_odd);
+    if (!__any_sync(~0u, nan) && some && lane == 0) atomicMax(odd + 2, static_cast<int>(t) + 1);
+  }
 }
 
 // All that a CTA has stored becomes NaN: a wait of it ran out, in whichever role, and nothing of it can be relied on.
@@ -262,12 +293,19 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
   // (UD) and P (PD) and O (OD) ready; outputs read (OE); drained (DR)
   constexpr int LF = 0, LE = LF + NS, TF = LE + NS, TE = TF + NT, XD = TE + NT, UD = XD + 2, PD = UD + 2, OD = PD + 2,
                 OE = OD + 1, DR = OE + 1, NBAR = DR + 1;
-  static_assert(NBAR * 8 + 40 <= 512, "barrier area");
+  static_assert(NBAR * 8 + 48 <= 512, "barrier area");
   uint64_t* bar = reinterpret_cast<uint64_t*>(sm + Cfg::kOffBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Cfg::kOffBar + NBAR * 8);
-  uint32_t* spoiled = tmem_slot + 1;  // bit c: some value of the CTA's c-th group of columns (DeltaAgain) is not finite
+  // bit c: some value of the CTA's c-th group of columns (DeltaAgain) is not finite; kGivenUp: so have some of the chain's
+  // or the outputs' warps
+  uint32_t* spoiled = tmem_slot + 1;
+  constexpr uint32_t kGivenUp = 1u << 31;
   uint32_t* stalled = tmem_slot + 2;  // a wait ran out
   int32_t* whose = reinterpret_cast<int32_t*>(tmem_slot + 3);  // sample, first and last token, whether the sample ends here
+  // groups with outputs that are not finite, the first and the last chunk of them, and the end of the last token that is
+  // made again for them
+  uint32_t* odd_groups = tmem_slot + 7;
+  int32_t* odd = reinterpret_cast<int32_t*>(tmem_slot + 8);
   const uint32_t base = smem_u32(sm), bars = smem_u32(bar);
   auto B = [&](int i) { return bars + 8 * i; };
   if (tid == 0) {
@@ -284,6 +322,9 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     whose[1] = static_cast<int>(bos);
     whose[2] = static_cast<int>(eos);
     whose[3] = seg + 1 == segs;
+    *odd_groups = 0;
+    odd[0] = INT32_MAX;
+    odd[1] = odd[2] = -1;
   }
   if (warp == 0) tc::alloc(smem_u32(tmem_slot), 512);
   tc::fence_before();
@@ -532,6 +573,11 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
     const int prow = 8 * (lane >> 4) + (lane & 7), pval = (lane >> 3) & 1;  // row of an stmatrix piece
     const int col = h * D + vblk * Cfg::kVB + 32 * quad % Cfg::kVB;
     constexpr int kPieces = D >= 128 ? 2 : 1;  // of 32 tokens
+    auto is_odd = [&](int value, int c) {  // of the warp's 32
+      atomicOr(odd_groups, 1u << ((32 * quad + value) % Cfg::kVB / DeltaAgain<D>::kCols));
+      atomicMin(odd, c);
+      atomicMax(odd + 1, c);
+    };
     for (int c = 0; OUT && c < nchunks; ++c) {
       const DeltaTable& t = tab[c % NT];
       const int len = chunk_len(c);
@@ -556,6 +602,7 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
             tc::fence_before();
             arrive(OE);
           }
+          uint32_t seen[2] = {0, 0};
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
             uint32_t z[4];  // tokens 8 (i + j) + pair, + 1: of value lane / 4, of value lane / 4 + 8
@@ -568,10 +615,16 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
                 const int k = 4 * (i + j) + 2 * v8;
                 z[2 * j + v8] = f32x2_to_bf16x2(fma_f32x2(ff, (static_cast<uint64_t>(x[k + 1]) << 32) | x[k],
                                                           (static_cast<uint64_t>(y[k + 1]) << 32) | y[k]));
+                seen[v8] = not_finite(z[2 * j + v8], seen[v8]);
               }
             }
             const int tok = 8 * i + prow;
             stsm_x4_t(turn + tok * 64 + (((2 * e + pval) ^ ((tok >> 1) & 3)) << 4), z[0], z[1], z[2], z[3]);
+          }
+          if (len == kTile) {
+#pragma unroll
+            for (int v8 = 0; v8 < 2; ++v8)
+              if (seen[v8] != 0) is_odd(16 * e + 8 * v8, c);
           }
         }
         const int64_t tok0 = bos + (int64_t)c * kTile + t0;
@@ -591,12 +644,14 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
                          : "=r"(z.x), "=r"(z.y), "=r"(z.z), "=r"(z.w)
                          : "r"(turn + tok * 64 + (((lane & 3) ^ ((tok >> 1) & 3)) << 4)) : "memory");
             *reinterpret_cast<uint4*>(o + tok * p.so) = z;
+            if (not_finite(z.x, not_finite(z.y, not_finite(z.z, not_finite(z.w, 0)))) != 0) is_odd(8 * (lane & 3), c);
           }
         }
       }
       arrive(TE + c % NT);
     }
     if (lane == 0) bulk_wait_all();
+    if (!alive) atomicOr(spoiled, kGivenUp);
     __syncwarp();
     bar_sync<640>(kBarEnd);
   } else {
@@ -761,12 +816,34 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
 #pragma unroll
     for (int i = 0; i < KT / 2; ++i) seen = fma_f32x2(S[i], 0, seen);
     if (f32x2_lo(seen) != 0.f || f32x2_hi(seen) != 0.f) atomicOr(spoiled, 1u << (vr / kGroup));
+    if (!alive) atomicOr(spoiled, kGivenUp);
     bar_sync<640>(kBarEnd);  // with the outputs' warps, once theirs have left
     float* end = out_slot >= 0 && !taken ? p.ht + (out_slot * p.H + h) * head : nullptr;
     if (OUT && seg + 1 < segs) end = nullptr;
     if (!OUT) end = (moves ? p.seg_moves : p.seg_states) + seg_state;
     // (what a segment that is not finite hands on is not made again: a column of it is spoiled as it is)
-    const uint32_t again = !OUT ? 0 : tokenwise ? ~0u : *spoiled;
+    const uint32_t again = !OUT ? 0 : tokenwise ? ~kGivenUp : *spoiled & ~kGivenUp;
+    if constexpr (OUT) {
+      const uint32_t rows = *odd_groups & ~again;
+      if ((again | rows) != 0 && !(*spoiled & kGivenUp)) {
+        // the states wait in shared memory, which no tile needs any more
+        uint64_t* keep = reinterpret_cast<uint64_t*>(sm) + tid - 256;
+        static_assert(512 * KT * 4 <= NS * Cfg::kBytesKQ, "room for the states");
+#pragma unroll
+        for (int i = 0; i < KT / 2; ++i) keep[512 * i] = S[i];
+        if (rows != 0) odd_tokens<D>(p, h, vblk * Cfg::kVB, whose[1], whose[2], odd, warp - 8);
+        bar_sync<512>(kBarAgain);
+        for (int g = warp - 8; g < Cfg::kVB / kGroup; g += 16) {
+          const bool whole = again >> g & 1;
+          if (whole || (rows >> g & 1))
+            delta_columns_again<D>(p, h, vblk * Cfg::kVB + g * kGroup, whose[1], whole ? whose[2] : odd[2],
+                                   first_state(sample), whole ? end : nullptr, !whole);
+        }
+        bar_sync<512>(kBarAgain);
+#pragma unroll
+        for (int i = 0; i < KT / 2; ++i) S[i] = keep[512 * i];
+      }
+    }
     if (writes && end != nullptr && !(again >> (vr / kGroup) & 1)) {
       if (moves) {  // [value column][key], as the join reads it
         ulonglong2* dst = reinterpret_cast<ulonglong2*>(end + (int64_t)(vblk * Cfg::kVB + vr) * D + KT * part);
@@ -780,11 +857,6 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
           dst[(i + 1) * D] = f32x2_hi(S[i / 2]);
         }
       }
-    }
-    if (OUT && again != 0 && alive) {
-      for (int g = warp - 8; g < Cfg::kVB / kGroup; g += 16)
-        if (again >> g & 1)
-          delta_columns_again<D>(p, h, vblk * Cfg::kVB + g * kGroup, whose[1], whose[2], first_state(sample), end);
     }
   }
   if (!alive) {
