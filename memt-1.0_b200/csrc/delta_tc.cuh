@@ -187,7 +187,8 @@ __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h,
       auto k = [&](int m) { return four(kAhead ? k1[kAhead ? m : 0] : raw(kt(t), m)); };
       auto q = [&](int m) { return four(kAhead ? q1[kAhead ? m : 0] : raw(qt(t), m)); };
       auto v = [&](int c) { return kAhead ? v1 : as_f32(vt(t)[c]); };  // (c is this lane's own column)
-      out = cols.template step<true>(k, q, v, a, p.g_layout == 1 ? 0.f : fixed_lo, beta);
+      // (a low half of zero would make NaN of an infinite state)
+      out = cols.template step<true>(k, q, v, a, p.g_layout == 1 ? low_half(a, 0.f) : fixed_lo, beta);
       bool nan = true;
 #pragma unroll
       for (int i = 0; i < Cols::kRows / 2; ++i)

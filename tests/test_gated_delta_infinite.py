@@ -118,3 +118,27 @@ def test_rows_of_the_next_sample_are_not_looked_at(cuda):
     bad[0][100:128] = float("inf")
     o2, f2 = M.gated_delta(*bad)
     assert torch.equal(f2, final) and torch.equal(o2[:100], o[:100]) and torch.equal(o2[128:], o[128:])
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("decay", ["none", "head", "token"])
+@pytest.mark.parametrize("first", [[150], [3]])
+def test_an_infinite_state(cuda, D, dtype, decay, first):
+    """One infinite element of the state that a sample of one token starts from: the correction is infinite, the other
+    rows become infinities and its own NaN, whichever form the sample goes in."""
+    H, r, c = 2, 9, 21
+    x = _inputs(55, first + [1], 1, H, D, dtype, decay=decay)
+    x[5][1, 1, r, c] = float("inf")
+    o, final = M.gated_delta(*x)
+    q, k, v, g, b, h0, cu = x
+    clean = h0.clone()
+    clean[1, 1, r, c] = 0.0
+    o2, f2 = M.gated_delta(q, k, v, g, b, clean, cu)
+    ref_o, ref, _, _ = _recurrence(*x, D ** -0.5)
+    assert int(torch.isinf(ref[1, 1, :, c]).sum()) == D - 1
+    assert torch.equal(_kinds(final), _kinds(ref)) and torch.equal(_kinds(o), _kinds(ref_o))
+    cols = torch.arange(D, device="cuda") // 16 != c // 16
+    assert torch.equal(final[1, 0], f2[1, 0]) and torch.equal(final[1, 1][:, cols], f2[1, 1][:, cols])
+    assert torch.equal(final[0], f2[0]) and torch.equal(o[:-1], o2[:-1])
