@@ -152,7 +152,15 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
     if constexpr (Cfg::kRowsPerWarp == 2) kq += __shfl_xor_sync(0xffffffffu, kq, 16);
     if (lane == 0) s_kq[warp] = kq;
   }
-  __syncthreads();
+  bool any_odd = false;  // some value of this CTA's is not finite, where its output would show it
+  if (DELTA && p.gated) {
+    float seen = kq + beta;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) seen = fmaf(0.f, o[e] + r[e], fmaf(0.f, v[e], seen));
+    any_odd = __syncthreads_or(!isfinite(seen));
+  } else {
+    __syncthreads();
+  }
   if constexpr (DELTA) {
     float d[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
@@ -173,6 +181,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
       __stcs(st + i * kStep, make_float4(fmaf(k, d[0], S[i].x), fmaf(k, d[1], S[i].y), fmaf(k, d[2], S[i].z),
                                   fmaf(k, d[3], S[i].w)));
     }
+    bool odd[4] = {};  // outputs that are not finite
     if (group == 0) {
       // o = S~^T q + (k'.q) d for the new state; the incoming one does not know d, which may not be finite
       float all = 0.f;
@@ -188,8 +197,32 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads) step_kernel(const StepPa
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < G; ++j) sum += s_o[j][col + e];
-        store_f32(static_cast<T*>(p.out), (int64_t)n * p.so + (int64_t)h * D + blk * C + col + e,
-                  p.scale * fmaf(all, d[e], sum));
+        const float out = fmaf(all, d[e], sum);
+        odd[e] = !isfinite(out);
+        store_f32(static_cast<T*>(p.out), (int64_t)n * p.so + (int64_t)h * D + blk * C + col + e, p.scale * out);
+      }
+    }
+    // A correction or a query that is not finite makes terms of either sign, which k.q and S~^T q do not show: the
+    // new state's sum.
+    if (any_odd) {
+      __syncthreads();
+      float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const float k = s_k[i * G + group], q = s_q[i * G + group];
+        const float x[4] = {S[i].x, S[i].y, S[i].z, S[i].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(q, fmaf(k, d[e], x[e]), y[e]);
+      }
+      *reinterpret_cast<float4*>(&s_o[group][col]) = make_float4(y[0], y[1], y[2], y[3]);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (!odd[e]) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < G; ++j) sum += s_o[j][col + e];
+        store_f32(static_cast<T*>(p.out), (int64_t)n * p.so + (int64_t)h * D + blk * C + col + e, p.scale * sum);
       }
     }
   } else {

@@ -142,3 +142,37 @@ def test_an_infinite_state(cuda, D, dtype, decay, first):
     cols = torch.arange(D, device="cuda") // 16 != c // 16
     assert torch.equal(final[1, 0], f2[1, 0]) and torch.equal(final[1, 1][:, cols], f2[1, 1][:, cols])
     assert torch.equal(final[0], f2[0]) and torch.equal(o[:-1], o2[:-1])
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("what,place", [("v", 1), ("v", -1), ("q", 1), ("q", -1), ("k", 1), ("state", 1), ("q", float("nan"))])
+def test_the_step(cuda, D, dtype, what, place):
+    """One session's output and state are the definition's, the other sessions keep their bits."""
+    N, H, c = 3, 2, 11
+    x = _inputs(56, [1] * N, 1, H, D, dtype)
+    clean = x[5].clone()
+    o = M.gated_delta_step(*x[:5], clean)
+    bad = [y.clone() if y is not None else None for y in x]
+    inf = place * float("inf")
+    if what == "v":
+        bad[2][1, 1, c] = inf
+    elif what == "state":
+        bad[5][1, 1, 9, c] = inf
+    else:
+        bad["qk".index(what)][1, 0, 9] = inf
+    states = bad[5].clone()
+    o2 = M.gated_delta_step(*bad[:5], states)
+    ref_o, ref, _, _ = _recurrence(*bad, D ** -0.5)
+    assert not bool(torch.isfinite(ref_o[1, 1, c])) and torch.equal(_kinds(states), _kinds(ref))
+    sure = torch.ones(N, H, D, dtype=torch.bool, device="cuda")
+    if what == "q":
+        sure[1] = ref[1, :, 9].abs() > 1e-3
+        assert float(sure[1].double().mean()) > 0.9
+    assert torch.equal(_kinds(o2)[sure], _kinds(ref_o)[sure])
+    keep = torch.isfinite(ref_o)
+    assert torch.equal(o2[keep], o[keep]) and torch.equal(states[torch.isfinite(ref)], clean[torch.isfinite(ref)])
+    # the same token as a prompt
+    o3, f3 = M.gated_delta(*bad)
+    assert torch.equal(_kinds(o3)[sure], _kinds(o2)[sure]) and torch.equal(_kinds(f3), _kinds(states))
