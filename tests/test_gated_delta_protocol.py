@@ -258,3 +258,17 @@ def test_a_wait_left_out_is_seen(name, role):
         with pytest.raises(AssertionError):
             for seed in range(40):
                 _run(3, 9, seed, edit, alias)
+
+
+@pytest.mark.parametrize("name,role", [("XD", "chain"), ("UD", "chain"), ("barW", "mma"), ("LF", "chain"),
+                                       ("TF", "chain")])
+def test_any_wait_left_out_is_seen(name, role):
+    """The waits that order X -> R, U -> w U and w U -> P, and those for tiles and tables."""
+    def edit(bars, roles):
+        for r in [r for r in roles if r.startswith(role)]:
+            roles[r] = (op for op in list(roles[r]) if not (op[0] in ("wait", "sync") and op[1][0] == name))
+
+    for alias in (False, True):
+        with pytest.raises(AssertionError):
+            for seed in range(40):
+                _run(3, 9, seed, edit, alias)
