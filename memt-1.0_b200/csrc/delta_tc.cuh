@@ -209,17 +209,30 @@ __device__ __forceinline__ void delta_columns_again(const DeltaParams& p, int h,
 template <int D>
 __device__ __forceinline__ void odd_tokens(const DeltaParams& p, int h, int col, int64_t bos, int64_t eos, int32_t* odd,
                                            int warp) {
-  constexpr int VB = DeltaTcCfg<D>::kVB;
+  constexpr int VB = DeltaTcCfg<D>::kVB, W = VB / 64, AT = 4;  // words of a lane, tokens at once
   const int lane = threadIdx.x & 31;
   const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(p.q) + (int64_t)(h / (p.H / p.Hk)) * D;
   const __nv_bfloat16* o = static_cast<const __nv_bfloat16*>(p.out) + (int64_t)h * D + col;
-  const int64_t end = bos + (int64_t)(odd[1] + 1) * kTile;
-  for (int64_t t = bos + (int64_t)odd[0] * kTile + warp; t < end && t < eos; t += 16) {
-    bool nan = false, is_odd = false;
-    for (int i = lane; i < D; i += 32) nan = nan || isnan(as_f32(q[t * p.sq + i]));
-    for (int i = lane; i < VB; i += 32) is_odd = is_odd || !isfinite(as_f32(o[t * p.so + i]));
-    const bool some = __any_sync(~0u, is_odd);
-    if (!__any_sync(~0u, nan) && some && lane == 0) atomicMax(odd + 2, static_cast<int>(t) + 1);
+  int64_t end = bos + (int64_t)(odd[1] + 1) * kTile;
+  if (end > eos) end = eos;
+  for (int64_t t0 = bos + (int64_t)odd[0] * kTile + AT * warp; t0 < end; t0 += 16 * AT) {
+    uint32_t x[AT][W] = {};
+#pragma unroll
+    for (int j = 0; j < AT; ++j)
+      if (t0 + j < end) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) x[j][i] = reinterpret_cast<const uint32_t*>(o + (t0 + j) * p.so)[lane + 32 * i];
+      }
+#pragma unroll
+    for (int j = 0; j < AT; ++j) {
+      uint32_t seen = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) seen = not_finite(x[j][i], seen);
+      if (!__any_sync(~0u, seen != 0)) continue;
+      bool nan = false;
+      for (int i = lane; i < D; i += 32) nan = nan || isnan(as_f32(q[(t0 + j) * p.sq + i]));
+      if (!__any_sync(~0u, nan) && lane == 0) atomicMax(odd + 2, static_cast<int>(t0) + j + 1);
+    }
   }
 }
 
