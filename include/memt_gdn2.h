@@ -457,8 +457,9 @@ int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
  * in the mean, samples of at most 40 / 20 / 14 tokens (D = 64 / 128 / 256) go token by token; few long samples are
  * split into segments. So results may differ within these roundings with what a sample is packed with.
  * A token that is not finite changes nothing before it. A column of a bf16 state that is not finite at the end is
- * made again token by token, its outputs too (2 us a token), and so are, by themselves, outputs that only their query makes
- * infinite: they have the definition's infinities and NaN.
+ * made again token by token, its outputs too (2 us a token), and with it its aligned group of 16 columns (D = 128 and 256:
+ * 8), whose roundings are then that form's. So are, by themselves, outputs that only their query makes infinite: they
+ * have the definition's infinities and NaN.
  */
 typedef struct memt_gated_delta_args {
   uint32_t struct_size;    /* sizeof(memt_gated_delta_args)                     */

@@ -49,7 +49,7 @@ constexpr int kPlanSms = 148;
 // (once for what they add to a zero state, once for what they make of an identity), a kernel joins them one after the other,
 // and a second pass over all makes the outputs. Measured at D = 64 / 128 / 256: a chunk of a whole sample takes
 // 1.9 / 2.4 / 5.5 us, 0.85 of it in a wave of the first pass, 1.25 in a full wave of the second; a segment's join
-// 2.1 / 3.7 / 8 and more; a start of a wave some 6. Samples of unequal length can make one segment more each.
+// 2.1 / 4 / 11 (the rule counts 8 for the last); a start of a wave some 6. Samples of unequal length can make one segment more each.
 // The rule counts samples, not tokens: short samples beside a long one can leave it whole.
 int plan_segment_chunks(int64_t N, int64_t L, int64_t H, int D) {
   const int64_t ctas = N * H * (D == 256 ? 2 : 1), chunks = (L + kTile - 1) / kTile / N;  // of a mean sample

@@ -5,8 +5,8 @@
 // (sample, head) state is shared out by value columns: a CTA has 16 of them and walks over the segments, in fp32, S in
 // shared memory, each H replaced in place by the state before its segment. All of M goes through every CTA: pieces
 // of it are copied ahead of the walk (they do not wait for S) and lie transposed, so that a thread with two rows and
-// eight columns of S reads pairs of rows beside its neighbours'. Measured: 2.1 / 3.7 / 10 us a segment at
-// D = 64 / 128 / 256, bound by the products (16 D^2 in a CTA); more threads that split the sum over keys were 20 to 60
+// eight columns of S reads pairs of rows beside its neighbours'. Measured: 2.1 / 4 / 11 us a segment at
+// D = 64 / 128 / 256 (2 heads, 16 and 10 segments), bound by the products (16 D^2 in a CTA); more threads that split the sum over keys were 20 to 60
 // percent faster for short segments and up to twice as slow behind long ones.
 #pragma once
 

@@ -30,6 +30,9 @@
 // half of R (T is lower triangular), P's sum over the first tokens only the first half of w U. V is fetched while P is
 // computed; S^T Q^T is issued behind U and O^T behind P. The MMA warp waits for the others at named barriers, which take
 // no issue slots. (Outputs made by the chain's warps beside X cost it a quarter more.)
+// At D = 256 a state thread has 64 keys in 96 registers and spills (1,354 bytes of stores, 1,472 of loads in the kernel, more
+// than half of them where columns are made again; D = 128: 96 and 244): 6.4 us a chunk, warps wait for tensor memory and for
+// what is spilled (4 x 2048 tokens, 16 heads: 205 us; tensor pipe 28 %).
 // At D = 64 the 64 values fill half of the 128 lanes; lanes 64-127 repeat them and store half of the output rows.
 //
 // Values that are not finite: the zeros of T and B meet them in tokens they must not reach. Whatever spoils a token
