@@ -498,7 +498,8 @@ int memt_gated_delta(const memt_gated_delta_args *args, void *workspace, size_t 
 
 /* As memt_linear_attention_status, of the bf16 calls of memt_gated_delta. What a thread block has stored is NaN where a
  * wait of it ran out: its sample's outputs (with segments, its segment's) and final state in up to 128 value columns of a
- * head, and all that starts from that state. */
+ * head, and all that starts from that state. Where it was the block that prepares a chunk, the sample's head is made
+ * again token by token (with segments: NaN behind the chunk's segment). */
 int memt_gated_delta_status(memt_stream_t stream, int32_t *status_out);
 
 /* ---- one token of a recurrence, states in place --------------------------

@@ -28,7 +28,7 @@
 // for S and P and of the tokens for R and U (warps 8-15 and 16-23), one half's threads working while the other
 // half's products are made: X's sum over the first keys needs the first half of S only, U's first tokens only the first
 // half of R (T is lower triangular), P's sum over the first tokens only the first half of w U. V is fetched while P is
-// computed; S^T Q^T is issued behind U and O^T behind P. The MMA warp waits for the others at named barriers, which take
+// computed; S^T Q^T is issued behind X and O^T behind P. The MMA warp waits for the others at named barriers, which take
 // no issue slots. (Outputs made by the chain's warps beside X cost it a quarter more.)
 // At D = 256 a state thread has 64 keys in 96 registers and spills (1,354 bytes of stores, 1,472 of loads in the kernel, more
 // than half of them where columns are made again; D = 128: 96 and 244): 6.4 us a chunk, warps wait for tensor memory and for
