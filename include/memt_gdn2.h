@@ -452,8 +452,8 @@ int memt_linear_attention_status(memt_stream_t stream, int32_t *status_out);
  *
  * dtype, rows, samples, states, pools and overlaps as in memt_linear_attention_args; beta is in q's dtype.
  * Keys are meant to be of unit length: beta |k|^2 above 2 lets a state grow.
- * fp32 goes token by token in fp32; bf16 in chunks of 64 tokens, with states exact to a few 1e-6 and scores, the
- * state that queries read and corrections rounded to bf16 for the outputs. In bf16 calls of up to 64 tokens a sample
+ * fp32 goes token by token in fp32; bf16 in chunks of 64 tokens, with states exact to a few 1e-6 and outputs
+ * that are rounded once. In bf16 calls of up to 64 tokens a sample
  * in the mean, samples of at most 40 / 20 / 14 tokens (D = 64 / 128 / 256) go token by token; few long samples are
  * split into segments. So results may differ within these roundings with what a sample is packed with.
  * A token that is not finite changes nothing before it. A column of a bf16 state that is not finite at the end is

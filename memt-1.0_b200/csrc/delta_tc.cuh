@@ -13,26 +13,25 @@
 //
 // Precision. The state is fp32 in registers. K and V are bf16 as given; every fp32 factor of a product that the state
 // depends on (S in S^T K^T, T, R, w U) is split into two bf16 terms, which leaves 2^-16 of each value at most and a few
-// 1e-6 of the state in all (one term would leave 1e-3). S^T Q^T reads the first term only, and
-// the U of O^T is bf16: what only the output sees is rounded like the output. (B has two terms: with one the outputs are
-// 2.9e-3 from the definition instead of 2.4e-3, where their own rounding is 1.7e-3. Two of U instead: the chain 9 to 16 %
-// slower.) Sums of log decays are formed in 64 bits; the decay of a
+// 1e-6 of the state in all (one term would leave 1e-3; a third of R and w U 0.3 to 1.7e-6, for 8 to 10 % of the time). S, U and
+// B are two terms for the outputs, too, which are then rounded once: 1.7e-3 from the definition, as the definition's own
+// are (with one term of S and U 2.4e-3, of B also 2.9e-3). Sums of log decays are formed in 64 bits; the decay of a
 // whole chunk is a pair of fp32 numbers where it is the same for every chunk.
 //
 // Roles (24 warps): warp 0 issues MMAs, warp 1 loads tiles, warps 2 and 3 make the decay tables of alternate chunks;
 // warps 4-7 make the outputs; warps 8-23 hold the state, a quarter of the keys each warpgroup, and walk the chain
 // X -> R -> U -> w U -> P -> S. What bounds a chunk is that chain: each of its three batches of MMAs has some 350
 // cycles from the first arrival to the threads that read the result, beside its own time and that of the threads
-// (8 x 8192 tokens, 16 heads, D = 128: 368 to 390 us in different runs, 3.0 us a chunk with 128 SMs at work and 2.4
-// with 16; tensor pipe 28 %, 1.4 TB/s). So it goes in two halves, of the keys
+// (8 x 8192 tokens, 16 heads, D = 128: 418 us in a run of its own, 3.3 us a chunk with 128 SMs at work; tensor pipe 34 %).
+// So it goes in two halves, of the keys
 // for S and P and of the tokens for R and U (warps 8-15 and 16-23), one half's threads working while the other
 // half's products are made: X's sum over the first keys needs the first half of S only, U's first tokens only the first
 // half of R (T is lower triangular), P's sum over the first tokens only the first half of w U. V is fetched while P is
-// computed; S^T Q^T is issued behind X and O^T behind P. The MMA warp waits for the others at named barriers, which take
+// computed, and U's terms for O^T are written then, over X; S^T Q^T is issued behind X and O^T behind P. The MMA warp waits for the others at named barriers, which take
 // no issue slots. (Outputs made by the chain's warps beside X cost it a quarter more.)
-// At D = 256 a state thread has 64 keys in 96 registers and spills (1,354 bytes of stores, 1,472 of loads in the kernel, more
-// than half of them where columns are made again; D = 128: 96 and 244): 6.4 us a chunk, warps wait for tensor memory and for
-// what is spilled (4 x 2048 tokens, 16 heads: 205 us; tensor pipe 28 %).
+// At D = 256 a state thread has 64 keys in 96 registers and spills (1,310 bytes of stores, 1,416 of loads in the kernel, more
+// than half of them where columns are made again; D = 128: 100 and 248): 6.3 us a chunk, warps wait for tensor memory and for
+// what is spilled (4 x 2048 tokens, 16 heads: 202 us; tensor pipe 34 %).
 // At D = 64 the 64 values fill half of the 128 lanes; lanes 64-127 repeat them and store half of the output rows.
 //
 // Values that are not finite: the zeros of T and B meet them in tokens they must not reach. Whatever spoils a token
@@ -85,12 +84,15 @@ struct DeltaTcCfg {
   static constexpr uint32_t kOffBar = kOffTab + kTables * sizeof(DeltaTable);
   static constexpr size_t kSmem = kOffBar + 512 + 1024;
   // Tensor memory columns. S: for each quarter of the keys its two terms, over which P^T is written once X has read
-  // them. X: S^T K^T, then in its first half bf16(U)^T. R: for each 16 tokens the two terms of R^T. U: U^T, then for each
-  // 16 tokens the two terms of (w U)^T. XQ: S^T Q^T of even and odd chunks. O has columns of its own. At D = 256 there is
+  // them. X: S^T K^T, then for each 16 tokens the two terms of U^T. R: for each 16 tokens the two terms of R^T. U: U^T, then
+  // for each 16 tokens the two terms of (w U)^T. XQ: S^T Q^T of even and odd chunks. O has columns of its own. At D = 256 there is
   // one XQ, and O lies on U, once P has read it.
   static constexpr bool kAlias = D == 256;
   static constexpr uint32_t kColS = 0, kColX = D, kColR = kColX + 64, kColU = kColR + 64, kColXQ = kColU + 64,
                             kColO = kAlias ? kColU : kColXQ + 128, kColEnd = kAlias ? kColXQ + 64 : kColO + 64;
+  // Whether the chain fetches the next chunk's V before it hands over U for the outputs. Before / after, us: D = 256, 4 x 4096
+  // tokens 512 / 535; D = 128, 8 x 8192 702 / 646; D = 64 593 / 543.
+  static constexpr bool kFetchFirst = D == 256;
   // registers per thread after the split of the launch's 6 x 80 over the warpgroups (40, 56, 96 at D = 128: the chain a sixth
   // slower; more for the outputs, fewer for the state: the same)
   static constexpr int kRegsControl = D == 256 ? 40 : 56, kRegsOut = D == 256 ? 56 : 72,
@@ -106,7 +108,8 @@ enum DeltaBarrier {
   kBarAgain = 8,  // the chain's, around columns that are made again
   kBarS = 2,    // the state's terms written: chain -> MMA
   kBarR = 4,    // R^T written: chain -> MMA
-  kBarW = 6     // (w U)^T and U^T written: chain -> MMA
+  kBarW = 6,    // (w U)^T written: chain -> MMA
+  kBarU = 9     // U^T written: chain -> MMA
 };
 template <int THREADS>
 __device__ __forceinline__ void bar_arrive(int id) {
@@ -431,8 +434,8 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
         if (OUT && Cfg::kAlias && c > 0) wait(OE, c - 1);
         if (OUT && go()) {
 #pragma unroll
-          for (int i = 0; i < D / 16; ++i)
-            tc::mma_bf16_ts(tXQ(c), state(0, i), dk + (kq(i) + (Cfg::kPanel >> 4)),
+          for (int i = 0; i < D / 8; ++i)
+            tc::mma_bf16_ts(tXQ(c), state(i < D / 16, i % (D / 16)), dk + (kq(i % (D / 16)) + (Cfg::kPanel >> 4)),
                             tc::idesc(tc::kBF16, 128, 64, false, false), i > 0);
         }
         __syncwarp();
@@ -483,12 +486,16 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
           if constexpr (kParts == 1) tc::commit(B(PD + 1));
         }
         __syncwarp();
-        if (OUT && !Cfg::kAlias && c > 0) wait(OE, c - 1);
+        if constexpr (OUT) {
+          bar_sync<288>(kBarU);
+          bar_sync<288>(kBarU + 1);
+          if (!Cfg::kAlias && c > 0) wait(OE, c - 1);
+        }
         if (go()) {
 #pragma unroll
-          for (int i = 0; OUT && i < 8; ++i) {  // B's second term, then its first
+          for (int i = 0; OUT && i < 12; ++i) {  // terms of U and B: first second, second first, first first
             const int j = i & 3;
-            tc::mma_bf16_ts(tO + 16 * j, tX + 8 * j, dt + ((i < 4 ? 3 : 2) * kTerm + rows(j, 16 * j)),
+            tc::mma_bf16_ts(tO + 16 * j, tX + 16 * j + 8 * (i >> 2 == 1), dt + ((i < 4 ? 3 : 2) * kTerm + rows(j, 16 * j)),
                             tc::idesc(tc::kBF16, 128, 64 - 16 * j, false, false), i > 0);
           }
           tc::commit(B(OD));
@@ -784,28 +791,37 @@ __global__ void __launch_bounds__(DeltaTcCfg<D>::kThreads, 1) delta_tc_kernel(co
       }
       const float a_hi = t.a_hi, a_lo = t.a_lo;
       ready(UD, c);
-      {
-        uint32_t x[2][8];
-        tc::ld_frag2<2>(tc::lane_addr(tU, 32 * quad, 16 * part), tc::lane_addr(tU, 32 * quad + 16, 16 * part), x[0], x[1]);
+      uint32_t x[2][8];
+      tc::ld_frag2<2>(tc::lane_addr(tU, 32 * quad, 16 * part), tc::lane_addr(tU, 32 * quad + 16, 16 * part), x[0], x[1]);
+      auto u = [&](int e, int j) { return (static_cast<uint64_t>(x[e][2 * j + 1]) << 32) | x[e][2 * j]; };
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t first[4], second[4], whole[4];
+      for (int e = 0; e < 2; ++e) {
+        uint32_t first[4], second[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint64_t u = (static_cast<uint64_t>(x[e][2 * j + 1]) << 32) | x[e][2 * j];
-            whole[j] = f32x2_to_bf16x2(u);
-            split2(mul_f32x2(ww[j >> 1], u), first[j], second[j]);
-          }
-          tc::st_frag8(tc::lane_addr(tU, 32 * quad + 16 * e, 16 * part), first);
-          tc::st_frag8(tc::lane_addr(tU, 32 * quad + 16 * e, 16 * part + 8), second);
-          tc::st_frag8(tc::lane_addr(tX, 32 * quad + 16 * e, 8 * part), whole);
-        }
+        for (int j = 0; j < 4; ++j) split2(mul_f32x2(ww[j >> 1], u(e, j)), first[j], second[j]);
+        tc::st_frag8(tc::lane_addr(tU, 32 * quad + 16 * e, 16 * part), first);
+        tc::st_frag8(tc::lane_addr(tU, 32 * quad + 16 * e, 16 * part + 8), second);
       }
       tc::wait_st();
       tc::fence_before();
       hand_over(kBarW + half);
+      auto hand_over_u = [&]() {  // in X's columns of the warp's own tokens, while P is made
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t first[4], second[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) split2(u(e, j), first[j], second[j]);
+          tc::st_frag8(tc::lane_addr(tX, 32 * quad + 16 * e, 16 * part), first);
+          tc::st_frag8(tc::lane_addr(tX, 32 * quad + 16 * e, 16 * part + 8), second);
+        }
+        tc::wait_st();
+        tc::fence_before();
+        hand_over(kBarU + half);
+      };
+      if (OUT && !Cfg::kFetchFirst) hand_over_u();
       arrive(TE + c % NT);
       if (c + 1 < nchunks) fetch(c + 1);
+      if (OUT && Cfg::kFetchFirst) hand_over_u();
       ready(PD, c);
       // A constant decay's rounding would be the same one every chunk and is left out by a pair of numbers.
       const uint64_t ah = f32x2_splat(fixed ? a_hi : a_hi + a_lo), al = f32x2_splat(a_lo);

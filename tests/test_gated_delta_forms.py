@@ -90,3 +90,69 @@ def test_the_same_call_twice_is_the_same(cuda, lengths, dtype):
     for _ in range(5):
         again = M.gated_delta(*x)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def _two_terms(q, k, v, g, beta, h0, cu, scale):
+    """(outputs, a bound of their error before they are rounded) of the chunked form, in which every factor of an output, the
+    state and U and the scores, is two bf16 terms: 2^-16 of each value is left out at most (two half steps of 2^-8), so
+    is the product of two remainders; sums are fp32, truncating: 2 u an addition. To it the errors of the state before the
+    chunk and of U, as test_gated_delta has them for the columns (there 2^-8 stands for these 2^-16)."""
+    L, H, D = v.shape
+    rep = H // q.shape[1]
+    u24, two = 2.0 ** -24, 2.0 ** -16
+    q, k = (x.double().repeat_interleave(rep, 1) for x in (q, k))
+    v = v.double()
+    a = torch.ones(L, H, dtype=torch.float64, device=v.device) if g is None else g.double().exp().expand(L, H)
+    b = beta.double()
+    S = h0.double().clone()
+    E = torch.zeros(S.shape[0], H, D, dtype=torch.float64, device=v.device)
+    o, A = torch.zeros_like(v), torch.zeros_like(v)
+    norm = lambda x: torch.linalg.matrix_norm(x, 2)[:, None]  # noqa: E731
+    cols = lambda x: x.norm(dim=1)  # noqa: E731
+    for n in range(len(cu) - 1):
+        for t0 in range(int(cu[n]), int(cu[n + 1]), 64):
+            t1 = min(t0 + 64, int(cu[n + 1]))
+            kc, qc, vc = (x[t0:t1].transpose(0, 1) for x in (k, q, v))
+            G = a[t0:t1].log().cumsum(0).T
+            f, w, bc = G.exp()[..., None], (G[:, -1:] - G).exp()[..., None], b[t0:t1].T[..., None]
+            i = torch.arange(t1 - t0, device=v.device)
+            weight = torch.where(i[:, None] >= i, G[:, :, None] - G[:, None, :], -torch.inf).exp()
+            low = (kc @ kc.transpose(1, 2)) * weight * bc * (i[:, None] > i)
+            T = torch.linalg.inv(torch.eye(t1 - t0, dtype=torch.float64, device=v.device) + low)
+            r = bc * (vc - f * (kc @ S[n]))
+            u = T @ r
+            scores = (qc @ kc.transpose(1, 2)) * weight
+            o[t0:t1] = scale * (f * (qc @ S[n]) + scores @ u).transpose(0, 1)
+            turns = min(float(G.abs().max()) * 1.4427, 30.0)
+            nk, nT = norm(kc), norm(T)
+            dr = nk * (two + 4 * D * u24) * cols(S[n]) + 4 * u24 * cols(vc) + (two + 4 * u24) * cols(r)
+            dT = (2 * two + 384 * u24) * T.flatten(1).norm(dim=1)[:, None] + 64 * u24 * nT * (1 + norm(low)) \
+                + (2 * D + 20 + 7 * turns) * u24 * nT ** 2 * low.flatten(1).norm(dim=1)[:, None]
+            du = nT * dr + dT * cols(r) + nk * nT * E[n]
+            inter, sums = f * (qc.abs() @ S[n].abs()), scores.abs() @ u.abs()
+            A[t0:t1] = abs(scale) * ((two + (4 * D + 16 + 7 * turns) * u24) * inter
+                                     + (3 * two + (384 + 2 * D + 20 + 7 * turns) * u24) * sums
+                                     + f * qc.norm(dim=2, keepdim=True) * E[n][:, None]
+                                     + scores.norm(dim=2, keepdim=True) * du[:, None]).transpose(0, 1)
+            keep = G[:, -1].exp()[:, None]
+            E[n] = keep * E[n] + norm(w * kc) * (nT * dr + dT * cols(r) + (two + (256 + 7 * turns) * u24) * cols(u)) \
+                + 4 * u24 * cols(S[n])
+            S[n] = keep[..., None] * S[n] + (w * kc).transpose(1, 2) @ u
+    return o, A
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("decay", ["none", "head", "token"])
+@pytest.mark.parametrize("lengths", [[300, 64, 70, 130], [800]])
+def test_outputs_in_chunks_are_rounded_once(cuda, D, decay, lengths):
+    """What an output loses besides its own rounding is some 2^-16 of its terms."""
+    x = _inputs(66, lengths, 1, 2, D, BF, decay=decay)
+    o, _ = M.gated_delta(*x)
+    ref, A = _two_terms(*x, D ** -0.5)
+    assert torch.allclose(ref, _recurrence(*x, D ** -0.5)[0], atol=1e-10)
+    err = (o.double() - ref).abs()
+    bound = A * 1.01 + HALF[BF] * (ref.abs() + A) + 1e-40
+    assert bool((err <= bound).all()), f"worst {float((err / bound).max()):.3g} of its bound"
+    rounding = (ref.bfloat16().double() - ref).norm()  # of the exact outputs alone
+    assert float(err.norm()) <= 1.02 * float(rounding) + float(A.norm())

@@ -1,6 +1,6 @@
 """What the chunked gated-delta kernel does when a wait runs out, on the host: no GPU is made to stall.
 
-The roles are those of test_gated_delta_protocol, with waits that give up: a role whose wait has run out waits for no
+The roles are those of test_gated_delta_order, with waits that give up: a role whose wait has run out waits for no
 mbarrier any more and goes through its code to the end, the MMA and load warps without issuing anything. Named barriers
 count arrivals, as the hardware does. The chain's warps, which otherwise only arrive at them, join them once they have
 given up (``hand_over`` in the kernel).
@@ -13,10 +13,10 @@ from pathlib import Path
 
 import pytest
 
-from test_gated_delta_protocol import _roles
+from test_gated_delta_order import roles as _roles
 
 CSRC = Path(__file__).resolve().parents[1] / "memt-1.0_b200" / "csrc"
-NAMED = ("barS", "barR", "barW", "barEnd")
+NAMED = ("barS", "barR", "barW", "barU", "barEnd")
 
 
 class _Stuck(Exception):
@@ -137,7 +137,7 @@ def test_the_chain_joins_named_barriers_once_it_has_given_up():
     body = re.search(r"auto hand_over = \[&\]\(int id\) \{(.*?)\};", code, re.S).group(1)
     assert re.sub(r"\s+", " ", body).strip() == "if (alive) bar_arrive<288>(id); else bar_sync<288>(id);"
     assert code.count("bar_arrive<288>") == 1  # nowhere else
-    for bar in ("kBarS", "kBarR", "kBarW"):
+    for bar in ("kBarS", "kBarR", "kBarW", "kBarU"):
         assert f"hand_over({bar} + half)" in code and f"bar_sync<288>({bar})" in code
     # a warp of the chain has given up as a whole: behind both places where it waits
     assert code.count("alive = __all_sync(~0u, alive);") == 2
