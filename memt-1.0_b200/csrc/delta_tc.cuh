@@ -27,8 +27,8 @@
 // for S and P and of the tokens for R and U (warps 8-15 and 16-23), one half's threads working while the other
 // half's products are made: X's sum over the first keys needs the first half of S only, U's first tokens only the first
 // half of R (T is lower triangular), P's sum over the first tokens only the first half of w U. V is fetched while P is
-// computed, and U's terms for O^T are written then, over X; S^T Q^T is issued behind X and O^T behind P. The MMA warp waits for the others at named barriers, which take
-// no issue slots. (Outputs made by the chain's warps beside X cost it a quarter more.)
+// computed, and U's terms for O^T are written then, over X; S^T Q^T is issued behind X and O^T behind P. The MMA warp
+// waits for the others at named barriers, which take no issue slots. (Outputs made by the chain's warps beside X cost it a quarter more.)
 // At D = 256 a state thread has 64 keys in 96 registers and spills (1,310 bytes of stores, 1,416 of loads in the kernel, more
 // than half of them where columns are made again; D = 128: 100 and 248): 6.3 us a chunk, warps wait for tensor memory and for
 // what is spilled (4 x 2048 tokens, 16 heads: 202 us; tensor pipe 34 %).
@@ -90,8 +90,8 @@ struct DeltaTcCfg {
   static constexpr bool kAlias = D == 256;
   static constexpr uint32_t kColS = 0, kColX = D, kColR = kColX + 64, kColU = kColR + 64, kColXQ = kColU + 64,
                             kColO = kAlias ? kColU : kColXQ + 128, kColEnd = kAlias ? kColXQ + 64 : kColO + 64;
-  // Whether the chain fetches the next chunk's V before it hands over U for the outputs. Before / after, us: D = 256, 4 x 4096
-  // tokens 512 / 535; D = 128, 8 x 8192 702 / 646; D = 64 593 / 543.
+  // Whether the chain fetches the next chunk's V before it hands over U for the outputs. V first / U first, us: D = 256,
+  // 4 x 4096 tokens 512 / 535; 8 x 8192 tokens at D = 128 702 / 646, at D = 64 593 / 543.
   static constexpr bool kFetchFirst = D == 256;
   // registers per thread after the split of the launch's 6 x 80 over the warpgroups (40, 56, 96 at D = 128: the chain a sixth
   // slower; more for the outputs, fewer for the state: the same)
